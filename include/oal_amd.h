@@ -265,6 +265,46 @@ int oal_check_labels(const void* labels, int wide, int per_head, int head_dim, i
 int oal_check_outputs(int wide, int out_kind, const void* num, const void* den, const void* out, size_t rows,
                       int width, int num_stride, int out_stride, int* flag, void* stream);
 
+/*
+ * Gated delta rule, per state head (exp, sums and state in fp32 or more):
+ *   S_t = e^(g_t) S_(t-1) + k_t u_t^T,  u_t = beta_t (v_t - e^(g_t) S_(t-1)^T k_t),  o_t = scale S_t^T q_t
+ * q [B][Hq][N][64], k [B][Hk][N][64], v [B][Hv][N][64] of dtype, g [B][Hv][N] f32, beta [B][Hv][N] of
+ * dtype or (beta_f32) f32; Hk divides Hv, one of Hq and Hv divides the other, and
+ * out [B][H][N][64] (dtype) has H = max(Hq, Hv) heads: output head o reads state head
+ * o Hv / H and query head o Hq / H, state head h key head h Hk / Hv. strides:
+ * of q, k, v, g, beta, three each (batch, head, token), in elements; rows of q, k
+ * and v are contiguous and 16-byte aligned. state (may be NULL: zero) and
+ * final_state [B][Hv][64][64] f32, rows the key's dimensions. saved
+ * (oal_gated_delta_saved_bytes) is what the backward reads.
+ */
+size_t oal_gated_delta_saved_bytes(int batch, int v_heads, int seq_len);
+int oal_gated_delta_forward(const void* q, const void* k, const void* v, const float* g, const void* beta,
+                            const int64_t* strides, int beta_f32, int batch, int q_heads, int k_heads, int v_heads,
+                            int seq_len, int dtype, float scale, const float* state, void* out, float* final_state,
+                            void* saved, void* stream);
+
+/*
+ * Its VJP: dout [B][H][N][64] (dtype) and dfinal [B][Hv][64][64] f32 (may be NULL)
+ * -> contiguous dq, dk, dv (dtype), dg f32, dbeta (beta's type) and dstate f32 (may be
+ * NULL). Heads that are shared are summed in a fixed order.
+ */
+size_t oal_gated_delta_workspace_bytes(int batch, int q_heads, int k_heads, int v_heads, int seq_len);
+int oal_gated_delta_backward(const void* q, const void* k, const void* v, const float* g, const void* beta,
+                             const int64_t* strides, int beta_f32, int batch, int q_heads, int k_heads, int v_heads,
+                             int seq_len, int dtype, float scale, const void* saved, const void* dout,
+                             const float* dfinal, void* dq, void* dk, void* dv, float* dg, void* dbeta, float* dstate,
+                             void* workspace, void* stream);
+
+/*
+ * The recurrence for a few tokens: state [B][Hv][key_dim][value_dim] f32 is updated
+ * in place, out [B][H][N][value_dim] is written; dimensions 1 to 64, rows of any
+ * alignment. kind: 0 float32, 1 bfloat16, 2 float16 (of q, k, v, out, and of beta unless beta_f32).
+ */
+int oal_gated_delta_step(const void* q, const void* k, const void* v, const float* g, const void* beta,
+                         const int64_t* strides, int beta_f32, int batch, int q_heads, int k_heads, int v_heads,
+                         int seq_len, int key_dim, int value_dim, int kind, float scale, float* state, void* out,
+                         void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -78,6 +78,11 @@ _SIGNATURES = {
     "oal_rotary_heads": ([_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp], _i),
     "oal_check_labels": ([_vp, _i, _i, _i, _i, _i, _vp, _vp, _vp], _i),
     "oal_check_outputs": ([_i, _i, _vp, _vp, _vp, _sz, _i, _i, _i, _vp, _vp], _i),
+    "oal_gated_delta_saved_bytes": ([_i] * 3, _sz),
+    "oal_gated_delta_workspace_bytes": ([_i] * 5, _sz),
+    "oal_gated_delta_forward": ([_vp] * 6 + [_i] * 7 + [_f] + [_vp] * 5, _i),
+    "oal_gated_delta_backward": ([_vp] * 6 + [_i] * 7 + [_f] + [_vp] * 11, _i),
+    "oal_gated_delta_step": ([_vp] * 6 + [_i] * 9 + [_f] + [_vp] * 3, _i),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
@@ -703,3 +708,83 @@ class Verdict:
             self._pending = False
         labels, outputs = self._words.tolist()
         return labels, outputs
+
+
+# ---------------------------------------------------------------------------
+# Gated delta rule (oal_delta.hip). The callers (gated_delta.py) have checked types,
+# shapes and devices; rows may lie at any strides.
+# ---------------------------------------------------------------------------
+def row_tensor(t: torch.Tensor) -> torch.Tensor:
+    """t, or a contiguous copy unless its rows are contiguous and 16-byte aligned."""
+    size = t.element_size()
+    strides = [s for s, n in zip(t.stride(), t.shape) if n > 1]
+    if (t.stride(-1) == 1 or t.shape[-1] == 1) and t.data_ptr() % 16 == 0 and all(
+            s * size % 16 == 0 for s in strides if s != 1):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _stride_array(*tensors: torch.Tensor):
+    """(batch, head, token) strides of each tensor; a dimension of one has none."""
+    values = [s if n > 1 else 0 for t in tensors for s, n in zip(t.stride()[:3], t.shape[:3])]
+    return (ctypes.c_int64 * len(values))(*values)
+
+
+def delta_forward(q, k, v, g, beta, state, *, scale: float):
+    """q, k, v [B, heads, N, 64] float32 or bfloat16 with aligned rows, g float32, beta
+    float32 or q's type, state float32 [B, Hv, 64, 64] or None. Returns (out, final_state, saved)."""
+    lib = load_library()
+    b, hq, n, _ = q.shape
+    hk, hv, dev = k.shape[1], v.shape[1], q.device
+    with _scope(dev, "oal_amd::gated_delta_forward"):
+        nbytes = lib.oal_gated_delta_saved_bytes(b, hv, n)
+        if nbytes == 0:
+            _check(1, lib, "oal_gated_delta_saved_bytes")
+        out = torch.empty((b, max(hq, hv), n, HEAD_DIM), dtype=q.dtype, device=dev)
+        final = torch.empty((b, hv, HEAD_DIM, HEAD_DIM), dtype=torch.float32, device=dev)
+        saved = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+        rc = lib.oal_gated_delta_forward(
+            _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(beta), _stride_array(q, k, v, g, beta),
+            int(beta.dtype == torch.float32), b, hq, hk, hv, n, _dtype_code(q.dtype), float(scale), _ptr(state),
+            _ptr(out), _ptr(final), _ptr(saved), _stream(dev))
+        _check(rc, lib, "oal_gated_delta_forward")
+    return out, final, saved
+
+
+def delta_backward(q, k, v, g, beta, saved, dout, dfinal, *, scale: float, need_state: bool):
+    """The VJP of :func:`delta_forward`: (dq, dk, dv, dg, dbeta, dstate or None)."""
+    lib = load_library()
+    b, hq, n, _ = q.shape
+    hk, hv, dev = k.shape[1], v.shape[1], q.device
+    with _scope(dev, "oal_amd::gated_delta_backward"):
+        nbytes = lib.oal_gated_delta_workspace_bytes(b, hq, hk, hv, n)
+        if nbytes == 0:
+            _check(1, lib, "oal_gated_delta_workspace_bytes")
+        work = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+        grads = [torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v, g, beta)]
+        dstate = torch.empty((b, hv, HEAD_DIM, HEAD_DIM), dtype=torch.float32, device=dev) if need_state else None
+        rc = lib.oal_gated_delta_backward(
+            _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(beta), _stride_array(q, k, v, g, beta),
+            int(beta.dtype == torch.float32), b, hq, hk, hv, n, _dtype_code(q.dtype), float(scale), _ptr(saved),
+            _ptr(dout), _ptr(dfinal), *(_ptr(t) for t in grads), _ptr(dstate), _ptr(work), _stream(dev))
+        _check(rc, lib, "oal_gated_delta_backward")
+    return (*grads, dstate)
+
+
+_KINDS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def delta_step(q, k, v, g, beta, state, *, scale: float) -> torch.Tensor:
+    """The recurrence over the N tokens of q, k, v [B, heads, N, D] (unit stride in a row);
+    state [B, Hv, Dk, Dv] contiguous float32 is updated in place."""
+    lib = load_library()
+    b, hq, n, dk = q.shape
+    hk, hv, dv, dev = k.shape[1], v.shape[1], v.shape[3], q.device
+    with _scope(dev, "oal_amd::gated_delta_step"):
+        out = torch.empty((b, max(hq, hv), n, dv), dtype=q.dtype, device=dev)
+        rc = lib.oal_gated_delta_step(
+            _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(beta), _stride_array(q, k, v, g, beta),
+            int(beta.dtype == torch.float32), b, hq, hk, hv, n, dk, dv, _KINDS[q.dtype], float(scale), _ptr(state),
+            _ptr(out), _stream(dev))
+        _check(rc, lib, "oal_gated_delta_step")
+    return out

@@ -30,6 +30,7 @@
 
 #include "oal_amd.h"
 #include "oal_common.hpp"
+#include "oal_delta.hpp"
 #include "oal_direct.hpp"
 #include "oal_internal.hpp"
 
@@ -1457,6 +1458,124 @@ int oal_check_outputs(int wide, int out_kind, const void* num, const void* den, 
                                 static_cast<hipStream_t>(stream)))
     return fail("oal_check_outputs: unknown output type");
   return launch_status("oal_check_outputs launch");
+}
+
+// ---------------------------------------------------------------------------
+// Gated delta rule
+// ---------------------------------------------------------------------------
+// A grid holds fewer than 2^32 threads; the kernels have at most 256 a block.
+static bool grid_fits(int64_t blocks) { return blocks < (int64_t(1) << 24); }
+
+static int check_delta(int batch, int q_heads, int k_heads, int v_heads, int seq_len) {
+  if (batch <= 0 || q_heads <= 0 || k_heads <= 0 || v_heads <= 0 || seq_len <= 0)
+    return fail("batch, head counts and sequence length must be positive");
+  if (v_heads % k_heads != 0) return fail("value head count must be divisible by key head count");
+  if (q_heads % v_heads != 0 && v_heads % q_heads != 0)
+    return fail("one of query and value head counts must be divisible by the other");
+  const int64_t heads = q_heads > v_heads ? q_heads : v_heads, chunks = (int64_t(seq_len) + 63) / 64;
+  // also the head sums of the backward: a thread per 4 of N 64 values
+  if (int64_t(batch) > (int64_t(1) << 24) / heads || !grid_fits(batch * heads * chunks) ||
+      !grid_fits(batch * heads * ((int64_t(seq_len) + 15) / 16)))
+    return fail("batch, heads and sequence length are too large for one launch");
+  return 0;
+}
+
+static oal::Strided strided(const void* p, const int64_t* s) { return {p, s[0], s[1], s[2]}; }
+
+static bool rows_aligned(const oal::Strided& s, int bytes) {
+  return aligned16(s.p) && (s.b * bytes) % 16 == 0 && (s.h * bytes) % 16 == 0 && (s.n * bytes) % 16 == 0;
+}
+
+static int delta_args(oal::DeltaArgs* a, const char* what, const void* q, const void* k, const void* v, const float* g,
+                      const void* beta, const int64_t* strides, int beta_f32, int batch, int q_heads, int k_heads,
+                      int v_heads, int seq_len, int dtype, float scale) {
+  if (check_delta(batch, q_heads, k_heads, v_heads, seq_len)) return 1;
+  if (dtype != OAL_DTYPE_F32 && dtype != OAL_DTYPE_BF16) return fail("dtype must be OAL_DTYPE_F32 or OAL_DTYPE_BF16");
+  if (!q || !k || !v || !g || !beta || !strides) return fail(std::string(what) + ": null pointer argument");
+  *a = {strided(q, strides), strided(k, strides + 3), strided(v, strides + 6), strided(g, strides + 9),
+        strided(beta, strides + 12), batch, q_heads, k_heads, v_heads, q_heads > v_heads ? q_heads : v_heads, seq_len,
+        (seq_len + 63) / 64, beta_f32 != 0 || dtype == OAL_DTYPE_F32, scale};
+  const int bytes = dtype == OAL_DTYPE_F32 ? 4 : 2;
+  if (!rows_aligned(a->q, bytes) || !rows_aligned(a->k, bytes) || !rows_aligned(a->v, bytes))
+    return fail(std::string(what) + ": rows must be 16-byte aligned");
+  return 0;
+}
+
+size_t oal_gated_delta_saved_bytes(int batch, int v_heads, int seq_len) {
+  if (check_delta(batch, v_heads, v_heads, v_heads, seq_len)) return 0;
+  return oal::delta_saved_view(nullptr, batch * v_heads, (seq_len + 63) / 64).bytes;
+}
+
+size_t oal_gated_delta_workspace_bytes(int batch, int q_heads, int k_heads, int v_heads, int seq_len) {
+  if (check_delta(batch, q_heads, k_heads, v_heads, seq_len)) return 0;
+  oal::DeltaArgs a{};
+  a.B = batch, a.Hq = q_heads, a.Hk = k_heads, a.Hv = v_heads, a.N = seq_len;
+  a.H = q_heads > v_heads ? q_heads : v_heads, a.NC = (seq_len + 63) / 64;
+  return oal::delta_work_view(nullptr, a).bytes;
+}
+
+int oal_gated_delta_forward(const void* q, const void* k, const void* v, const float* g, const void* beta,
+                            const int64_t* strides, int beta_f32, int batch, int q_heads, int k_heads, int v_heads,
+                            int seq_len, int dtype, float scale, const float* state, void* out, float* final_state,
+                            void* saved, void* stream) {
+  Range range("oal_gated_delta_forward");
+  oal::DeltaArgs a;
+  if (delta_args(&a, "oal_gated_delta_forward", q, k, v, g, beta, strides, beta_f32, batch, q_heads, k_heads, v_heads,
+                 seq_len, dtype, scale))
+    return 1;
+  if (!out || !final_state || !saved) return fail("oal_gated_delta_forward: null pointer argument");
+  const void* ptrs[] = {state, out, final_state, saved};
+  for (const void* p : ptrs)
+    if (!aligned16(p)) return fail("oal_gated_delta_forward: tensor pointers must be 16-byte aligned");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (dtype == OAL_DTYPE_F32)
+    oal::launch_delta_forward<float>(a, state, out, final_state, saved, st, make_timer());
+  else
+    oal::launch_delta_forward<uint16_t>(a, state, out, final_state, saved, st, make_timer());
+  return launch_status("oal_gated_delta_forward launch");
+}
+
+int oal_gated_delta_backward(const void* q, const void* k, const void* v, const float* g, const void* beta,
+                             const int64_t* strides, int beta_f32, int batch, int q_heads, int k_heads, int v_heads,
+                             int seq_len, int dtype, float scale, const void* saved, const void* dout,
+                             const float* dfinal, void* dq, void* dk, void* dv, float* dg, void* dbeta, float* dstate,
+                             void* workspace, void* stream) {
+  Range range("oal_gated_delta_backward");
+  oal::DeltaArgs a;
+  if (delta_args(&a, "oal_gated_delta_backward", q, k, v, g, beta, strides, beta_f32, batch, q_heads, k_heads, v_heads,
+                 seq_len, dtype, scale))
+    return 1;
+  if (!saved || !dout || !dq || !dk || !dv || !dg || !dbeta || !workspace)
+    return fail("oal_gated_delta_backward: null pointer argument");
+  const void* ptrs[] = {saved, dout, dfinal, dq, dk, dv, dstate, workspace};
+  for (const void* p : ptrs)
+    if (!aligned16(p)) return fail("oal_gated_delta_backward: tensor pointers must be 16-byte aligned");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (dtype == OAL_DTYPE_F32)
+    oal::launch_delta_backward<float>(a, saved, dout, dfinal, dq, dk, dv, dg, dbeta, dstate, workspace, st, make_timer());
+  else
+    oal::launch_delta_backward<uint16_t>(a, saved, dout, dfinal, dq, dk, dv, dg, dbeta, dstate, workspace, st,
+                                         make_timer());
+  return launch_status("oal_gated_delta_backward launch");
+}
+
+int oal_gated_delta_step(const void* q, const void* k, const void* v, const float* g, const void* beta,
+                         const int64_t* strides, int beta_f32, int batch, int q_heads, int k_heads, int v_heads,
+                         int seq_len, int key_dim, int value_dim, int kind, float scale, float* state, void* out,
+                         void* stream) {
+  Range range("oal_gated_delta_step");
+  if (check_delta(batch, q_heads, k_heads, v_heads, seq_len)) return 1;
+  if (key_dim < 1 || key_dim > 64 || value_dim < 1 || value_dim > 64)
+    return fail("oal_gated_delta_step: dimensions must be in [1, 64]");
+  if (kind < 0 || kind > 2) return fail("oal_gated_delta_step: unknown type");
+  if (!q || !k || !v || !g || !beta || !strides || !state || !out)
+    return fail("oal_gated_delta_step: null pointer argument");
+  const oal::DeltaStepArgs a = {strided(q, strides), strided(k, strides + 3), strided(v, strides + 6),
+                                strided(g, strides + 9), strided(beta, strides + 12), batch, q_heads, k_heads, v_heads,
+                                q_heads > v_heads ? q_heads : v_heads, seq_len, key_dim, value_dim,
+                                beta_f32 != 0 || kind == 0, scale, state, out};
+  oal::launch_delta_step(kind, a, static_cast<hipStream_t>(stream), make_timer());
+  return launch_status("oal_gated_delta_step launch");
 }
 
 }  // extern "C"

@@ -1,0 +1,204 @@
+// Products of 64 x 64 tiles on the matrix cores whose operands are one or three
+// bf16 parts, for the chunked and the windowed attention kernels on gfx950.
+//
+// A value in three bf16 parts (the value rounded, what that left, what that
+// left) carries 24 bits, so products of such parts that leave out only the terms below
+// 2^-24 are as exact as fp32, at 3 (one operand a bf16 value as it is) or 6 matrix
+// instructions in place of the 16 times slower fp32 ones. bf16 tensors enter as
+// one part, fp32 tensors and intermediate results that have to stay fp32 as three.
+//
+// An accumulator tile of v_mfma_f32_16x16x32_bf16 holds rows 4 g + i in lane group
+// g = lane / 16, and an operand's lane group g holds 8 of the 32 indexes that the
+// product sums over. Which 8 does not matter as long as both operands agree, so
+// two accumulator tiles (32 rows) are, lane for lane, an operand of a product
+// that sums over their rows, in the order
+//   slot (g, j) -> row 4 g + j (j < 4), 16 + 4 g + j - 4 (j >= 4),
+// and the other operand is read from LDS in that order: chains of products
+// pass through registers. "perm" marks that order below.
+#pragma once
+
+#include "oal_mfma_common.hpp"
+
+namespace oal {
+
+constexpr int kTileRow = 72;  // bf16 of an LDS row: 144 bytes, 16 rows start in distinct banks
+constexpr int kTileElems = 64 * kTileRow;
+
+template <int NP>
+struct Frag {
+  bf16x8 p[NP];
+};
+
+// Parts per value of an element type.
+template <typename T>
+constexpr int kPartsOf = sizeof(T) == 4 ? 3 : 1;
+
+__device__ __forceinline__ float bf16_part(float x) { return static_cast<float>(static_cast<__bf16>(x)); }
+
+template <int NP>
+__device__ __forceinline__ Frag<NP> split(const float (&v)[8]) {
+  Frag<NP> f;
+  float r[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) r[e] = v[e];
+#pragma unroll
+  for (int p = 0; p < NP; ++p) {
+    f.p[p] = pack8(r);
+    if (p + 1 < NP) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) r[e] -= static_cast<float>(f.p[p][e]);
+    }
+  }
+  return f;
+}
+
+// c += a b without the terms of parts below fp32's last bit; small terms first.
+template <int NA, int NB>
+__device__ __forceinline__ f32x4 mma(const Frag<NA>& a, const Frag<NB>& b, f32x4 c) {
+  constexpr int kLast = (NA > NB ? NA : NB) - 1;
+#pragma unroll
+  for (int s = kLast; s >= 0; --s)
+#pragma unroll
+    for (int i = 0; i < NA; ++i) {
+      const int j = s - i;
+      if (j >= 0 && j < NB) c = mfma16(a.p[i], b.p[j], c);
+    }
+  return c;
+}
+
+// LDS tile: NP parts of 64 rows of kTileRow bf16.
+template <int NP>
+struct Tile {
+  __bf16 x[NP * kTileElems];
+};
+
+typedef __bf16 lds_bf16x4 __attribute__((ext_vector_type(4)));
+
+// Operand row r0 + lane % 16, sum indexes 32 t + 8 g + j.
+template <int NP>
+__device__ __forceinline__ Frag<NP> row_frag(const Tile<NP>& s, int r0, int t, int lane) {
+  Frag<NP> f;
+  const __bf16* p = s.x + (r0 + (lane & 15)) * kTileRow + 32 * t + 8 * (lane >> 4);
+#pragma unroll
+  for (int e = 0; e < NP; ++e) f.p[e] = *reinterpret_cast<const bf16x8*>(p + e * kTileElems);
+  return f;
+}
+// The same row with the sum indexes in perm order.
+template <int NP>
+__device__ __forceinline__ Frag<NP> row_frag_perm(const Tile<NP>& s, int r0, int t, int lane) {
+  Frag<NP> f;
+  const __bf16* p = s.x + (r0 + (lane & 15)) * kTileRow + 32 * t + 4 * (lane >> 4);
+#pragma unroll
+  for (int e = 0; e < NP; ++e) {
+    const bf16x4 lo = *reinterpret_cast<const bf16x4*>(p + e * kTileElems);
+    const bf16x4 hi = *reinterpret_cast<const bf16x4*>(p + e * kTileElems + 16);
+    f.p[e] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+  return f;
+}
+
+// Transposed read: operand row c0 + lane % 16 is a column of the tile, the sum
+// indexes are its rows. ds_read_b64_tr_b16 hands lane i of a 16-lane group column i
+// of the 4 x 16 block whose row j lanes 4 j .. 4 j + 3 address.
+__device__ __forceinline__ bf16x8 tr_rows(const __bf16* lo_row, const __bf16* hi_row) {
+  typedef __attribute__((address_space(3))) trv4 lds_trv4;
+  const trv4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_trv4*)(lo_row));
+  const trv4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_trv4*)(hi_row));
+  typedef short trv8 __attribute__((ext_vector_type(8)));
+  const trv8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  return __builtin_bit_cast(bf16x8, v);
+}
+template <int NP>
+__device__ __forceinline__ Frag<NP> col_frag_perm(const Tile<NP>& s, int c0, int t, int lane) {
+  Frag<NP> f;
+  const int g = lane >> 4, i = lane & 15;
+  const __bf16* p = s.x + (32 * t + 4 * g + (i >> 2)) * kTileRow + c0 + 4 * (i & 3);
+#pragma unroll
+  for (int e = 0; e < NP; ++e) f.p[e] = tr_rows(p + e * kTileElems, p + e * kTileElems + 16 * kTileRow);
+  return f;
+}
+template <int NP>
+__device__ __forceinline__ Frag<NP> col_frag(const Tile<NP>& s, int c0, int t, int lane) {
+  Frag<NP> f;
+  const int g = lane >> 4, i = lane & 15;
+  const __bf16* p = s.x + (32 * t + 8 * g + (i >> 2)) * kTileRow + c0 + 4 * (i & 3);
+#pragma unroll
+  for (int e = 0; e < NP; ++e) f.p[e] = tr_rows(p + e * kTileElems, p + e * kTileElems + 4 * kTileRow);
+  return f;
+}
+
+// Two accumulator tiles as the operand of a sum over their 32 rows (perm order).
+template <int NP>
+__device__ __forceinline__ Frag<NP> acc_frag(const f32x4& lo, const f32x4& hi) {
+  const float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  return split<NP>(v);
+}
+
+// 8 consecutive values of a row in global memory as floats.
+__device__ __forceinline__ void load_row8(float (&x)[8], const float* p) {
+  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+  x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+}
+
+// Operand row straight from global memory: 8 values at p (not read unless live: zero then).
+template <int NP, typename T>
+__device__ __forceinline__ Frag<NP> global_frag(const T* p, bool live) {
+  Frag<NP> f;
+  if constexpr (sizeof(T) == 2) {
+    static_assert(NP == 1, "a bf16 value is one part");
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (live) v = *reinterpret_cast<const uint4*>(p);
+    f.p[0] = __builtin_bit_cast(bf16x8, v);
+  } else {
+    float x[8] = {};
+    if (live) load_row8(x, p);
+    f = split<NP>(x);
+  }
+  return f;
+}
+
+// ROWS rows of 64 values (row stride in elements) into rows 0 .. of an LDS tile,
+// NT threads; rows at and past `live` are zero. 16-byte aligned rows.
+template <int ROWS, int NT, int NP, typename T>
+__device__ __forceinline__ void load_tile(Tile<NP>& s, const T* __restrict__ src, int64_t stride, int live, int t) {
+  if constexpr (sizeof(T) == 2) {
+    static_assert(NP == 1, "a bf16 value is one part");
+    constexpr int kIt = (ROWS * 8 + NT - 1) / NT;
+    uint4 v[kIt];
+#pragma unroll
+    for (int x = 0; x < kIt; ++x) {
+      const int i = t + NT * x, r = i >> 3;
+      v[x] = make_uint4(0, 0, 0, 0);
+      if (r < live && i < ROWS * 8) v[x] = *reinterpret_cast<const uint4*>(src + r * stride + 8 * (i & 7));
+    }
+#pragma unroll
+    for (int x = 0; x < kIt; ++x) {
+      const int i = t + NT * x;
+      if (i < ROWS * 8) *reinterpret_cast<uint4*>(s.x + (i >> 3) * kTileRow + 8 * (i & 7)) = v[x];
+    }
+  } else {
+    constexpr int kIt = (ROWS * 8 + NT - 1) / NT;
+#pragma unroll
+    for (int x = 0; x < kIt; ++x) {
+      const int i = t + NT * x, r = i >> 3;
+      if (i < ROWS * 8) {
+        const Frag<NP> f = global_frag<NP>(src + r * stride + 8 * (i & 7), r < live);
+#pragma unroll
+        for (int e = 0; e < NP; ++e)
+          *reinterpret_cast<bf16x8*>(s.x + e * kTileElems + r * kTileRow + 8 * (i & 7)) = f.p[e];
+      }
+    }
+  }
+}
+
+// Sum over the four lane groups of a wave (lanes of one column).
+__device__ __forceinline__ float group_sum(float x) {
+  x += __shfl_xor(x, 16, 64);
+  return x + __shfl_xor(x, 32, 64);
+}
+__device__ __forceinline__ float group_max(float x) {
+  x = fmaxf(x, __shfl_xor(x, 16, 64));
+  return fmaxf(x, __shfl_xor(x, 32, 64));
+}
+
+}  // namespace oal
