@@ -305,6 +305,43 @@ int oal_gated_delta_step(const void* q, const void* k, const void* v, const floa
                          int seq_len, int key_dim, int value_dim, int kind, float scale, float* state, void* out,
                          void* stream);
 
+/*
+ * Causal softmax attention over a sliding window and first keys that stay visible:
+ * out_i = sum_j softmax_j(scale q_i.k_j) v_j over keys j <= p_i with p_i - j < window or
+ * j < sinks, p_i = key_len - query_len + i (the queries are the last tokens). q, out
+ * [B][Hq][query_len][64], k, v [B][Hkv][key_len][64] of dtype; query head h reads KV head
+ * h / (Hq / Hkv). strides: of q, k, v, three each (batch, head, token), in elements;
+ * rows contiguous and 16-byte aligned; out is contiguous. lse [B][Hq][query_len] f32 is what the
+ * backward reads (log2 of the sums of exponentials). 1 <= query_len <= key_len, window >= 1, sinks >= 0.
+ */
+int oal_window_attention_forward(const void* q, const void* k, const void* v, const int64_t* strides, int batch,
+                                 int q_heads, int kv_heads, int query_len, int key_len, int window, int sinks,
+                                 int dtype, float scale, void* out, float* lse, void* stream);
+
+/* Its VJP: out, lse and dout [B][Hq][query_len][64] -> contiguous dq, dk, dv (dtype). */
+size_t oal_window_attention_workspace_bytes(int batch, int q_heads, int kv_heads, int query_len, int key_len,
+                                            int window, int sinks, int dtype);
+int oal_window_attention_backward(const void* q, const void* k, const void* v, const int64_t* strides, int batch,
+                                  int q_heads, int kv_heads, int query_len, int key_len, int window, int sinks,
+                                  int dtype, float scale, const void* out, const float* lse, const void* dout,
+                                  void* dq, void* dk, void* dv, void* workspace, void* stream);
+
+/*
+ * One token per sequence over ring caches [B][Hkv][sinks + window][D]: the token at
+ * position p (tokens before it) is written to slot p < sinks ? p : sinks + (p - sinks) % window
+ * and sees the min(p + 1, sinks + window) filled slots. position [B] int64 on the
+ * device; a negative one means no token: nothing is written, out is zero. strides: of q, k, v,
+ * k_cache, v_cache, three each (batch, head, slot; those of q, k, v unused for the slot). key_dim and
+ * value_dim multiples of 8 up to 64, all rows 16-byte aligned; out [B][Hq][value_dim]
+ * contiguous. kind: 0 float32, 1 bfloat16, 2 float16.
+ */
+size_t oal_window_attention_step_workspace_bytes(int batch, int q_heads, int kv_heads, int value_dim, int window,
+                                                 int sinks);
+int oal_window_attention_step(const void* q, const void* k, const void* v, void* k_cache, void* v_cache,
+                              const int64_t* strides, const int64_t* position, int batch, int q_heads, int kv_heads,
+                              int key_dim, int value_dim, int window, int sinks, int kind, float scale, void* out,
+                              void* workspace, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -83,6 +83,11 @@ _SIGNATURES = {
     "oal_gated_delta_forward": ([_vp] * 6 + [_i] * 7 + [_f] + [_vp] * 5, _i),
     "oal_gated_delta_backward": ([_vp] * 6 + [_i] * 7 + [_f] + [_vp] * 11, _i),
     "oal_gated_delta_step": ([_vp] * 6 + [_i] * 9 + [_f] + [_vp] * 3, _i),
+    "oal_window_attention_forward": ([_vp] * 4 + [_i] * 8 + [_f] + [_vp] * 3, _i),
+    "oal_window_attention_workspace_bytes": ([_i] * 8, _sz),
+    "oal_window_attention_backward": ([_vp] * 4 + [_i] * 8 + [_f] + [_vp] * 8, _i),
+    "oal_window_attention_step_workspace_bytes": ([_i] * 6, _sz),
+    "oal_window_attention_step": ([_vp] * 7 + [_i] * 8 + [_f] + [_vp] * 3, _i),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
@@ -787,4 +792,61 @@ def delta_step(q, k, v, g, beta, state, *, scale: float) -> torch.Tensor:
             int(beta.dtype == torch.float32), b, hq, hk, hv, n, dk, dv, _KINDS[q.dtype], float(scale), _ptr(state),
             _ptr(out), _stream(dev))
         _check(rc, lib, "oal_gated_delta_step")
+    return out
+
+
+# ---------------------------------------------------------------------------
+# Windowed attention (oal_window.hip). The callers (window_attention.py) have checked
+# types, shapes and devices; rows are contiguous and aligned, at any strides.
+# ---------------------------------------------------------------------------
+def window_forward(q, k, v, *, window: int, sinks: int, scale: float):
+    """q [B, Hq, Nq, 64], k and v [B, Hkv, Nk, 64], float32 or bfloat16. Returns (out, lse)."""
+    lib = load_library()
+    b, hq, nq, _ = q.shape
+    hk, nk, dev = k.shape[1], k.shape[2], q.device
+    with _scope(dev, "oal_amd::window_attention_forward"):
+        out = torch.empty((b, hq, nq, HEAD_DIM), dtype=q.dtype, device=dev)
+        lse = torch.empty((b, hq, nq), dtype=torch.float32, device=dev)
+        rc = lib.oal_window_attention_forward(
+            _ptr(q), _ptr(k), _ptr(v), _stride_array(q, k, v), b, hq, hk, nq, nk, window, sinks, _dtype_code(q.dtype),
+            float(scale), _ptr(out), _ptr(lse), _stream(dev))
+        _check(rc, lib, "oal_window_attention_forward")
+    return out, lse
+
+
+def window_backward(q, k, v, out, lse, dout, *, window: int, sinks: int, scale: float):
+    """The VJP of :func:`window_forward`: (dq, dk, dv)."""
+    lib = load_library()
+    b, hq, nq, _ = q.shape
+    hk, nk, dev, code = k.shape[1], k.shape[2], q.device, _dtype_code(q.dtype)
+    with _scope(dev, "oal_amd::window_attention_backward"):
+        nbytes = lib.oal_window_attention_workspace_bytes(b, hq, hk, nq, nk, window, sinks, code)
+        if nbytes == 0:
+            _check(1, lib, "oal_window_attention_workspace_bytes")
+        work = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+        grads = [torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v)]
+        rc = lib.oal_window_attention_backward(
+            _ptr(q), _ptr(k), _ptr(v), _stride_array(q, k, v), b, hq, hk, nq, nk, window, sinks, code, float(scale),
+            _ptr(out), _ptr(lse), _ptr(dout), *(_ptr(t) for t in grads), _ptr(work), _stream(dev))
+        _check(rc, lib, "oal_window_attention_backward")
+    return tuple(grads)
+
+
+def window_step(q, k, v, k_cache, v_cache, positions, *, window: int, sinks: int, scale: float) -> torch.Tensor:
+    """One token q [B, Hq, 1, D], k, v [B, Hkv, 1, D] over the ring caches
+    [B, Hkv, sinks + window, D], which it is written into; positions int64 [B]."""
+    lib = load_library()
+    b, hq, _, d = q.shape
+    hk, dv, dev = k.shape[1], v.shape[3], q.device
+    with _scope(dev, "oal_amd::window_attention_step"):
+        nbytes = lib.oal_window_attention_step_workspace_bytes(b, hq, hk, dv, window, sinks)
+        if nbytes == 0:
+            _check(1, lib, "oal_window_attention_step_workspace_bytes")
+        work = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+        out = torch.empty((b, hq, 1, dv), dtype=q.dtype, device=dev)
+        rc = lib.oal_window_attention_step(
+            _ptr(q), _ptr(k), _ptr(v), _ptr(k_cache), _ptr(v_cache), _stride_array(q, k, v, k_cache, v_cache),
+            _ptr(positions), b, hq, hk, d, dv, window, sinks, _KINDS[q.dtype], float(scale), _ptr(out), _ptr(work),
+            _stream(dev))
+        _check(rc, lib, "oal_window_attention_step")
     return out

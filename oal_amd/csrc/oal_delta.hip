@@ -109,7 +109,7 @@ __global__ __launch_bounds__(kThr) void k_delta_solve(DeltaArgs a, uint16_t* __r
   constexpr int NP = kPartsOf<T>;
   __shared__ Tile<NP> K;
   __shared__ Gates gate;
-  __shared__ float L[64 * kRow32], S[64 * kRow32], Y[32 * kRow32];
+  __shared__ alignas(16) float L[64 * kRow32], S[64 * kRow32], Y[32 * kRow32];
   const int t = threadIdx.x, lane = t & 63, w = t >> 6, g = lane >> 4, c = lane & 15;
   const int ch = blockIdx.x % a.NC, u = blockIdx.x / a.NC, b = u / a.Hv, h = u % a.Hv;
   const int tok0 = 64 * ch, live = min(64, a.N - tok0);

@@ -33,6 +33,7 @@
 #include "oal_delta.hpp"
 #include "oal_direct.hpp"
 #include "oal_internal.hpp"
+#include "oal_window.hpp"
 
 namespace oal {
 
@@ -1576,6 +1577,129 @@ int oal_gated_delta_step(const void* q, const void* k, const void* v, const floa
                                 beta_f32 != 0 || kind == 0, scale, state, out};
   oal::launch_delta_step(kind, a, static_cast<hipStream_t>(stream), make_timer());
   return launch_status("oal_gated_delta_step launch");
+}
+
+// ---------------------------------------------------------------------------
+// Windowed attention
+// ---------------------------------------------------------------------------
+static int check_window(int batch, int q_heads, int kv_heads, int query_len, int key_len, int window, int sinks) {
+  if (batch <= 0 || q_heads <= 0 || kv_heads <= 0 || query_len <= 0)
+    return fail("batch, head counts and sequence length must be positive");
+  if (q_heads % kv_heads != 0) return fail("query head count must be divisible by KV head count");
+  if (query_len > key_len) return fail("there must be a key for every query");
+  if (window < 1 || sinks < 0) return fail("window must be positive and sinks not negative");
+  // the grids' blocks: 32 queries of a head or fewer; a thread per 4 of the keys' 64 values, twice
+  if (int64_t(batch) > (int64_t(1) << 24) / q_heads ||
+      !grid_fits(int64_t(batch) * q_heads * ((int64_t(query_len) + 15) / 16)) ||
+      !grid_fits(int64_t(batch) * q_heads * ((int64_t(key_len) + 7) / 8)) || key_len > (1 << 30))
+    return fail("batch, heads and sequence length are too large for one launch");
+  return 0;
+}
+
+static int window_args(oal::WindowArgs* a, const char* what, const void* q, const void* k, const void* v,
+                       const int64_t* strides, int batch, int q_heads, int kv_heads, int query_len, int key_len,
+                       int window, int sinks, int dtype, float scale) {
+  if (check_window(batch, q_heads, kv_heads, query_len, key_len, window, sinks)) return 1;
+  if (dtype != OAL_DTYPE_F32 && dtype != OAL_DTYPE_BF16) return fail("dtype must be OAL_DTYPE_F32 or OAL_DTYPE_BF16");
+  if (!q || !k || !v || !strides) return fail(std::string(what) + ": null pointer argument");
+  *a = {strided(q, strides), strided(k, strides + 3), strided(v, strides + 6), batch, q_heads, kv_heads, query_len,
+        key_len, window, sinks, scale};
+  const int bytes = dtype == OAL_DTYPE_F32 ? 4 : 2;
+  if (!rows_aligned(a->q, bytes) || !rows_aligned(a->k, bytes) || !rows_aligned(a->v, bytes))
+    return fail(std::string(what) + ": rows must be 16-byte aligned");
+  return 0;
+}
+
+int oal_window_attention_forward(const void* q, const void* k, const void* v, const int64_t* strides, int batch,
+                                 int q_heads, int kv_heads, int query_len, int key_len, int window, int sinks,
+                                 int dtype, float scale, void* out, float* lse, void* stream) {
+  Range range("oal_window_attention_forward");
+  oal::WindowArgs a;
+  if (window_args(&a, "oal_window_attention_forward", q, k, v, strides, batch, q_heads, kv_heads, query_len, key_len,
+                  window, sinks, dtype, scale))
+    return 1;
+  if (!out || !lse) return fail("oal_window_attention_forward: null pointer argument");
+  if (!aligned16(out)) return fail("oal_window_attention_forward: tensor pointers must be 16-byte aligned");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (dtype == OAL_DTYPE_F32)
+    oal::launch_window_forward<float>(a, out, lse, st, make_timer());
+  else
+    oal::launch_window_forward<uint16_t>(a, out, lse, st, make_timer());
+  return launch_status("oal_window_attention_forward launch");
+}
+
+size_t oal_window_attention_workspace_bytes(int batch, int q_heads, int kv_heads, int query_len, int key_len,
+                                            int window, int sinks, int dtype) {
+  if (check_window(batch, q_heads, kv_heads, query_len, key_len, window, sinks)) return 0;
+  oal::WindowArgs a{};
+  a.B = batch, a.Hq = q_heads, a.Hk = kv_heads, a.Nq = query_len, a.Nk = key_len;
+  return oal::window_work_view(nullptr, a, oal::window_plan(batch, q_heads, kv_heads, query_len, key_len, window, sinks,
+                                                            dtype == OAL_DTYPE_F32)).bytes;
+}
+
+int oal_window_attention_backward(const void* q, const void* k, const void* v, const int64_t* strides, int batch,
+                                  int q_heads, int kv_heads, int query_len, int key_len, int window, int sinks,
+                                  int dtype, float scale, const void* out, const float* lse, const void* dout,
+                                  void* dq, void* dk, void* dv, void* workspace, void* stream) {
+  Range range("oal_window_attention_backward");
+  oal::WindowArgs a;
+  if (window_args(&a, "oal_window_attention_backward", q, k, v, strides, batch, q_heads, kv_heads, query_len, key_len,
+                  window, sinks, dtype, scale))
+    return 1;
+  if (!lse) return fail("oal_window_attention_backward: null pointer argument");
+  const void* ptrs[] = {out, dout, dq, dk, dv, workspace};
+  for (const void* p : ptrs) {
+    if (!p) return fail("oal_window_attention_backward: null pointer argument");
+    if (!aligned16(p)) return fail("oal_window_attention_backward: tensor pointers must be 16-byte aligned");
+  }
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (dtype == OAL_DTYPE_F32)
+    oal::launch_window_backward<float>(a, out, lse, dout, dq, dk, dv, workspace, st, make_timer());
+  else
+    oal::launch_window_backward<uint16_t>(a, out, lse, dout, dq, dk, dv, workspace, st, make_timer());
+  return launch_status("oal_window_attention_backward launch");
+}
+
+static int check_window_step(int batch, int q_heads, int kv_heads, int value_dim, int window, int sinks) {
+  if (batch <= 0 || q_heads <= 0 || kv_heads <= 0) return fail("batch and head counts must be positive");
+  if (q_heads % kv_heads != 0) return fail("query head count must be divisible by KV head count");
+  if (window < 1 || sinks < 0) return fail("window must be positive and sinks not negative");
+  if (int64_t(sinks) + window > (1 << 30)) return fail("the cache has too many slots");
+  if (value_dim < 8 || value_dim > 64 || value_dim % 8)
+    return fail("oal_window_attention_step: dimensions must be multiples of 8 up to 64");
+  // at most 512 blocks more than there are head groups
+  if (int64_t(batch) > (int64_t(1) << 23) / q_heads) return fail("batch and heads are too large for one launch");
+  return 0;
+}
+
+size_t oal_window_attention_step_workspace_bytes(int batch, int q_heads, int kv_heads, int value_dim, int window,
+                                                 int sinks) {
+  if (check_window_step(batch, q_heads, kv_heads, value_dim, window, sinks)) return 0;
+  int splits, span;
+  oal::window_step_plan(batch, q_heads, kv_heads, int64_t(sinks) + window, &splits, &span);
+  return splits > 1 ? sizeof(float) * splits * batch * q_heads * (value_dim + 2) : 256;
+}
+
+int oal_window_attention_step(const void* q, const void* k, const void* v, void* k_cache, void* v_cache,
+                              const int64_t* strides, const int64_t* position, int batch, int q_heads, int kv_heads,
+                              int key_dim, int value_dim, int window, int sinks, int kind, float scale, void* out,
+                              void* workspace, void* stream) {
+  Range range("oal_window_attention_step");
+  if (check_window_step(batch, q_heads, kv_heads, value_dim, window, sinks)) return 1;
+  if (key_dim < 8 || key_dim > 64 || key_dim % 8)
+    return fail("oal_window_attention_step: dimensions must be multiples of 8 up to 64");
+  if (kind < 0 || kind > 2) return fail("oal_window_attention_step: unknown type");
+  if (!q || !k || !v || !k_cache || !v_cache || !strides || !position || !out || !workspace)
+    return fail("oal_window_attention_step: null pointer argument");
+  oal::WindowStepArgs a = {strided(q, strides), strided(k, strides + 3), strided(v, strides + 6),
+                           strided(k_cache, strides + 9), strided(v_cache, strides + 12), position, batch, q_heads,
+                           kv_heads, key_dim, value_dim, window, sinks, 1, 0, scale, out, static_cast<float*>(workspace)};
+  const int bytes = kind == 0 ? 4 : 2;
+  for (const oal::Strided* s : {&a.q, &a.k, &a.v, &a.kc, &a.vc})
+    if (!rows_aligned(*s, bytes)) return fail("oal_window_attention_step: rows must be 16-byte aligned");
+  oal::window_step_plan(batch, q_heads, kv_heads, int64_t(sinks) + window, &a.splits, &a.span);
+  oal::launch_window_step(kind, a, static_cast<hipStream_t>(stream), make_timer());
+  return launch_status("oal_window_attention_step launch");
 }
 
 }  // extern "C"

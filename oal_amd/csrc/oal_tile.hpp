@@ -68,7 +68,7 @@ __device__ __forceinline__ f32x4 mma(const Frag<NA>& a, const Frag<NB>& b, f32x4
 
 // LDS tile: NP parts of 64 rows of kTileRow bf16.
 template <int NP>
-struct Tile {
+struct alignas(16) Tile {
   __bf16 x[NP * kTileElems];
 };
 
