@@ -275,13 +275,13 @@ int oal_check_outputs(int wide, int out_kind, const void* num, const void* den, 
  * of q, k, v, g, beta, three each (batch, head, token), in elements; rows of q, k
  * and v are contiguous and 16-byte aligned. state (may be NULL: zero) and
  * final_state [B][Hv][64][64] f32, rows the key's dimensions. saved
- * (oal_gated_delta_saved_bytes) is what the backward reads.
+ * (oal_gated_delta_saved_bytes) is the call's room and, with keep, what the backward reads.
  */
-size_t oal_gated_delta_saved_bytes(int batch, int v_heads, int seq_len);
+size_t oal_gated_delta_saved_bytes(int batch, int v_heads, int seq_len, int keep);
 int oal_gated_delta_forward(const void* q, const void* k, const void* v, const float* g, const void* beta,
                             const int64_t* strides, int beta_f32, int batch, int q_heads, int k_heads, int v_heads,
                             int seq_len, int dtype, float scale, const float* state, void* out, float* final_state,
-                            void* saved, void* stream);
+                            void* saved, int keep, void* stream);
 
 /*
  * Its VJP: dout [B][H][N][64] (dtype) and dfinal [B][Hv][64][64] f32 (may be NULL)

@@ -78,9 +78,9 @@ _SIGNATURES = {
     "oal_rotary_heads": ([_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp], _i),
     "oal_check_labels": ([_vp, _i, _i, _i, _i, _i, _vp, _vp, _vp], _i),
     "oal_check_outputs": ([_i, _i, _vp, _vp, _vp, _sz, _i, _i, _i, _vp, _vp], _i),
-    "oal_gated_delta_saved_bytes": ([_i] * 3, _sz),
+    "oal_gated_delta_saved_bytes": ([_i] * 4, _sz),
     "oal_gated_delta_workspace_bytes": ([_i] * 5, _sz),
-    "oal_gated_delta_forward": ([_vp] * 6 + [_i] * 7 + [_f] + [_vp] * 5, _i),
+    "oal_gated_delta_forward": ([_vp] * 6 + [_i] * 7 + [_f] + [_vp] * 4 + [_i, _vp], _i),
     "oal_gated_delta_backward": ([_vp] * 6 + [_i] * 7 + [_f] + [_vp] * 11, _i),
     "oal_gated_delta_step": ([_vp] * 6 + [_i] * 9 + [_f] + [_vp] * 3, _i),
     "oal_window_attention_forward": ([_vp] * 4 + [_i] * 8 + [_f] + [_vp] * 3, _i),
@@ -735,14 +735,15 @@ def _stride_array(*tensors: torch.Tensor):
     return (ctypes.c_int64 * len(values))(*values)
 
 
-def delta_forward(q, k, v, g, beta, state, *, scale: float):
+def delta_forward(q, k, v, g, beta, state, *, scale: float, keep: bool):
     """q, k, v [B, heads, N, 64] float32 or bfloat16 with aligned rows, g float32, beta
-    float32 or q's type, state float32 [B, Hv, 64, 64] or None. Returns (out, final_state, saved)."""
+    float32 or q's type, state float32 [B, Hv, 64, 64] or None. Returns (out,
+    final_state, saved); saved serves the backward if kept."""
     lib = load_library()
     b, hq, n, _ = q.shape
     hk, hv, dev = k.shape[1], v.shape[1], q.device
     with _scope(dev, "oal_amd::gated_delta_forward"):
-        nbytes = lib.oal_gated_delta_saved_bytes(b, hv, n)
+        nbytes = lib.oal_gated_delta_saved_bytes(b, hv, n, int(keep))
         if nbytes == 0:
             _check(1, lib, "oal_gated_delta_saved_bytes")
         out = torch.empty((b, max(hq, hv), n, HEAD_DIM), dtype=q.dtype, device=dev)
@@ -751,7 +752,7 @@ def delta_forward(q, k, v, g, beta, state, *, scale: float):
         rc = lib.oal_gated_delta_forward(
             _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(beta), _stride_array(q, k, v, g, beta),
             int(beta.dtype == torch.float32), b, hq, hk, hv, n, _dtype_code(q.dtype), float(scale), _ptr(state),
-            _ptr(out), _ptr(final), _ptr(saved), _stream(dev))
+            _ptr(out), _ptr(final), _ptr(saved), int(keep), _stream(dev))
         _check(rc, lib, "oal_gated_delta_forward")
     return out, final, saved
 

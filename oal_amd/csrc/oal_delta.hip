@@ -8,15 +8,19 @@
 //   A_ij = exp(G_i - G_j) k_i.k_j (j < i),  T = (I + A diag(beta))^-1
 //   Z = T (V - e^G K S),  U = beta Z,  S' = e^(G_63) S + K^T (e^(G_63 - G) U)
 //   O = scale (e^G Q S + (exp(G_i - G_j) q_i.k_j)_(j <= i) U)
-// T and O are formed chunk by chunk at once, S and Z in a walk over the chunks.
-// The walk's products are exact to fp32 whatever the tensors' type (oal_tile.hpp):
-// a state is a sum over all tokens before it and is handed on in fp32.
+// A chunk maps the state before it to M S + D, with M and D of its own tokens alone:
+// T, M and D are formed chunk by chunk at once, then S in a walk of one product per
+// chunk, then Z and O chunk by chunk at once. What makes the state is exact to fp32
+// whatever the tensors' type (oal_tile.hpp): a state is a sum over all tokens before it and is handed on in fp32.
 //
 // Decays enter as differences of sums, held in two floats (48 bits): a token that
 // forgets nearly everything leaves large sums whose differences still matter.
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+
+#include <algorithm>
+#include <type_traits>
 
 #include "oal_common.hpp"
 #include "oal_delta.hpp"
@@ -30,8 +34,6 @@ constexpr int kThr = 256;
 constexpr int kTile2 = 64 * 64;
 // Smallest log-decay: exp of it is zero, and 64 of them leave the sums' differences exact.
 constexpr double kLeast = -1e4;
-
-typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
 struct Gates {
   float hi[64], lo[64], beta[64];  // log2 of the decay up to and with token i, in two parts
@@ -101,20 +103,43 @@ __device__ __forceinline__ f32x4 mma_f32(const float* a, const float* b, f32x4 c
 
 }  // namespace
 
-// T of one chunk. Diagonal blocks of 16 rows by substitution (a lane per
-// column), then twice the rule for two blocks, [L11 0; L21 L22]^-1 =
-// [T11 0; -T22 L21 T11, T22], on the fp32 matrix cores.
+// Two 64 x 64 products' results in C layout go to LDS rows as bf16 parts.
+template <int NP>
+__device__ __forceinline__ void put_parts(Tile<NP>& s, int row, int col, float x) {
+#pragma unroll
+  for (int e = 0; e < NP; ++e) {
+    const __bf16 y = static_cast<__bf16>(x);
+    s.x[e * kTileElems + row * kTileRow + col] = y;
+    x -= static_cast<float>(y);
+  }
+}
+
+// One chunk by itself: T, and the chunk's map of the state S' = M S + D,
+//   M = e^(G_63) - (e^(G_63 - G) beta K)^T T e^G K,  D = (e^(G_63 - G) beta K)^T T V.
+// T's diagonal blocks of 16 rows by substitution (a lane per column), then twice
+// the rule for two blocks, [L11 0; L21 L22]^-1 = [T11 0; -T22 L21 T11, T22], on the
+// fp32 matrix cores. In the products a wave owns 16 columns of M and of D.
 template <typename T>
-__global__ __launch_bounds__(kThr) void k_delta_solve(DeltaArgs a, uint16_t* __restrict__ out) {
+__global__ __launch_bounds__(kThr) void k_delta_chunk(DeltaArgs a, float* __restrict__ Tout, float* __restrict__ Mout,
+                                                      float* __restrict__ Dout) {
   constexpr int NP = kPartsOf<T>;
-  __shared__ Tile<NP> K;
+  __shared__ Tile<NP> K, V;
   __shared__ Gates gate;
-  __shared__ alignas(16) float L[64 * kRow32], S[64 * kRow32], Y[32 * kRow32];
+  __shared__ alignas(16) float S[64 * kRow32];
+  struct Solve {
+    float L[64 * kRow32], Y[32 * kRow32];
+  };
+  __shared__ alignas(16) char room[sizeof(Tile<3>) > sizeof(Solve) ? sizeof(Tile<3>) : sizeof(Solve)];
+  float* const L = reinterpret_cast<Solve*>(room)->L;
+  float* const Y = reinterpret_cast<Solve*>(room)->Y;
+  Tile<3>& P = *reinterpret_cast<Tile<3>*>(room);
   const int t = threadIdx.x, lane = t & 63, w = t >> 6, g = lane >> 4, c = lane & 15;
   const int ch = blockIdx.x % a.NC, u = blockIdx.x / a.NC, b = u / a.Hv, h = u % a.Hv;
   const int tok0 = 64 * ch, live = min(64, a.N - tok0);
-  load_gates<T>(gate, a, b, h, tok0, t);
+  const size_t at = ((size_t)u * a.NC + ch) * kTile2;
   load_tile<64, kThr>(K, rows_of<T>(a.k, b, h / (a.Hv / a.Hk), tok0), a.k.n, live, t);
+  load_tile<64, kThr>(V, rows_of<T>(a.v, b, h, tok0), a.v.n, live, t);
+  load_gates<T>(gate, a, b, h, tok0, t);
   __syncthreads();
   for (int n = 0; n < 4; ++n) {
     f32x4 kk = {};
@@ -156,107 +181,171 @@ __global__ __launch_bounds__(kThr) void k_delta_solve(DeltaArgs a, uint16_t* __r
     for (int r = 0; r < 4; ++r) S[(o + 16 + 4 * g + r) * kRow32 + o + c] = -y[r];
   }
   __syncthreads();
-  const int m = 16 * (w >> 1), n = 16 * (w & 1);
-  y = mma_f32<32>(L + (32 + m) * kRow32, S + n, f32x4{}, lane);
+  const int m2 = 16 * (w >> 1), n2 = 16 * (w & 1);
+  y = mma_f32<32>(L + (32 + m2) * kRow32, S + n2, f32x4{}, lane);
 #pragma unroll
-  for (int r = 0; r < 4; ++r) Y[(m + 4 * g + r) * kRow32 + n + c] = y[r];
+  for (int r = 0; r < 4; ++r) Y[(m2 + 4 * g + r) * kRow32 + n2 + c] = y[r];
   __syncthreads();
-  y = mma_f32<32>(S + (32 + m) * kRow32 + 32, Y + n, f32x4{}, lane);
+  y = mma_f32<32>(S + (32 + m2) * kRow32 + 32, Y + n2, f32x4{}, lane);
 #pragma unroll
-  for (int r = 0; r < 4; ++r) S[(32 + m + 4 * g + r) * kRow32 + n + c] = -y[r];
+  for (int r = 0; r < 4; ++r) S[(32 + m2 + 4 * g + r) * kRow32 + n2 + c] = -y[r];
   __syncthreads();
-  uint16_t* dst = out + ((size_t)u * a.NC + ch) * 3 * kTile2;
+  // twice: T's columns scaled by e^G times K, T times V; then what the chunk writes of it
 #pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    const int i = t + kThr * x;
-    float v[8];
-    load_row8(v, S + (i >> 3) * kRow32 + 8 * (i & 7));
-    const Frag<3> f = split<3>(v);
+  for (int side = 0; side < 2; ++side) {
 #pragma unroll
-    for (int e = 0; e < 3; ++e) *reinterpret_cast<bf16x8*>(dst + e * kTile2 + 8 * i) = f.p[e];
+    for (int x = 0; x < 2; ++x) {
+      const int i = t + kThr * x, r = i >> 3, col = 8 * (i & 7);
+      float v[8];
+      load_row8(v, S + r * kRow32 + col);
+      if (side == 0) {
+        float4* dst = reinterpret_cast<float4*>(Tout + at + 8 * i);
+        dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+        dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= gate.since(col + e);
+      }
+      const Frag<3> f = split<3>(v);
+#pragma unroll
+      for (int e = 0; e < 3; ++e) *reinterpret_cast<bf16x8*>(P.x + e * kTileElems + r * kTileRow + col) = f.p[e];
+    }
+    __syncthreads();
+    const Tile<NP>& B = side == 0 ? K : V;
+    const Frag<NP> b0 = col_frag(B, 16 * w, 0, lane), b1 = col_frag(B, 16 * w, 1, lane);
+    f32x4 z[4];
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+      z[m] = mma(row_frag(P, 16 * m, 0, lane), b0, f32x4{});
+      if (m >= 2) z[m] = mma(row_frag(P, 16 * m, 1, lane), b1, z[m]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = 16 * m + 4 * g + i;
+        const float x = gate.beta[row] * gate.between(63, row);
+        z[m][i] *= side == 0 ? -x : x;
+      }
+    }
+    const Frag<3> z0 = acc_frag<3>(z[0], z[1]), z1 = acc_frag<3>(z[2], z[3]);
+    const float last = gate.since(63);
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+      f32x4 x = mma(col_frag_perm(K, 16 * m, 0, lane), z0, f32x4{});
+      x = mma(col_frag_perm(K, 16 * m, 1, lane), z1, x);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = 16 * m + 4 * g + i, col = 16 * w + c;
+        (side == 0 ? Mout : Dout)[at + row * 64 + col] = side == 0 && row == col ? x[i] + last : x[i];
+      }
+    }
+    __syncthreads();
   }
 }
 
-// The walk over the chunks: a block per unit, a wave per 16 columns of the state,
-// whose products stay in its registers.
-template <typename T>
-__global__ __launch_bounds__(kThr) void k_delta_scan(DeltaArgs a, const uint16_t* __restrict__ Tm,
-                                                     const float* __restrict__ state, float* __restrict__ Sout,
-                                                     float* __restrict__ Zout, float* __restrict__ final_state) {
-  constexpr int NP = kPartsOf<T>;
-  __shared__ Tile<NP> K;
-  __shared__ Tile<3> M;
-  __shared__ Gates gate;
-  const int t = threadIdx.x, lane = t & 63, w = t >> 6, g = lane >> 4, col = 16 * w + (lane & 15);
-  const int u = blockIdx.x, b = u / a.Hv, h = u % a.Hv;
-  f32x4 S[4];
+// A walk over maps of 64 x 64 states, S -> M S + D, or back through them, S -> M^T S + D
+// (M's transpose where TR): a block per chain and 16 columns, a wave per 16 rows, who
+// hand each other their rows in three parts through LDS once per map. What a map
+// needs of memory is loaded kAhead maps before.
+struct Walk {
+  const float* M;     // [units][maps][64][64]
+  const float* D;
+  const float* init;  // state the walk starts from, by unit (segs == 1) or segment (null: zero)
+  float* each;        // [units][maps][64][64]: the state before each map (null: not wanted)
+  float* end;         // by unit or segment: the state after the last (null: not wanted)
+  float* mend;        // with 8 column groups: the product of the segment's maps
+  int maps, segs, len, units;
+  bool back;
+};
+
+constexpr int kAhead = 4;
+
+template <bool TR, int COLS>
+__global__ __launch_bounds__(kThr) void k_delta_walk(Walk a) {
+  struct Rows {
+    bf16x4 x[3][4][64];
+  };
+  __shared__ Rows rows[2];
+  const int t = threadIdx.x, lane = t & 63, w = t >> 6, g = lane >> 4, c = lane & 15;
+  // a chain's column groups on one XCD (blocks go round the 8 of them): they share its maps
+  const int chains = a.units * a.segs, id = blockIdx.x, whole = chains / 8 * 8 * COLS;
+  const int chain = id < whole ? id % 8 + id / (8 * COLS) * 8 : chains / 8 * 8 + (id - whole) / COLS;
+  const int group = id < whole ? id / 8 % COLS : (id - whole) % COLS;
+  const int u = chain / a.segs, seg = chain % a.segs;
+  const bool unit = group >= 4;  // columns of the maps' product: from the unit matrix, nothing added
+  const int first = seg * a.len, count = min(a.len, a.maps - first);
+  const int col = 16 * (group & 3) + c, row = 16 * w + 4 * g;
+  const size_t base = ((size_t)u * a.maps + first) * kTile2;
+  const size_t slot = (size_t)chain * kTile2;
+  float m[kAhead][16], d[kAhead][4];
+  auto fetch = [&](int n, float (&mm)[16], float (&dd)[4]) {
+    n = min(n, count - 1);
+    const size_t at = base + (size_t)(a.back ? count - 1 - n : n) * kTile2;
 #pragma unroll
-  for (int m = 0; m < 4; ++m)
+    for (int q = 0; q < 4; ++q) {
+      const int k = 16 * q + 4 * g;  // perm order: tiles 2 t, 2 t + 1
+      if constexpr (TR) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) S[m][i] = state ? state[(size_t)u * kTile2 + (16 * m + 4 * g + i) * 64 + col] : 0.f;
-  for (int ch = 0; ch < a.NC; ++ch) {
-    const int tok0 = 64 * ch, live = min(64, a.N - tok0);
-    const size_t at = ((size_t)u * a.NC + ch) * kTile2;
-    __syncthreads();
-    load_gates<T>(gate, a, b, h, tok0, t);
-    load_tile<64, kThr>(K, rows_of<T>(a.k, b, h / (a.Hv / a.Hk), tok0), a.k.n, live, t);
-#pragma unroll
-    for (int x = 0; x < 6; ++x) {
-      const int i = t + kThr * x;
-      *reinterpret_cast<uint4*>(M.x + (i >> 9) * kTileElems + ((i & 511) >> 3) * kTileRow + 8 * (i & 7)) =
-          reinterpret_cast<const uint4*>(Tm + 3 * at)[i];
+        for (int e = 0; e < 4; ++e) mm[4 * q + e] = a.M[at + (k + e) * 64 + 16 * w + c];
+      } else {
+        const float4 v = *reinterpret_cast<const float4*>(a.M + at + (16 * w + c) * 64 + k);
+        mm[4 * q] = v.x, mm[4 * q + 1] = v.y, mm[4 * q + 2] = v.z, mm[4 * q + 3] = v.w;
+      }
+      dd[q] = unit ? 0.f : a.D[at + (row + q) * 64 + col];
     }
-    const T* v = rows_of<T>(a.v, b, h, tok0);
-    f32x4 r[4];
+  };
 #pragma unroll
-    for (int m = 0; m < 4; ++m)
+  for (int n = 0; n < kAhead; ++n) fetch(n, m[n], d[n]);
+  f32x4 S;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = 16 * m + 4 * g + i;
-        r[m][i] = row < live ? to_f(v[row * a.v.n + col]) : 0.f;
-        Sout[at + row * 64 + col] = S[m][i];
+  for (int i = 0; i < 4; ++i)
+    S[i] = unit ? (row + i == col ? 1.f : 0.f) : a.init ? a.init[slot + (row + i) * 64 + col] : 0.f;
+  for (int n0 = 0; n0 < count; n0 += kAhead) {
+#pragma unroll
+    for (int x = 0; x < kAhead; ++x) {
+      const int n = n0 + x;
+      if (n >= count) break;
+      Rows& r = rows[x & 1];
+      float v[4] = {S[0], S[1], S[2], S[3]};
+#pragma unroll
+      for (int p = 0; p < 3; ++p) {
+        const bf16x4 y = __builtin_bit_cast(bf16x4, pack4(v));
+        r.x[p][w][lane] = y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] -= static_cast<float>(y[e]);
       }
-    __syncthreads();
-    {
-      const Frag<3> s0 = acc_frag<3>(S[0], S[1]), s1 = acc_frag<3>(S[2], S[3]);
+      if (a.each) {
+        const size_t at = base + (size_t)(a.back ? count - 1 - n : n) * kTile2;
 #pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        f32x4 x = mma(row_frag_perm(K, 16 * m, 0, lane), s0, f32x4{});
-        x = mma(row_frag_perm(K, 16 * m, 1, lane), s1, x);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) r[m][i] -= gate.since(16 * m + 4 * g + i) * x[i];
+        for (int i = 0; i < 4; ++i) a.each[at + (row + i) * 64 + col] = S[i];
       }
-    }
-    f32x4 z[4];
-    {
-      const Frag<3> r0 = acc_frag<3>(r[0], r[1]), r1 = acc_frag<3>(r[2], r[3]);
+      Frag<3> mf[2];
 #pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        z[m] = mma(row_frag_perm(M, 16 * m, 0, lane), r0, f32x4{});
-        if (m >= 2) z[m] = mma(row_frag_perm(M, 16 * m, 1, lane), r1, z[m]);
+      for (int s = 0; s < 2; ++s) {
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = m[x][8 * s + e];
+        mf[s] = split<3>(y);
       }
-    }
-    const float last = gate.since(63);
+      S = f32x4{d[x][0], d[x][1], d[x][2], d[x][3]};
+      fetch(n + kAhead, m[x], d[x]);
+      lds_sync();
+      f32x4 half = {};
 #pragma unroll
-    for (int m = 0; m < 4; ++m)
+      for (int s = 0; s < 2; ++s) {
+        Frag<3> f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = 16 * m + 4 * g + i;
-        Zout[at + row * 64 + col] = z[m][i];
-        z[m][i] *= gate.beta[row] * gate.between(63, row);
-        S[m][i] *= last;
+        for (int p = 0; p < 3; ++p)
+          f.p[p] = __builtin_shufflevector(r.x[p][2 * s][lane], r.x[p][2 * s + 1][lane], 0, 1, 2, 3, 4, 5, 6, 7);
+        if (s == 0)
+          S = mma(mf[s], f, S);
+        else
+          half = mma(mf[s], f, half);
       }
-    const Frag<3> u0 = acc_frag<3>(z[0], z[1]), u1 = acc_frag<3>(z[2], z[3]);
-#pragma unroll
-    for (int m = 0; m < 4; ++m) {
-      S[m] = mma(col_frag_perm(K, 16 * m, 0, lane), u0, S[m]);
-      S[m] = mma(col_frag_perm(K, 16 * m, 1, lane), u1, S[m]);
+      S += half;
     }
   }
+  float* end = unit ? a.mend : a.end;
+  if (!end) return;
 #pragma unroll
-  for (int m = 0; m < 4; ++m)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) final_state[(size_t)u * kTile2 + (16 * m + 4 * g + i) * 64 + col] = S[m][i];
+  for (int i = 0; i < 4; ++i) end[slot + (row + i) * 64 + col] = S[i];
 }
 
 // Four consecutive values of a row.
@@ -272,213 +361,206 @@ __device__ __forceinline__ f32x4 load4(const uint16_t* p) {
                __uint_as_float(v.y & 0xffff0000u)};
 }
 
-// The outputs of one chunk and output head, transposed: a wave's 16 queries are
-// the columns, so the scores are an operand of the product with U as they are. The
-// scores, U and S enter in the output's own precision.
-template <typename T>
-__global__ __launch_bounds__(kThr) void k_delta_out(DeltaArgs a, const float* __restrict__ Sin,
-                                                    const float* __restrict__ Zin, T* __restrict__ out) {
-  constexpr int NP = kPartsOf<T>;
-  __shared__ Tile<NP> K, U, S;
+
+__device__ __forceinline__ void put(float* p, float x) { *p = x; }
+__device__ __forceinline__ void put(uint16_t* p, float x) { *p = from_f<uint16_t>(x); }
+__device__ __forceinline__ void put(_Float16* p, float x) { *p = static_cast<_Float16>(x); }
+
+// The outputs of one chunk for `each` output heads of a state head. First Z = T (V -
+// e^G K S), a wave per 16 columns, to LDS as U = beta Z; then per output head, transposed: a
+// wave's 16 queries are the columns, so the scores are an operand of the product
+// with U as they are. What goes on to the backward (KEEP) is exact to fp32; the outputs take
+// two parts per value for 16-bit tensors, twice their precision: one rounding is the output's own.
+template <typename T, bool KEEP>
+__global__ __launch_bounds__(kThr) void k_delta_out(DeltaArgs a, int each, const float* __restrict__ Tin,
+                                                    const float* __restrict__ Sin, float* __restrict__ Zout,
+                                                    T* __restrict__ out) {
+  constexpr int NP = kPartsOf<T>, NZ = KEEP || NP == 3 ? 3 : 2, NO = NP == 3 ? 3 : 2;
+  __shared__ Tile<NP> K;
+  __shared__ Tile<NZ> S, U;
   __shared__ Gates gate;
   const int t = threadIdx.x, lane = t & 63, w = t >> 6, g = lane >> 4, c = lane & 15;
-  const int ch = blockIdx.x % a.NC, b = blockIdx.x / a.NC / a.H, o = blockIdx.x / a.NC % a.H;
-  const int h = o / (a.H / a.Hv), u = b * a.Hv + h;
-  const int tok0 = 64 * ch, live = min(64, a.N - tok0), qrow = 16 * w + c;
+  const int rep = a.H / a.Hv, parts = (rep + each - 1) / each;
+  const int part = blockIdx.x % parts, ch = blockIdx.x / parts % a.NC, u = blockIdx.x / parts / a.NC;
+  const int b = u / a.Hv, h = u % a.Hv;
+  const int tok0 = 64 * ch, live = min(64, a.N - tok0), own = 16 * w + c;
   const size_t at = ((size_t)u * a.NC + ch) * kTile2;
-  load_gates<T>(gate, a, b, h, tok0, t);
   load_tile<64, kThr>(K, rows_of<T>(a.k, b, h / (a.Hv / a.Hk), tok0), a.k.n, live, t);
-  load_f32(U, Zin + at, t);
   load_f32(S, Sin + at, t);
-  const T* q = rows_of<T>(a.q, b, o / (a.H / a.Hq), tok0) + qrow * a.q.n;
-  Frag<NP> qf[2];
+  load_f32(U, Tin + at, t);
+  const T* v = rows_of<T>(a.v, b, h, tok0) + own;
+  f32x4 z[4];
 #pragma unroll
-  for (int s = 0; s < 2; ++s) qf[s] = global_frag<NP>(q + 32 * s + 8 * g, qrow < live);
-  __syncthreads();
-  f32x4 acc[4] = {}, p[4] = {};
-  const float since = a.scale * gate.since(qrow);
-#pragma unroll
-  for (int m = 0; m < 4; ++m) {
-#pragma unroll
-    for (int s = 0; s < 2; ++s) acc[m] = mma(col_frag(S, 16 * m, s, lane), qf[s], acc[m]);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[m][i] *= since;
-    if (m > w) continue;
-#pragma unroll
-    for (int s = 0; s < 2; ++s) p[m] = mma(row_frag(K, 16 * m, s, lane), qf[s], p[m]);
+  for (int m = 0; m < 4; ++m)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int j = 16 * m + 4 * g + i;
-      p[m][i] = j <= qrow ? p[m][i] * a.scale * gate.between(qrow, j) * gate.beta[j] : 0.f;
+      const int row = 16 * m + 4 * g + i;
+      z[m][i] = to_f(v[min(row, live - 1) * a.v.n]);
+      z[m][i] = row < live ? z[m][i] : 0.f;
+    }
+  load_gates<T>(gate, a, b, h, tok0, t);
+  __syncthreads();
+  {
+    const Frag<NZ> s0 = col_frag(S, 16 * w, 0, lane), s1 = col_frag(S, 16 * w, 1, lane);
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+      f32x4 x = mma(row_frag(K, 16 * m, 0, lane), s0, f32x4{});
+      x = mma(row_frag(K, 16 * m, 1, lane), s1, x);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) z[m][i] -= gate.since(16 * m + 4 * g + i) * x[i];
     }
   }
-  const Frag<NP> p0 = acc_frag<NP>(p[0], p[1]), p1 = acc_frag<NP>(p[2], p[3]);
-  T* dst = out + (((size_t)b * a.H + o) * a.N + tok0 + qrow) * 64;
+  {
+    const Frag<NZ> r0 = acc_frag<NZ>(z[0], z[1]), r1 = acc_frag<NZ>(z[2], z[3]);
 #pragma unroll
-  for (int m = 0; m < 4; ++m) {
-    acc[m] = mma(col_frag_perm(U, 16 * m, 0, lane), p0, acc[m]);
-    if (w >= 2) acc[m] = mma(col_frag_perm(U, 16 * m, 1, lane), p1, acc[m]);
-    if (qrow < live) store4(dst + 16 * m + 4 * g, acc[m]);
+    for (int m = 0; m < 4; ++m) {
+      z[m] = mma(row_frag_perm(U, 16 * m, 0, lane), r0, f32x4{});
+      if (m >= 2) z[m] = mma(row_frag_perm(U, 16 * m, 1, lane), r1, z[m]);
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int m = 0; m < 4; ++m)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = 16 * m + 4 * g + i;
+      if (KEEP && part == 0) Zout[at + row * 64 + own] = z[m][i];
+      put_parts(U, row, own, gate.beta[row] * z[m][i]);
+    }
+  __syncthreads();
+  const float since = a.scale * gate.since(own);
+  for (int o = h * rep + part * each; o < min(h * rep + (part + 1) * each, (h + 1) * rep); ++o) {
+    const T* q = rows_of<T>(a.q, b, o / (a.H / a.Hq), tok0) + own * a.q.n;
+    Frag<NP> qf[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) qf[s] = global_frag<NP>(q + 32 * s + 8 * g, own < live);
+    f32x4 acc[4] = {}, p[4] = {};
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) acc[m] = mma(col_frag<NO>(S, 16 * m, s, lane), qf[s], acc[m]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[m][i] *= since;
+      if (m > w) continue;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) p[m] = mma(row_frag(K, 16 * m, s, lane), qf[s], p[m]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int j = 16 * m + 4 * g + i;
+        p[m][i] = j <= own ? p[m][i] * a.scale * gate.between(own, j) : 0.f;
+      }
+    }
+    const Frag<NO> p0 = acc_frag<NO>(p[0], p[1]), p1 = acc_frag<NO>(p[2], p[3]);
+    T* dst = out + (((size_t)b * a.H + o) * a.N + tok0 + own) * 64;
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+      acc[m] = mma(col_frag_perm<NO>(U, 16 * m, 0, lane), p0, acc[m]);
+      if (w >= 2) acc[m] = mma(col_frag_perm<NO>(U, 16 * m, 1, lane), p1, acc[m]);
+      if (own < live) store4(dst + 16 * m + 4 * g, acc[m]);
+    }
   }
 }
 
 // ---------------------------------------------------------------------------
-// Backward. Gradients of a chunk's u and of the state before it from its own outputs
-// (E, F), at once; then the walk back:
-//   dU = E + e^(G_63 - G) K dS',  dZ = T^T (beta dU),
-//   dS = F + e^(G_63) dS' - K^T (e^G dZ)
-// and from dZ = dV, dU, dS', S and Z everything else of the chunk at once.
+// Backward. Per chunk at once, from its own outputs: the gradient E of its u and, with
+// what it does to the state before through them, F; the walk back over the chunks'
+// maps, dS = M^T dS' + F; and from dS', S and Z everything else of the chunk at once:
+//   E = D^T dO,  F = scale (e^G Q)^T dO - (e^G K)^T T^T (beta E)
+//   dU = E + e^(G_63 - G) K dS',  dZ = dV = T^T (beta dU)
 // Decays' gradients are sums of terms that cancel, so all of it is exact to fp32.
 // ---------------------------------------------------------------------------
 template <typename T>
 __global__ __launch_bounds__(kThr) void k_delta_bwd_local(DeltaArgs a, const T* __restrict__ dout,
-                                                          float* __restrict__ E, float* __restrict__ F) {
+                                                          const float* __restrict__ Tin, float* __restrict__ E,
+                                                          float* __restrict__ F) {
   constexpr int NP = kPartsOf<T>;
-  __shared__ Tile<NP> Q, O;
+  __shared__ Tile<NP> K, Q, O;
+  __shared__ Tile<3> P;
   __shared__ Gates gate;
   const int t = threadIdx.x, lane = t & 63, w = t >> 6, g = lane >> 4, c = lane & 15;
   const int ch = blockIdx.x % a.NC, u = blockIdx.x / a.NC, b = u / a.Hv, h = u % a.Hv;
   const int tok0 = 64 * ch, live = min(64, a.N - tok0), own = 16 * w + c;
+  const size_t at = ((size_t)u * a.NC + ch) * kTile2;
+  load_tile<64, kThr>(K, rows_of<T>(a.k, b, h / (a.Hv / a.Hk), tok0), a.k.n, live, t);
   load_gates<T>(gate, a, b, h, tok0, t);
-  const T* k = rows_of<T>(a.k, b, h / (a.Hv / a.Hk), tok0) + own * a.k.n;
-  Frag<NP> kf[2];
-#pragma unroll
-  for (int s = 0; s < 2; ++s) kf[s] = global_frag<NP>(k + 32 * s + 8 * g, own < live);
   f32x4 e[4] = {}, f[4] = {};
   const int each = a.H / a.Hv;
   for (int o = h * each; o < (h + 1) * each; ++o) {
-    __syncthreads();
+    if (o > h * each) __syncthreads();
     load_tile<64, kThr>(Q, rows_of<T>(a.q, b, o / (a.H / a.Hq), tok0), a.q.n, live, t);
     load_tile<64, kThr>(O, dout + (((size_t)b * a.H + o) * a.N + tok0) * 64, (int64_t)64, live, t);
     __syncthreads();
-    f32x4 p[4] = {};
+    // the scores, queries by keys = own: to LDS with the queries along a row
 #pragma unroll
     for (int m = 0; m < 4; ++m) {
-      if (m < w) continue;
+      f32x4 p = {};
+      if (m >= w)
 #pragma unroll
-      for (int s = 0; s < 2; ++s) p[m] = mma(row_frag(Q, 16 * m, s, lane), kf[s], p[m]);
+        for (int s = 0; s < 2; ++s) p = mma(row_frag(Q, 16 * m, s, lane), row_frag(K, 16 * w, s, lane), p);
+      float v[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int row = 16 * m + 4 * g + i;
-        p[m][i] = own <= row ? p[m][i] * a.scale * gate.between(row, own) : 0.f;
+        v[i] = own <= row ? p[i] * a.scale * gate.between(row, own) : 0.f;
+      }
+#pragma unroll
+      for (int x = 0; x < 3; ++x) {
+        const bf16x4 y = __builtin_bit_cast(bf16x4, pack4(v));
+        *reinterpret_cast<bf16x4*>(P.x + x * kTileElems + own * kTileRow + 16 * m + 4 * g) = y;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] -= static_cast<float>(y[i]);
       }
     }
-    const Frag<3> p0 = acc_frag<3>(p[0], p[1]), p1 = acc_frag<3>(p[2], p[3]);
-    Frag<3> of[2];
+    Frag<NP> of[2];
+    Frag<3> og[2];
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      const Frag<NP> x = col_frag(O, 16 * w, s, lane);
+      of[s] = col_frag(O, 16 * w, s, lane);
       float v[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        v[j] = static_cast<float>(x.p[0][j]);
-        if constexpr (NP == 3) v[j] = (v[j] + static_cast<float>(x.p[1][j])) + static_cast<float>(x.p[2][j]);
+        v[j] = static_cast<float>(of[s].p[0][j]);
+        if constexpr (NP == 3) v[j] = (v[j] + static_cast<float>(of[s].p[1][j])) + static_cast<float>(of[s].p[2][j]);
         v[j] *= a.scale * gate.since(32 * s + 8 * g + j);
       }
-      of[s] = split<3>(v);
+      og[s] = split<3>(v);
     }
+    __syncthreads();
 #pragma unroll
     for (int m = 0; m < 4; ++m) {
-      if (w < 2) e[m] = mma(col_frag_perm(O, 16 * m, 0, lane), p0, e[m]);
-      e[m] = mma(col_frag_perm(O, 16 * m, 1, lane), p1, e[m]);
+      if (m < 2) e[m] = mma(row_frag(P, 16 * m, 0, lane), of[0], e[m]);
+      e[m] = mma(row_frag(P, 16 * m, 1, lane), of[1], e[m]);
 #pragma unroll
-      for (int s = 0; s < 2; ++s) f[m] = mma(col_frag(Q, 16 * m, s, lane), of[s], f[m]);
+      for (int s = 0; s < 2; ++s) f[m] = mma(col_frag(Q, 16 * m, s, lane), og[s], f[m]);
     }
   }
-  const size_t at = ((size_t)u * a.NC + ch) * kTile2;
-#pragma unroll
-  for (int m = 0; m < 4; ++m) {
-    store4(E + at + own * 64 + 16 * m + 4 * g, e[m]);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) F[at + (16 * m + 4 * g + i) * 64 + 16 * w + c] = f[m][i];
-  }
-}
-
-template <typename T>
-__global__ __launch_bounds__(kThr) void k_delta_bwd_scan(DeltaArgs a, const uint16_t* __restrict__ Tm,
-                                                         const float* __restrict__ dfinal, float* __restrict__ E,
-                                                         const float* __restrict__ F, float* __restrict__ dSout,
-                                                         float* __restrict__ dZout, float* __restrict__ dstate) {
-  constexpr int NP = kPartsOf<T>;
-  __shared__ Tile<NP> K;
-  __shared__ Tile<3> M;
-  __shared__ Gates gate;
-  const int t = threadIdx.x, lane = t & 63, w = t >> 6, g = lane >> 4, col = 16 * w + (lane & 15);
-  const int u = blockIdx.x, b = u / a.Hv, h = u % a.Hv;
-  f32x4 S[4];
+  __syncthreads();
+  load_f32(P, Tin + at, t);
+  f32x4 z[4];
 #pragma unroll
   for (int m = 0; m < 4; ++m)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) S[m][i] = dfinal ? dfinal[(size_t)u * kTile2 + (16 * m + 4 * g + i) * 64 + col] : 0.f;
-  for (int ch = a.NC - 1; ch >= 0; --ch) {
-    const int tok0 = 64 * ch, live = min(64, a.N - tok0);
-    const size_t at = ((size_t)u * a.NC + ch) * kTile2;
-    __syncthreads();
-    load_gates<T>(gate, a, b, h, tok0, t);
-    load_tile<64, kThr>(K, rows_of<T>(a.k, b, h / (a.Hv / a.Hk), tok0), a.k.n, live, t);
-#pragma unroll
-    for (int x = 0; x < 6; ++x) {
-      const int i = t + kThr * x;
-      *reinterpret_cast<uint4*>(M.x + (i >> 9) * kTileElems + ((i & 511) >> 3) * kTileRow + 8 * (i & 7)) =
-          reinterpret_cast<const uint4*>(Tm + 3 * at)[i];
+    for (int i = 0; i < 4; ++i) {
+      const int row = 16 * m + 4 * g + i;
+      E[at + row * 64 + own] = e[m][i];
+      e[m][i] *= gate.beta[row];
     }
-    f32x4 r[4], f[4];
+  const Frag<3> e0 = acc_frag<3>(e[0], e[1]), e1 = acc_frag<3>(e[2], e[3]);
+  __syncthreads();
 #pragma unroll
-    for (int m = 0; m < 4; ++m)
+  for (int m = 0; m < 4; ++m) {
+    z[m] = mma(col_frag_perm(P, 16 * m, 1, lane), e1, f32x4{});
+    if (m < 2) z[m] = mma(col_frag_perm(P, 16 * m, 0, lane), e0, z[m]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const size_t x = at + (16 * m + 4 * g + i) * 64 + col;
-        r[m][i] = E[x];
-        f[m][i] = F[x];
-        dSout[x] = S[m][i];
-      }
-    __syncthreads();
-    {
-      const Frag<3> s0 = acc_frag<3>(S[0], S[1]), s1 = acc_frag<3>(S[2], S[3]);
-#pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        f32x4 x = mma(row_frag_perm(K, 16 * m, 0, lane), s0, f32x4{});
-        x = mma(row_frag_perm(K, 16 * m, 1, lane), s1, x);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int row = 16 * m + 4 * g + i;
-          r[m][i] += gate.between(63, row) * x[i];
-          E[at + row * 64 + col] = r[m][i];
-          r[m][i] *= gate.beta[row];
-        }
-      }
-    }
-    f32x4 z[4];
-    {
-      const Frag<3> r0 = acc_frag<3>(r[0], r[1]), r1 = acc_frag<3>(r[2], r[3]);
-#pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        z[m] = mma(col_frag_perm(M, 16 * m, 1, lane), r1, f32x4{});
-        if (m < 2) z[m] = mma(col_frag_perm(M, 16 * m, 0, lane), r0, z[m]);
-      }
-    }
-    const float last = gate.since(63);
-#pragma unroll
-    for (int m = 0; m < 4; ++m)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = 16 * m + 4 * g + i;
-        dZout[at + row * 64 + col] = z[m][i];
-        z[m][i] *= -gate.since(row);
-        S[m][i] = S[m][i] * last + f[m][i];
-      }
-    const Frag<3> u0 = acc_frag<3>(z[0], z[1]), u1 = acc_frag<3>(z[2], z[3]);
-#pragma unroll
-    for (int m = 0; m < 4; ++m) {
-      S[m] = mma(col_frag_perm(K, 16 * m, 0, lane), u0, S[m]);
-      S[m] = mma(col_frag_perm(K, 16 * m, 1, lane), u1, S[m]);
-    }
+    for (int i = 0; i < 4; ++i) z[m][i] *= -gate.since(16 * m + 4 * g + i);
   }
-  if (dstate) {
+  const Frag<3> z0 = acc_frag<3>(z[0], z[1]), z1 = acc_frag<3>(z[2], z[3]);
 #pragma unroll
-    for (int m = 0; m < 4; ++m)
+  for (int m = 0; m < 4; ++m) {
+    f[m] = mma(col_frag_perm(K, 16 * m, 0, lane), z0, f[m]);
+    f[m] = mma(col_frag_perm(K, 16 * m, 1, lane), z1, f[m]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) dstate[(size_t)u * kTile2 + (16 * m + 4 * g + i) * 64 + col] = S[m][i];
+    for (int i = 0; i < 4; ++i) F[at + (16 * m + 4 * g + i) * 64 + own] = f[m][i];
   }
 }
 
@@ -504,9 +586,9 @@ __device__ __forceinline__ void own_row(Frag<3> (&f)[2], const float* row, int g
 // tokens are the columns.
 template <typename T>
 __global__ __launch_bounds__(kThr) void k_delta_bwd_out(DeltaArgs a, const T* __restrict__ dout,
-                                                        const float* __restrict__ Sin, const float* __restrict__ Zin,
-                                                        const float* __restrict__ dU, const float* __restrict__ dSin,
-                                                        const float* __restrict__ dZ, T* __restrict__ dq,
+                                                        const float* __restrict__ Tin, const float* __restrict__ Sin,
+                                                        const float* __restrict__ Zin, const float* __restrict__ E,
+                                                        const float* __restrict__ dSin, T* __restrict__ dq,
                                                         float* __restrict__ dqh, T* __restrict__ dk,
                                                         float* __restrict__ dkh, T* __restrict__ dv,
                                                         float* __restrict__ dg, void* __restrict__ dbeta) {
@@ -514,24 +596,106 @@ __global__ __launch_bounds__(kThr) void k_delta_bwd_out(DeltaArgs a, const T* __
   __shared__ Tile<NP> K, Q, O;
   __shared__ Tile<3> Z, X;
   __shared__ Gates gate;
-  __shared__ float dG[64], part[4];
+  __shared__ float dG[64], part[4], dotU[4][64];
   const int t = threadIdx.x, lane = t & 63, w = t >> 6, g = lane >> 4, c = lane & 15;
   const int ch = blockIdx.x % a.NC, u = blockIdx.x / a.NC, b = u / a.Hv, h = u % a.Hv;
   const int tok0 = 64 * ch, live = min(64, a.N - tok0), own = 16 * w + c;
   const size_t at = ((size_t)u * a.NC + ch) * kTile2;
-  load_gates<T>(gate, a, b, h, tok0, t);
   const T* krows = rows_of<T>(a.k, b, h / (a.Hv / a.Hk), tok0);
   load_tile<64, kThr>(K, krows, a.k.n, live, t);
-  load_f32(Z, Zin + at, t);
-  load_f32(X, dZ + at, t);
+  load_f32(X, dSin + at, t);
+  load_f32(Z, Tin + at, t);
   Frag<3> zf[2], dzf[2];
   own_row(zf, Zin + at + own * 64, g);
-  own_row(dzf, dZ + at + own * 64, g);
+  f32x4 e[4];
+#pragma unroll
+  for (int m = 0; m < 4; ++m)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e[m][i] = E[at + (16 * m + 4 * g + i) * 64 + own];
+  // <S, dS'>
+  float ends = 0.f;
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    const int i = 4 * (t + kThr * x);
+    const f32x4 s = load4(Sin + at + i), d = load4(dSin + at + i);
+    ends += s[0] * d[0] + s[1] * d[1] + s[2] * d[2] + s[3] * d[3];
+  }
+  load_gates<T>(gate, a, b, h, tok0, t);
   __syncthreads();
+  ends *= gate.since(63);
   const float beta = gate.beta[own];
   f32x4 reads[4] = {}, writes[4] = {};
   float dot = 0.f;    // of dbeta
   float decay = 0.f;  // of dG
+  f32x4 kv[4];
+  {
+    const float until = beta * gate.between(63, own);
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      kv[n] = f32x4{};
+      if (own < live) kv[n] = load4(krows + own * a.k.n + 16 * n + 4 * g);
+      f32x4 x = {};
+#pragma unroll
+      for (int s = 0; s < 2; ++s) x = mma(row_frag(X, 16 * n, s, lane), zf[s], x);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float y = until * x[i];
+        writes[n][i] += y;
+        // what the last token writes does not decay
+        const float z = own < live - 1 ? kv[n][i] * y : 0.f;
+        ends += z;
+        decay -= z;
+      }
+    }
+  }
+  ends = wave_sum(ends);
+  if (lane == 0) part[w] = ends;
+  {
+    // dU and dZ, columns of the values: own
+    const Frag<3> s0 = col_frag(X, 16 * w, 0, lane), s1 = col_frag(X, 16 * w, 1, lane);
+    float dots[16];
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+      f32x4 x = mma(row_frag(K, 16 * m, 0, lane), s0, f32x4{});
+      x = mma(row_frag(K, 16 * m, 1, lane), s1, x);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = 16 * m + 4 * g + i;
+        e[m][i] += gate.between(63, row) * x[i];
+        dots[4 * m + i] = e[m][i] * Zin[at + row * 64 + own];
+        e[m][i] *= gate.beta[row];
+      }
+    }
+    // sums over the 16 lanes of a row group; lane c ends with row 16 (c / 4) + 4 g + c % 4
+#pragma unroll
+    for (int half = 8; half > 0; half >>= 1)
+#pragma unroll
+      for (int i = 0; i < half; ++i) {
+        const bool up = c & half;
+        const float mine = up ? dots[i + half] : dots[i], other = up ? dots[i] : dots[i + half];
+        dots[i] = mine + __shfl_xor(other, half, 64);
+      }
+    dotU[w][16 * (c >> 2) + 4 * g + (c & 3)] = dots[0];
+    const Frag<3> e0 = acc_frag<3>(e[0], e[1]), e1 = acc_frag<3>(e[2], e[3]);
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+      e[m] = mma(col_frag_perm(Z, 16 * m, 1, lane), e1, f32x4{});
+      if (m < 2) e[m] = mma(col_frag_perm(Z, 16 * m, 0, lane), e0, e[m]);
+    }
+  }
+  __syncthreads();
+  load_f32(Z, Zin + at, t);
+#pragma unroll
+  for (int m = 0; m < 4; ++m)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = 16 * m + 4 * g + i;
+      put_parts(X, row, own, e[m][i]);
+      if (row < live) put(dv + ((size_t)u * a.N + tok0 + row) * 64 + own, e[m][i]);
+    }
+  __syncthreads();
+#pragma unroll
+  for (int s = 0; s < 2; ++s) dzf[s] = row_frag(X, 16 * w, s, lane);
   {
     // M^T: rows j, columns i = own
     f32x4 m[4] = {};
@@ -586,15 +750,7 @@ __global__ __launch_bounds__(kThr) void k_delta_bwd_out(DeltaArgs a, const T* __
       writes[n] = mma(col_frag_perm(K, 16 * n, 1, lane), m1, writes[n]);
     }
   }
-#pragma unroll
-  for (int n = 0; n < 4; ++n) {
-    const int x = own * 64 + 16 * n + 4 * g;
-    const f32x4 du = load4(dU + at + x), z = load4(Zin + at + x), dz = load4(dZ + at + x);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) dot += du[i] * z[i];
-    if (own < live) store4(dv + ((size_t)u * a.N + tok0) * 64 + x, dz);
-  }
-  dot = group_sum(dot);
+  dot = group_sum(dot) + ((dotU[0][own] + dotU[1][own]) + (dotU[2][own] + dotU[3][own]));
   if (g == 0 && own < live) {
     const size_t x = (size_t)u * a.N + tok0 + own;
     if (sizeof(T) == 2 && !a.beta32)
@@ -602,43 +758,6 @@ __global__ __launch_bounds__(kThr) void k_delta_bwd_out(DeltaArgs a, const T* __
     else
       static_cast<float*>(dbeta)[x] = dot;
   }
-  // the state after the chunk: its share of dk, and <S', dS'>
-  __syncthreads();
-  load_f32(X, dSin + at, t);
-  float ends = 0.f;
-  {
-    const float last = gate.since(63);
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const int i = 4 * (t + kThr * x);
-      const f32x4 s = load4(Sin + at + i), d = load4(dSin + at + i);
-      ends += last * (s[0] * d[0] + s[1] * d[1] + s[2] * d[2] + s[3] * d[3]);
-    }
-  }
-  __syncthreads();
-  f32x4 kv[4];
-  {
-    const float until = beta * gate.between(63, own);
-#pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      kv[n] = f32x4{};
-      if (own < live) kv[n] = load4(krows + own * a.k.n + 16 * n + 4 * g);
-      f32x4 x = {};
-#pragma unroll
-      for (int s = 0; s < 2; ++s) x = mma(row_frag(X, 16 * n, s, lane), zf[s], x);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float y = until * x[i];
-        writes[n][i] += y;
-        // what the last token writes does not decay
-        const float z = own < live - 1 ? kv[n][i] * y : 0.f;
-        ends += z;
-        decay -= z;
-      }
-    }
-  }
-  ends = wave_sum(ends);
-  if (lane == 0) part[w] = ends;
   __syncthreads();
   load_f32(X, Sin + at, t);
   __syncthreads();
@@ -775,9 +894,6 @@ namespace {
 __device__ __forceinline__ float value(const float* p, int64_t i) { return p[i]; }
 __device__ __forceinline__ float value(const uint16_t* p, int64_t i) { return to_f(p[i]); }
 __device__ __forceinline__ float value(const _Float16* p, int64_t i) { return static_cast<float>(p[i]); }
-__device__ __forceinline__ void put(float* p, int64_t i, float x) { p[i] = x; }
-__device__ __forceinline__ void put(uint16_t* p, int64_t i, float x) { p[i] = from_f<uint16_t>(x); }
-__device__ __forceinline__ void put(_Float16* p, int64_t i, float x) { p[i] = static_cast<_Float16>(x); }
 }  // namespace
 
 template <typename T>
@@ -844,7 +960,7 @@ __global__ __launch_bounds__(kThr) void k_delta_step(DeltaStepArgs a) {
       if (t < 16)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (c0 + j < a.Dv) put(out, c0 + j, a.scale * y[j]);
+          if (c0 + j < a.Dv) put(out + c0 + j, a.scale * y[j]);
     }
   }
 #pragma unroll
@@ -857,52 +973,112 @@ __global__ __launch_bounds__(kThr) void k_delta_step(DeltaStepArgs a) {
 // ---------------------------------------------------------------------------
 // Launches
 // ---------------------------------------------------------------------------
-DeltaSaved delta_saved_view(void* base, int U, int NC) {
-  DeltaSaved s;
+namespace {
+struct Room {
+  char* base;
   size_t off = 0;
-  const size_t tiles = (size_t)U * NC * kTile2;
-  auto take = [&](size_t bytes) {
-    char* p = static_cast<char*>(base) + off;
-    off += align256(bytes);
+  float* take(size_t values) {
+    float* p = reinterpret_cast<float*>(base + off);
+    off += align256(4 * values);
     return p;
+  }
+};
+
+// A chunk takes a walk about the same time whatever happens beside it, so long walks
+// of few chains are cut into segments: their maps' products at once (twice the
+// columns), a walk over those, then the segments from their own states. In units of a chunk's
+// time; a further launch costs about 10, and 512 blocks run at once.
+struct Segments {
+  int count, len;
+};
+Segments segments(int U, int NC) {
+  auto rounds = [](int64_t blocks) { return (double)((blocks + 511) / 512); };
+  Segments best{1, NC};
+  double least = NC * rounds(4LL * U);
+  for (int len = 4; 2 * len <= NC; ++len) {
+    const int n = (NC + len - 1) / len;
+    const double cost = len * (rounds(8LL * U * n) + rounds(4LL * U * n)) + n * rounds(4LL * U) + 20;
+    if (cost < least) least = cost, best = {n, len};
+  }
+  return best;
+}
+
+template <bool TR>
+void walk(const float* M, const float* D, const float* init, float* each, float* end, float* scratch, int U, int NC,
+          bool back, hipStream_t st, const Timer& timed) {
+  const Segments sg = segments(U, NC);
+  auto launch = [&](const Walk& a, auto tr, int cols) {
+    timed("k_delta_walk", st, [&] {
+      if (cols == 8)
+        hipLaunchKernelGGL((k_delta_walk<decltype(tr)::value, 8>), dim3(a.units * a.segs * 8), dim3(kThr), 0, st, a);
+      else
+        hipLaunchKernelGGL((k_delta_walk<decltype(tr)::value, 4>), dim3(a.units * a.segs * 4), dim3(kThr), 0, st, a);
+    });
   };
-  s.T = reinterpret_cast<uint16_t*>(take(tiles * 6));
-  s.S = reinterpret_cast<float*>(take(tiles * 4));
-  s.Z = reinterpret_cast<float*>(take(tiles * 4));
-  s.bytes = off;
+  using Tr = std::integral_constant<bool, TR>;
+  if (sg.count == 1) {
+    launch({M, D, init, each, end, nullptr, NC, 1, NC, U, back}, Tr{}, 4);
+    return;
+  }
+  const size_t part = (size_t)U * sg.count * kTile2;
+  float *segM = scratch, *segD = scratch + part, *segS = scratch + 2 * part;
+  launch({M, D, nullptr, nullptr, segD, segM, NC, sg.count, sg.len, U, back}, Tr{}, 8);
+  // the products stand as they act, whichever way the walk goes
+  launch({segM, segD, init, segS, end, nullptr, sg.count, 1, sg.count, U, back}, std::false_type{}, 4);
+  launch({M, D, segS, each, nullptr, nullptr, NC, sg.count, sg.len, U, back}, Tr{}, 4);
+}
+size_t walk_scratch(int U, int NC) {
+  const Segments sg = segments(U, NC);
+  return sg.count == 1 ? 0 : (size_t)3 * U * sg.count * kTile2;
+}
+}  // namespace
+
+DeltaSaved delta_saved_view(void* base, int U, int NC, bool keep) {
+  DeltaSaved s;
+  Room r{static_cast<char*>(base)};
+  const size_t tiles = (size_t)U * NC * kTile2;
+  s.T = r.take(tiles);
+  s.M = r.take(tiles);
+  s.S = r.take(tiles);
+  s.Z = keep ? r.take(tiles) : nullptr;
+  // needed by the forward alone: after what the backward reads
+  s.D = r.take(tiles);
+  s.scratch = r.take(walk_scratch(U, NC));
+  s.bytes = r.off;
   return s;
 }
 
 DeltaWork delta_work_view(void* base, const DeltaArgs& a) {
   DeltaWork w;
-  size_t off = 0;
-  auto take = [&](size_t values) {
-    float* p = reinterpret_cast<float*>(static_cast<char*>(base) + off);
-    off += align256(4 * values);
-    return p;
-  };
-  const size_t tiles = (size_t)a.B * a.Hv * a.NC * kTile2;
-  w.E = take(tiles);
-  w.F = take(tiles);
-  w.dS = take(tiles);
-  w.dZ = take(tiles);
-  w.dqh = a.H != a.Hq ? take((size_t)a.B * a.H * a.N * 64) : nullptr;
-  w.dkh = a.Hv != a.Hk ? take((size_t)a.B * a.Hv * a.N * 64) : nullptr;
-  w.bytes = off;
+  Room r{static_cast<char*>(base)};
+  const int U = a.B * a.Hv;
+  const size_t tiles = (size_t)U * a.NC * kTile2;
+  w.E = r.take(tiles);
+  w.F = r.take(tiles);
+  w.dS = r.take(tiles);
+  w.scratch = r.take(walk_scratch(U, a.NC));
+  w.dqh = a.H != a.Hq ? r.take((size_t)a.B * a.H * a.N * 64) : nullptr;
+  w.dkh = a.Hv != a.Hk ? r.take((size_t)a.B * a.Hv * a.N * 64) : nullptr;
+  w.bytes = r.off;
   return w;
 }
 
 template <typename T>
-void launch_delta_forward(const DeltaArgs& a, const float* state, void* out, float* final_state, void* saved,
+void launch_delta_forward(const DeltaArgs& a, const float* state, void* out, float* final_state, void* saved, bool keep,
                           hipStream_t st, const Timer& timed) {
-  const int U = a.B * a.Hv;
-  const DeltaSaved s = delta_saved_view(saved, U, a.NC);
-  timed("k_delta_solve", st, [&] { hipLaunchKernelGGL(k_delta_solve<T>, dim3(a.NC * U), dim3(kThr), 0, st, a, s.T); });
-  timed("k_delta_scan", st, [&] {
-    hipLaunchKernelGGL(k_delta_scan<T>, dim3(U), dim3(kThr), 0, st, a, s.T, state, s.S, s.Z, final_state);
-  });
+  const int U = a.B * a.Hv, rep = a.H / a.Hv;
+  const DeltaSaved s = delta_saved_view(saved, U, a.NC, keep);
+  timed("k_delta_chunk", st,
+        [&] { hipLaunchKernelGGL(k_delta_chunk<T>, dim3(a.NC * U), dim3(kThr), 0, st, a, s.T, s.M, s.D); });
+  walk<false>(s.M, s.D, state, s.S, final_state, s.scratch, U, a.NC, false, st, timed);
+  // all heads of a state in one block, unless that leaves CUs without one
+  const int parts = std::clamp((1024 + U * a.NC - 1) / (U * a.NC), 1, rep), each = (rep + parts - 1) / parts;
+  const dim3 grid(U * a.NC * ((rep + each - 1) / each));
   timed("k_delta_out", st, [&] {
-    hipLaunchKernelGGL(k_delta_out<T>, dim3(a.NC * a.B * a.H), dim3(kThr), 0, st, a, s.S, s.Z, static_cast<T*>(out));
+    if (keep)
+      hipLaunchKernelGGL((k_delta_out<T, true>), grid, dim3(kThr), 0, st, a, each, s.T, s.S, s.Z, static_cast<T*>(out));
+    else
+      hipLaunchKernelGGL((k_delta_out<T, false>), grid, dim3(kThr), 0, st, a, each, s.T, s.S, s.Z, static_cast<T*>(out));
   });
 }
 
@@ -911,17 +1087,15 @@ void launch_delta_backward(const DeltaArgs& a, const void* saved, const void* do
                            void* dk, void* dv, float* dg, void* dbeta, float* dstate, void* work, hipStream_t st,
                            const Timer& timed) {
   const int U = a.B * a.Hv;
-  const DeltaSaved s = delta_saved_view(const_cast<void*>(saved), U, a.NC);
+  const DeltaSaved s = delta_saved_view(const_cast<void*>(saved), U, a.NC, true);
   const DeltaWork w = delta_work_view(work, a);
   const T* od = static_cast<const T*>(dout);
   timed("k_delta_bwd_local", st, [&] {
-    hipLaunchKernelGGL(k_delta_bwd_local<T>, dim3(a.NC * U), dim3(kThr), 0, st, a, od, w.E, w.F);
+    hipLaunchKernelGGL(k_delta_bwd_local<T>, dim3(a.NC * U), dim3(kThr), 0, st, a, od, s.T, w.E, w.F);
   });
-  timed("k_delta_bwd_scan", st, [&] {
-    hipLaunchKernelGGL(k_delta_bwd_scan<T>, dim3(U), dim3(kThr), 0, st, a, s.T, dfinal, w.E, w.F, w.dS, w.dZ, dstate);
-  });
+  walk<true>(s.M, w.F, dfinal, w.dS, dstate, w.scratch, U, a.NC, true, st, timed);
   timed("k_delta_bwd_out", st, [&] {
-    hipLaunchKernelGGL(k_delta_bwd_out<T>, dim3(a.NC * U), dim3(kThr), 0, st, a, od, s.S, s.Z, w.E, w.dS, w.dZ,
+    hipLaunchKernelGGL(k_delta_bwd_out<T>, dim3(a.NC * U), dim3(kThr), 0, st, a, od, s.T, s.S, s.Z, w.E, w.dS,
                        static_cast<T*>(dq), w.dqh, static_cast<T*>(dk), w.dkh, static_cast<T*>(dv), dg, dbeta);
   });
   auto sum = [&](const float* src, void* dst, int heads, int each) {
@@ -935,10 +1109,10 @@ void launch_delta_backward(const DeltaArgs& a, const void* saved, const void* do
   if (w.dkh) sum(w.dkh, dk, a.Hk, a.Hv / a.Hk);
 }
 
-template void launch_delta_forward<float>(const DeltaArgs&, const float*, void*, float*, void*, hipStream_t,
+template void launch_delta_forward<float>(const DeltaArgs&, const float*, void*, float*, void*, bool, hipStream_t,
                                           const Timer&);
-template void launch_delta_forward<uint16_t>(const DeltaArgs&, const float*, void*, float*, void*, hipStream_t,
-                                             const Timer&);
+template void launch_delta_forward<uint16_t>(const DeltaArgs&, const float*, void*, float*, void*, bool,
+                                             hipStream_t, const Timer&);
 template void launch_delta_backward<float>(const DeltaArgs&, const void*, const void*, const float*, void*, void*,
                                            void*, float*, void*, float*, void*, hipStream_t, const Timer&);
 template void launch_delta_backward<uint16_t>(const DeltaArgs&, const void*, const void*, const float*, void*, void*,

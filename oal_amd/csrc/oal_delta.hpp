@@ -21,28 +21,32 @@ struct DeltaArgs {
   float scale;
 };
 
-// What the forward keeps for the backward, per unit u = b Hv + state head and chunk.
+// What the forward computes per unit u = b Hv + state head and chunk, and the backward reads (T to Z).
 struct DeltaSaved {
-  uint16_t* T;  // [U][NC][3][64][64] bf16 parts of the chunk's solved triangle
-  float* S;     // [U][NC][64][64] state before the chunk
-  float* Z;     // [U][NC][64][64] what each token found missing in its state, unscaled by beta
+  float* T;  // [U][NC][64][64] the chunk's solved triangle
+  float* M;  // [U][NC][64][64] its map of the state, S' = M S + D
+  float* S;  // [U][NC][64][64] state before the chunk
+  float* Z;  // [U][NC][64][64] what each token found missing in its state, unscaled by beta (null: not kept)
+  float* D;
+  float* scratch;
   size_t bytes;
 };
-DeltaSaved delta_saved_view(void* base, int U, int NC);
+DeltaSaved delta_saved_view(void* base, int U, int NC, bool keep);
 
 struct DeltaWork {
-  float* E;    // [U][NC][64][64] gradient of u from the chunk's own outputs; then of all
-  float* F;    // [U][NC][64][64] gradient of the state before the chunk from its outputs
-  float* dS;   // [U][NC][64][64] gradient of the state after the chunk
-  float* dZ;   // [U][NC][64][64]
+  float* E;   // [U][NC][64][64] gradient of u from the chunk's own outputs
+  float* F;   // [U][NC][64][64] gradient of the state before the chunk from its outputs
+  float* dS;  // [U][NC][64][64] gradient of the state after the chunk
+  float* scratch;
   float* dqh;  // [B][H][N][64] dq of every output head (null: heads are not shared)
   float* dkh;  // [B][Hv][N][64] dk of every state head (null: heads are not shared)
   size_t bytes;
 };
 DeltaWork delta_work_view(void* base, const DeltaArgs& a);
 
+// keep: for a backward
 template <typename T>
-void launch_delta_forward(const DeltaArgs& a, const float* state, void* out, float* final_state, void* saved,
+void launch_delta_forward(const DeltaArgs& a, const float* state, void* out, float* final_state, void* saved, bool keep,
                           hipStream_t st, const Timer& timed);
 // dout [B][H][N][64]; dfinal [U][64][64] may be null (no gradient).
 template <typename T>

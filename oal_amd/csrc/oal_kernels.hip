@@ -1502,9 +1502,9 @@ static int delta_args(oal::DeltaArgs* a, const char* what, const void* q, const 
   return 0;
 }
 
-size_t oal_gated_delta_saved_bytes(int batch, int v_heads, int seq_len) {
+size_t oal_gated_delta_saved_bytes(int batch, int v_heads, int seq_len, int keep) {
   if (check_delta(batch, v_heads, v_heads, v_heads, seq_len)) return 0;
-  return oal::delta_saved_view(nullptr, batch * v_heads, (seq_len + 63) / 64).bytes;
+  return oal::delta_saved_view(nullptr, batch * v_heads, (seq_len + 63) / 64, keep != 0).bytes;
 }
 
 size_t oal_gated_delta_workspace_bytes(int batch, int q_heads, int k_heads, int v_heads, int seq_len) {
@@ -1518,7 +1518,7 @@ size_t oal_gated_delta_workspace_bytes(int batch, int q_heads, int k_heads, int 
 int oal_gated_delta_forward(const void* q, const void* k, const void* v, const float* g, const void* beta,
                             const int64_t* strides, int beta_f32, int batch, int q_heads, int k_heads, int v_heads,
                             int seq_len, int dtype, float scale, const float* state, void* out, float* final_state,
-                            void* saved, void* stream) {
+                            void* saved, int keep, void* stream) {
   Range range("oal_gated_delta_forward");
   oal::DeltaArgs a;
   if (delta_args(&a, "oal_gated_delta_forward", q, k, v, g, beta, strides, beta_f32, batch, q_heads, k_heads, v_heads,
@@ -1530,9 +1530,9 @@ int oal_gated_delta_forward(const void* q, const void* k, const void* v, const f
     if (!aligned16(p)) return fail("oal_gated_delta_forward: tensor pointers must be 16-byte aligned");
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == OAL_DTYPE_F32)
-    oal::launch_delta_forward<float>(a, state, out, final_state, saved, st, make_timer());
+    oal::launch_delta_forward<float>(a, state, out, final_state, saved, keep != 0, st, make_timer());
   else
-    oal::launch_delta_forward<uint16_t>(a, state, out, final_state, saved, st, make_timer());
+    oal::launch_delta_forward<uint16_t>(a, state, out, final_state, saved, keep != 0, st, make_timer());
   return launch_status("oal_gated_delta_forward launch");
 }
 

@@ -74,22 +74,22 @@ struct alignas(16) Tile {
 
 typedef __bf16 lds_bf16x4 __attribute__((ext_vector_type(4)));
 
-// Operand row r0 + lane % 16, sum indexes 32 t + 8 g + j.
-template <int NP>
-__device__ __forceinline__ Frag<NP> row_frag(const Tile<NP>& s, int r0, int t, int lane) {
-  Frag<NP> f;
+// Operand row r0 + lane % 16, sum indexes 32 t + 8 g + j; its first N parts (0: all).
+template <int N = 0, int NP>
+__device__ __forceinline__ Frag<(N ? N : NP)> row_frag(const Tile<NP>& s, int r0, int t, int lane) {
+  Frag<(N ? N : NP)> f;
   const __bf16* p = s.x + (r0 + (lane & 15)) * kTileRow + 32 * t + 8 * (lane >> 4);
 #pragma unroll
-  for (int e = 0; e < NP; ++e) f.p[e] = *reinterpret_cast<const bf16x8*>(p + e * kTileElems);
+  for (int e = 0; e < (N ? N : NP); ++e) f.p[e] = *reinterpret_cast<const bf16x8*>(p + e * kTileElems);
   return f;
 }
 // The same row with the sum indexes in perm order.
-template <int NP>
-__device__ __forceinline__ Frag<NP> row_frag_perm(const Tile<NP>& s, int r0, int t, int lane) {
-  Frag<NP> f;
+template <int N = 0, int NP>
+__device__ __forceinline__ Frag<(N ? N : NP)> row_frag_perm(const Tile<NP>& s, int r0, int t, int lane) {
+  Frag<(N ? N : NP)> f;
   const __bf16* p = s.x + (r0 + (lane & 15)) * kTileRow + 32 * t + 4 * (lane >> 4);
 #pragma unroll
-  for (int e = 0; e < NP; ++e) {
+  for (int e = 0; e < (N ? N : NP); ++e) {
     const bf16x4 lo = *reinterpret_cast<const bf16x4*>(p + e * kTileElems);
     const bf16x4 hi = *reinterpret_cast<const bf16x4*>(p + e * kTileElems + 16);
     f.p[e] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
@@ -108,22 +108,22 @@ __device__ __forceinline__ bf16x8 tr_rows(const __bf16* lo_row, const __bf16* hi
   const trv8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
   return __builtin_bit_cast(bf16x8, v);
 }
-template <int NP>
-__device__ __forceinline__ Frag<NP> col_frag_perm(const Tile<NP>& s, int c0, int t, int lane) {
-  Frag<NP> f;
+template <int N = 0, int NP>
+__device__ __forceinline__ Frag<(N ? N : NP)> col_frag_perm(const Tile<NP>& s, int c0, int t, int lane) {
+  Frag<(N ? N : NP)> f;
   const int g = lane >> 4, i = lane & 15;
   const __bf16* p = s.x + (32 * t + 4 * g + (i >> 2)) * kTileRow + c0 + 4 * (i & 3);
 #pragma unroll
-  for (int e = 0; e < NP; ++e) f.p[e] = tr_rows(p + e * kTileElems, p + e * kTileElems + 16 * kTileRow);
+  for (int e = 0; e < (N ? N : NP); ++e) f.p[e] = tr_rows(p + e * kTileElems, p + e * kTileElems + 16 * kTileRow);
   return f;
 }
-template <int NP>
-__device__ __forceinline__ Frag<NP> col_frag(const Tile<NP>& s, int c0, int t, int lane) {
-  Frag<NP> f;
+template <int N = 0, int NP>
+__device__ __forceinline__ Frag<(N ? N : NP)> col_frag(const Tile<NP>& s, int c0, int t, int lane) {
+  Frag<(N ? N : NP)> f;
   const int g = lane >> 4, i = lane & 15;
   const __bf16* p = s.x + (32 * t + 8 * g + (i >> 2)) * kTileRow + c0 + 4 * (i & 3);
 #pragma unroll
-  for (int e = 0; e < NP; ++e) f.p[e] = tr_rows(p + e * kTileElems, p + e * kTileElems + 4 * kTileRow);
+  for (int e = 0; e < (N ? N : NP); ++e) f.p[e] = tr_rows(p + e * kTileElems, p + e * kTileElems + 4 * kTileRow);
   return f;
 }
 

@@ -100,8 +100,10 @@ class _GatedDeltaFunction(torch.autograd.Function):
         q, k, v = (_native.row_tensor(t.detach()) for t in (q, k, v))
         g, beta = g.detach(), beta.detach()
         start = None if state is None else _native._aligned(state.detach().contiguous())
-        out, final, saved = _native.delta_forward(q, k, v, g, beta, start, scale=scale)
-        ctx.save_for_backward(q, k, v, g, beta, saved)
+        keep = any(ctx.needs_input_grad)
+        out, final, saved = _native.delta_forward(q, k, v, g, beta, start, scale=scale, keep=keep)
+        if keep:
+            ctx.save_for_backward(q, k, v, g, beta, saved)
         ctx.scale = scale
         return out, final
 

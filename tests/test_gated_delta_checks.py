@@ -69,18 +69,19 @@ def _lib():
 
 def test_c_entries_check_before_they_launch():
     lib = _lib()
-    assert lib.oal_gated_delta_saved_bytes(2, 2, 65) == 4 * 2 * (6 + 4 + 4) * 4096
-    assert lib.oal_gated_delta_saved_bytes(0, 2, 65) == 0 and b"positive" in lib.oal_last_error()
+    assert lib.oal_gated_delta_saved_bytes(2, 2, 65, 1) == 4 * 2 * 5 * 4 * 4096
+    assert lib.oal_gated_delta_saved_bytes(2, 2, 65, 0) == 4 * 2 * 4 * 4 * 4096
+    assert lib.oal_gated_delta_saved_bytes(0, 2, 65, 1) == 0 and b"positive" in lib.oal_last_error()
     assert lib.oal_gated_delta_workspace_bytes(1, 3, 2, 2, 64) == 0 and b"divisible" in lib.oal_last_error()
     # shared heads need room for what is summed
     assert lib.oal_gated_delta_workspace_bytes(1, 2, 2, 4, 64) > lib.oal_gated_delta_workspace_bytes(1, 4, 4, 4, 64)
-    assert lib.oal_gated_delta_saved_bytes(1 << 20, 64, 1 << 20) == 0 and b"too large" in lib.oal_last_error()
+    assert lib.oal_gated_delta_saved_bytes(1 << 20, 64, 1 << 20, 1) == 0 and b"too large" in lib.oal_last_error()
     p, odd = ctypes.c_void_p(1 << 20), ctypes.c_void_p((1 << 20) + 8)
     rows = (ctypes.c_int64 * 15)(*[64] * 15)
     lib_f = lib.oal_gated_delta_forward
 
     def forward(q=p, strides=rows, dtype=1, out=p):
-        return lib_f(q, p, p, p, p, strides, 1, 1, 2, 2, 2, 64, dtype, 0.1, None, out, p, p, None)
+        return lib_f(q, p, p, p, p, strides, 1, 1, 2, 2, 2, 64, dtype, 0.1, None, out, p, p, 1, None)
 
     assert forward(q=None) and b"null" in lib.oal_last_error()
     assert forward(dtype=2) and b"dtype" in lib.oal_last_error()

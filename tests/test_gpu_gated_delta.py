@@ -38,12 +38,12 @@ def _inputs(b, heads, n, d=64, dv=None, dtype=torch.float32, beta_dtype=None, se
     return [q, k, v, g, beta, state], [dout, dstate]
 
 
-def _check(ins, ups, scale=0.125, tol=None, with_state=True):
+def _check(ins, ups, scale=0.125, with_state=True, on="cpu"):
     dev = _dev()
-    want_ins = [t.double().requires_grad_() for t in ins]
+    want_ins = [t.to(on).double().requires_grad_() for t in ins]
     want = gated_delta(*want_ins[:5], want_ins[5] if with_state else None, scale=scale)
     leaves = want_ins if with_state else want_ins[:5]
-    want = [*want, *torch.autograd.grad(want, leaves, [t.double() for t in ups])]
+    want = [*want, *torch.autograd.grad(want, leaves, [t.to(on).double() for t in ups])]
     got_ins = [t.to(dev).requires_grad_() for t in ins]
     got = gated_delta_attention(*got_ins[:5], scale=scale, initial_state=got_ins[5] if with_state else None)
     got = [*got, *torch.autograd.grad(got, got_ins if with_state else got_ins[:5], [t.to(dev) for t in ups])]
@@ -51,14 +51,20 @@ def _check(ins, ups, scale=0.125, tol=None, with_state=True):
     for name, x, y, dtype in zip(_NAMES, got, want, types):
         x, y = x.detach(), y.detach()
         assert x.dtype == dtype and x.shape == y.shape, name
-        err = float((x.double().cpu() - y).norm()) / max(float(y.norm()), 1e-30)
-        assert err <= (tol or _TOL)[dtype], f"{name}: {err:.3g}"
+        err = float((x.double().to(on) - y).norm()) / max(float(y.norm()), 1e-30)
+        assert err <= _TOL[dtype], f"{name}: {err:.3g}"
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("n", [1, 2, 16, 63, 64, 65, 127, 129, 300])
 def test_lengths(n, dtype):
     _check(*_inputs(2, (2, 2, 2), n, dtype=dtype, seed=n))
+
+
+@pytest.mark.parametrize("heads,n", [((2, 1, 1), 6001), ((2, 2, 2), 2688)])
+def test_long_sequences_walk_in_segments(heads, n):
+    ins, ups = _inputs(1, heads, n, dtype=torch.bfloat16, seed=n, decay=0.02)
+    _check(ins, ups, on=_dev())
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
