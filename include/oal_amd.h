@@ -44,6 +44,7 @@ extern "C" {
 
 #define OAL_DTYPE_F32 0
 #define OAL_DTYPE_BF16 1
+#define OAL_DTYPE_F16 2 /* the gated delta rule and the windowed attention alone */
 
 /* Arithmetic precision (reference HD planner "precision", hd_block_gemm.py:132-153):
  * OAL_PRECISION_FP32  fp32 arithmetic throughout (VALU kernels), any group count.
@@ -268,62 +269,64 @@ int oal_check_outputs(int wide, int out_kind, const void* num, const void* den, 
 /*
  * Gated delta rule, per state head (exp, sums and state in fp32 or more):
  *   S_t = e^(g_t) S_(t-1) + k_t u_t^T,  u_t = beta_t (v_t - e^(g_t) S_(t-1)^T k_t),  o_t = scale S_t^T q_t
- * q [B][Hq][N][64], k [B][Hk][N][64], v [B][Hv][N][64] of dtype, g [B][Hv][N] f32, beta [B][Hv][N] of
+ * q [B][Hq][N][key_dim], k [B][Hk][N][key_dim], v [B][Hv][N][value_dim] of dtype, dimensions
+ * multiples of 8 up to 64, g [B][Hv][N] f32, beta [B][Hv][N] of
  * dtype or (beta_f32) f32; Hk divides Hv, one of Hq and Hv divides the other, and
- * out [B][H][N][64] (dtype) has H = max(Hq, Hv) heads: output head o reads state head
+ * out [B][H][N][value_dim] (dtype) has H = max(Hq, Hv) heads: output head o reads state head
  * o Hv / H and query head o Hq / H, state head h key head h Hk / Hv. strides:
  * of q, k, v, g, beta, three each (batch, head, token), in elements; rows of q, k
  * and v are contiguous and 16-byte aligned. state (may be NULL: zero) and
- * final_state [B][Hv][64][64] f32, rows the key's dimensions. saved
+ * final_state [B][Hv][key_dim][value_dim] f32. saved
  * (oal_gated_delta_saved_bytes) is the call's room and, with keep, what the backward reads.
  */
 size_t oal_gated_delta_saved_bytes(int batch, int v_heads, int seq_len, int keep);
 int oal_gated_delta_forward(const void* q, const void* k, const void* v, const float* g, const void* beta,
                             const int64_t* strides, int beta_f32, int batch, int q_heads, int k_heads, int v_heads,
-                            int seq_len, int dtype, float scale, const float* state, void* out, float* final_state,
+                            int seq_len, int key_dim, int value_dim, int dtype, float scale, const float* state, void* out, float* final_state,
                             void* saved, int keep, void* stream);
 
 /*
- * Its VJP: dout [B][H][N][64] (dtype) and dfinal [B][Hv][64][64] f32 (may be NULL)
+ * Its VJP: dout [B][H][N][value_dim] (dtype) and dfinal [B][Hv][key_dim][value_dim] f32 (may be NULL)
  * -> contiguous dq, dk, dv (dtype), dg f32, dbeta (beta's type) and dstate f32 (may be
  * NULL). Heads that are shared are summed in a fixed order.
  */
-size_t oal_gated_delta_workspace_bytes(int batch, int q_heads, int k_heads, int v_heads, int seq_len);
+size_t oal_gated_delta_workspace_bytes(int batch, int q_heads, int k_heads, int v_heads, int seq_len, int key_dim);
 int oal_gated_delta_backward(const void* q, const void* k, const void* v, const float* g, const void* beta,
                              const int64_t* strides, int beta_f32, int batch, int q_heads, int k_heads, int v_heads,
-                             int seq_len, int dtype, float scale, const void* saved, const void* dout,
+                             int seq_len, int key_dim, int value_dim, int dtype, float scale, const void* saved, const void* dout,
                              const float* dfinal, void* dq, void* dk, void* dv, float* dg, void* dbeta, float* dstate,
                              void* workspace, void* stream);
 
 /*
  * The recurrence for a few tokens: state [B][Hv][key_dim][value_dim] f32 is updated
  * in place, out [B][H][N][value_dim] is written; dimensions 1 to 64, rows of any
- * alignment. kind: 0 float32, 1 bfloat16, 2 float16 (of q, k, v, out, and of beta unless beta_f32).
+ * alignment. dtype: of q, k, v, out, and of beta unless beta_f32.
  */
 int oal_gated_delta_step(const void* q, const void* k, const void* v, const float* g, const void* beta,
                          const int64_t* strides, int beta_f32, int batch, int q_heads, int k_heads, int v_heads,
-                         int seq_len, int key_dim, int value_dim, int kind, float scale, float* state, void* out,
+                         int seq_len, int key_dim, int value_dim, int dtype, float scale, float* state, void* out,
                          void* stream);
 
 /*
  * Causal softmax attention over a sliding window and first keys that stay visible:
  * out_i = sum_j softmax_j(scale q_i.k_j) v_j over keys j <= p_i with p_i - j < window or
- * j < sinks, p_i = key_len - query_len + i (the queries are the last tokens). q, out
- * [B][Hq][query_len][64], k, v [B][Hkv][key_len][64] of dtype; query head h reads KV head
+ * j < sinks, p_i = key_len - query_len + i (the queries are the last tokens). q
+ * [B][Hq][query_len][key_dim], k [B][Hkv][key_len][key_dim], v [..][value_dim], out
+ * [B][Hq][query_len][value_dim] of dtype, dimensions multiples of 8 up to 64; query head h reads KV head
  * h / (Hq / Hkv). strides: of q, k, v, three each (batch, head, token), in elements;
  * rows contiguous and 16-byte aligned; out is contiguous. lse [B][Hq][query_len] f32 is what the
  * backward reads (log2 of the sums of exponentials). 1 <= query_len <= key_len, window >= 1, sinks >= 0.
  */
 int oal_window_attention_forward(const void* q, const void* k, const void* v, const int64_t* strides, int batch,
-                                 int q_heads, int kv_heads, int query_len, int key_len, int window, int sinks,
-                                 int dtype, float scale, void* out, float* lse, void* stream);
+                                 int q_heads, int kv_heads, int query_len, int key_len, int key_dim,
+                                 int value_dim, int window, int sinks, int dtype, float scale, void* out, float* lse, void* stream);
 
-/* Its VJP: out, lse and dout [B][Hq][query_len][64] -> contiguous dq, dk, dv (dtype). */
+/* Its VJP: out, lse and dout [B][Hq][query_len][value_dim] -> contiguous dq, dk, dv (dtype). */
 size_t oal_window_attention_workspace_bytes(int batch, int q_heads, int kv_heads, int query_len, int key_len,
                                             int window, int sinks, int dtype);
 int oal_window_attention_backward(const void* q, const void* k, const void* v, const int64_t* strides, int batch,
-                                  int q_heads, int kv_heads, int query_len, int key_len, int window, int sinks,
-                                  int dtype, float scale, const void* out, const float* lse, const void* dout,
+                                  int q_heads, int kv_heads, int query_len, int key_len, int key_dim,
+                                  int value_dim, int window, int sinks, int dtype, float scale, const void* out, const float* lse, const void* dout,
                                   void* dq, void* dk, void* dv, void* workspace, void* stream);
 
 /*
@@ -333,13 +336,13 @@ int oal_window_attention_backward(const void* q, const void* k, const void* v, c
  * device; a negative one means no token: nothing is written, out is zero. strides: of q, k, v,
  * k_cache, v_cache, three each (batch, head, slot; those of q, k, v unused for the slot). key_dim and
  * value_dim multiples of 8 up to 64, all rows 16-byte aligned; out [B][Hq][value_dim]
- * contiguous. kind: 0 float32, 1 bfloat16, 2 float16.
+ * contiguous.
  */
 size_t oal_window_attention_step_workspace_bytes(int batch, int q_heads, int kv_heads, int value_dim, int window,
                                                  int sinks);
 int oal_window_attention_step(const void* q, const void* k, const void* v, void* k_cache, void* v_cache,
                               const int64_t* strides, const int64_t* position, int batch, int q_heads, int kv_heads,
-                              int key_dim, int value_dim, int window, int sinks, int kind, float scale, void* out,
+                              int key_dim, int value_dim, int window, int sinks, int dtype, float scale, void* out,
                               void* workspace, void* stream);
 
 #ifdef __cplusplus

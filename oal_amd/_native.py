@@ -79,13 +79,13 @@ _SIGNATURES = {
     "oal_check_labels": ([_vp, _i, _i, _i, _i, _i, _vp, _vp, _vp], _i),
     "oal_check_outputs": ([_i, _i, _vp, _vp, _vp, _sz, _i, _i, _i, _vp, _vp], _i),
     "oal_gated_delta_saved_bytes": ([_i] * 4, _sz),
-    "oal_gated_delta_workspace_bytes": ([_i] * 5, _sz),
-    "oal_gated_delta_forward": ([_vp] * 6 + [_i] * 7 + [_f] + [_vp] * 4 + [_i, _vp], _i),
-    "oal_gated_delta_backward": ([_vp] * 6 + [_i] * 7 + [_f] + [_vp] * 11, _i),
+    "oal_gated_delta_workspace_bytes": ([_i] * 6, _sz),
+    "oal_gated_delta_forward": ([_vp] * 6 + [_i] * 9 + [_f] + [_vp] * 4 + [_i, _vp], _i),
+    "oal_gated_delta_backward": ([_vp] * 6 + [_i] * 9 + [_f] + [_vp] * 11, _i),
     "oal_gated_delta_step": ([_vp] * 6 + [_i] * 9 + [_f] + [_vp] * 3, _i),
-    "oal_window_attention_forward": ([_vp] * 4 + [_i] * 8 + [_f] + [_vp] * 3, _i),
+    "oal_window_attention_forward": ([_vp] * 4 + [_i] * 10 + [_f] + [_vp] * 3, _i),
     "oal_window_attention_workspace_bytes": ([_i] * 8, _sz),
-    "oal_window_attention_backward": ([_vp] * 4 + [_i] * 8 + [_f] + [_vp] * 8, _i),
+    "oal_window_attention_backward": ([_vp] * 4 + [_i] * 10 + [_f] + [_vp] * 8, _i),
     "oal_window_attention_step_workspace_bytes": ([_i] * 6, _sz),
     "oal_window_attention_step": ([_vp] * 7 + [_i] * 8 + [_f] + [_vp] * 3, _i),
 }
@@ -716,43 +716,44 @@ class Verdict:
 
 
 # ---------------------------------------------------------------------------
-# Gated delta rule (oal_delta.hip). The callers (gated_delta.py) have checked types,
-# shapes and devices; rows may lie at any strides.
+# Gated delta rule (oal_delta.hip) and windowed attention (oal_window.hip). The callers
+# (gated_delta.py, window_attention.py) have checked types, shapes and devices; rows
+# are contiguous and 16-byte aligned, at any strides.
 # ---------------------------------------------------------------------------
+_DTYPES = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float16: 2}
+_Strides3, _Strides5 = ctypes.c_int64 * 9, ctypes.c_int64 * 15
+
+
 def row_tensor(t: torch.Tensor) -> torch.Tensor:
     """t, or a contiguous copy unless its rows are contiguous and 16-byte aligned."""
-    size = t.element_size()
-    strides = [s for s, n in zip(t.stride(), t.shape) if n > 1]
-    if (t.stride(-1) == 1 or t.shape[-1] == 1) and t.data_ptr() % 16 == 0 and all(
-            s * size % 16 == 0 for s in strides if s != 1):
-        return t
+    if t.data_ptr() % 16 == 0:
+        if t.is_contiguous() and t.shape[-1] % 8 == 0:
+            return t
+        size = t.element_size()
+        if t.stride(-1) == 1 and all(s * size % 16 == 0 for s, n in zip(t.stride()[:-1], t.shape) if n > 1):
+            return t
     return t.clone(memory_format=torch.contiguous_format)
 
 
-def _stride_array(*tensors: torch.Tensor):
-    """(batch, head, token) strides of each tensor; a dimension of one has none."""
-    values = [s if n > 1 else 0 for t in tensors for s, n in zip(t.stride()[:3], t.shape[:3])]
-    return (ctypes.c_int64 * len(values))(*values)
-
-
 def delta_forward(q, k, v, g, beta, state, *, scale: float, keep: bool):
-    """q, k, v [B, heads, N, 64] float32 or bfloat16 with aligned rows, g float32, beta
-    float32 or q's type, state float32 [B, Hv, 64, 64] or None. Returns (out,
-    final_state, saved); saved serves the backward if kept."""
+    """q, k [B, heads, N, D], v [B, Hv, N, DV], D and DV multiples of 8; g float32, beta
+    float32 or q's type, state contiguous float32 [B, Hv, D, DV] or None. Returns (out, final_state,
+    saved); saved serves the backward if kept."""
     lib = load_library()
-    b, hq, n, _ = q.shape
-    hk, hv, dev = k.shape[1], v.shape[1], q.device
+    b, hq, n, d = q.shape
+    hk, hv, dv, dev = k.shape[1], v.shape[1], v.shape[3], q.device
     with _scope(dev, "oal_amd::gated_delta_forward"):
-        nbytes = lib.oal_gated_delta_saved_bytes(b, hv, n, int(keep))
+        nbytes = lib.oal_gated_delta_saved_bytes(b, hv, n, keep)
         if nbytes == 0:
             _check(1, lib, "oal_gated_delta_saved_bytes")
-        out = torch.empty((b, max(hq, hv), n, HEAD_DIM), dtype=q.dtype, device=dev)
-        final = torch.empty((b, hv, HEAD_DIM, HEAD_DIM), dtype=torch.float32, device=dev)
+        out = q.new_empty((b, max(hq, hv), n, dv))
+        final = g.new_empty((b, hv, d, dv))
         saved = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
         rc = lib.oal_gated_delta_forward(
-            _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(beta), _stride_array(q, k, v, g, beta),
-            int(beta.dtype == torch.float32), b, hq, hk, hv, n, _dtype_code(q.dtype), float(scale), _ptr(state),
-            _ptr(out), _ptr(final), _ptr(saved), int(keep), _stream(dev))
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(),
+            _Strides5(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *g.stride(), *beta.stride()),
+            beta.dtype == torch.float32, b, hq, hk, hv, n, d, dv, _DTYPES[q.dtype], scale, _ptr(state),
+            out.data_ptr(), final.data_ptr(), saved.data_ptr(), keep, _stream(dev))
         _check(rc, lib, "oal_gated_delta_forward")
     return out, final, saved
 
@@ -760,57 +761,53 @@ def delta_forward(q, k, v, g, beta, state, *, scale: float, keep: bool):
 def delta_backward(q, k, v, g, beta, saved, dout, dfinal, *, scale: float, need_state: bool):
     """The VJP of :func:`delta_forward`: (dq, dk, dv, dg, dbeta, dstate or None)."""
     lib = load_library()
-    b, hq, n, _ = q.shape
-    hk, hv, dev = k.shape[1], v.shape[1], q.device
+    b, hq, n, d = q.shape
+    hk, hv, dv, dev = k.shape[1], v.shape[1], v.shape[3], q.device
     with _scope(dev, "oal_amd::gated_delta_backward"):
-        nbytes = lib.oal_gated_delta_workspace_bytes(b, hq, hk, hv, n)
+        nbytes = lib.oal_gated_delta_workspace_bytes(b, hq, hk, hv, n, d)
         if nbytes == 0:
             _check(1, lib, "oal_gated_delta_workspace_bytes")
         work = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
-        grads = [torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v, g, beta)]
-        dstate = torch.empty((b, hv, HEAD_DIM, HEAD_DIM), dtype=torch.float32, device=dev) if need_state else None
+        grads = [t.new_empty(t.shape) for t in (q, k, v, g, beta)]
+        dstate = g.new_empty((b, hv, d, dv)) if need_state else None
         rc = lib.oal_gated_delta_backward(
-            _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(beta), _stride_array(q, k, v, g, beta),
-            int(beta.dtype == torch.float32), b, hq, hk, hv, n, _dtype_code(q.dtype), float(scale), _ptr(saved),
-            _ptr(dout), _ptr(dfinal), *(_ptr(t) for t in grads), _ptr(dstate), _ptr(work), _stream(dev))
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(),
+            _Strides5(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *g.stride(), *beta.stride()),
+            beta.dtype == torch.float32, b, hq, hk, hv, n, d, dv, _DTYPES[q.dtype], scale, saved.data_ptr(),
+            dout.data_ptr(), _ptr(dfinal), *[t.data_ptr() for t in grads], _ptr(dstate), work.data_ptr(), _stream(dev))
         _check(rc, lib, "oal_gated_delta_backward")
     return (*grads, dstate)
 
 
-_KINDS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-
-
 def delta_step(q, k, v, g, beta, state, *, scale: float) -> torch.Tensor:
-    """The recurrence over the N tokens of q, k, v [B, heads, N, D] (unit stride in a row);
-    state [B, Hv, Dk, Dv] contiguous float32 is updated in place."""
+    """The recurrence over the N tokens of q, k, v [B, heads, N, D] (unit stride in a row, any
+    alignment); state [B, Hv, D, DV] contiguous float32 is updated in place."""
     lib = load_library()
-    b, hq, n, dk = q.shape
+    b, hq, n, d = q.shape
     hk, hv, dv, dev = k.shape[1], v.shape[1], v.shape[3], q.device
     with _scope(dev, "oal_amd::gated_delta_step"):
-        out = torch.empty((b, max(hq, hv), n, dv), dtype=q.dtype, device=dev)
+        out = q.new_empty((b, max(hq, hv), n, dv))
         rc = lib.oal_gated_delta_step(
-            _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(beta), _stride_array(q, k, v, g, beta),
-            int(beta.dtype == torch.float32), b, hq, hk, hv, n, dk, dv, _KINDS[q.dtype], float(scale), _ptr(state),
-            _ptr(out), _stream(dev))
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(),
+            _Strides5(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *g.stride(), *beta.stride()),
+            beta.dtype == torch.float32, b, hq, hk, hv, n, d, dv, _DTYPES[q.dtype], scale, state.data_ptr(),
+            out.data_ptr(), _stream(dev))
         _check(rc, lib, "oal_gated_delta_step")
     return out
 
 
-# ---------------------------------------------------------------------------
-# Windowed attention (oal_window.hip). The callers (window_attention.py) have checked
-# types, shapes and devices; rows are contiguous and aligned, at any strides.
-# ---------------------------------------------------------------------------
 def window_forward(q, k, v, *, window: int, sinks: int, scale: float):
-    """q [B, Hq, Nq, 64], k and v [B, Hkv, Nk, 64], float32 or bfloat16. Returns (out, lse)."""
+    """q [B, Hq, Nq, D], k [B, Hkv, Nk, D], v [B, Hkv, Nk, DV], D and DV multiples of 8. Returns (out, lse)."""
     lib = load_library()
-    b, hq, nq, _ = q.shape
-    hk, nk, dev = k.shape[1], k.shape[2], q.device
+    b, hq, nq, d = q.shape
+    _, hk, nk, dv = v.shape
+    dev = q.device
     with _scope(dev, "oal_amd::window_attention_forward"):
-        out = torch.empty((b, hq, nq, HEAD_DIM), dtype=q.dtype, device=dev)
+        out = q.new_empty((b, hq, nq, dv))
         lse = torch.empty((b, hq, nq), dtype=torch.float32, device=dev)
         rc = lib.oal_window_attention_forward(
-            _ptr(q), _ptr(k), _ptr(v), _stride_array(q, k, v), b, hq, hk, nq, nk, window, sinks, _dtype_code(q.dtype),
-            float(scale), _ptr(out), _ptr(lse), _stream(dev))
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), _Strides3(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3]),
+            b, hq, hk, nq, nk, d, dv, window, sinks, _DTYPES[q.dtype], scale, out.data_ptr(), lse.data_ptr(), _stream(dev))
         _check(rc, lib, "oal_window_attention_forward")
     return out, lse
 
@@ -818,17 +815,19 @@ def window_forward(q, k, v, *, window: int, sinks: int, scale: float):
 def window_backward(q, k, v, out, lse, dout, *, window: int, sinks: int, scale: float):
     """The VJP of :func:`window_forward`: (dq, dk, dv)."""
     lib = load_library()
-    b, hq, nq, _ = q.shape
-    hk, nk, dev, code = k.shape[1], k.shape[2], q.device, _dtype_code(q.dtype)
+    b, hq, nq, d = q.shape
+    _, hk, nk, dv = v.shape
+    dev, code = q.device, _DTYPES[q.dtype]
     with _scope(dev, "oal_amd::window_attention_backward"):
         nbytes = lib.oal_window_attention_workspace_bytes(b, hq, hk, nq, nk, window, sinks, code)
         if nbytes == 0:
             _check(1, lib, "oal_window_attention_workspace_bytes")
         work = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
-        grads = [torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v)]
+        grads = [t.new_empty(t.shape) for t in (q, k, v)]
         rc = lib.oal_window_attention_backward(
-            _ptr(q), _ptr(k), _ptr(v), _stride_array(q, k, v), b, hq, hk, nq, nk, window, sinks, code, float(scale),
-            _ptr(out), _ptr(lse), _ptr(dout), *(_ptr(t) for t in grads), _ptr(work), _stream(dev))
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), _Strides3(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3]),
+            b, hq, hk, nq, nk, d, dv, window, sinks, code, scale, out.data_ptr(), lse.data_ptr(), dout.data_ptr(),
+            *[t.data_ptr() for t in grads], work.data_ptr(), _stream(dev))
         _check(rc, lib, "oal_window_attention_backward")
     return tuple(grads)
 
@@ -844,10 +843,11 @@ def window_step(q, k, v, k_cache, v_cache, positions, *, window: int, sinks: int
         if nbytes == 0:
             _check(1, lib, "oal_window_attention_step_workspace_bytes")
         work = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
-        out = torch.empty((b, hq, 1, dv), dtype=q.dtype, device=dev)
+        out = q.new_empty((b, hq, 1, dv))
         rc = lib.oal_window_attention_step(
-            _ptr(q), _ptr(k), _ptr(v), _ptr(k_cache), _ptr(v_cache), _stride_array(q, k, v, k_cache, v_cache),
-            _ptr(positions), b, hq, hk, d, dv, window, sinks, _KINDS[q.dtype], float(scale), _ptr(out), _ptr(work),
-            _stream(dev))
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+            _Strides5(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *k_cache.stride()[:3], *v_cache.stride()[:3]),
+            positions.data_ptr(), b, hq, hk, d, dv, window, sinks, _DTYPES[q.dtype], scale, out.data_ptr(),
+            work.data_ptr(), _stream(dev))
         _check(rc, lib, "oal_window_attention_step")
     return out

@@ -43,9 +43,10 @@ struct Gates {
   __device__ float since(int i) const { return __builtin_amdgcn_exp2f(hi[i] + lo[i]); }
 };
 
-__device__ __forceinline__ float beta_at(const DeltaArgs& a, int b, int h, int tok, bool bf16) {
+template <typename T>
+__device__ __forceinline__ float beta_at(const DeltaArgs& a, int b, int h, int tok) {
   const int64_t at = b * a.beta.b + h * a.beta.h + tok * a.beta.n;
-  return bf16 && !a.beta32 ? to_f(static_cast<const uint16_t*>(a.beta.p)[at]) : static_cast<const float*>(a.beta.p)[at];
+  return a.beta32 ? static_cast<const float*>(a.beta.p)[at] : get(static_cast<const T*>(a.beta.p) + at);
 }
 
 // The first wave of the block; tokens past N decay nothing and write nothing.
@@ -58,7 +59,7 @@ __device__ __forceinline__ void load_gates(Gates& s, const DeltaArgs& a, int b, 
   if (tok < a.N) {
     x = static_cast<const float*>(a.g.p)[b * a.g.b + h * a.g.h + tok * a.g.n];
     x = (x < kLeast ? kLeast : x) * 1.4426950408889634;
-    beta = beta_at(a, b, h, tok, sizeof(T) == 2);
+    beta = beta_at<T>(a, b, h, tok);
   }
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
@@ -137,8 +138,8 @@ __global__ __launch_bounds__(kThr) void k_delta_chunk(DeltaArgs a, float* __rest
   const int ch = blockIdx.x % a.NC, u = blockIdx.x / a.NC, b = u / a.Hv, h = u % a.Hv;
   const int tok0 = 64 * ch, live = min(64, a.N - tok0);
   const size_t at = ((size_t)u * a.NC + ch) * kTile2;
-  load_tile<64, kThr>(K, rows_of<T>(a.k, b, h / (a.Hv / a.Hk), tok0), a.k.n, live, t);
-  load_tile<64, kThr>(V, rows_of<T>(a.v, b, h, tok0), a.v.n, live, t);
+  load_tile<64, kThr>(K, rows_of<T>(a.k, b, h / (a.Hv / a.Hk), tok0), a.k.n, a.D, live, t);
+  load_tile<64, kThr>(V, rows_of<T>(a.v, b, h, tok0), a.v.n, a.DV, live, t);
   load_gates<T>(gate, a, b, h, tok0, t);
   __syncthreads();
   for (int n = 0; n < 4; ++n) {
@@ -247,11 +248,11 @@ __global__ __launch_bounds__(kThr) void k_delta_chunk(DeltaArgs a, float* __rest
 struct Walk {
   const float* M;     // [units][maps][64][64]
   const float* D;
-  const float* init;  // state the walk starts from, by unit (segs == 1) or segment (null: zero)
+  const float* init;  // [rows][cols] state the walk starts from, by unit (segs == 1) or segment (null: zero)
   float* each;        // [units][maps][64][64]: the state before each map (null: not wanted)
-  float* end;         // by unit or segment: the state after the last (null: not wanted)
+  float* end;         // the same: the state after the last map (null: not wanted)
   float* mend;        // with 8 column groups: the product of the segment's maps
-  int maps, segs, len, units;
+  int maps, segs, len, units, rows, cols;
   bool back;
 };
 
@@ -273,7 +274,8 @@ __global__ __launch_bounds__(kThr) void k_delta_walk(Walk a) {
   const int first = seg * a.len, count = min(a.len, a.maps - first);
   const int col = 16 * (group & 3) + c, row = 16 * w + 4 * g;
   const size_t base = ((size_t)u * a.maps + first) * kTile2;
-  const size_t slot = (size_t)chain * kTile2;
+  auto slot = [&](int i) { return ((size_t)chain * a.rows + row + i) * a.cols + col; };
+  auto held = [&](int i) { return row + i < a.rows && col < a.cols; };
   float m[kAhead][16], d[kAhead][4];
   auto fetch = [&](int n, float (&mm)[16], float (&dd)[4]) {
     n = min(n, count - 1);
@@ -296,7 +298,7 @@ __global__ __launch_bounds__(kThr) void k_delta_walk(Walk a) {
   f32x4 S;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    S[i] = unit ? (row + i == col ? 1.f : 0.f) : a.init ? a.init[slot + (row + i) * 64 + col] : 0.f;
+    S[i] = unit ? (row + i == col ? 1.f : 0.f) : a.init && held(i) ? a.init[slot(i)] : 0.f;
   for (int n0 = 0; n0 < count; n0 += kAhead) {
 #pragma unroll
     for (int x = 0; x < kAhead; ++x) {
@@ -345,26 +347,9 @@ __global__ __launch_bounds__(kThr) void k_delta_walk(Walk a) {
   float* end = unit ? a.mend : a.end;
   if (!end) return;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) end[slot + (row + i) * 64 + col] = S[i];
+  for (int i = 0; i < 4; ++i)
+    if (held(i)) end[slot(i)] = S[i];
 }
-
-// Four consecutive values of a row.
-__device__ __forceinline__ void store4(float* p, const f32x4& x) { *reinterpret_cast<f32x4*>(p) = x; }
-__device__ __forceinline__ void store4(uint16_t* p, const f32x4& x) {
-  uint2 v = make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]));
-  *reinterpret_cast<uint2*>(p) = v;
-}
-__device__ __forceinline__ f32x4 load4(const float* p) { return *reinterpret_cast<const f32x4*>(p); }
-__device__ __forceinline__ f32x4 load4(const uint16_t* p) {
-  const uint2 v = *reinterpret_cast<const uint2*>(p);
-  return f32x4{__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16),
-               __uint_as_float(v.y & 0xffff0000u)};
-}
-
-
-__device__ __forceinline__ void put(float* p, float x) { *p = x; }
-__device__ __forceinline__ void put(uint16_t* p, float x) { *p = from_f<uint16_t>(x); }
-__device__ __forceinline__ void put(_Float16* p, float x) { *p = static_cast<_Float16>(x); }
 
 // The outputs of one chunk for `each` output heads of a state head. First Z = T (V -
 // e^G K S), a wave per 16 columns, to LDS as U = beta Z; then per output head, transposed: a
@@ -385,18 +370,18 @@ __global__ __launch_bounds__(kThr) void k_delta_out(DeltaArgs a, int each, const
   const int b = u / a.Hv, h = u % a.Hv;
   const int tok0 = 64 * ch, live = min(64, a.N - tok0), own = 16 * w + c;
   const size_t at = ((size_t)u * a.NC + ch) * kTile2;
-  load_tile<64, kThr>(K, rows_of<T>(a.k, b, h / (a.Hv / a.Hk), tok0), a.k.n, live, t);
+  load_tile<64, kThr>(K, rows_of<T>(a.k, b, h / (a.Hv / a.Hk), tok0), a.k.n, a.D, live, t);
   load_f32(S, Sin + at, t);
   load_f32(U, Tin + at, t);
-  const T* v = rows_of<T>(a.v, b, h, tok0) + own;
+  const T* v = rows_of<T>(a.v, b, h, tok0) + min(own, a.DV - 1);
   f32x4 z[4];
 #pragma unroll
   for (int m = 0; m < 4; ++m)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int row = 16 * m + 4 * g + i;
-      z[m][i] = to_f(v[min(row, live - 1) * a.v.n]);
-      z[m][i] = row < live ? z[m][i] : 0.f;
+      z[m][i] = get(v + min(row, live - 1) * a.v.n);
+      z[m][i] = row < live && own < a.DV ? z[m][i] : 0.f;
     }
   load_gates<T>(gate, a, b, h, tok0, t);
   __syncthreads();
@@ -433,7 +418,7 @@ __global__ __launch_bounds__(kThr) void k_delta_out(DeltaArgs a, int each, const
     const T* q = rows_of<T>(a.q, b, o / (a.H / a.Hq), tok0) + own * a.q.n;
     Frag<NP> qf[2];
 #pragma unroll
-    for (int s = 0; s < 2; ++s) qf[s] = global_frag<NP>(q + 32 * s + 8 * g, own < live);
+    for (int s = 0; s < 2; ++s) qf[s] = global_frag<NP>(q + 32 * s + 8 * g, own < live && 32 * s + 8 * g < a.D);
     f32x4 acc[4] = {}, p[4] = {};
 #pragma unroll
     for (int m = 0; m < 4; ++m) {
@@ -451,12 +436,12 @@ __global__ __launch_bounds__(kThr) void k_delta_out(DeltaArgs a, int each, const
       }
     }
     const Frag<NO> p0 = acc_frag<NO>(p[0], p[1]), p1 = acc_frag<NO>(p[2], p[3]);
-    T* dst = out + (((size_t)b * a.H + o) * a.N + tok0 + own) * 64;
+    T* dst = out + (((size_t)b * a.H + o) * a.N + tok0 + own) * a.DV;
 #pragma unroll
     for (int m = 0; m < 4; ++m) {
       acc[m] = mma(col_frag_perm<NO>(U, 16 * m, 0, lane), p0, acc[m]);
       if (w >= 2) acc[m] = mma(col_frag_perm<NO>(U, 16 * m, 1, lane), p1, acc[m]);
-      if (own < live) store4(dst + 16 * m + 4 * g, acc[m]);
+      if (own < live && 16 * m + 4 * g < a.DV) store4(dst + 16 * m + 4 * g, acc[m]);
     }
   }
 }
@@ -481,14 +466,14 @@ __global__ __launch_bounds__(kThr) void k_delta_bwd_local(DeltaArgs a, const T* 
   const int ch = blockIdx.x % a.NC, u = blockIdx.x / a.NC, b = u / a.Hv, h = u % a.Hv;
   const int tok0 = 64 * ch, live = min(64, a.N - tok0), own = 16 * w + c;
   const size_t at = ((size_t)u * a.NC + ch) * kTile2;
-  load_tile<64, kThr>(K, rows_of<T>(a.k, b, h / (a.Hv / a.Hk), tok0), a.k.n, live, t);
+  load_tile<64, kThr>(K, rows_of<T>(a.k, b, h / (a.Hv / a.Hk), tok0), a.k.n, a.D, live, t);
   load_gates<T>(gate, a, b, h, tok0, t);
   f32x4 e[4] = {}, f[4] = {};
   const int each = a.H / a.Hv;
   for (int o = h * each; o < (h + 1) * each; ++o) {
     if (o > h * each) __syncthreads();
-    load_tile<64, kThr>(Q, rows_of<T>(a.q, b, o / (a.H / a.Hq), tok0), a.q.n, live, t);
-    load_tile<64, kThr>(O, dout + (((size_t)b * a.H + o) * a.N + tok0) * 64, (int64_t)64, live, t);
+    load_tile<64, kThr>(Q, rows_of<T>(a.q, b, o / (a.H / a.Hq), tok0), a.q.n, a.D, live, t);
+    load_tile<64, kThr>(O, dout + (((size_t)b * a.H + o) * a.N + tok0) * a.DV, (int64_t)a.DV, a.DV, live, t);
     __syncthreads();
     // the scores, queries by keys = own: to LDS with the queries along a row
 #pragma unroll
@@ -519,8 +504,9 @@ __global__ __launch_bounds__(kThr) void k_delta_bwd_local(DeltaArgs a, const T* 
       float v[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        v[j] = static_cast<float>(of[s].p[0][j]);
-        if constexpr (NP == 3) v[j] = (v[j] + static_cast<float>(of[s].p[1][j])) + static_cast<float>(of[s].p[2][j]);
+        v[j] = 0.f;
+#pragma unroll
+        for (int x = NP - 1; x >= 0; --x) v[j] += static_cast<float>(of[s].p[x][j]);
         v[j] *= a.scale * gate.since(32 * s + 8 * g + j);
       }
       og[s] = split<3>(v);
@@ -602,7 +588,7 @@ __global__ __launch_bounds__(kThr) void k_delta_bwd_out(DeltaArgs a, const T* __
   const int tok0 = 64 * ch, live = min(64, a.N - tok0), own = 16 * w + c;
   const size_t at = ((size_t)u * a.NC + ch) * kTile2;
   const T* krows = rows_of<T>(a.k, b, h / (a.Hv / a.Hk), tok0);
-  load_tile<64, kThr>(K, krows, a.k.n, live, t);
+  load_tile<64, kThr>(K, krows, a.k.n, a.D, live, t);
   load_f32(X, dSin + at, t);
   load_f32(Z, Tin + at, t);
   Frag<3> zf[2], dzf[2];
@@ -633,7 +619,7 @@ __global__ __launch_bounds__(kThr) void k_delta_bwd_out(DeltaArgs a, const T* __
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
       kv[n] = f32x4{};
-      if (own < live) kv[n] = load4(krows + own * a.k.n + 16 * n + 4 * g);
+      if (own < live && 16 * n + 4 * g < a.D) kv[n] = load4(krows + own * a.k.n + 16 * n + 4 * g);
       f32x4 x = {};
 #pragma unroll
       for (int s = 0; s < 2; ++s) x = mma(row_frag(X, 16 * n, s, lane), zf[s], x);
@@ -691,7 +677,7 @@ __global__ __launch_bounds__(kThr) void k_delta_bwd_out(DeltaArgs a, const T* __
     for (int i = 0; i < 4; ++i) {
       const int row = 16 * m + 4 * g + i;
       put_parts(X, row, own, e[m][i]);
-      if (row < live) put(dv + ((size_t)u * a.N + tok0 + row) * 64 + own, e[m][i]);
+      if (row < live && own < a.DV) put(dv + ((size_t)u * a.N + tok0 + row) * a.DV + own, e[m][i]);
     }
   __syncthreads();
 #pragma unroll
@@ -753,10 +739,10 @@ __global__ __launch_bounds__(kThr) void k_delta_bwd_out(DeltaArgs a, const T* __
   dot = group_sum(dot) + ((dotU[0][own] + dotU[1][own]) + (dotU[2][own] + dotU[3][own]));
   if (g == 0 && own < live) {
     const size_t x = (size_t)u * a.N + tok0 + own;
-    if (sizeof(T) == 2 && !a.beta32)
-      static_cast<uint16_t*>(dbeta)[x] = from_f<uint16_t>(dot);
-    else
+    if (a.beta32)
       static_cast<float*>(dbeta)[x] = dot;
+    else
+      put(static_cast<T*>(dbeta) + x, dot);
   }
   __syncthreads();
   load_f32(X, Sin + at, t);
@@ -778,8 +764,8 @@ __global__ __launch_bounds__(kThr) void k_delta_bwd_out(DeltaArgs a, const T* __
     if (o > h * each) __syncthreads();
     const T* qrows = rows_of<T>(a.q, b, o / (a.H / a.Hq), tok0);
     const size_t orow = ((size_t)b * a.H + o) * a.N + tok0;
-    load_tile<64, kThr>(Q, qrows, a.q.n, live, t);
-    load_tile<64, kThr>(O, dout + orow * 64, (int64_t)64, live, t);
+    load_tile<64, kThr>(Q, qrows, a.q.n, a.D, live, t);
+    load_tile<64, kThr>(O, dout + orow * a.DV, (int64_t)a.DV, a.DV, live, t);
     __syncthreads();
     Frag<NP> of[2];
 #pragma unroll
@@ -788,7 +774,7 @@ __global__ __launch_bounds__(kThr) void k_delta_bwd_out(DeltaArgs a, const T* __
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
       f32x4 x = {}, qk = {}, qv = {};
-      if (own < live) qv = load4(qrows + own * a.q.n + 16 * n + 4 * g);
+      if (own < live && 16 * n + 4 * g < a.D) qv = load4(qrows + own * a.q.n + 16 * n + 4 * g);
 #pragma unroll
       for (int s = 0; s < 2; ++s) x = mma(row_frag(X, 16 * n, s, lane), of[s], x);
 #pragma unroll
@@ -815,11 +801,11 @@ __global__ __launch_bounds__(kThr) void k_delta_bwd_out(DeltaArgs a, const T* __
       for (int n = 0; n < 4; ++n) {
         acc[n] = mma(col_frag_perm(K, 16 * n, 0, lane), p0, acc[n]);
         if (w >= 2) acc[n] = mma(col_frag_perm(K, 16 * n, 1, lane), p1, acc[n]);
-        if (own < live) {
+        if (own < live && 16 * n + 4 * g < a.D) {
           if (dqh)
-            store4(dqh + (orow + own) * 64 + 16 * n + 4 * g, acc[n]);
+            store4(dqh + (orow + own) * a.D + 16 * n + 4 * g, acc[n]);
           else
-            store4(dq + (orow + own) * 64 + 16 * n + 4 * g, acc[n]);
+            store4(dq + (orow + own) * a.D + 16 * n + 4 * g, acc[n]);
         }
       }
     }
@@ -849,9 +835,9 @@ __global__ __launch_bounds__(kThr) void k_delta_bwd_out(DeltaArgs a, const T* __
   }
 #pragma unroll
   for (int n = 0; n < 4; ++n) {
-    if (own < live) {
+    if (own < live && 16 * n + 4 * g < a.D) {
       const f32x4 x = reads[n] + writes[n];
-      const size_t row = ((size_t)u * a.N + tok0 + own) * 64 + 16 * n + 4 * g;
+      const size_t row = ((size_t)u * a.N + tok0 + own) * a.D + 16 * n + 4 * g;
       if (dkh)
         store4(dkh + row, x);
       else
@@ -874,7 +860,7 @@ __global__ __launch_bounds__(kThr) void k_delta_bwd_out(DeltaArgs a, const T* __
 }
 
 // Gradients of heads that several heads share: their sums, in order. dst
-// [B][heads][N][64] of src [B][heads each][N][64].
+// [B][heads][N][D] of src [B][heads each][N][D].
 template <typename T>
 __global__ __launch_bounds__(kThr) void k_delta_sum_heads(const float* __restrict__ src, T* __restrict__ dst, int each,
                                                           int64_t head, int64_t total) {
@@ -890,12 +876,6 @@ __global__ __launch_bounds__(kThr) void k_delta_sum_heads(const float* __restric
 // The recurrence itself, for single tokens: a block per state head holds the
 // state, 4 x 4 values per thread, for all N tokens and writes it back.
 // ---------------------------------------------------------------------------
-namespace {
-__device__ __forceinline__ float value(const float* p, int64_t i) { return p[i]; }
-__device__ __forceinline__ float value(const uint16_t* p, int64_t i) { return to_f(p[i]); }
-__device__ __forceinline__ float value(const _Float16* p, int64_t i) { return static_cast<float>(p[i]); }
-}  // namespace
-
 template <typename T>
 __global__ __launch_bounds__(kThr) void k_delta_step(DeltaStepArgs a) {
   __shared__ float sum[4][64];
@@ -927,11 +907,11 @@ __global__ __launch_bounds__(kThr) void k_delta_step(DeltaStepArgs a) {
   for (int n = 0; n < a.N; ++n) {
     const float decay = expf(static_cast<const float*>(a.g.p)[b * a.g.b + h * a.g.h + n * a.g.n]);
     const int64_t bx = b * a.beta.b + h * a.beta.h + n * a.beta.n;
-    const float beta = a.beta32 ? static_cast<const float*>(a.beta.p)[bx] : value(static_cast<const T*>(a.beta.p), bx);
+    const float beta = a.beta32 ? static_cast<const float*>(a.beta.p)[bx] : get(static_cast<const T*>(a.beta.p) + bx);
     float kr[4], x[4] = {};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      kr[i] = d0 + i < a.Dk ? value(k, n * a.k.n + d0 + i) : 0.f;
+      kr[i] = d0 + i < a.Dk ? get(k + n * a.k.n + d0 + i) : 0.f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         s[i][j] *= decay;
@@ -941,7 +921,7 @@ __global__ __launch_bounds__(kThr) void k_delta_step(DeltaStepArgs a) {
     over_rows(x);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float vj = c0 + j < a.Dv ? value(v, n * a.v.n + c0 + j) : 0.f;
+      const float vj = c0 + j < a.Dv ? get(v + n * a.v.n + c0 + j) : 0.f;
       const float uj = beta * (vj - x[j]);
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[i][j] += kr[i] * uj;
@@ -951,7 +931,7 @@ __global__ __launch_bounds__(kThr) void k_delta_step(DeltaStepArgs a) {
       float y[4] = {};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float qi = d0 + i < a.Dk ? value(q, d0 + i) : 0.f;
+        const float qi = d0 + i < a.Dk ? get(q + d0 + i) : 0.f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) y[j] += qi * s[i][j];
       }
@@ -1004,8 +984,9 @@ Segments segments(int U, int NC) {
 }
 
 template <bool TR>
-void walk(const float* M, const float* D, const float* init, float* each, float* end, float* scratch, int U, int NC,
-          bool back, hipStream_t st, const Timer& timed) {
+void walk(const DeltaArgs& g, const float* M, const float* D, const float* init, float* each, float* end,
+          float* scratch, bool back, hipStream_t st, const Timer& timed) {
+  const int U = g.B * g.Hv, NC = g.NC;
   const Segments sg = segments(U, NC);
   auto launch = [&](const Walk& a, auto tr, int cols) {
     timed("k_delta_walk", st, [&] {
@@ -1017,15 +998,15 @@ void walk(const float* M, const float* D, const float* init, float* each, float*
   };
   using Tr = std::integral_constant<bool, TR>;
   if (sg.count == 1) {
-    launch({M, D, init, each, end, nullptr, NC, 1, NC, U, back}, Tr{}, 4);
+    launch({M, D, init, each, end, nullptr, NC, 1, NC, U, g.D, g.DV, back}, Tr{}, 4);
     return;
   }
   const size_t part = (size_t)U * sg.count * kTile2;
   float *segM = scratch, *segD = scratch + part, *segS = scratch + 2 * part;
-  launch({M, D, nullptr, nullptr, segD, segM, NC, sg.count, sg.len, U, back}, Tr{}, 8);
+  launch({M, D, nullptr, nullptr, segD, segM, NC, sg.count, sg.len, U, 64, 64, back}, Tr{}, 8);
   // the products stand as they act, whichever way the walk goes
-  launch({segM, segD, init, segS, end, nullptr, sg.count, 1, sg.count, U, back}, std::false_type{}, 4);
-  launch({M, D, segS, each, nullptr, nullptr, NC, sg.count, sg.len, U, back}, Tr{}, 4);
+  launch({segM, segD, init, segS, end, nullptr, sg.count, 1, sg.count, U, g.D, g.DV, back}, std::false_type{}, 4);
+  launch({M, D, segS, each, nullptr, nullptr, NC, sg.count, sg.len, U, 64, 64, back}, Tr{}, 4);
 }
 size_t walk_scratch(int U, int NC) {
   const Segments sg = segments(U, NC);
@@ -1057,8 +1038,8 @@ DeltaWork delta_work_view(void* base, const DeltaArgs& a) {
   w.F = r.take(tiles);
   w.dS = r.take(tiles);
   w.scratch = r.take(walk_scratch(U, a.NC));
-  w.dqh = a.H != a.Hq ? r.take((size_t)a.B * a.H * a.N * 64) : nullptr;
-  w.dkh = a.Hv != a.Hk ? r.take((size_t)a.B * a.Hv * a.N * 64) : nullptr;
+  w.dqh = a.H != a.Hq ? r.take((size_t)a.B * a.H * a.N * a.D) : nullptr;
+  w.dkh = a.Hv != a.Hk ? r.take((size_t)a.B * a.Hv * a.N * a.D) : nullptr;
   w.bytes = r.off;
   return w;
 }
@@ -1070,7 +1051,7 @@ void launch_delta_forward(const DeltaArgs& a, const float* state, void* out, flo
   const DeltaSaved s = delta_saved_view(saved, U, a.NC, keep);
   timed("k_delta_chunk", st,
         [&] { hipLaunchKernelGGL(k_delta_chunk<T>, dim3(a.NC * U), dim3(kThr), 0, st, a, s.T, s.M, s.D); });
-  walk<false>(s.M, s.D, state, s.S, final_state, s.scratch, U, a.NC, false, st, timed);
+  walk<false>(a, s.M, s.D, state, s.S, final_state, s.scratch, false, st, timed);
   // all heads of a state in one block, unless that leaves CUs without one
   const int parts = std::clamp((1024 + U * a.NC - 1) / (U * a.NC), 1, rep), each = (rep + parts - 1) / parts;
   const dim3 grid(U * a.NC * ((rep + each - 1) / each));
@@ -1093,13 +1074,13 @@ void launch_delta_backward(const DeltaArgs& a, const void* saved, const void* do
   timed("k_delta_bwd_local", st, [&] {
     hipLaunchKernelGGL(k_delta_bwd_local<T>, dim3(a.NC * U), dim3(kThr), 0, st, a, od, s.T, w.E, w.F);
   });
-  walk<true>(s.M, w.F, dfinal, w.dS, dstate, w.scratch, U, a.NC, true, st, timed);
+  walk<true>(a, s.M, w.F, dfinal, w.dS, dstate, w.scratch, true, st, timed);
   timed("k_delta_bwd_out", st, [&] {
     hipLaunchKernelGGL(k_delta_bwd_out<T>, dim3(a.NC * U), dim3(kThr), 0, st, a, od, s.T, s.S, s.Z, w.E, w.dS,
                        static_cast<T*>(dq), w.dqh, static_cast<T*>(dk), w.dkh, static_cast<T*>(dv), dg, dbeta);
   });
   auto sum = [&](const float* src, void* dst, int heads, int each) {
-    const int64_t head = (int64_t)a.N * 64, total = (int64_t)a.B * heads * head;
+    const int64_t head = (int64_t)a.N * a.D, total = (int64_t)a.B * heads * head;
     timed("k_delta_sum_heads", st, [&] {
       hipLaunchKernelGGL(k_delta_sum_heads<T>, dim3((unsigned)((total / 4 + kThr - 1) / kThr)), dim3(kThr), 0, st, src,
                          static_cast<T*>(dst), each, head, total);
@@ -1109,14 +1090,15 @@ void launch_delta_backward(const DeltaArgs& a, const void* saved, const void* do
   if (w.dkh) sum(w.dkh, dk, a.Hk, a.Hv / a.Hk);
 }
 
-template void launch_delta_forward<float>(const DeltaArgs&, const float*, void*, float*, void*, bool, hipStream_t,
-                                          const Timer&);
-template void launch_delta_forward<uint16_t>(const DeltaArgs&, const float*, void*, float*, void*, bool,
-                                             hipStream_t, const Timer&);
-template void launch_delta_backward<float>(const DeltaArgs&, const void*, const void*, const float*, void*, void*,
-                                           void*, float*, void*, float*, void*, hipStream_t, const Timer&);
-template void launch_delta_backward<uint16_t>(const DeltaArgs&, const void*, const void*, const float*, void*, void*,
-                                              void*, float*, void*, float*, void*, hipStream_t, const Timer&);
+#define OAL_DELTA(T)                                                                                                 \
+  template void launch_delta_forward<T>(const DeltaArgs&, const float*, void*, float*, void*, bool, hipStream_t,     \
+                                        const Timer&);                                                              \
+  template void launch_delta_backward<T>(const DeltaArgs&, const void*, const void*, const float*, void*, void*,     \
+                                         void*, float*, void*, float*, void*, hipStream_t, const Timer&);
+OAL_DELTA(float)
+OAL_DELTA(uint16_t)
+OAL_DELTA(_Float16)
+#undef OAL_DELTA
 
 void launch_delta_step(int kind, const DeltaStepArgs& a, hipStream_t st, const Timer& timed) {
   timed("k_delta_step", st, [&] {

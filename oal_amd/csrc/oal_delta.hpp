@@ -15,8 +15,8 @@ struct Strided {
 };
 
 struct DeltaArgs {
-  Strided q, k, v, g, beta;  // rows of 64 values; g and beta one value
-  int B, Hq, Hk, Hv, H, N, NC;
+  Strided q, k, v, g, beta;  // rows of D, D and DV values; g and beta one value
+  int B, Hq, Hk, Hv, H, N, NC, D, DV;
   bool beta32;  // beta is float32 whatever the other operands are
   float scale;
 };
@@ -38,8 +38,8 @@ struct DeltaWork {
   float* F;   // [U][NC][64][64] gradient of the state before the chunk from its outputs
   float* dS;  // [U][NC][64][64] gradient of the state after the chunk
   float* scratch;
-  float* dqh;  // [B][H][N][64] dq of every output head (null: heads are not shared)
-  float* dkh;  // [B][Hv][N][64] dk of every state head (null: heads are not shared)
+  float* dqh;  // [B][H][N][D] dq of every output head (null: heads are not shared)
+  float* dkh;  // [B][Hv][N][D] dk of every state head (null: heads are not shared)
   size_t bytes;
 };
 DeltaWork delta_work_view(void* base, const DeltaArgs& a);
@@ -48,7 +48,7 @@ DeltaWork delta_work_view(void* base, const DeltaArgs& a);
 template <typename T>
 void launch_delta_forward(const DeltaArgs& a, const float* state, void* out, float* final_state, void* saved, bool keep,
                           hipStream_t st, const Timer& timed);
-// dout [B][H][N][64]; dfinal [U][64][64] may be null (no gradient).
+// dout [B][H][N][DV]; dfinal [U][D][DV] may be null (no gradient).
 template <typename T>
 void launch_delta_backward(const DeltaArgs& a, const void* saved, const void* dout, const float* dfinal, void* dq,
                            void* dk, void* dv, float* dg, void* dbeta, float* dstate, void* work, hipStream_t st,

@@ -1483,21 +1483,29 @@ static int check_delta(int batch, int q_heads, int k_heads, int v_heads, int seq
 
 static oal::Strided strided(const void* p, const int64_t* s) { return {p, s[0], s[1], s[2]}; }
 
-static bool rows_aligned(const oal::Strided& s, int bytes) {
-  return aligned16(s.p) && (s.b * bytes) % 16 == 0 && (s.h * bytes) % 16 == 0 && (s.n * bytes) % 16 == 0;
+// Strides of dimensions of one do not matter.
+static bool rows_aligned(const oal::Strided& s, int dtype, int batch, int heads, int64_t len) {
+  const int bytes = dtype == OAL_DTYPE_F32 ? 4 : 2;
+  return aligned16(s.p) && (batch == 1 || (s.b * bytes) % 16 == 0) && (heads == 1 || (s.h * bytes) % 16 == 0) &&
+         (len == 1 || (s.n * bytes) % 16 == 0);
 }
+
+static bool dim_ok(int d) { return d >= 8 && d <= 64 && d % 8 == 0; }
 
 static int delta_args(oal::DeltaArgs* a, const char* what, const void* q, const void* k, const void* v, const float* g,
                       const void* beta, const int64_t* strides, int beta_f32, int batch, int q_heads, int k_heads,
-                      int v_heads, int seq_len, int dtype, float scale) {
+                      int v_heads, int seq_len, int key_dim, int value_dim, int dtype, float scale) {
   if (check_delta(batch, q_heads, k_heads, v_heads, seq_len)) return 1;
-  if (dtype != OAL_DTYPE_F32 && dtype != OAL_DTYPE_BF16) return fail("dtype must be OAL_DTYPE_F32 or OAL_DTYPE_BF16");
+  if (!dim_ok(key_dim) || !dim_ok(value_dim))
+    return fail(std::string(what) + ": dimensions must be multiples of 8 up to 64");
+  if (dtype < OAL_DTYPE_F32 || dtype > OAL_DTYPE_F16)
+    return fail("dtype must be OAL_DTYPE_F32, OAL_DTYPE_BF16 or OAL_DTYPE_F16");
   if (!q || !k || !v || !g || !beta || !strides) return fail(std::string(what) + ": null pointer argument");
   *a = {strided(q, strides), strided(k, strides + 3), strided(v, strides + 6), strided(g, strides + 9),
         strided(beta, strides + 12), batch, q_heads, k_heads, v_heads, q_heads > v_heads ? q_heads : v_heads, seq_len,
-        (seq_len + 63) / 64, beta_f32 != 0 || dtype == OAL_DTYPE_F32, scale};
-  const int bytes = dtype == OAL_DTYPE_F32 ? 4 : 2;
-  if (!rows_aligned(a->q, bytes) || !rows_aligned(a->k, bytes) || !rows_aligned(a->v, bytes))
+        (seq_len + 63) / 64, key_dim, value_dim, beta_f32 != 0 || dtype == OAL_DTYPE_F32, scale};
+  if (!rows_aligned(a->q, dtype, batch, q_heads, seq_len) || !rows_aligned(a->k, dtype, batch, k_heads, seq_len) ||
+      !rows_aligned(a->v, dtype, batch, v_heads, seq_len))
     return fail(std::string(what) + ": rows must be 16-byte aligned");
   return 0;
 }
@@ -1507,44 +1515,48 @@ size_t oal_gated_delta_saved_bytes(int batch, int v_heads, int seq_len, int keep
   return oal::delta_saved_view(nullptr, batch * v_heads, (seq_len + 63) / 64, keep != 0).bytes;
 }
 
-size_t oal_gated_delta_workspace_bytes(int batch, int q_heads, int k_heads, int v_heads, int seq_len) {
+size_t oal_gated_delta_workspace_bytes(int batch, int q_heads, int k_heads, int v_heads, int seq_len, int key_dim) {
   if (check_delta(batch, q_heads, k_heads, v_heads, seq_len)) return 0;
+  if (!dim_ok(key_dim)) {
+    fail("oal_gated_delta_workspace_bytes: dimensions must be multiples of 8 up to 64");
+    return 0;
+  }
   oal::DeltaArgs a{};
-  a.B = batch, a.Hq = q_heads, a.Hk = k_heads, a.Hv = v_heads, a.N = seq_len;
+  a.B = batch, a.Hq = q_heads, a.Hk = k_heads, a.Hv = v_heads, a.N = seq_len, a.D = key_dim;
   a.H = q_heads > v_heads ? q_heads : v_heads, a.NC = (seq_len + 63) / 64;
   return oal::delta_work_view(nullptr, a).bytes;
 }
 
 int oal_gated_delta_forward(const void* q, const void* k, const void* v, const float* g, const void* beta,
                             const int64_t* strides, int beta_f32, int batch, int q_heads, int k_heads, int v_heads,
-                            int seq_len, int dtype, float scale, const float* state, void* out, float* final_state,
+                            int seq_len, int key_dim, int value_dim, int dtype, float scale, const float* state, void* out, float* final_state,
                             void* saved, int keep, void* stream) {
   Range range("oal_gated_delta_forward");
   oal::DeltaArgs a;
   if (delta_args(&a, "oal_gated_delta_forward", q, k, v, g, beta, strides, beta_f32, batch, q_heads, k_heads, v_heads,
-                 seq_len, dtype, scale))
+                 seq_len, key_dim, value_dim, dtype, scale))
     return 1;
   if (!out || !final_state || !saved) return fail("oal_gated_delta_forward: null pointer argument");
   const void* ptrs[] = {state, out, final_state, saved};
   for (const void* p : ptrs)
     if (!aligned16(p)) return fail("oal_gated_delta_forward: tensor pointers must be 16-byte aligned");
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (dtype == OAL_DTYPE_F32)
-    oal::launch_delta_forward<float>(a, state, out, final_state, saved, keep != 0, st, make_timer());
-  else
-    oal::launch_delta_forward<uint16_t>(a, state, out, final_state, saved, keep != 0, st, make_timer());
+  const auto launch = dtype == OAL_DTYPE_F32    ? oal::launch_delta_forward<float>
+                      : dtype == OAL_DTYPE_BF16 ? oal::launch_delta_forward<uint16_t>
+                                                : oal::launch_delta_forward<_Float16>;
+  launch(a, state, out, final_state, saved, keep != 0, st, make_timer());
   return launch_status("oal_gated_delta_forward launch");
 }
 
 int oal_gated_delta_backward(const void* q, const void* k, const void* v, const float* g, const void* beta,
                              const int64_t* strides, int beta_f32, int batch, int q_heads, int k_heads, int v_heads,
-                             int seq_len, int dtype, float scale, const void* saved, const void* dout,
+                             int seq_len, int key_dim, int value_dim, int dtype, float scale, const void* saved, const void* dout,
                              const float* dfinal, void* dq, void* dk, void* dv, float* dg, void* dbeta, float* dstate,
                              void* workspace, void* stream) {
   Range range("oal_gated_delta_backward");
   oal::DeltaArgs a;
   if (delta_args(&a, "oal_gated_delta_backward", q, k, v, g, beta, strides, beta_f32, batch, q_heads, k_heads, v_heads,
-                 seq_len, dtype, scale))
+                 seq_len, key_dim, value_dim, dtype, scale))
     return 1;
   if (!saved || !dout || !dq || !dk || !dv || !dg || !dbeta || !workspace)
     return fail("oal_gated_delta_backward: null pointer argument");
@@ -1552,30 +1564,29 @@ int oal_gated_delta_backward(const void* q, const void* k, const void* v, const 
   for (const void* p : ptrs)
     if (!aligned16(p)) return fail("oal_gated_delta_backward: tensor pointers must be 16-byte aligned");
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (dtype == OAL_DTYPE_F32)
-    oal::launch_delta_backward<float>(a, saved, dout, dfinal, dq, dk, dv, dg, dbeta, dstate, workspace, st, make_timer());
-  else
-    oal::launch_delta_backward<uint16_t>(a, saved, dout, dfinal, dq, dk, dv, dg, dbeta, dstate, workspace, st,
-                                         make_timer());
+  const auto launch = dtype == OAL_DTYPE_F32    ? oal::launch_delta_backward<float>
+                      : dtype == OAL_DTYPE_BF16 ? oal::launch_delta_backward<uint16_t>
+                                                : oal::launch_delta_backward<_Float16>;
+  launch(a, saved, dout, dfinal, dq, dk, dv, dg, dbeta, dstate, workspace, st, make_timer());
   return launch_status("oal_gated_delta_backward launch");
 }
 
 int oal_gated_delta_step(const void* q, const void* k, const void* v, const float* g, const void* beta,
                          const int64_t* strides, int beta_f32, int batch, int q_heads, int k_heads, int v_heads,
-                         int seq_len, int key_dim, int value_dim, int kind, float scale, float* state, void* out,
+                         int seq_len, int key_dim, int value_dim, int dtype, float scale, float* state, void* out,
                          void* stream) {
   Range range("oal_gated_delta_step");
   if (check_delta(batch, q_heads, k_heads, v_heads, seq_len)) return 1;
   if (key_dim < 1 || key_dim > 64 || value_dim < 1 || value_dim > 64)
     return fail("oal_gated_delta_step: dimensions must be in [1, 64]");
-  if (kind < 0 || kind > 2) return fail("oal_gated_delta_step: unknown type");
+  if (dtype < OAL_DTYPE_F32 || dtype > OAL_DTYPE_F16) return fail("oal_gated_delta_step: unknown type");
   if (!q || !k || !v || !g || !beta || !strides || !state || !out)
     return fail("oal_gated_delta_step: null pointer argument");
   const oal::DeltaStepArgs a = {strided(q, strides), strided(k, strides + 3), strided(v, strides + 6),
                                 strided(g, strides + 9), strided(beta, strides + 12), batch, q_heads, k_heads, v_heads,
                                 q_heads > v_heads ? q_heads : v_heads, seq_len, key_dim, value_dim,
-                                beta_f32 != 0 || kind == 0, scale, state, out};
-  oal::launch_delta_step(kind, a, static_cast<hipStream_t>(stream), make_timer());
+                                beta_f32 != 0 || dtype == OAL_DTYPE_F32, scale, state, out};
+  oal::launch_delta_step(dtype, a, static_cast<hipStream_t>(stream), make_timer());
   return launch_status("oal_gated_delta_step launch");
 }
 
@@ -1598,33 +1609,36 @@ static int check_window(int batch, int q_heads, int kv_heads, int query_len, int
 
 static int window_args(oal::WindowArgs* a, const char* what, const void* q, const void* k, const void* v,
                        const int64_t* strides, int batch, int q_heads, int kv_heads, int query_len, int key_len,
-                       int window, int sinks, int dtype, float scale) {
+                       int key_dim, int value_dim, int window, int sinks, int dtype, float scale) {
   if (check_window(batch, q_heads, kv_heads, query_len, key_len, window, sinks)) return 1;
-  if (dtype != OAL_DTYPE_F32 && dtype != OAL_DTYPE_BF16) return fail("dtype must be OAL_DTYPE_F32 or OAL_DTYPE_BF16");
+  if (!dim_ok(key_dim) || !dim_ok(value_dim))
+    return fail(std::string(what) + ": dimensions must be multiples of 8 up to 64");
+  if (dtype < OAL_DTYPE_F32 || dtype > OAL_DTYPE_F16)
+    return fail("dtype must be OAL_DTYPE_F32, OAL_DTYPE_BF16 or OAL_DTYPE_F16");
   if (!q || !k || !v || !strides) return fail(std::string(what) + ": null pointer argument");
   *a = {strided(q, strides), strided(k, strides + 3), strided(v, strides + 6), batch, q_heads, kv_heads, query_len,
-        key_len, window, sinks, scale};
-  const int bytes = dtype == OAL_DTYPE_F32 ? 4 : 2;
-  if (!rows_aligned(a->q, bytes) || !rows_aligned(a->k, bytes) || !rows_aligned(a->v, bytes))
+        key_len, key_dim, value_dim, window, sinks, scale};
+  if (!rows_aligned(a->q, dtype, batch, q_heads, query_len) || !rows_aligned(a->k, dtype, batch, kv_heads, key_len) ||
+      !rows_aligned(a->v, dtype, batch, kv_heads, key_len))
     return fail(std::string(what) + ": rows must be 16-byte aligned");
   return 0;
 }
 
 int oal_window_attention_forward(const void* q, const void* k, const void* v, const int64_t* strides, int batch,
-                                 int q_heads, int kv_heads, int query_len, int key_len, int window, int sinks,
-                                 int dtype, float scale, void* out, float* lse, void* stream) {
+                                 int q_heads, int kv_heads, int query_len, int key_len, int key_dim,
+                                 int value_dim, int window, int sinks, int dtype, float scale, void* out, float* lse, void* stream) {
   Range range("oal_window_attention_forward");
   oal::WindowArgs a;
   if (window_args(&a, "oal_window_attention_forward", q, k, v, strides, batch, q_heads, kv_heads, query_len, key_len,
-                  window, sinks, dtype, scale))
+                  key_dim, value_dim, window, sinks, dtype, scale))
     return 1;
   if (!out || !lse) return fail("oal_window_attention_forward: null pointer argument");
   if (!aligned16(out)) return fail("oal_window_attention_forward: tensor pointers must be 16-byte aligned");
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (dtype == OAL_DTYPE_F32)
-    oal::launch_window_forward<float>(a, out, lse, st, make_timer());
-  else
-    oal::launch_window_forward<uint16_t>(a, out, lse, st, make_timer());
+  const auto launch = dtype == OAL_DTYPE_F32    ? oal::launch_window_forward<float>
+                      : dtype == OAL_DTYPE_BF16 ? oal::launch_window_forward<uint16_t>
+                                                : oal::launch_window_forward<_Float16>;
+  launch(a, out, lse, st, make_timer());
   return launch_status("oal_window_attention_forward launch");
 }
 
@@ -1634,17 +1648,17 @@ size_t oal_window_attention_workspace_bytes(int batch, int q_heads, int kv_heads
   oal::WindowArgs a{};
   a.B = batch, a.Hq = q_heads, a.Hk = kv_heads, a.Nq = query_len, a.Nk = key_len;
   return oal::window_work_view(nullptr, a, oal::window_plan(batch, q_heads, kv_heads, query_len, key_len, window, sinks,
-                                                            dtype == OAL_DTYPE_F32)).bytes;
+                                                            dtype == OAL_DTYPE_BF16 ? 128 : 64)).bytes;
 }
 
 int oal_window_attention_backward(const void* q, const void* k, const void* v, const int64_t* strides, int batch,
-                                  int q_heads, int kv_heads, int query_len, int key_len, int window, int sinks,
-                                  int dtype, float scale, const void* out, const float* lse, const void* dout,
+                                  int q_heads, int kv_heads, int query_len, int key_len, int key_dim,
+                                  int value_dim, int window, int sinks, int dtype, float scale, const void* out, const float* lse, const void* dout,
                                   void* dq, void* dk, void* dv, void* workspace, void* stream) {
   Range range("oal_window_attention_backward");
   oal::WindowArgs a;
   if (window_args(&a, "oal_window_attention_backward", q, k, v, strides, batch, q_heads, kv_heads, query_len, key_len,
-                  window, sinks, dtype, scale))
+                  key_dim, value_dim, window, sinks, dtype, scale))
     return 1;
   if (!lse) return fail("oal_window_attention_backward: null pointer argument");
   const void* ptrs[] = {out, dout, dq, dk, dv, workspace};
@@ -1653,10 +1667,10 @@ int oal_window_attention_backward(const void* q, const void* k, const void* v, c
     if (!aligned16(p)) return fail("oal_window_attention_backward: tensor pointers must be 16-byte aligned");
   }
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (dtype == OAL_DTYPE_F32)
-    oal::launch_window_backward<float>(a, out, lse, dout, dq, dk, dv, workspace, st, make_timer());
-  else
-    oal::launch_window_backward<uint16_t>(a, out, lse, dout, dq, dk, dv, workspace, st, make_timer());
+  const auto launch = dtype == OAL_DTYPE_F32    ? oal::launch_window_backward<float>
+                      : dtype == OAL_DTYPE_BF16 ? oal::launch_window_backward<uint16_t>
+                                                : oal::launch_window_backward<_Float16>;
+  launch(a, out, lse, dout, dq, dk, dv, workspace, st, make_timer());
   return launch_status("oal_window_attention_backward launch");
 }
 
@@ -1665,7 +1679,7 @@ static int check_window_step(int batch, int q_heads, int kv_heads, int value_dim
   if (q_heads % kv_heads != 0) return fail("query head count must be divisible by KV head count");
   if (window < 1 || sinks < 0) return fail("window must be positive and sinks not negative");
   if (int64_t(sinks) + window > (1 << 30)) return fail("the cache has too many slots");
-  if (value_dim < 8 || value_dim > 64 || value_dim % 8)
+  if (!dim_ok(value_dim))
     return fail("oal_window_attention_step: dimensions must be multiples of 8 up to 64");
   // at most 512 blocks more than there are head groups
   if (int64_t(batch) > (int64_t(1) << 23) / q_heads) return fail("batch and heads are too large for one launch");
@@ -1682,23 +1696,25 @@ size_t oal_window_attention_step_workspace_bytes(int batch, int q_heads, int kv_
 
 int oal_window_attention_step(const void* q, const void* k, const void* v, void* k_cache, void* v_cache,
                               const int64_t* strides, const int64_t* position, int batch, int q_heads, int kv_heads,
-                              int key_dim, int value_dim, int window, int sinks, int kind, float scale, void* out,
+                              int key_dim, int value_dim, int window, int sinks, int dtype, float scale, void* out,
                               void* workspace, void* stream) {
   Range range("oal_window_attention_step");
   if (check_window_step(batch, q_heads, kv_heads, value_dim, window, sinks)) return 1;
-  if (key_dim < 8 || key_dim > 64 || key_dim % 8)
+  if (!dim_ok(key_dim))
     return fail("oal_window_attention_step: dimensions must be multiples of 8 up to 64");
-  if (kind < 0 || kind > 2) return fail("oal_window_attention_step: unknown type");
+  if (dtype < OAL_DTYPE_F32 || dtype > OAL_DTYPE_F16) return fail("oal_window_attention_step: unknown type");
   if (!q || !k || !v || !k_cache || !v_cache || !strides || !position || !out || !workspace)
     return fail("oal_window_attention_step: null pointer argument");
   oal::WindowStepArgs a = {strided(q, strides), strided(k, strides + 3), strided(v, strides + 6),
                            strided(k_cache, strides + 9), strided(v_cache, strides + 12), position, batch, q_heads,
                            kv_heads, key_dim, value_dim, window, sinks, 1, 0, scale, out, static_cast<float*>(workspace)};
-  const int bytes = kind == 0 ? 4 : 2;
-  for (const oal::Strided* s : {&a.q, &a.k, &a.v, &a.kc, &a.vc})
-    if (!rows_aligned(*s, bytes)) return fail("oal_window_attention_step: rows must be 16-byte aligned");
-  oal::window_step_plan(batch, q_heads, kv_heads, int64_t(sinks) + window, &a.splits, &a.span);
-  oal::launch_window_step(kind, a, static_cast<hipStream_t>(stream), make_timer());
+  const int64_t slots = int64_t(sinks) + window;
+  if (!rows_aligned(a.q, dtype, batch, q_heads, 1) || !rows_aligned(a.k, dtype, batch, kv_heads, 1) ||
+      !rows_aligned(a.v, dtype, batch, kv_heads, 1) || !rows_aligned(a.kc, dtype, batch, kv_heads, slots) ||
+      !rows_aligned(a.vc, dtype, batch, kv_heads, slots))
+    return fail("oal_window_attention_step: rows must be 16-byte aligned");
+  oal::window_step_plan(batch, q_heads, kv_heads, slots, &a.splits, &a.span);
+  oal::launch_window_step(dtype, a, static_cast<hipStream_t>(stream), make_timer());
   return launch_status("oal_window_attention_step launch");
 }
 

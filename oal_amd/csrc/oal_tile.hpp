@@ -1,11 +1,11 @@
-// Products of 64 x 64 tiles on the matrix cores whose operands are one or three
+// Products of 64 x 64 tiles on the matrix cores whose operands are one to three
 // bf16 parts, for the chunked and the windowed attention kernels on gfx950.
 //
 // A value in three bf16 parts (the value rounded, what that left, what that
 // left) carries 24 bits, so products of such parts that leave out only the terms below
 // 2^-24 are as exact as fp32, at 3 (one operand a bf16 value as it is) or 6 matrix
 // instructions in place of the 16 times slower fp32 ones. bf16 tensors enter as
-// one part, fp32 tensors and intermediate results that have to stay fp32 as three.
+// one part, fp16 tensors as two, fp32 tensors and intermediate results that have to stay fp32 as three.
 //
 // An accumulator tile of v_mfma_f32_16x16x32_bf16 holds rows 4 g + i in lane group
 // g = lane / 16, and an operand's lane group g holds 8 of the 32 indexes that the
@@ -16,6 +16,8 @@
 // and the other operand is read from LDS in that order: chains of products
 // pass through registers. "perm" marks that order below.
 #pragma once
+
+#include <type_traits>
 
 #include "oal_mfma_common.hpp"
 
@@ -29,11 +31,9 @@ struct Frag {
   bf16x8 p[NP];
 };
 
-// Parts per value of an element type.
+// Exact parts per value of an element type: 24, 8 and 11 bits.
 template <typename T>
-constexpr int kPartsOf = sizeof(T) == 4 ? 3 : 1;
-
-__device__ __forceinline__ float bf16_part(float x) { return static_cast<float>(static_cast<__bf16>(x)); }
+inline constexpr int kPartsOf = std::is_same_v<T, float> ? 3 : std::is_same_v<T, _Float16> ? 2 : 1;
 
 template <int NP>
 __device__ __forceinline__ Frag<NP> split(const float (&v)[8]) {
@@ -71,8 +71,6 @@ template <int NP>
 struct alignas(16) Tile {
   __bf16 x[NP * kTileElems];
 };
-
-typedef __bf16 lds_bf16x4 __attribute__((ext_vector_type(4)));
 
 // Operand row r0 + lane % 16, sum indexes 32 t + 8 g + j; its first N parts (0: all).
 template <int N = 0, int NP>
@@ -134,18 +132,53 @@ __device__ __forceinline__ Frag<NP> acc_frag(const f32x4& lo, const f32x4& hi) {
   return split<NP>(v);
 }
 
-// 8 consecutive values of a row in global memory as floats.
+// 8 consecutive values of a row as floats, 16-byte aligned.
 __device__ __forceinline__ void load_row8(float (&x)[8], const float* p) {
   const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
   x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
 }
+__device__ __forceinline__ void load_row8(float (&x)[8], const uint16_t* p) {
+  const bf16x8 v = *reinterpret_cast<const bf16x8*>(p);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = static_cast<float>(v[e]);
+}
+__device__ __forceinline__ void load_row8(float (&x)[8], const _Float16* p) {
+  typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+  const f16x8 v = *reinterpret_cast<const f16x8*>(p);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = static_cast<float>(v[e]);
+}
+
+// Four consecutive values of a row, aligned to their size.
+__device__ __forceinline__ f32x4 load4(const float* p) { return *reinterpret_cast<const f32x4*>(p); }
+__device__ __forceinline__ f32x4 load4(const uint16_t* p) {
+  const bf16x4 v = *reinterpret_cast<const bf16x4*>(p);
+  return __builtin_convertvector(v, f32x4);
+}
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ f32x4 load4(const _Float16* p) {
+  return __builtin_convertvector(*reinterpret_cast<const f16x4*>(p), f32x4);
+}
+__device__ __forceinline__ void store4(float* p, const f32x4& x) { *reinterpret_cast<f32x4*>(p) = x; }
+__device__ __forceinline__ void store4(uint16_t* p, const f32x4& x) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]));
+}
+__device__ __forceinline__ void store4(_Float16* p, const f32x4& x) {
+  *reinterpret_cast<f16x4*>(p) = __builtin_convertvector(x, f16x4);
+}
+__device__ __forceinline__ float get(const float* p) { return *p; }
+__device__ __forceinline__ float get(const uint16_t* p) { return to_f(*p); }
+__device__ __forceinline__ float get(const _Float16* p) { return static_cast<float>(*p); }
+__device__ __forceinline__ void put(float* p, float x) { *p = x; }
+__device__ __forceinline__ void put(uint16_t* p, float x) { *p = from_f<uint16_t>(x); }
+__device__ __forceinline__ void put(_Float16* p, float x) { *p = static_cast<_Float16>(x); }
 
 // Operand row straight from global memory: 8 values at p (not read unless live: zero then).
 template <int NP, typename T>
 __device__ __forceinline__ Frag<NP> global_frag(const T* p, bool live) {
   Frag<NP> f;
-  if constexpr (sizeof(T) == 2) {
-    static_assert(NP == 1, "a bf16 value is one part");
+  if constexpr (NP == 1) {
+    static_assert(std::is_same_v<T, uint16_t>, "a bf16 value is one part");
     uint4 v = make_uint4(0, 0, 0, 0);
     if (live) v = *reinterpret_cast<const uint4*>(p);
     f.p[0] = __builtin_bit_cast(bf16x8, v);
@@ -157,35 +190,32 @@ __device__ __forceinline__ Frag<NP> global_frag(const T* p, bool live) {
   return f;
 }
 
-// ROWS rows of 64 values (row stride in elements) into rows 0 .. of an LDS tile,
-// NT threads; rows at and past `live` are zero. 16-byte aligned rows.
+// ROWS rows of D values, a multiple of 8 up to 64 (row stride in elements), into rows
+// 0 .. of an LDS tile, NT threads; rows at and past `live` and columns from D are zero. 16-byte aligned rows.
 template <int ROWS, int NT, int NP, typename T>
-__device__ __forceinline__ void load_tile(Tile<NP>& s, const T* __restrict__ src, int64_t stride, int live, int t) {
-  if constexpr (sizeof(T) == 2) {
-    static_assert(NP == 1, "a bf16 value is one part");
-    constexpr int kIt = (ROWS * 8 + NT - 1) / NT;
-    uint4 v[kIt];
+__device__ __forceinline__ void load_tile(Tile<NP>& s, const T* __restrict__ src, int64_t stride, int D, int live, int t) {
+  constexpr int kIt = (ROWS * 8 + NT - 1) / NT;
+  if constexpr (NP == 1) {
+    // every load before the first store
+    Frag<1> f[kIt];
 #pragma unroll
     for (int x = 0; x < kIt; ++x) {
-      const int i = t + NT * x, r = i >> 3;
-      v[x] = make_uint4(0, 0, 0, 0);
-      if (r < live && i < ROWS * 8) v[x] = *reinterpret_cast<const uint4*>(src + r * stride + 8 * (i & 7));
+      const int i = t + NT * x, r = i >> 3, c = 8 * (i & 7);
+      f[x] = global_frag<1>(src + r * stride + c, r < live && c < D && i < ROWS * 8);
     }
 #pragma unroll
     for (int x = 0; x < kIt; ++x) {
       const int i = t + NT * x;
-      if (i < ROWS * 8) *reinterpret_cast<uint4*>(s.x + (i >> 3) * kTileRow + 8 * (i & 7)) = v[x];
+      if (i < ROWS * 8) *reinterpret_cast<bf16x8*>(s.x + (i >> 3) * kTileRow + 8 * (i & 7)) = f[x].p[0];
     }
   } else {
-    constexpr int kIt = (ROWS * 8 + NT - 1) / NT;
 #pragma unroll
     for (int x = 0; x < kIt; ++x) {
-      const int i = t + NT * x, r = i >> 3;
+      const int i = t + NT * x, r = i >> 3, c = 8 * (i & 7);
       if (i < ROWS * 8) {
-        const Frag<NP> f = global_frag<NP>(src + r * stride + 8 * (i & 7), r < live);
+        const Frag<NP> f = global_frag<NP>(src + r * stride + c, r < live && c < D);
 #pragma unroll
-        for (int e = 0; e < NP; ++e)
-          *reinterpret_cast<bf16x8*>(s.x + e * kTileElems + r * kTileRow + 8 * (i & 7)) = f.p[e];
+        for (int e = 0; e < NP; ++e) *reinterpret_cast<bf16x8*>(s.x + e * kTileElems + r * kTileRow + c) = f.p[e];
       }
     }
   }

@@ -31,15 +31,10 @@ __device__ __forceinline__ const T* rows_at(const Strided& s, int b, int h, int6
   return static_cast<const T*>(s.p) + b * s.b + h * s.h + row * s.n;
 }
 
-__device__ __forceinline__ void store4(float* p, const f32x4& x) { *reinterpret_cast<f32x4*>(p) = x; }
-__device__ __forceinline__ void store4(uint16_t* p, const f32x4& x) {
-  *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]));
-}
-
-// Columns per wave: two tiles of 16 share each operand read from LDS; with three parts
+// Columns per wave: two tiles of 16 share each operand read from LDS; with several parts
 // per value the registers hold one.
 template <typename T>
-constexpr int kColTiles = sizeof(T) == 4 ? 1 : 2;
+constexpr int kColTiles = kPartsOf<T> > 1 ? 1 : 2;
 template <typename T>
 constexpr int kCols = 16 * kColTiles<T>;
 
@@ -104,7 +99,7 @@ __global__ __launch_bounds__(512) void k_window_fwd(WindowArgs a, Shape sh, int 
     for (int s = 0; s < 2; ++s) {
       const int row = q0 + 16 * x + c;
       const bool live = row < a.Nq;
-      qf[x][s] = global_frag<NP>(rows_at<T>(a.q, b, h, live ? row : 0) + 32 * s + 8 * g, live);
+      qf[x][s] = global_frag<NP>(rows_at<T>(a.q, b, h, live ? row : 0) + 32 * s + 8 * g, live && 32 * s + 8 * g < a.D);
     }
   f32x4 acc[CT][4] = {};
   float top[CT], sum[CT];
@@ -118,8 +113,8 @@ __global__ __launch_bounds__(512) void k_window_fwd(WindowArgs a, Shape sh, int 
     __syncthreads();
     const int live = min(64, a.Nk - j0);
     if (t < 256) {
-      load_tile<64, 256>(K, rows_at<T>(a.k, b, hk, j0), a.k.n, live, t);
-      load_tile<64, 256>(V, rows_at<T>(a.v, b, hk, j0), a.v.n, live, t);
+      load_tile<64, 256>(K, rows_at<T>(a.k, b, hk, j0), a.k.n, a.D, live, t);
+      load_tile<64, 256>(V, rows_at<T>(a.v, b, hk, j0), a.v.n, a.DV, live, t);
     }
     __syncthreads();
     if (!works || !sees_any(a, far, i0, i1, j0)) continue;
@@ -184,7 +179,8 @@ __global__ __launch_bounds__(512) void k_window_fwd(WindowArgs a, Shape sh, int 
     if (row >= a.Nq) continue;
     const size_t at = ((size_t)b * a.Hq + h) * a.Nq + row;
 #pragma unroll
-    for (int m = 0; m < 4; ++m) store4(out + at * 64 + 16 * m + 4 * g, acc[x][m] * inv);
+    for (int m = 0; m < 4; ++m)
+      if (16 * m + 4 * g < a.DV) store4(out + at * a.DV + 16 * m + 4 * g, acc[x][m] * inv);
     if (g == 0) lse[at] = top[x] + __builtin_amdgcn_logf(all);
   }
 }
@@ -221,18 +217,13 @@ __global__ __launch_bounds__(512) void k_window_dq(WindowArgs a, Shape sh, int q
     float y = 0.f;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      qf[x][s] = global_frag<NP>(rows_at<T>(a.q, b, h, live ? row : 0) + 32 * s + 8 * g, live);
-      of[x][s] = global_frag<NP>(dout + at * 64 + 32 * s + 8 * g, live);
+      const int col = 32 * s + 8 * g;
+      qf[x][s] = global_frag<NP>(rows_at<T>(a.q, b, h, live ? row : 0) + col, live && col < a.D);
+      of[x][s] = global_frag<NP>(dout + at * a.DV + col, live && col < a.DV);
       float o[8] = {}, d[8] = {};
-      if (live) {
-        if constexpr (NP == 3) {
-          load_row8(o, out + at * 64 + 32 * s + 8 * g);
-          load_row8(d, dout + at * 64 + 32 * s + 8 * g);
-        } else {
-          const Frag<1> f = global_frag<1>(out + at * 64 + 32 * s + 8 * g, true);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) o[e] = static_cast<float>(f.p[0][e]), d[e] = static_cast<float>(of[x][s].p[0][e]);
-        }
+      if (live && col < a.DV) {
+        load_row8(o, out + at * a.DV + col);
+        load_row8(d, dout + at * a.DV + col);
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) y += o[e] * d[e];
@@ -250,8 +241,8 @@ __global__ __launch_bounds__(512) void k_window_dq(WindowArgs a, Shape sh, int q
     __syncthreads();
     const int live = min(64, a.Nk - j0);
     if (t < 256) {
-      load_tile<64, 256>(K, rows_at<T>(a.k, b, hk, j0), a.k.n, live, t);
-      load_tile<64, 256>(V, rows_at<T>(a.v, b, hk, j0), a.v.n, live, t);
+      load_tile<64, 256>(K, rows_at<T>(a.k, b, hk, j0), a.k.n, a.D, live, t);
+      load_tile<64, 256>(V, rows_at<T>(a.v, b, hk, j0), a.v.n, a.DV, live, t);
     }
     __syncthreads();
     if (!works || !sees_any(a, far, i0, i1, j0)) continue;
@@ -302,7 +293,8 @@ __global__ __launch_bounds__(512) void k_window_dq(WindowArgs a, Shape sh, int q
     if (row >= a.Nq) continue;
     const size_t at = ((size_t)b * a.Hq + h) * a.Nq + row;
 #pragma unroll
-    for (int m = 0; m < 4; ++m) store4(dq + at * 64 + 16 * m + 4 * g, acc[x][m] * a.scale);
+    for (int m = 0; m < 4; ++m)
+      if (16 * m + 4 * g < a.D) store4(dq + at * a.D + 16 * m + 4 * g, acc[x][m] * a.scale);
   }
 }
 
@@ -343,8 +335,9 @@ __global__ __launch_bounds__(256) void k_window_dkv(WindowArgs a, WindowPlan pla
     for (int s = 0; s < 2; ++s) {
       const int row = j0 + 16 * x + c;
       const bool live = row < rows;
-      kf[x][s] = global_frag<NP>(rows_at<T>(a.k, b, hk, live ? row : 0) + 32 * s + 8 * g, live);
-      vf[x][s] = global_frag<NP>(rows_at<T>(a.v, b, hk, live ? row : 0) + 32 * s + 8 * g, live);
+      const int col = 32 * s + 8 * g;
+      kf[x][s] = global_frag<NP>(rows_at<T>(a.k, b, hk, live ? row : 0) + col, live && col < a.D);
+      vf[x][s] = global_frag<NP>(rows_at<T>(a.v, b, hk, live ? row : 0) + col, live && col < a.DV);
     }
   f32x4 dk[CT][4] = {}, dv[CT][4] = {};
   const float scale = a.scale * kLog2e;
@@ -353,8 +346,8 @@ __global__ __launch_bounds__(256) void k_window_dkv(WindowArgs a, WindowPlan pla
     const int live = min(64, a.Nk - i0);
     const size_t at = ((size_t)b * a.Hq + h) * a.Nq + (i0 - off);
     __syncthreads();
-    load_tile<64, 256>(Q, rows_at<T>(a.q, b, h, i0 - off), a.q.n, live, t);
-    load_tile<64, 256>(O, dout + at * 64, (int64_t)64, live, t);
+    load_tile<64, 256>(Q, rows_at<T>(a.q, b, h, i0 - off), a.q.n, a.D, live, t);
+    load_tile<64, 256>(O, dout + at * a.DV, (int64_t)a.DV, a.DV, live, t);
     if (t < 64) {
       base[t] = t < live ? lse[at + t] : 0.f;
       dot[t] = t < live ? delta[at + t] : 0.f;
@@ -430,7 +423,7 @@ __global__ __launch_bounds__(256) void k_window_dkv(WindowArgs a, WindowPlan pla
   }
 }
 
-// The parts' sums, in order: dk and dv [B][Hk][Nk][64].
+// The parts' sums, in order: dk [B][Hk][Nk][D] and dv [B][Hk][Nk][DV].
 template <typename T>
 __global__ __launch_bounds__(256) void k_window_sum(WindowArgs a, WindowPlan plan, const float* __restrict__ part,
                                                     const float* __restrict__ farpart, T* __restrict__ dk,
@@ -447,7 +440,8 @@ __global__ __launch_bounds__(256) void k_window_sum(WindowArgs a, WindowPlan pla
   if (in < rows)
     for (int p = 0; p < plan.chunks; ++p)
       s += *reinterpret_cast<const f32x4*>(farpart + ((v ? plan.chunks : 0) + p) * far + bh * rows + in);
-  store4((v ? dv : dk) + y, s);
+  const int col = (int)(y & 63), width = v ? a.DV : a.D;
+  if (col < width) store4((v ? dv : dk) + (y >> 6) * width + col, s);
 }
 
 // ---------------------------------------------------------------------------
@@ -456,13 +450,6 @@ __global__ __launch_bounds__(256) void k_window_sum(WindowArgs a, WindowPlan pla
 // columns are query heads of one KV head. The slot's row comes from the token itself.
 // ---------------------------------------------------------------------------
 namespace {
-
-template <typename T>
-constexpr int kStepParts = 1;  // exact parts of a value: 8, 11, 24 bits
-template <>
-constexpr int kStepParts<_Float16> = 2;
-template <>
-constexpr int kStepParts<float> = 3;
 
 template <typename T>
 struct alignas(16) Row8 {
@@ -475,7 +462,7 @@ __device__ __forceinline__ Row8<T> row8(const T* p, int d, int D, bool live) {
   if (live && d < D) r = *reinterpret_cast<const Row8<T>*>(p + d);
   return r;
 }
-template <typename T, int NP = kStepParts<T>>
+template <typename T, int NP = kPartsOf<T>>
 __device__ __forceinline__ Frag<NP> frag_of(const Row8<T>& r) {
   if constexpr (sizeof(T) == 2 && NP == 1) {
     return Frag<1>{{__builtin_bit_cast(bf16x8, r)}};
@@ -487,15 +474,11 @@ __device__ __forceinline__ Frag<NP> frag_of(const Row8<T>& r) {
   }
 }
 
-__device__ __forceinline__ void put(float* p, float x) { *p = x; }
-__device__ __forceinline__ void put(uint16_t* p, float x) { *p = from_f<uint16_t>(x); }
-__device__ __forceinline__ void put(_Float16* p, float x) { *p = static_cast<_Float16>(x); }
-
 }  // namespace
 
 template <typename T>
 __global__ __launch_bounds__(256) void k_window_step(WindowStepArgs a) {
-  constexpr int NP = kStepParts<T>;
+  constexpr int NP = kPartsOf<T>;
   // 32 rows of V per wave; after the walk the waves' sums
   struct alignas(16) Rows {
     __bf16 x[NP * 32 * kTileRow];
@@ -642,9 +625,9 @@ __global__ __launch_bounds__(64) void k_window_step_join(WindowStepArgs a) {
 // ---------------------------------------------------------------------------
 // Launches
 // ---------------------------------------------------------------------------
-WindowPlan window_plan(int B, int Hq, int Hk, int Nq, int Nk, int window, int sinks, bool f32) {
+WindowPlan window_plan(int B, int Hq, int Hk, int Nq, int Nk, int window, int sinks, int keys) {
   WindowPlan p;
-  const int keys = f32 ? 64 : 128, R = Hq / Hk;
+  const int R = Hq / Hk;
   const int64_t blocks = (int64_t)B * Hk * ((Nk + keys - 1) / keys);
   // parts until every CU has a few blocks
   p.splits = (int)std::clamp<int64_t>((768 + blocks - 1) / blocks, 1, R);
@@ -688,7 +671,7 @@ void launch_window_backward(const WindowArgs& a, const void* out, const float* l
   const Shape sh = block_shape(a.Hq / a.Hk);
   const int qblocks = (a.Nq + sh.subs * kCols<T> - 1) / (sh.subs * kCols<T>);
   const int waves = std::max(4, sh.heads * sh.subs);
-  const WindowPlan plan = window_plan(a.B, a.Hq, a.Hk, a.Nq, a.Nk, a.window, a.sinks, sizeof(T) == 4);
+  const WindowPlan plan = window_plan(a.B, a.Hq, a.Hk, a.Nq, a.Nk, a.window, a.sinks, 4 * kCols<T>);
   const WindowWork w = window_work_view(work, a, plan);
   timed("k_window_dq", st, [&] {
     hipLaunchKernelGGL(k_window_dq<T>, dim3((unsigned)((int64_t)a.B * a.Hk * sh.groups * qblocks)), dim3(64 * waves), 0,
@@ -708,12 +691,14 @@ void launch_window_backward(const WindowArgs& a, const void* out, const float* l
   });
 }
 
-template void launch_window_forward<float>(const WindowArgs&, void*, float*, hipStream_t, const Timer&);
-template void launch_window_forward<uint16_t>(const WindowArgs&, void*, float*, hipStream_t, const Timer&);
-template void launch_window_backward<float>(const WindowArgs&, const void*, const float*, const void*, void*, void*,
-                                            void*, void*, hipStream_t, const Timer&);
-template void launch_window_backward<uint16_t>(const WindowArgs&, const void*, const float*, const void*, void*, void*,
-                                               void*, void*, hipStream_t, const Timer&);
+#define OAL_WINDOW(T)                                                                                              \
+  template void launch_window_forward<T>(const WindowArgs&, void*, float*, hipStream_t, const Timer&);             \
+  template void launch_window_backward<T>(const WindowArgs&, const void*, const float*, const void*, void*, void*, \
+                                          void*, void*, hipStream_t, const Timer&);
+OAL_WINDOW(float)
+OAL_WINDOW(uint16_t)
+OAL_WINDOW(_Float16)
+#undef OAL_WINDOW
 
 void window_step_plan(int B, int Hq, int Hk, int64_t slots, int* splits, int* span) {
   // blocks of 128 slots and more, until every CU has two

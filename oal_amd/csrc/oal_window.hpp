@@ -11,17 +11,18 @@ namespace oal {
 // Query i of Nq has position off + i, off = Nk - Nq; it sees keys j <= off + i with
 // off + i - j < window or j < sinks.
 struct WindowArgs {
-  Strided q, k, v;  // rows of 64 values
-  int B, Hq, Hk, Nq, Nk, window, sinks;
+  Strided q, k, v;  // rows of D, D and DV values
+  int B, Hq, Hk, Nq, Nk, D, DV, window, sinks;
   float scale;
 };
 
-// How the key side of the backward is cut: `splits` parts of each 128 keys' steps (a
+// How the key side of the backward is cut: `splits` parts of each block of keys' steps (a
 // step: one query head and 64 queries), `chunks` of the steps over which the first keys are seen from afar.
 struct WindowPlan {
   int splits, chunks, sink_rows, sink_blocks;
 };
-WindowPlan window_plan(int B, int Hq, int Hk, int Nq, int Nk, int window, int sinks, bool f32);
+// keys: of a block, 128 for bf16 and 64 for the other types
+WindowPlan window_plan(int B, int Hq, int Hk, int Nq, int Nk, int window, int sinks, int keys);
 
 struct WindowWork {
   float* delta;   // [B][Hq][Nq] sum of dout * out

@@ -18,9 +18,8 @@ divides the other; the output has H = max(Hq, Hv) heads, of which head o reads w
 query head o // (H / Hq) from state head o // (H / Hv).
 
 The rule is a stable memory for keys of length one (normalise them before the call)
-and beta up to 2. The arithmetic does not depend on the type of q, k and v where sums over tokens are
-concerned: states, decays and their gradients are exact to float32 in both.
-float16 tensors run the float32 kernels. A token with beta = 0 and g = 0 leaves the
+and beta up to 2. Sums over tokens do not depend on the type of q, k and v, which may be
+float32, bfloat16 or float16: states, decays and their gradients are exact to float32. A token with beta = 0 and g = 0 leaves the
 state as it is: pad batches of ragged lengths with such tokens. Values have to be
 finite: a token that is not spoils the 64 tokens of its chunk.
 """
@@ -33,7 +32,6 @@ from typing import Any, Optional
 import torch
 
 from . import _native
-from .hd_block_gemm_autograd import _kernel_dtype, _pad_last
 
 HEAD_DIM = _native.HEAD_DIM
 _FLOATS = (torch.float16, torch.bfloat16, torch.float32)
@@ -49,7 +47,26 @@ def _validate_scale(scale, dim: int) -> float:
     return float(scale)
 
 
-def _validate(q, k, v, g, beta, state, name: str):
+def _plain(q, k, v, g, beta, state) -> bool:
+    """Whether the operands are as they should be, in one look: it is asked in every call."""
+    try:
+        (b, hq, n, d), (_, hv, _, dv), hk, dev = q.shape, v.shape, k.shape[1], q.device
+        return (
+            q.dtype in _FLOATS and k.dtype is v.dtype is q.dtype and g.dtype is torch.float32
+            and (beta.dtype is q.dtype or beta.dtype is torch.float32)
+            and k.device == dev and v.device == dev and g.device == dev and beta.device == dev
+            and k.shape == (b, hk, n, d) and v.shape == (b, hv, n, dv) and g.shape == beta.shape == (b, hv, n)
+            and b > 0 and hq > 0 and hk > 0 and hv > 0 and n > 0 and 0 < d <= HEAD_DIM and 0 < dv <= HEAD_DIM
+            and hv % hk == 0 and (hq % hv == 0 or hv % hq == 0)
+            and (state is None or (state.dtype is torch.float32 and state.shape == (b, hv, d, dv) and state.device == dev))
+        )
+    except (AttributeError, ValueError, IndexError):
+        return False
+
+
+def _validate(q, k, v, g, beta, state, name: str) -> None:
+    if _plain(q, k, v, g, beta, state):
+        return
     if not all(isinstance(t, torch.Tensor) for t in (q, k, v, g, beta)):
         raise TypeError("q, k, v, g and beta must be torch.Tensor objects")
     if q.ndim != 4 or k.ndim != 4 or v.ndim != 4:
@@ -92,19 +109,17 @@ def _validate(q, k, v, g, beta, state, name: str):
 
 
 class _GatedDeltaFunction(torch.autograd.Function):
-    """(q, k, v, g, beta, state or None, scale) -> (out, final state); q, k, v
-    [B, H, N, 64] float32 or bfloat16, beta float32 or q's dtype, on one ROCm device."""
+    """(q, k, v, g, beta, state or None, scale) -> (out, final state); dimensions multiples of 8, on one ROCm device."""
 
     @staticmethod
     def forward(ctx: Any, q, k, v, g, beta, state, scale: float):
-        q, k, v = (_native.row_tensor(t.detach()) for t in (q, k, v))
-        g, beta = g.detach(), beta.detach()
-        start = None if state is None else _native._aligned(state.detach().contiguous())
+        q, k, v = map(_native.row_tensor, (q, k, v))
+        start = None if state is None else _native._aligned(state.contiguous())
         keep = any(ctx.needs_input_grad)
         out, final, saved = _native.delta_forward(q, k, v, g, beta, start, scale=scale, keep=keep)
         if keep:
             ctx.save_for_backward(q, k, v, g, beta, saved)
-        ctx.scale = scale
+            ctx.scale = scale
         return out, final
 
     @staticmethod
@@ -116,6 +131,11 @@ class _GatedDeltaFunction(torch.autograd.Function):
         grads = _native.delta_backward(q, k, v, g, beta, saved, dout, dfinal, scale=ctx.scale,
                                        need_state=ctx.needs_input_grad[5])
         return (*(d if need else None for d, need in zip(grads, ctx.needs_input_grad)), None)
+
+
+def _pad8(x: torch.Tensor) -> torch.Tensor:
+    """x with its last dimension at the next multiple of 8, zeros behind."""
+    return torch.nn.functional.pad(x, (0, -x.shape[-1] % 8))
 
 
 def gated_delta_attention(
@@ -133,14 +153,13 @@ def gated_delta_attention(
     d, dv = q.shape[3], v.shape[3]
     scale = _validate_scale(scale, d)
     _native._require_device(q)
-    kd = _kernel_dtype(q.dtype)
-    wide = kd == torch.float32
-    qp, kp, vp = (t.to(kd) if t.shape[3] == HEAD_DIM else _pad_last(t.to(kd)) for t in (q, k, v))
+    if d % 8 == 0 and dv % 8 == 0:
+        return _GatedDeltaFunction.apply(q, k, v, g, beta, initial_state, scale)
     state = initial_state
-    if state is not None and (d, dv) != (HEAD_DIM, HEAD_DIM):
-        state = torch.nn.functional.pad(state, (0, HEAD_DIM - dv, 0, HEAD_DIM - d))
-    out, final = _GatedDeltaFunction.apply(qp, kp, vp, g, beta.float() if wide else beta, state, scale)
-    return out[..., :dv].to(q.dtype), final[..., :d, :dv]
+    if state is not None:
+        state = torch.nn.functional.pad(state, (0, -dv % 8, 0, -d % 8))
+    out, final = _GatedDeltaFunction.apply(_pad8(q), _pad8(k), _pad8(v), g, beta, state, scale)
+    return out[..., :dv], final[..., :d, :dv]
 
 
 def gated_delta_step(
@@ -163,7 +182,7 @@ def gated_delta_step(
     scale = _validate_scale(scale, q.shape[3])
     _native._require_device(q)
     q, k, v = (t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous() for t in (q, k, v))
-    out = _native.delta_step(q.detach(), k.detach(), v.detach(), g.detach(), beta.detach(), state, scale=scale)
+    out = _native.delta_step(q, k, v, g, beta, state, scale=scale)
     torch.autograd.graph.increment_version(state)
     return out
 

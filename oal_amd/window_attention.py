@@ -16,8 +16,8 @@ else in slot sinks + (p - sinks) % window: the filled slots are just what the to
 the caches never grow and nothing is masked.
 
 bfloat16 tensors run on the matrix cores as they are, with the softmax in
-float32; float32 tensors are exact to float32 (three bfloat16 parts per value); float16
-tensors run the float32 kernels in window_attention and their own in window_attention_step.
+float32; float32 and float16 tensors in three and two exact bfloat16 parts per value, so that
+results are exact to their type.
 Padding at the end of a sequence changes nothing before it; its values have to be finite
 all the same, in k, v and the gradients (a masked weight of zero times infinity is not zero).
 """
@@ -29,8 +29,7 @@ from typing import Any, Optional
 import torch
 
 from . import _native
-from .gated_delta import _FLOATS, _validate_scale
-from .hd_block_gemm_autograd import _kernel_dtype, _pad_last
+from .gated_delta import _FLOATS, _pad8, _validate_scale
 
 HEAD_DIM = _native.HEAD_DIM
 _MOST = 1 << 30
@@ -45,6 +44,14 @@ def _validate_window(window, sinks) -> None:
 
 
 def _validate(q, k, v) -> None:
+    try:  # as they should be, in one look: it is asked in every call
+        (b, hq, nq, d), (_, hk, nk, dv), dev = q.shape, v.shape, q.device
+        if (q.dtype in _FLOATS and k.dtype is v.dtype is q.dtype and k.device == dev and v.device == dev
+                and k.shape == (b, hk, nk, d) and v.shape[0] == b and b > 0 and hq > 0 and hk > 0 and nq > 0 and nk > 0
+                and 0 < d <= HEAD_DIM and 0 < dv <= HEAD_DIM and hq % hk == 0):
+            return
+    except (AttributeError, ValueError, IndexError):
+        pass
     if not all(isinstance(t, torch.Tensor) for t in (q, k, v)):
         raise TypeError("q, k and v must be torch.Tensor objects")
     if q.ndim != 4 or k.ndim != 4 or v.ndim != 4:
@@ -68,12 +75,12 @@ def _validate(q, k, v) -> None:
 
 
 class _WindowFunction(torch.autograd.Function):
-    """(q, k, v, window, sinks, scale) -> out; q, k, v [B, H, N, 64] float32 or bfloat16 on one ROCm device."""
+    """(q, k, v, window, sinks, scale) -> out; dimensions multiples of 8, on one ROCm device."""
 
     @staticmethod
     def forward(ctx: Any, q, k, v, window: int, sinks: int, scale: float):
         ctx.set_materialize_grads(False)
-        q, k, v = (_native.row_tensor(t.detach()) for t in (q, k, v))
+        q, k, v = map(_native.row_tensor, (q, k, v))
         out, lse = _native.window_forward(q, k, v, window=window, sinks=sinks, scale=scale)
         ctx.save_for_backward(q, k, v, out, lse)
         ctx.options = dict(window=window, sinks=sinks, scale=scale)
@@ -104,13 +111,12 @@ def window_attention(
     _validate_window(window, sinks)
     if q.shape[2] > k.shape[2]:
         raise ValueError("there must be a key for every query")
-    dv = v.shape[3]
-    scale = _validate_scale(scale, q.shape[3])
+    d, dv = q.shape[3], v.shape[3]
+    scale = _validate_scale(scale, d)
     _native._require_device(q)
-    kd = _kernel_dtype(q.dtype)
-    qp, kp, vp = (t.to(kd) if t.shape[3] == HEAD_DIM else _pad_last(t.to(kd)) for t in (q, k, v))
-    out = _WindowFunction.apply(qp, kp, vp, window, sinks, scale)
-    return out[..., :dv].to(q.dtype)
+    if d % 8 == 0 and dv % 8 == 0:
+        return _WindowFunction.apply(q, k, v, window, sinks, scale)
+    return _WindowFunction.apply(_pad8(q), _pad8(k), _pad8(v), window, sinks, scale)[..., :dv]
 
 
 def window_cache(
@@ -166,6 +172,9 @@ def window_attention_step(
     if size > _MOST:
         raise ValueError(f"the cache must have at most {_MOST} slots")
     for name, t, width in (("k_cache", k_cache, d), ("v_cache", v_cache, dv)):
+        if (isinstance(t, torch.Tensor) and t.dtype is q.dtype and t.device == q.device and t.shape == (b, hk, size, width)
+                and t.is_contiguous() and t.data_ptr() % 16 == 0):
+            continue
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{name} must be a torch.Tensor")
         if t.dtype != q.dtype or t.device != q.device:
@@ -186,9 +195,10 @@ def window_attention_step(
     _native._require_device(q)
     if k_cache.data_ptr() == v_cache.data_ptr():
         raise ValueError("k_cache and v_cache must be two tensors")
-    q, k, v = (_native.row_tensor(t.detach()) for t in (q, k, v))
-    out = _native.window_step(q, k, v, k_cache, v_cache, positions.to(torch.int64).contiguous(), window=window,
-                              sinks=sinks, scale=scale)
+    q, k, v = map(_native.row_tensor, (q, k, v))
+    if positions.dtype is not torch.int64 or not positions.is_contiguous():
+        positions = positions.to(torch.int64).contiguous()
+    out = _native.window_step(q, k, v, k_cache, v_cache, positions, window=window, sinks=sinks, scale=scale)
     for t in (k_cache, v_cache):
         torch.autograd.graph.increment_version(t)
     return out

@@ -72,23 +72,24 @@ def test_c_entries_check_before_they_launch():
     assert lib.oal_gated_delta_saved_bytes(2, 2, 65, 1) == 4 * 2 * 5 * 4 * 4096
     assert lib.oal_gated_delta_saved_bytes(2, 2, 65, 0) == 4 * 2 * 4 * 4 * 4096
     assert lib.oal_gated_delta_saved_bytes(0, 2, 65, 1) == 0 and b"positive" in lib.oal_last_error()
-    assert lib.oal_gated_delta_workspace_bytes(1, 3, 2, 2, 64) == 0 and b"divisible" in lib.oal_last_error()
+    assert lib.oal_gated_delta_workspace_bytes(1, 3, 2, 2, 64, 64) == 0 and b"divisible" in lib.oal_last_error()
     # shared heads need room for what is summed
-    assert lib.oal_gated_delta_workspace_bytes(1, 2, 2, 4, 64) > lib.oal_gated_delta_workspace_bytes(1, 4, 4, 4, 64)
+    assert lib.oal_gated_delta_workspace_bytes(1, 2, 2, 4, 64, 64) > lib.oal_gated_delta_workspace_bytes(1, 4, 4, 4, 64, 64)
     assert lib.oal_gated_delta_saved_bytes(1 << 20, 64, 1 << 20, 1) == 0 and b"too large" in lib.oal_last_error()
     p, odd = ctypes.c_void_p(1 << 20), ctypes.c_void_p((1 << 20) + 8)
     rows = (ctypes.c_int64 * 15)(*[64] * 15)
     lib_f = lib.oal_gated_delta_forward
 
-    def forward(q=p, strides=rows, dtype=1, out=p):
-        return lib_f(q, p, p, p, p, strides, 1, 1, 2, 2, 2, 64, dtype, 0.1, None, out, p, p, 1, None)
+    def forward(q=p, strides=rows, dtype=1, out=p, dim=64):
+        return lib_f(q, p, p, p, p, strides, 1, 1, 2, 2, 2, 64, dim, 64, dtype, 0.1, None, out, p, p, 1, None)
 
     assert forward(q=None) and b"null" in lib.oal_last_error()
-    assert forward(dtype=2) and b"dtype" in lib.oal_last_error()
+    assert forward(dtype=3) and b"dtype" in lib.oal_last_error()
+    assert forward(dim=12) and b"multiples of 8" in lib.oal_last_error()
     assert forward(q=odd) and b"16-byte" in lib.oal_last_error()
     assert forward(strides=(ctypes.c_int64 * 15)(*[63] * 15)) and b"16-byte" in lib.oal_last_error()
     assert forward(out=odd) and b"16-byte" in lib.oal_last_error()
-    rc = lib.oal_gated_delta_backward(p, p, p, p, p, rows, 1, 1, 2, 2, 2, 64, 1, 0.1, p, None, None, p, p, p, p, p, None, p, None)
+    rc = lib.oal_gated_delta_backward(p, p, p, p, p, rows, 1, 1, 2, 2, 2, 64, 64, 64, 1, 0.1, p, None, None, p, p, p, p, p, None, p, None)
     assert rc and b"null" in lib.oal_last_error()
     rc = lib.oal_gated_delta_step(p, p, p, p, p, rows, 1, 1, 2, 2, 2, 1, 65, 64, 0, 0.1, p, p, None)
     assert rc and b"[1, 64]" in lib.oal_last_error()

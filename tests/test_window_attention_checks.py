@@ -103,11 +103,11 @@ def test_c_entries_check_before_they_launch():
     p, odd = ctypes.c_void_p(1 << 20), ctypes.c_void_p((1 << 20) + 8)
     rows = (ctypes.c_int64 * 15)(*[64] * 15)
     forward = lib.oal_window_attention_forward
-    assert forward(p, p, None, rows, 1, 2, 2, 5, 5, 3, 0, 1, 0.1, p, p, None) and b"null" in lib.oal_last_error()
-    assert forward(p, odd, p, rows, 1, 2, 2, 5, 5, 3, 0, 1, 0.1, p, p, None) and b"16-byte" in lib.oal_last_error()
-    assert forward(p, p, p, rows, 1, 2, 2, 5, 5, 3, 0, 7, 0.1, p, p, None) and b"dtype" in lib.oal_last_error()
+    assert forward(p, p, None, rows, 1, 2, 2, 5, 5, 64, 64, 3, 0, 1, 0.1, p, p, None) and b"null" in lib.oal_last_error()
+    assert forward(p, odd, p, rows, 1, 2, 2, 5, 5, 64, 64, 3, 0, 1, 0.1, p, p, None) and b"16-byte" in lib.oal_last_error()
+    assert forward(p, p, p, rows, 1, 2, 2, 5, 5, 64, 64, 3, 0, 7, 0.1, p, p, None) and b"dtype" in lib.oal_last_error()
     backward = lib.oal_window_attention_backward
-    assert backward(p, p, p, rows, 1, 2, 2, 5, 5, 3, 0, 1, 0.1, p, p, None, p, p, p, p, None) and b"null" in lib.oal_last_error()
+    assert backward(p, p, p, rows, 1, 2, 2, 5, 5, 64, 64, 3, 0, 1, 0.1, p, p, None, p, p, p, p, None) and b"null" in lib.oal_last_error()
     step = lib.oal_window_attention_step
     assert step(p, p, p, p, p, rows, p, 1, 2, 2, 64, 64, 3, 0, 5, 0.1, p, p, None) and b"type" in lib.oal_last_error()
     assert step(p, p, p, p, odd, rows, p, 1, 2, 2, 64, 64, 3, 0, 1, 0.1, p, p, None) and b"16-byte" in lib.oal_last_error()
