@@ -134,7 +134,7 @@ __global__ __launch_bounds__(kThr) void k_delta_chunk(DeltaArgs a, float* __rest
   float* const L = reinterpret_cast<Solve*>(room)->L;
   float* const Y = reinterpret_cast<Solve*>(room)->Y;
   Tile<3>& P = *reinterpret_cast<Tile<3>*>(room);
-  const int t = threadIdx.x, lane = t & 63, w = t >> 6, g = lane >> 4, c = lane & 15;
+  const int t = threadIdx.x, lane = t & 63, w = wave_of(t), g = lane >> 4, c = lane & 15;
   const int ch = blockIdx.x % a.NC, u = blockIdx.x / a.NC, b = u / a.Hv, h = u % a.Hv;
   const int tok0 = 64 * ch, live = min(64, a.N - tok0);
   const size_t at = ((size_t)u * a.NC + ch) * kTile2;
@@ -264,7 +264,7 @@ __global__ __launch_bounds__(kThr) void k_delta_walk(Walk a) {
     bf16x4 x[3][4][64];
   };
   __shared__ Rows rows[2];
-  const int t = threadIdx.x, lane = t & 63, w = t >> 6, g = lane >> 4, c = lane & 15;
+  const int t = threadIdx.x, lane = t & 63, w = wave_of(t), g = lane >> 4, c = lane & 15;
   // a chain's column groups on one XCD (blocks go round the 8 of them): they share its maps
   const int chains = a.units * a.segs, id = blockIdx.x, whole = chains / 8 * 8 * COLS;
   const int chain = id < whole ? id % 8 + id / (8 * COLS) * 8 : chains / 8 * 8 + (id - whole) / COLS;
@@ -364,7 +364,7 @@ __global__ __launch_bounds__(kThr) void k_delta_out(DeltaArgs a, int each, const
   __shared__ Tile<NP> K;
   __shared__ Tile<NZ> S, U;
   __shared__ Gates gate;
-  const int t = threadIdx.x, lane = t & 63, w = t >> 6, g = lane >> 4, c = lane & 15;
+  const int t = threadIdx.x, lane = t & 63, w = wave_of(t), g = lane >> 4, c = lane & 15;
   const int rep = a.H / a.Hv, parts = (rep + each - 1) / each;
   const int part = blockIdx.x % parts, ch = blockIdx.x / parts % a.NC, u = blockIdx.x / parts / a.NC;
   const int b = u / a.Hv, h = u % a.Hv;
@@ -462,7 +462,7 @@ __global__ __launch_bounds__(kThr) void k_delta_bwd_local(DeltaArgs a, const T* 
   __shared__ Tile<NP> K, Q, O;
   __shared__ Tile<3> P;
   __shared__ Gates gate;
-  const int t = threadIdx.x, lane = t & 63, w = t >> 6, g = lane >> 4, c = lane & 15;
+  const int t = threadIdx.x, lane = t & 63, w = wave_of(t), g = lane >> 4, c = lane & 15;
   const int ch = blockIdx.x % a.NC, u = blockIdx.x / a.NC, b = u / a.Hv, h = u % a.Hv;
   const int tok0 = 64 * ch, live = min(64, a.N - tok0), own = 16 * w + c;
   const size_t at = ((size_t)u * a.NC + ch) * kTile2;
@@ -583,7 +583,7 @@ __global__ __launch_bounds__(kThr) void k_delta_bwd_out(DeltaArgs a, const T* __
   __shared__ Tile<3> Z, X;
   __shared__ Gates gate;
   __shared__ float dG[64], part[4], dotU[4][64];
-  const int t = threadIdx.x, lane = t & 63, w = t >> 6, g = lane >> 4, c = lane & 15;
+  const int t = threadIdx.x, lane = t & 63, w = wave_of(t), g = lane >> 4, c = lane & 15;
   const int ch = blockIdx.x % a.NC, u = blockIdx.x / a.NC, b = u / a.Hv, h = u % a.Hv;
   const int tok0 = 64 * ch, live = min(64, a.N - tok0), own = 16 * w + c;
   const size_t at = ((size_t)u * a.NC + ch) * kTile2;
@@ -879,7 +879,7 @@ __global__ __launch_bounds__(kThr) void k_delta_sum_heads(const float* __restric
 template <typename T>
 __global__ __launch_bounds__(kThr) void k_delta_step(DeltaStepArgs a) {
   __shared__ float sum[4][64];
-  const int t = threadIdx.x, lane = t & 63, w = t >> 6;
+  const int t = threadIdx.x, lane = t & 63, w = wave_of(t);
   const int u = blockIdx.x, b = u / a.Hv, h = u % a.Hv;
   const int d0 = 4 * (t >> 4), c0 = 4 * (t & 15);
   float* state = a.state + (size_t)u * a.Dk * a.Dv;

@@ -221,6 +221,9 @@ __device__ __forceinline__ void load_tile(Tile<NP>& s, const T* __restrict__ src
   }
 }
 
+// A thread's wave as a scalar: what depends on it branches once per wave.
+__device__ __forceinline__ int wave_of(int t) { return __builtin_amdgcn_readfirstlane(t >> 6); }
+
 // Sum over the four lane groups of a wave (lanes of one column).
 __device__ __forceinline__ float group_sum(float x) {
   x += __shfl_xor(x, 16, 64);

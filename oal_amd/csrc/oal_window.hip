@@ -25,6 +25,7 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNone = -__builtin_inff();
+constexpr float kFloor = -1e30f;  // before the first maximum: below every finite score
 
 template <typename T>
 __device__ __forceinline__ const T* rows_at(const Strided& s, int b, int h, int64_t row) {
@@ -42,9 +43,16 @@ constexpr int kCols = 16 * kColTiles<T>;
 struct Shape {
   int heads, subs, groups;
 };
-inline Shape block_shape(int R) {
-  const int groups = (R + 7) / 8, heads = (R + groups - 1) / groups;
+inline Shape block_shape(int R, int most) {
+  const int groups = (R + most - 1) / most, heads = (R + groups - 1) / groups;
   return {heads, std::max(1, 4 / heads), groups};
+}
+
+// The chip's 8 dies take workgroups in turn and each has its own L2: item of
+// workgroup id such that every die works on a contiguous range of items.
+__device__ __forceinline__ int die_item(int id, int total) {
+  const int each = total / 8, more = total % 8, die = id & 7;
+  return die * each + min(die, more) + (id >> 3);
 }
 
 struct Keys {
@@ -59,201 +67,292 @@ struct Keys {
   __device__ int start(int t) const { return t < far ? 64 * t : lo + 64 * (t - far); }
 };
 
-__device__ __forceinline__ bool sees(const WindowArgs& a, bool far, int i, int j) {
-  return far ? j < a.sinks && i - j >= a.window : j <= i && i - j < a.window;
+// The pairs of a tile that are seen: distances i - j from `least` on, `count` of them, of
+// keys before `keys`.
+struct Sight {
+  int least;
+  unsigned count;
+  int keys;
+  __device__ Sight(const WindowArgs& a, bool far)
+      : least(far ? a.window : 0), count(far ? ~0u >> 1 : a.window), keys(far ? a.sinks : a.Nk) {}
+  __device__ bool operator()(int i, int j) const { return ((unsigned)(i - j - least) < count) & (j < keys); }
+};
+// The largest of 8 results of VALU instructions (no operand is quieted first, as fmaxf does).
+__device__ __forceinline__ float max3(float x, float y, float z) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
+  return r;
 }
-// Whether positions i0 .. i1 see any, or all, of keys j0 .. j0 + 63.
-__device__ __forceinline__ bool sees_any(const WindowArgs& a, bool far, int i0, int i1, int j0) {
-  return far ? j0 < a.sinks && i1 - j0 >= a.window : j0 <= i1 && i0 - (j0 + 63) < a.window;
+__device__ __forceinline__ float largest(const float (&y)[8]) {
+  return max3(max3(y[0], y[1], y[2]), max3(y[3], y[4], y[5]), max3(y[6], y[7], y[7]));
 }
-__device__ __forceinline__ bool sees_all(const WindowArgs& a, bool far, int i0, int i1, int j0) {
-  return far ? j0 + 63 < a.sinks && i0 - (j0 + 63) >= a.window : j0 + 63 <= i0 && i1 - j0 < a.window;
+template <int NP>
+__device__ __forceinline__ Frag<NP> negated(Frag<NP> f) {
+#pragma unroll
+  for (int e = 0; e < NP; ++e) f.p[e] = -f.p[e];
+  return f;
+}
+// Whether positions i0 .. i1 see any, or all, of keys j0 .. j1.
+__device__ __forceinline__ bool sees_any(const WindowArgs& a, bool far, int i0, int i1, int j0, int j1) {
+  return far ? j0 < a.sinks && i1 - j0 >= a.window : j0 <= i1 && i0 - j1 < a.window;
+}
+__device__ __forceinline__ bool sees_all(const WindowArgs& a, bool far, int i0, int i1, int j0, int j1) {
+  return far ? j1 < a.sinks && i0 - j1 >= a.window : j1 <= i0 && i1 - j0 < a.window;
 }
 
-}  // namespace
-
+// 64 rows of a tensor in LDS as a block's 256 threads bring them there. bf16 rows
+// go there without passing registers, 16 bytes a lane in the order of the lanes: the 16-byte pieces of row r
+// stand at c ^ r % 8, so that reads of 8 rows meet all banks. Other types are split into parts on the way.
+// Rows past the last and columns past the width repeat others: what they meet is
+// masked or a zero of the other operand. Two barriers around bring(): all waves past their
+// reads before it, all rows there behind it (__syncthreads waits for the copies).
 template <typename T>
-__global__ __launch_bounds__(512) void k_window_fwd(WindowArgs a, Shape sh, int qblocks, T* __restrict__ out,
-                                                    float* __restrict__ lse) {
-  constexpr int NP = kPartsOf<T>, CT = kColTiles<T>;
-  __shared__ Tile<NP> K, V;
-  const int t = threadIdx.x, lane = t & 63, w = t >> 6, g = lane >> 4, c = lane & 15;
-  const int R = a.Hq / a.Hk;
-  int id = blockIdx.x;
+struct Board {
+  static constexpr int NP = kPartsOf<T>;
+  Tile<NP> tile;
+  __device__ void bring(const T* src, int64_t stride, int D, int live, int t) {
+    load_rows(src, stride, D, live, t);
+  }
+  __device__ Frag<NP> rows(int r0, int t, int lane) const { return row_frag(tile, r0, t, lane); }
+  __device__ Frag<NP> columns(int c0, int t, int lane) const { return col_frag_perm(tile, c0, t, lane); }
+
+ private:
+  __device__ void load_rows(const T* src, int64_t stride, int D, int live, int t) {
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      const int r = (t >> 3) + 32 * n, c = 8 * (t & 7);
+      float x[8];
+      load_row8(x, src + min(r, live - 1) * stride + min(c, D - 8));
+      const Frag<NP> f = split<NP>(x);
+#pragma unroll
+      for (int e = 0; e < NP; ++e) *reinterpret_cast<bf16x8*>(tile.x + e * kTileElems + r * kTileRow + c) = f.p[e];
+    }
+  }
+};
+template <>
+struct Board<uint16_t> {
+  alignas(16) __bf16 x[64 * 64];
+  __device__ void bring(const uint16_t* src, int64_t stride, int D, int live, int t) {
+    const int lane = t & 63, w = wave_of(t), c = 8 * ((lane & 7) ^ (lane >> 3));
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      const int r = 32 * n + 8 * w + (lane >> 3);
+      copy16_to_lds(src + min(r, live - 1) * stride + min(c, D - 8), x + (32 * n + 8 * w) * 64);
+    }
+  }
+  __device__ Frag<1> rows(int r0, int t, int lane) const {
+    const int r = lane & 15;
+    return {{*reinterpret_cast<const bf16x8*>(x + (r0 + r) * 64 + 8 * ((4 * t + (lane >> 4)) ^ (r & 7)))}};
+  }
+  __device__ Frag<1> columns(int c0, int t, int lane) const {
+    const int g = lane >> 4, i = lane & 15, r = 4 * g + (i >> 2);
+    const __bf16* p = x + (32 * t + r) * 64 + 8 * (((c0 >> 3) + ((i >> 1) & 1)) ^ (r & 7)) + 4 * (i & 1);
+    return {{tr_rows(p, p + 16 * 64)}};
+  }
+};
+// What a block of the query side works on.
+struct Block {
+  int b, hk, h, q0, i0, i1, first, last;
+  bool works;
+};
+template <typename T>
+__device__ __forceinline__ Block query_block(const WindowArgs& a, const Shape& sh, int qblocks, int w) {
+  Block x;
+  const int R = a.Hq / a.Hk, off = a.Nk - a.Nq;
+  int id = die_item(blockIdx.x, gridDim.x);
   const int qb = id % qblocks;
   id /= qblocks;
   const int hg = id % sh.groups;
   id /= sh.groups;
-  const int hk = id % a.Hk, b = id / a.Hk;
-  const int r = hg * sh.heads + w / sh.subs, off = a.Nk - a.Nq;
-  const int span = sh.subs * kCols<T>, q0 = qb * span + (w % sh.subs) * kCols<T>;
-  const bool works = r < R && q0 < a.Nq;
-  const int h = hk * R + (r < R ? r : R - 1);
-  const Keys keys(a, off + qb * span, off + min(a.Nq, (qb + 1) * span) - 1);
-  const int i0 = off + q0, i1 = off + min(a.Nq, q0 + kCols<T>) - 1;
+  x.hk = id % a.Hk, x.b = id / a.Hk;
+  const int r = hg * sh.heads + w / sh.subs, span = sh.subs * kCols<T>;
+  x.q0 = qb * span + (w % sh.subs) * kCols<T>;
+  x.works = w < sh.heads * sh.subs && r < R && x.q0 < a.Nq;
+  x.h = x.hk * R + min(r, R - 1);
+  x.first = off + qb * span, x.last = off + min(a.Nq, (qb + 1) * span) - 1;
+  x.i0 = off + x.q0, x.i1 = off + min(a.Nq, x.q0 + kCols<T>) - 1;
+  return x;
+}
+
+}  // namespace
+
+// Bound by the exponentials: of the 6 issue slots per pair (a multiply-add, half a
+// maximum, an exponential of 4, half a conversion) they take 4, the two products 2.7 on
+// the matrix cores beside. The sums of the weights are a third product, with ones, of
+// the weights as the values meet them. A row's maximum is moved only when a score
+// exceeds it by 2^8, which float32 sums do not mind: else nothing is rescaled.
+template <typename T>
+__global__ __launch_bounds__(256, kPartsOf<T> == 1 ? 3 : 1) void k_window_fwd(WindowArgs a, Shape sh, int qblocks, T* __restrict__ out,
+                                                       float* __restrict__ lse) {
+  constexpr int NP = kPartsOf<T>, CT = kColTiles<T>;
+  __shared__ Board<T> K, V;
+  const int t = threadIdx.x, lane = t & 63, w = wave_of(t), g = lane >> 4, c = lane & 15;
+  const Block at = query_block<T>(a, sh, qblocks, w);
+  const Keys keys(a, at.first, at.last);
 
   Frag<NP> qf[CT][2];
 #pragma unroll
   for (int x = 0; x < CT; ++x)
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      const int row = q0 + 16 * x + c;
+      const int row = at.q0 + 16 * x + c;
       const bool live = row < a.Nq;
-      qf[x][s] = global_frag<NP>(rows_at<T>(a.q, b, h, live ? row : 0) + 32 * s + 8 * g, live && 32 * s + 8 * g < a.D);
+      qf[x][s] = global_frag<NP>(rows_at<T>(a.q, at.b, at.h, live ? row : 0) + 32 * s + 8 * g, live && 32 * s + 8 * g < a.D);
+      if (a.scale < 0.f) qf[x][s] = negated(qf[x][s]);
     }
-  f32x4 acc[CT][4] = {};
-  float top[CT], sum[CT];
+  Frag<1> ones;
 #pragma unroll
-  for (int x = 0; x < CT; ++x) top[x] = kNone, sum[x] = 0.f;
-  const float scale = a.scale * kLog2e;
+  for (int e = 0; e < 8; ++e) ones.p[0][e] = static_cast<__bf16>(1.f);
+  f32x4 acc[CT][4] = {}, sum[CT] = {};
+  float top[CT];
+#pragma unroll
+  for (int x = 0; x < CT; ++x) top[x] = kFloor;
+  const float scale = fabsf(a.scale) * kLog2e;
 
-  for (int tile = 0; tile < keys.tiles; ++tile) {
-    const int j0 = keys.start(tile);
-    const bool far = tile < keys.far;
-    __syncthreads();
-    const int live = min(64, a.Nk - j0);
-    if (t < 256) {
-      load_tile<64, 256>(K, rows_at<T>(a.k, b, hk, j0), a.k.n, a.D, live, t);
-      load_tile<64, 256>(V, rows_at<T>(a.v, b, hk, j0), a.v.n, a.DV, live, t);
-    }
-    __syncthreads();
-    if (!works || !sees_any(a, far, i0, i1, j0)) continue;
-    f32x4 s[CT][4];
+  // 32 keys
+  auto half_tile = [&](auto masked, bool far, int jh, int half) {
+    // the scores that are hidden become none
+    auto hide = [&](float (&y)[8], int x) {
+      if constexpr (decltype(masked)::value) {
+        const Sight sees(a, far);
 #pragma unroll
-    for (int m = 0; m < 4; ++m) {
+        for (int e = 0; e < 8; ++e)
+          y[e] = sees(at.i0 + 16 * x + c, jh + 16 * (e >> 2) + 4 * g + (e & 3)) ? y[e] : kNone;
+      }
+    };
+    f32x4 s[CT][2] = {};
 #pragma unroll
-      for (int x = 0; x < CT; ++x) s[x][m] = f32x4{};
+    for (int m = 0; m < 2; ++m)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const Frag<NP> k = row_frag(K, 16 * m, e, lane);
+        const Frag<NP> k = K.rows(32 * half + 16 * m, e, lane);
 #pragma unroll
         for (int x = 0; x < CT; ++x) s[x][m] = mma(k, qf[x][e], s[x][m]);
       }
-    }
-    const bool all = sees_all(a, far, i0, i1, j0);
-    Frag<NP> p[CT][2];
+    Frag<NP> vf[4];
+#pragma unroll
+    for (int m = 0; m < 4; ++m) vf[m] = V.columns(16 * m, half, lane);
+    float y[CT][8], most[CT];
 #pragma unroll
     for (int x = 0; x < CT; ++x) {
-      const int i = i0 + 16 * x + c;
-      float most = kNone;
 #pragma unroll
-      for (int m = 0; m < 4; ++m)
+      for (int e = 0; e < 8; ++e) y[x][e] = __builtin_fmaf(s[x][e >> 2][e & 3], scale, -top[x]);
+      hide(y[x], x);
+      most[x] = largest(y[x]);
+    }
+    if (__any(max3(most[0], most[CT - 1], most[0]) > 8.f)) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float y = s[x][m][e] * scale;
-          s[x][m][e] = all || sees(a, far, i, j0 + 16 * m + 4 * g + e) ? y : kNone;
-          most = fmaxf(most, s[x][m][e]);
-        }
-      most = fmaxf(top[x], group_max(most));
-      const float base = most == kNone ? 0.f : most;
-      const float keep = __builtin_amdgcn_exp2f(top[x] - base);
-      top[x] = most;
-      float part = 0.f;
+      for (int x = 0; x < CT; ++x) {
+        // from the stand-in of the start the differences are not exact
 #pragma unroll
-      for (int m = 0; m < 4; ++m)
+        for (int e = 0; e < 8; ++e) y[x][e] = s[x][e >> 2][e & 3] * scale;
+        hide(y[x], x);
+        const float peak = fmaxf(top[x], group_max(largest(y[x]))), less = __builtin_amdgcn_exp2f(top[x] - peak);
+        top[x] = peak;
+        sum[x] *= less;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[x][m][e] = __builtin_amdgcn_exp2f(s[x][m][e] - base);
-          part += s[x][m][e];
-        }
-      sum[x] = sum[x] * keep + part;
+        for (int m = 0; m < 4; ++m) acc[x][m] *= less;
 #pragma unroll
-      for (int m = 0; m < 4; ++m) acc[x][m] *= keep;
-      p[x][0] = acc_frag<NP>(s[x][0], s[x][1]);
-      p[x][1] = acc_frag<NP>(s[x][2], s[x][3]);
+        for (int e = 0; e < 8; ++e) y[x][e] -= peak;
+      }
+    }
+    Frag<NP> p[CT];
+#pragma unroll
+    for (int x = 0; x < CT; ++x) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[x][e] = __builtin_amdgcn_exp2f(y[x][e]);
+      p[x] = split<NP>(y[x]);
+      sum[x] = mma(ones, p[x], sum[x]);
     }
 #pragma unroll
-    for (int m = 0; m < 4; ++m)
+    for (int m = 0; m < 4; ++m) {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const Frag<NP> v = col_frag_perm(V, 16 * m, e, lane);
-#pragma unroll
-        for (int x = 0; x < CT; ++x) acc[x][m] = mma(v, p[x][e], acc[x][m]);
-      }
+      for (int x = 0; x < CT; ++x) acc[x][m] = mma(vf[m], p[x], acc[x][m]);
+    }
+  };
+  for (int tile = 0; tile < keys.tiles; ++tile) {
+    const int j0 = keys.start(tile), live = min(64, at.last + 1 - j0);
+    const bool far = tile < keys.far;
+    if (tile) lds_sync();
+    K.bring(rows_at<T>(a.k, at.b, at.hk, j0), a.k.n, a.D, live, t);
+    V.bring(rows_at<T>(a.v, at.b, at.hk, j0), a.v.n, a.DV, live, t);
+    __syncthreads();
+    if (!at.works) continue;
+#pragma nounroll
+    for (int half = 0; half < 2; ++half) {
+      const int jh = j0 + 32 * half;
+      if (!sees_any(a, far, at.i0, at.i1, jh, jh + 31)) continue;
+      if (sees_all(a, far, at.i0, at.i1, jh, jh + 31))
+        half_tile(std::false_type{}, far, jh, half);
+      else
+        half_tile(std::true_type{}, far, jh, half);
+    }
   }
-  if (!works) return;
+  if (!at.works) return;
 #pragma unroll
   for (int x = 0; x < CT; ++x) {
-    const int row = q0 + 16 * x + c;
-    const float all = group_sum(sum[x]), inv = 1.f / all;
+    const int row = at.q0 + 16 * x + c;
     if (row >= a.Nq) continue;
-    const size_t at = ((size_t)b * a.Hq + h) * a.Nq + row;
+    const float all = sum[x][0], inv = 1.f / all;
+    const size_t to = ((size_t)at.b * a.Hq + at.h) * a.Nq + row;
 #pragma unroll
     for (int m = 0; m < 4; ++m)
-      if (16 * m + 4 * g < a.DV) store4(out + at * a.DV + 16 * m + 4 * g, acc[x][m] * inv);
-    if (g == 0) lse[at] = top[x] + __builtin_amdgcn_logf(all);
+      if (16 * m + 4 * g < a.DV) store4(out + to * a.DV + 16 * m + 4 * g, acc[x][m] * inv);
+    if (g == 0) lse[to] = top[x] + __builtin_amdgcn_logf(all);
   }
 }
 
 // dq, and for the other side delta_i = do_i.o_i: the forward's walk again.
 template <typename T>
-__global__ __launch_bounds__(512) void k_window_dq(WindowArgs a, Shape sh, int qblocks, const T* __restrict__ out,
-                                                   const float* __restrict__ lse, const T* __restrict__ dout,
-                                                   float* __restrict__ delta, T* __restrict__ dq) {
+__global__ __launch_bounds__(256, kPartsOf<T> == 1 ? 3 : 1) void k_window_dq(WindowArgs a, Shape sh, int qblocks, const T* __restrict__ out,
+                                                      const float* __restrict__ lse, const T* __restrict__ dout,
+                                                      float* __restrict__ delta, T* __restrict__ dq) {
   constexpr int NP = kPartsOf<T>, CT = kColTiles<T>;
-  __shared__ Tile<NP> K, V;
-  const int t = threadIdx.x, lane = t & 63, w = t >> 6, g = lane >> 4, c = lane & 15;
-  const int R = a.Hq / a.Hk;
-  int id = blockIdx.x;
-  const int qb = id % qblocks;
-  id /= qblocks;
-  const int hg = id % sh.groups;
-  id /= sh.groups;
-  const int hk = id % a.Hk, b = id / a.Hk;
-  const int r = hg * sh.heads + w / sh.subs, off = a.Nk - a.Nq;
-  const int span = sh.subs * kCols<T>, q0 = qb * span + (w % sh.subs) * kCols<T>;
-  const bool works = r < R && q0 < a.Nq;
-  const int h = hk * R + (r < R ? r : R - 1);
-  const Keys keys(a, off + qb * span, off + min(a.Nq, (qb + 1) * span) - 1);
-  const int i0 = off + q0, i1 = off + min(a.Nq, q0 + kCols<T>) - 1;
+  __shared__ Board<T> K, V;
+  const int t = threadIdx.x, lane = t & 63, w = wave_of(t), g = lane >> 4, c = lane & 15;
+  const Block at = query_block<T>(a, sh, qblocks, w);
+  const Keys keys(a, at.first, at.last);
 
   Frag<NP> qf[CT][2], of[CT][2];
   float base[CT], dot[CT];
 #pragma unroll
   for (int x = 0; x < CT; ++x) {
-    const int row = q0 + 16 * x + c;
-    const bool live = works && row < a.Nq;
-    const size_t at = ((size_t)b * a.Hq + h) * a.Nq + (live ? row : 0);
+    const int row = at.q0 + 16 * x + c;
+    const bool live = at.works && row < a.Nq;
+    const size_t from = ((size_t)at.b * a.Hq + at.h) * a.Nq + (live ? row : 0);
     float y = 0.f;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       const int col = 32 * s + 8 * g;
-      qf[x][s] = global_frag<NP>(rows_at<T>(a.q, b, h, live ? row : 0) + col, live && col < a.D);
-      of[x][s] = global_frag<NP>(dout + at * a.DV + col, live && col < a.DV);
+      qf[x][s] = global_frag<NP>(rows_at<T>(a.q, at.b, at.h, live ? row : 0) + col, live && col < a.D);
+      of[x][s] = global_frag<NP>(dout + from * a.DV + col, live && col < a.DV);
       float o[8] = {}, d[8] = {};
       if (live && col < a.DV) {
-        load_row8(o, out + at * a.DV + col);
-        load_row8(d, dout + at * a.DV + col);
+        load_row8(o, out + from * a.DV + col);
+        load_row8(d, dout + from * a.DV + col);
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) y += o[e] * d[e];
     }
     dot[x] = group_sum(y);
-    base[x] = live ? lse[at] : 0.f;
-    if (live && g == 0) delta[at] = dot[x];
+    base[x] = live ? lse[from] : 0.f;
+    if (live && g == 0) delta[from] = dot[x];
   }
   f32x4 acc[CT][4] = {};
   const float scale = a.scale * kLog2e;
 
-  for (int tile = 0; tile < keys.tiles; ++tile) {
-    const int j0 = keys.start(tile);
-    const bool far = tile < keys.far;
-    __syncthreads();
-    const int live = min(64, a.Nk - j0);
-    if (t < 256) {
-      load_tile<64, 256>(K, rows_at<T>(a.k, b, hk, j0), a.k.n, a.D, live, t);
-      load_tile<64, 256>(V, rows_at<T>(a.v, b, hk, j0), a.v.n, a.DV, live, t);
-    }
-    __syncthreads();
-    if (!works || !sees_any(a, far, i0, i1, j0)) continue;
-    f32x4 s[CT][4], d[CT][4];
+  auto half_tile = [&](auto masked, bool far, int jh, int half) {
+    f32x4 s[CT][2], d[CT][2];
 #pragma unroll
-    for (int m = 0; m < 4; ++m) {
+    for (int m = 0; m < 2; ++m) {
 #pragma unroll
-      for (int x = 0; x < CT; ++x) s[x][m] = f32x4{}, d[x][m] = f32x4{};
+      for (int x = 0; x < CT; ++x) {
+        s[x][m] = f32x4{};
+        d[x][m] = f32x4{-dot[x], -dot[x], -dot[x], -dot[x]};
+      }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const Frag<NP> k = row_frag(K, 16 * m, e, lane), v = row_frag(V, 16 * m, e, lane);
+        const Frag<NP> k = K.rows(32 * half + 16 * m, e, lane), v = V.rows(32 * half + 16 * m, e, lane);
 #pragma unroll
         for (int x = 0; x < CT; ++x) {
           s[x][m] = mma(k, qf[x][e], s[x][m]);
@@ -261,73 +360,89 @@ __global__ __launch_bounds__(512) void k_window_dq(WindowArgs a, Shape sh, int q
         }
       }
     }
-    const bool all = sees_all(a, far, i0, i1, j0);
-    Frag<NP> p[CT][2];
+    Frag<NP> p[CT];
 #pragma unroll
     for (int x = 0; x < CT; ++x) {
-      const int i = i0 + 16 * x + c;
+      float y[8];
 #pragma unroll
-      for (int m = 0; m < 4; ++m)
+      for (int e = 0; e < 8; ++e)
+        y[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][e >> 2][e & 3], scale, -base[x])) * d[x][e >> 2][e & 3];
+      if constexpr (decltype(masked)::value) {
+        const Sight sees(a, far);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float y = __builtin_amdgcn_exp2f(s[x][m][e] * scale - base[x]);
-          const float z = y * (d[x][m][e] - dot[x]);
-          s[x][m][e] = all || sees(a, far, i, j0 + 16 * m + 4 * g + e) ? z : 0.f;
-        }
-      p[x][0] = acc_frag<NP>(s[x][0], s[x][1]);
-      p[x][1] = acc_frag<NP>(s[x][2], s[x][3]);
+        for (int e = 0; e < 8; ++e)
+          y[e] = sees(at.i0 + 16 * x + c, jh + 16 * (e >> 2) + 4 * g + (e & 3)) ? y[e] : 0.f;
+      }
+      p[x] = split<NP>(y);
     }
 #pragma unroll
-    for (int m = 0; m < 4; ++m)
+    for (int m = 0; m < 4; ++m) {
+      const Frag<NP> k = K.columns(16 * m, half, lane);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const Frag<NP> k = col_frag_perm(K, 16 * m, e, lane);
-#pragma unroll
-        for (int x = 0; x < CT; ++x) acc[x][m] = mma(k, p[x][e], acc[x][m]);
-      }
+      for (int x = 0; x < CT; ++x) acc[x][m] = mma(k, p[x], acc[x][m]);
+    }
+  };
+  for (int tile = 0; tile < keys.tiles; ++tile) {
+    const int j0 = keys.start(tile), live = min(64, at.last + 1 - j0);
+    const bool far = tile < keys.far;
+    if (tile) lds_sync();
+    K.bring(rows_at<T>(a.k, at.b, at.hk, j0), a.k.n, a.D, live, t);
+    V.bring(rows_at<T>(a.v, at.b, at.hk, j0), a.v.n, a.DV, live, t);
+    __syncthreads();
+    if (!at.works) continue;
+#pragma nounroll
+    for (int half = 0; half < 2; ++half) {
+      const int jh = j0 + 32 * half;
+      if (!sees_any(a, far, at.i0, at.i1, jh, jh + 31)) continue;
+      if (sees_all(a, far, at.i0, at.i1, jh, jh + 31))
+        half_tile(std::false_type{}, far, jh, half);
+      else
+        half_tile(std::true_type{}, far, jh, half);
+    }
   }
-  if (!works) return;
+  if (!at.works) return;
 #pragma unroll
   for (int x = 0; x < CT; ++x) {
-    const int row = q0 + 16 * x + c;
+    const int row = at.q0 + 16 * x + c;
     if (row >= a.Nq) continue;
-    const size_t at = ((size_t)b * a.Hq + h) * a.Nq + row;
+    const size_t to = ((size_t)at.b * a.Hq + at.h) * a.Nq + row;
 #pragma unroll
     for (int m = 0; m < 4; ++m)
-      if (16 * m + 4 * g < a.D) store4(dq + at * a.D + 16 * m + 4 * g, acc[x][m] * a.scale);
+      if (16 * m + 4 * g < a.D) store4(dq + to * a.D + 16 * m + 4 * g, acc[x][m] * a.scale);
   }
 }
 
 // dk and dv of 4 waves' keys over a part of the queries that see them. Blocks
 // 0 .. near - 1: through the window; the others: first keys seen from afar.
 template <typename T>
-__global__ __launch_bounds__(256) void k_window_dkv(WindowArgs a, WindowPlan plan, int kblocks, int near,
-                                                    const float* __restrict__ lse, const T* __restrict__ dout,
-                                                    const float* __restrict__ delta, float* __restrict__ part,
-                                                    float* __restrict__ farpart) {
-  constexpr int NP = kPartsOf<T>, CT = kColTiles<T>;
-  __shared__ Tile<NP> Q, O;
+__global__ __launch_bounds__(256, kPartsOf<T> == 1 ? 2 : 1) void k_window_dkv(WindowArgs a, WindowPlan plan, int kblocks, int near,
+                                                       const float* __restrict__ lse, const T* __restrict__ dout,
+                                                       const float* __restrict__ delta, float* __restrict__ part,
+                                                       float* __restrict__ farpart) {
+  constexpr int NP = kPartsOf<T>, CT = kColTiles<T>, kKeys = 4 * kCols<T>;
+  __shared__ Board<T> Q, O;
   __shared__ alignas(16) float base[64], dot[64];
-  const int t = threadIdx.x, lane = t & 63, w = t >> 6, g = lane >> 4, c = lane & 15;
+  const int t = threadIdx.x, lane = t & 63, w = wave_of(t), g = lane >> 4, c = lane & 15;
   const int R = a.Hq / a.Hk, off = a.Nk - a.Nq;
   const bool far = (int)blockIdx.x >= near;
   const int blocks = far ? plan.sink_blocks : kblocks, parts = far ? plan.chunks : plan.splits;
   const int rows = far ? plan.sink_rows : a.Nk;
-  int id = far ? blockIdx.x - near : blockIdx.x;
+  int id = far ? blockIdx.x - near : die_item(blockIdx.x, near);
   const int kb = id % blocks;
   id /= blocks;
   const int piece = id % parts;
   id /= parts;
   const int hk = id % a.Hk, b = id / a.Hk;
-  const int jb = kb * 4 * kCols<T>, j0 = jb + w * kCols<T>;
+  const int jb = kb * kKeys, j0 = jb + w * kCols<T>, j1 = j0 + kCols<T> - 1;
   // positions of the queries that see these keys
-  const int last = min(rows, jb + 4 * kCols<T>) - 1;
+  const int last = min(rows, jb + kKeys) - 1;
   const int lo = max(off, far ? jb + a.window : jb);
   const int64_t until = far ? a.Nk - 1 : min((int64_t)a.Nk - 1, (int64_t)last + a.window - 1);
   const int tiles = until >= lo ? (int)(until - lo) / 64 + 1 : 0;
   const int64_t steps = (int64_t)R * tiles;
-  const int64_t s0 = steps * piece / parts, s1 = steps * (piece + 1) / parts;
-
+  const int64_t s0 = steps * piece / parts;
+  const int count = (int)(steps * (piece + 1) / parts - s0);
+  int r = tiles ? (int)(s0 / tiles) : 0, tile = tiles ? (int)(s0 % tiles) : 0;  // of the step
   Frag<NP> kf[CT][2], vf[CT][2];
 #pragma unroll
   for (int x = 0; x < CT; ++x)
@@ -341,31 +456,16 @@ __global__ __launch_bounds__(256) void k_window_dkv(WindowArgs a, WindowPlan pla
     }
   f32x4 dk[CT][4] = {}, dv[CT][4] = {};
   const float scale = a.scale * kLog2e;
-  for (int64_t step = s0; step < s1; ++step) {
-    const int h = hk * R + (int)(step / tiles), i0 = lo + 64 * (int)(step % tiles);  // position of the tile's first query
-    const int live = min(64, a.Nk - i0);
-    const size_t at = ((size_t)b * a.Hq + h) * a.Nq + (i0 - off);
-    __syncthreads();
-    load_tile<64, 256>(Q, rows_at<T>(a.q, b, h, i0 - off), a.q.n, a.D, live, t);
-    load_tile<64, 256>(O, dout + at * a.DV, (int64_t)a.DV, a.DV, live, t);
-    if (t < 64) {
-      base[t] = t < live ? lse[at + t] : 0.f;
-      dot[t] = t < live ? delta[at + t] : 0.f;
-    }
-    __syncthreads();
-    if (j0 >= rows) continue;
-    const int j1 = j0 + kCols<T> - 1, i1 = i0 + live - 1;
-    // none, or all, of the pairs in sight
-    if (far ? j0 >= a.sinks || i1 - j0 < a.window : j0 > i1 || i0 - j1 >= a.window) continue;
-    const bool all = live == 64 && (far ? j1 < a.sinks && i0 - j1 >= a.window : j1 <= i0 && i1 - j0 < a.window);
-    f32x4 s[CT][4], d[CT][4];
+  auto half_tile = [&](auto masked, int ih, int half) {
+    f32x4 s[CT][2], d[CT][2];
 #pragma unroll
-    for (int m = 0; m < 4; ++m) {
+    for (int m = 0; m < 2; ++m) {
+      const f32x4 dt = *reinterpret_cast<const f32x4*>(dot + 32 * half + 16 * m + 4 * g);
 #pragma unroll
-      for (int x = 0; x < CT; ++x) s[x][m] = f32x4{}, d[x][m] = f32x4{};
+      for (int x = 0; x < CT; ++x) s[x][m] = f32x4{}, d[x][m] = dt;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const Frag<NP> q = row_frag(Q, 16 * m, e, lane), o = row_frag(O, 16 * m, e, lane);
+        const Frag<NP> q = Q.rows(32 * half + 16 * m, e, lane), o = O.rows(32 * half + 16 * m, e, lane);
 #pragma unroll
         for (int x = 0; x < CT; ++x) {
           s[x][m] = mma(q, kf[x][e], s[x][m]);
@@ -373,40 +473,62 @@ __global__ __launch_bounds__(256) void k_window_dkv(WindowArgs a, WindowPlan pla
         }
       }
     }
-    Frag<NP> p[CT][2], z[CT][2];
+    Frag<NP> p[CT], z[CT];
 #pragma unroll
     for (int x = 0; x < CT; ++x) {
-      const int j = j0 + 16 * x + c;
+      float y[8], yd[8];
 #pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        const f32x4 bs = *reinterpret_cast<const f32x4*>(base + 16 * m + 4 * g);
-        const f32x4 dt = *reinterpret_cast<const f32x4*>(dot + 16 * m + 4 * g);
+      for (int m = 0; m < 2; ++m) {
+        const f32x4 bs = *reinterpret_cast<const f32x4*>(base + 32 * half + 16 * m + 4 * g);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int row = 16 * m + 4 * g + e;
-          const float y = __builtin_amdgcn_exp2f(s[x][m][e] * scale - bs[e]);
-          const bool seen = all || (row < live && sees(a, far, i0 + row, j));
-          s[x][m][e] = seen ? y : 0.f;
-          d[x][m][e] = seen ? y * (d[x][m][e] - dt[e]) : 0.f;
+          y[4 * m + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][m][e], scale, -bs[e]));
+          yd[4 * m + e] = y[4 * m + e] * d[x][m][e];
         }
       }
+      if constexpr (decltype(masked)::value) {
+        const Sight sees(a, far);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        p[x][e] = acc_frag<NP>(s[x][2 * e], s[x][2 * e + 1]);
-        z[x][e] = acc_frag<NP>(d[x][2 * e], d[x][2 * e + 1]);
+        for (int e = 0; e < 8; ++e) {
+          const int i = ih + 16 * (e >> 2) + 4 * g + (e & 3);
+          const bool seen = (i < a.Nk) & sees(i, j0 + 16 * x + c);
+          y[e] = seen ? y[e] : 0.f;
+          yd[e] = seen ? yd[e] : 0.f;
+        }
       }
+      p[x] = split<NP>(y);
+      z[x] = split<NP>(yd);
     }
 #pragma unroll
-    for (int m = 0; m < 4; ++m)
+    for (int m = 0; m < 4; ++m) {
+      const Frag<NP> q = Q.columns(16 * m, half, lane), o = O.columns(16 * m, half, lane);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const Frag<NP> q = col_frag_perm(Q, 16 * m, e, lane), o = col_frag_perm(O, 16 * m, e, lane);
-#pragma unroll
-        for (int x = 0; x < CT; ++x) {
-          dk[x][m] = mma(q, z[x][e], dk[x][m]);
-          dv[x][m] = mma(o, p[x][e], dv[x][m]);
-        }
+      for (int x = 0; x < CT; ++x) {
+        dk[x][m] = mma(q, z[x], dk[x][m]);
+        dv[x][m] = mma(o, p[x], dv[x][m]);
       }
+    }
+  };
+  for (int step = 0; step < count; ++step) {
+    const int h = hk * R + r, i0 = lo + 64 * tile, live = min(64, a.Nk - i0);
+    if (++tile == tiles) tile = 0, ++r;
+    const size_t at = ((size_t)b * a.Hq + h) * a.Nq + (i0 - off);
+    if (step) lds_sync();
+    Q.bring(rows_at<T>(a.q, b, h, i0 - off), a.q.n, a.D, live, t);
+    O.bring(dout + at * a.DV, a.DV, a.DV, live, t);
+    if (t < 64) base[t] = lse[at + min(t, live - 1)];
+    if (t >= 64 && t < 128) dot[t - 64] = -delta[at + min(t - 64, live - 1)];
+    __syncthreads();
+    if (j0 >= rows) continue;
+#pragma nounroll
+    for (int half = 0; half < 2; ++half) {
+      const int ih = i0 + 32 * half, ie = min(a.Nk - 1, ih + 31);
+      if (ih >= a.Nk || !sees_any(a, far, ih, ie, j0, j1)) continue;
+      if (ie == ih + 31 && sees_all(a, far, ih, ie, j0, j1))
+        half_tile(std::false_type{}, ih, half);
+      else
+        half_tile(std::true_type{}, ih, half);
+    }
   }
   float* to = far ? farpart : part;
   const size_t half = (size_t)parts * a.B * a.Hk * rows * 64;
@@ -486,7 +608,7 @@ __global__ __launch_bounds__(256) void k_window_step(WindowStepArgs a) {
   __shared__ Rows V[4];
   __shared__ alignas(16) float acc4[4][16][68];
   __shared__ float top4[4][16], sum4[4][16];
-  const int t = threadIdx.x, lane = t & 63, w = t >> 6, g = lane >> 4, c = lane & 15;
+  const int t = threadIdx.x, lane = t & 63, w = wave_of(t), g = lane >> 4, c = lane & 15;
   const int R = a.Hq / a.Hk, groups = (R + 15) / 16;
   int id = blockIdx.x;
   const int piece = id % a.splits;
@@ -655,12 +777,10 @@ WindowWork window_work_view(void* base, const WindowArgs& a, const WindowPlan& p
 
 template <typename T>
 void launch_window_forward(const WindowArgs& a, void* out, float* lse, hipStream_t st, const Timer& timed) {
-  const Shape sh = block_shape(a.Hq / a.Hk);
+  const Shape sh = block_shape(a.Hq / a.Hk, 4);
   const int qblocks = (a.Nq + sh.subs * kCols<T> - 1) / (sh.subs * kCols<T>);
-  // at least the four waves that load the tiles
-  const int waves = std::max(4, sh.heads * sh.subs);
   timed("k_window_fwd", st, [&] {
-    hipLaunchKernelGGL(k_window_fwd<T>, dim3((unsigned)((int64_t)a.B * a.Hk * sh.groups * qblocks)), dim3(64 * waves), 0,
+    hipLaunchKernelGGL(k_window_fwd<T>, dim3((unsigned)((int64_t)a.B * a.Hk * sh.groups * qblocks)), dim3(256), 0,
                        st, a, sh, qblocks, static_cast<T*>(out), lse);
   });
 }
@@ -668,13 +788,12 @@ void launch_window_forward(const WindowArgs& a, void* out, float* lse, hipStream
 template <typename T>
 void launch_window_backward(const WindowArgs& a, const void* out, const float* lse, const void* dout, void* dq,
                             void* dk, void* dv, void* work, hipStream_t st, const Timer& timed) {
-  const Shape sh = block_shape(a.Hq / a.Hk);
+  const Shape sh = block_shape(a.Hq / a.Hk, 4);
   const int qblocks = (a.Nq + sh.subs * kCols<T> - 1) / (sh.subs * kCols<T>);
-  const int waves = std::max(4, sh.heads * sh.subs);
   const WindowPlan plan = window_plan(a.B, a.Hq, a.Hk, a.Nq, a.Nk, a.window, a.sinks, 4 * kCols<T>);
   const WindowWork w = window_work_view(work, a, plan);
   timed("k_window_dq", st, [&] {
-    hipLaunchKernelGGL(k_window_dq<T>, dim3((unsigned)((int64_t)a.B * a.Hk * sh.groups * qblocks)), dim3(64 * waves), 0,
+    hipLaunchKernelGGL(k_window_dq<T>, dim3((unsigned)((int64_t)a.B * a.Hk * sh.groups * qblocks)), dim3(256), 0,
                        st, a, sh, qblocks, static_cast<const T*>(out), lse, static_cast<const T*>(dout), w.delta,
                        static_cast<T*>(dq));
   });
