@@ -730,7 +730,8 @@ def row_tensor(t: torch.Tensor) -> torch.Tensor:
         if t.is_contiguous() and t.shape[-1] % 8 == 0:
             return t
         size = t.element_size()
-        if t.stride(-1) == 1 and all(s * size % 16 == 0 for s, n in zip(t.stride()[:-1], t.shape) if n > 1):
+        if t.stride(-1) == 1 and t.stride(-2) < 1 << 24 and all(
+                s * size % 16 == 0 for s, n in zip(t.stride()[:-1], t.shape) if n > 1):
             return t
     return t.clone(memory_format=torch.contiguous_format)
 

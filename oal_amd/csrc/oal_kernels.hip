@@ -1621,6 +1621,9 @@ static int window_args(oal::WindowArgs* a, const char* what, const void* q, cons
   if (!rows_aligned(a->q, dtype, batch, q_heads, query_len) || !rows_aligned(a->k, dtype, batch, kv_heads, key_len) ||
       !rows_aligned(a->v, dtype, batch, kv_heads, key_len))
     return fail(std::string(what) + ": rows must be 16-byte aligned");
+  // 32-bit offsets inside a tile of 64 rows
+  for (const oal::Strided* s : {&a->q, &a->k, &a->v})
+    if (key_len > 1 && (s->n < 0 || s->n >= (1 << 24))) return fail(std::string(what) + ": rows are too far apart");
   return 0;
 }
 

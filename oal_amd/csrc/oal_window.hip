@@ -122,7 +122,7 @@ struct Board {
     for (int n = 0; n < 2; ++n) {
       const int r = (t >> 3) + 32 * n, c = 8 * (t & 7);
       float x[8];
-      load_row8(x, src + min(r, live - 1) * stride + min(c, D - 8));
+      load_row8(x, src + (unsigned)(min(r, live - 1) * (int)stride + min(c, D - 8)));
       const Frag<NP> f = split<NP>(x);
 #pragma unroll
       for (int e = 0; e < NP; ++e) *reinterpret_cast<bf16x8*>(tile.x + e * kTileElems + r * kTileRow + c) = f.p[e];
@@ -137,7 +137,7 @@ struct Board<uint16_t> {
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
       const int r = 32 * n + 8 * w + (lane >> 3);
-      copy16_to_lds(src + min(r, live - 1) * stride + min(c, D - 8), x + (32 * n + 8 * w) * 64);
+      copy16_to_lds(src + (unsigned)(min(r, live - 1) * (int)stride + min(c, D - 8)), x + (32 * n + 8 * w) * 64);
     }
   }
   __device__ Frag<1> rows(int r0, int t, int lane) const {
@@ -182,7 +182,7 @@ __device__ __forceinline__ Block query_block(const WindowArgs& a, const Shape& s
 // the weights as the values meet them. A row's maximum is moved only when a score
 // exceeds it by 2^8, which float32 sums do not mind: else nothing is rescaled.
 template <typename T>
-__global__ __launch_bounds__(256, kPartsOf<T> == 1 ? 3 : 1) void k_window_fwd(WindowArgs a, Shape sh, int qblocks, T* __restrict__ out,
+__global__ __launch_bounds__(256, kPartsOf<T> == 1 ? 4 : 1) void k_window_fwd(WindowArgs a, Shape sh, int qblocks, T* __restrict__ out,
                                                        float* __restrict__ lse) {
   constexpr int NP = kPartsOf<T>, CT = kColTiles<T>;
   __shared__ Board<T> K, V;
@@ -210,10 +210,10 @@ __global__ __launch_bounds__(256, kPartsOf<T> == 1 ? 3 : 1) void k_window_fwd(Wi
   const float scale = fabsf(a.scale) * kLog2e;
 
   // 32 keys
-  auto half_tile = [&](auto masked, bool far, int jh, int half) {
+  auto half_tile = [&](bool masked, bool far, int jh, int half) {
     // the scores that are hidden become none
     auto hide = [&](float (&y)[8], int x) {
-      if constexpr (decltype(masked)::value) {
+      if (masked) {
         const Sight sees(a, far);
 #pragma unroll
         for (int e = 0; e < 8; ++e)
@@ -229,9 +229,6 @@ __global__ __launch_bounds__(256, kPartsOf<T> == 1 ? 3 : 1) void k_window_fwd(Wi
 #pragma unroll
         for (int x = 0; x < CT; ++x) s[x][m] = mma(k, qf[x][e], s[x][m]);
       }
-    Frag<NP> vf[4];
-#pragma unroll
-    for (int m = 0; m < 4; ++m) vf[m] = V.columns(16 * m, half, lane);
     float y[CT][8], most[CT];
 #pragma unroll
     for (int x = 0; x < CT; ++x) {
@@ -266,8 +263,9 @@ __global__ __launch_bounds__(256, kPartsOf<T> == 1 ? 3 : 1) void k_window_fwd(Wi
     }
 #pragma unroll
     for (int m = 0; m < 4; ++m) {
+      const Frag<NP> v = V.columns(16 * m, half, lane);
 #pragma unroll
-      for (int x = 0; x < CT; ++x) acc[x][m] = mma(vf[m], p[x], acc[x][m]);
+      for (int x = 0; x < CT; ++x) acc[x][m] = mma(v, p[x], acc[x][m]);
     }
   };
   for (int tile = 0; tile < keys.tiles; ++tile) {
@@ -282,10 +280,7 @@ __global__ __launch_bounds__(256, kPartsOf<T> == 1 ? 3 : 1) void k_window_fwd(Wi
     for (int half = 0; half < 2; ++half) {
       const int jh = j0 + 32 * half;
       if (!sees_any(a, far, at.i0, at.i1, jh, jh + 31)) continue;
-      if (sees_all(a, far, at.i0, at.i1, jh, jh + 31))
-        half_tile(std::false_type{}, far, jh, half);
-      else
-        half_tile(std::true_type{}, far, jh, half);
+      half_tile(!sees_all(a, far, at.i0, at.i1, jh, jh + 31), far, jh, half);
     }
   }
   if (!at.works) return;
@@ -341,7 +336,7 @@ __global__ __launch_bounds__(256, kPartsOf<T> == 1 ? 3 : 1) void k_window_dq(Win
   f32x4 acc[CT][4] = {};
   const float scale = a.scale * kLog2e;
 
-  auto half_tile = [&](auto masked, bool far, int jh, int half) {
+  auto half_tile = [&](bool masked, bool far, int jh, int half) {
     f32x4 s[CT][2], d[CT][2];
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
@@ -367,7 +362,7 @@ __global__ __launch_bounds__(256, kPartsOf<T> == 1 ? 3 : 1) void k_window_dq(Win
 #pragma unroll
       for (int e = 0; e < 8; ++e)
         y[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][e >> 2][e & 3], scale, -base[x])) * d[x][e >> 2][e & 3];
-      if constexpr (decltype(masked)::value) {
+      if (masked) {
         const Sight sees(a, far);
 #pragma unroll
         for (int e = 0; e < 8; ++e)
@@ -394,10 +389,7 @@ __global__ __launch_bounds__(256, kPartsOf<T> == 1 ? 3 : 1) void k_window_dq(Win
     for (int half = 0; half < 2; ++half) {
       const int jh = j0 + 32 * half;
       if (!sees_any(a, far, at.i0, at.i1, jh, jh + 31)) continue;
-      if (sees_all(a, far, at.i0, at.i1, jh, jh + 31))
-        half_tile(std::false_type{}, far, jh, half);
-      else
-        half_tile(std::true_type{}, far, jh, half);
+      half_tile(!sees_all(a, far, at.i0, at.i1, jh, jh + 31), far, jh, half);
     }
   }
   if (!at.works) return;
@@ -415,7 +407,7 @@ __global__ __launch_bounds__(256, kPartsOf<T> == 1 ? 3 : 1) void k_window_dq(Win
 // dk and dv of 4 waves' keys over a part of the queries that see them. Blocks
 // 0 .. near - 1: through the window; the others: first keys seen from afar.
 template <typename T>
-__global__ __launch_bounds__(256, kPartsOf<T> == 1 ? 2 : 1) void k_window_dkv(WindowArgs a, WindowPlan plan, int kblocks, int near,
+__global__ __launch_bounds__(256, kPartsOf<T> == 1 ? 3 : 1) void k_window_dkv(WindowArgs a, WindowPlan plan, int kblocks, int near,
                                                        const float* __restrict__ lse, const T* __restrict__ dout,
                                                        const float* __restrict__ delta, float* __restrict__ part,
                                                        float* __restrict__ farpart) {
@@ -456,7 +448,7 @@ __global__ __launch_bounds__(256, kPartsOf<T> == 1 ? 2 : 1) void k_window_dkv(Wi
     }
   f32x4 dk[CT][4] = {}, dv[CT][4] = {};
   const float scale = a.scale * kLog2e;
-  auto half_tile = [&](auto masked, int ih, int half) {
+  auto half_tile = [&](bool masked, int ih, int half) {
     f32x4 s[CT][2], d[CT][2];
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
@@ -486,7 +478,7 @@ __global__ __launch_bounds__(256, kPartsOf<T> == 1 ? 2 : 1) void k_window_dkv(Wi
           yd[4 * m + e] = y[4 * m + e] * d[x][m][e];
         }
       }
-      if constexpr (decltype(masked)::value) {
+      if (masked) {
         const Sight sees(a, far);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -524,10 +516,7 @@ __global__ __launch_bounds__(256, kPartsOf<T> == 1 ? 2 : 1) void k_window_dkv(Wi
     for (int half = 0; half < 2; ++half) {
       const int ih = i0 + 32 * half, ie = min(a.Nk - 1, ih + 31);
       if (ih >= a.Nk || !sees_any(a, far, ih, ie, j0, j1)) continue;
-      if (ie == ih + 31 && sees_all(a, far, ih, ie, j0, j1))
-        half_tile(std::false_type{}, ih, half);
-      else
-        half_tile(std::true_type{}, ih, half);
+      half_tile(ie < ih + 31 || !sees_all(a, far, ih, ie, j0, j1), ih, half);
     }
   }
   float* to = far ? farpart : part;
