@@ -87,7 +87,7 @@ __device__ __forceinline__ void load_f32(Tile<NP>& s, const float* __restrict__ 
     const Frag<NP> f = split<NP>(v);
 #pragma unroll
     for (int e = 0; e < NP; ++e)
-      *reinterpret_cast<bf16x8*>(s.x + e * kTileElems + (i >> 3) * kTileRow + 8 * (i & 7)) = f.p[e];
+      *reinterpret_cast<bf16x8*>(s.x + e * kTileElems + tile_at(i >> 3, 8 * (i & 7))) = f.p[e];
   }
 }
 
@@ -110,7 +110,7 @@ __device__ __forceinline__ void put_parts(Tile<NP>& s, int row, int col, float x
 #pragma unroll
   for (int e = 0; e < NP; ++e) {
     const __bf16 y = static_cast<__bf16>(x);
-    s.x[e * kTileElems + row * kTileRow + col] = y;
+    s.x[e * kTileElems + tile_at(row, col)] = y;
     x -= static_cast<float>(y);
   }
 }
@@ -208,7 +208,7 @@ __global__ __launch_bounds__(kThr) void k_delta_chunk(DeltaArgs a, float* __rest
       }
       const Frag<3> f = split<3>(v);
 #pragma unroll
-      for (int e = 0; e < 3; ++e) *reinterpret_cast<bf16x8*>(P.x + e * kTileElems + r * kTileRow + col) = f.p[e];
+      for (int e = 0; e < 3; ++e) *reinterpret_cast<bf16x8*>(P.x + e * kTileElems + tile_at(r, col)) = f.p[e];
     }
     __syncthreads();
     const Tile<NP>& B = side == 0 ? K : V;
@@ -243,8 +243,10 @@ __global__ __launch_bounds__(kThr) void k_delta_chunk(DeltaArgs a, float* __rest
 
 // A walk over maps of 64 x 64 states, S -> M S + D, or back through them, S -> M^T S + D
 // (M's transpose where TR): a block per chain and 16 columns, a wave per 16 rows, who
-// hand each other their rows in three parts through LDS once per map. What a map
-// needs of memory is loaded kAhead maps before.
+// hand each other their rows through LDS once per map. What a map needs of memory is
+// loaded kAhead maps before. On the fp32 matrix cores, whose operands are M and S as
+// they lie in registers and LDS (sum index 16 q + 4 g + e of instruction q, e): their
+// 16 instructions per map are slower than 12 of bf16 parts, but there is nothing to split.
 struct Walk {
   const float* M;     // [units][maps][64][64]
   const float* D;
@@ -260,10 +262,7 @@ constexpr int kAhead = 4;
 
 template <bool TR, int COLS>
 __global__ __launch_bounds__(kThr) void k_delta_walk(Walk a) {
-  struct Rows {
-    bf16x4 x[3][4][64];
-  };
-  __shared__ Rows rows[2];
+  __shared__ f32x4 rows[2][4][64];
   const int t = threadIdx.x, lane = t & 63, w = wave_of(t), g = lane >> 4, c = lane & 15;
   // a chain's column groups on one XCD (blocks go round the 8 of them): they share its maps
   const int chains = a.units * a.segs, id = blockIdx.x, whole = chains / 8 * 8 * COLS;
@@ -282,7 +281,7 @@ __global__ __launch_bounds__(kThr) void k_delta_walk(Walk a) {
     const size_t at = base + (size_t)(a.back ? count - 1 - n : n) * kTile2;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const int k = 16 * q + 4 * g;  // perm order: tiles 2 t, 2 t + 1
+      const int k = 16 * q + 4 * g;
       if constexpr (TR) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) mm[4 * q + e] = a.M[at + (k + e) * 64 + 16 * w + c];
@@ -304,44 +303,25 @@ __global__ __launch_bounds__(kThr) void k_delta_walk(Walk a) {
     for (int x = 0; x < kAhead; ++x) {
       const int n = n0 + x;
       if (n >= count) break;
-      Rows& r = rows[x & 1];
-      float v[4] = {S[0], S[1], S[2], S[3]};
-#pragma unroll
-      for (int p = 0; p < 3; ++p) {
-        const bf16x4 y = __builtin_bit_cast(bf16x4, pack4(v));
-        r.x[p][w][lane] = y;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] -= static_cast<float>(y[e]);
-      }
+      rows[x & 1][w][lane] = S;
       if (a.each) {
         const size_t at = base + (size_t)(a.back ? count - 1 - n : n) * kTile2;
 #pragma unroll
         for (int i = 0; i < 4; ++i) a.each[at + (row + i) * 64 + col] = S[i];
       }
-      Frag<3> mf[2];
+      f32x4 next[4] = {{d[x][0], d[x][1], d[x][2], d[x][3]}};
+      float mm[16];
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        float y[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = m[x][8 * s + e];
-        mf[s] = split<3>(y);
-      }
-      S = f32x4{d[x][0], d[x][1], d[x][2], d[x][3]};
+      for (int e = 0; e < 16; ++e) mm[e] = m[x][e];
       fetch(n + kAhead, m[x], d[x]);
       lds_sync();
-      f32x4 half = {};
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        Frag<3> f;
+      for (int q = 0; q < 4; ++q) {
+        const f32x4 v = rows[x & 1][q][lane];
 #pragma unroll
-        for (int p = 0; p < 3; ++p)
-          f.p[p] = __builtin_shufflevector(r.x[p][2 * s][lane], r.x[p][2 * s + 1][lane], 0, 1, 2, 3, 4, 5, 6, 7);
-        if (s == 0)
-          S = mma(mf[s], f, S);
-        else
-          half = mma(mf[s], f, half);
+        for (int e = 0; e < 4; ++e) next[q] = __builtin_amdgcn_mfma_f32_16x16x4f32(mm[4 * q + e], v[e], next[q], 0, 0, 0);
       }
-      S += half;
+      S = (next[0] + next[1]) + (next[2] + next[3]);
     }
   }
   float* end = unit ? a.mend : a.end;
@@ -491,7 +471,7 @@ __global__ __launch_bounds__(kThr) void k_delta_bwd_local(DeltaArgs a, const T* 
 #pragma unroll
       for (int x = 0; x < 3; ++x) {
         const bf16x4 y = __builtin_bit_cast(bf16x4, pack4(v));
-        *reinterpret_cast<bf16x4*>(P.x + x * kTileElems + own * kTileRow + 16 * m + 4 * g) = y;
+        *reinterpret_cast<bf16x4*>(P.x + x * kTileElems + tile_at(own, 16 * m + 4 * g)) = y;
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] -= static_cast<float>(y[i]);
       }

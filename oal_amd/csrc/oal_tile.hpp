@@ -23,8 +23,7 @@
 
 namespace oal {
 
-constexpr int kTileRow = 72;  // bf16 of an LDS row: 144 bytes, 16 rows start in distinct banks
-constexpr int kTileElems = 64 * kTileRow;
+constexpr int kTileElems = 64 * 64;
 
 template <int NP>
 struct Frag {
@@ -66,7 +65,9 @@ __device__ __forceinline__ f32x4 mma(const Frag<NA>& a, const Frag<NB>& b, f32x4
   return c;
 }
 
-// LDS tile: NP parts of 64 rows of kTileRow bf16.
+// LDS tile: NP parts of 64 rows of 64 bf16. The 16-byte piece c of row r stands at c ^ r % 8:
+// reads of one column's pieces over 8 rows, and of rows, meet all banks.
+__device__ __forceinline__ int tile_at(int r, int c) { return r * 64 + 8 * ((c >> 3) ^ (r & 7)) + (c & 7); }
 template <int NP>
 struct alignas(16) Tile {
   __bf16 x[NP * kTileElems];
@@ -76,7 +77,7 @@ struct alignas(16) Tile {
 template <int N = 0, int NP>
 __device__ __forceinline__ Frag<(N ? N : NP)> row_frag(const Tile<NP>& s, int r0, int t, int lane) {
   Frag<(N ? N : NP)> f;
-  const __bf16* p = s.x + (r0 + (lane & 15)) * kTileRow + 32 * t + 8 * (lane >> 4);
+  const __bf16* p = s.x + tile_at(r0 + (lane & 15), 32 * t + 8 * (lane >> 4));
 #pragma unroll
   for (int e = 0; e < (N ? N : NP); ++e) f.p[e] = *reinterpret_cast<const bf16x8*>(p + e * kTileElems);
   return f;
@@ -85,11 +86,12 @@ __device__ __forceinline__ Frag<(N ? N : NP)> row_frag(const Tile<NP>& s, int r0
 template <int N = 0, int NP>
 __device__ __forceinline__ Frag<(N ? N : NP)> row_frag_perm(const Tile<NP>& s, int r0, int t, int lane) {
   Frag<(N ? N : NP)> f;
-  const __bf16* p = s.x + (r0 + (lane & 15)) * kTileRow + 32 * t + 4 * (lane >> 4);
+  const int r = r0 + (lane & 15), c = 32 * t + 4 * (lane >> 4);
+  const __bf16 *p = s.x + tile_at(r, c), *q = s.x + tile_at(r, c + 16);
 #pragma unroll
   for (int e = 0; e < (N ? N : NP); ++e) {
     const bf16x4 lo = *reinterpret_cast<const bf16x4*>(p + e * kTileElems);
-    const bf16x4 hi = *reinterpret_cast<const bf16x4*>(p + e * kTileElems + 16);
+    const bf16x4 hi = *reinterpret_cast<const bf16x4*>(q + e * kTileElems);
     f.p[e] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
   }
   return f;
@@ -110,18 +112,19 @@ template <int N = 0, int NP>
 __device__ __forceinline__ Frag<(N ? N : NP)> col_frag_perm(const Tile<NP>& s, int c0, int t, int lane) {
   Frag<(N ? N : NP)> f;
   const int g = lane >> 4, i = lane & 15;
-  const __bf16* p = s.x + (32 * t + 4 * g + (i >> 2)) * kTileRow + c0 + 4 * (i & 3);
+  const __bf16* p = s.x + tile_at(32 * t + 4 * g + (i >> 2), c0 + 4 * (i & 3));
 #pragma unroll
-  for (int e = 0; e < (N ? N : NP); ++e) f.p[e] = tr_rows(p + e * kTileElems, p + e * kTileElems + 16 * kTileRow);
+  for (int e = 0; e < (N ? N : NP); ++e) f.p[e] = tr_rows(p + e * kTileElems, p + e * kTileElems + 16 * 64);
   return f;
 }
 template <int N = 0, int NP>
 __device__ __forceinline__ Frag<(N ? N : NP)> col_frag(const Tile<NP>& s, int c0, int t, int lane) {
   Frag<(N ? N : NP)> f;
   const int g = lane >> 4, i = lane & 15;
-  const __bf16* p = s.x + (32 * t + 8 * g + (i >> 2)) * kTileRow + c0 + 4 * (i & 3);
+  const int r = 32 * t + 8 * g + (i >> 2), c = c0 + 4 * (i & 3);
+  const __bf16 *p = s.x + tile_at(r, c), *q = s.x + tile_at(r + 4, c);
 #pragma unroll
-  for (int e = 0; e < (N ? N : NP); ++e) f.p[e] = tr_rows(p + e * kTileElems, p + e * kTileElems + 4 * kTileRow);
+  for (int e = 0; e < (N ? N : NP); ++e) f.p[e] = tr_rows(p + e * kTileElems, q + e * kTileElems);
   return f;
 }
 
@@ -206,7 +209,7 @@ __device__ __forceinline__ void load_tile(Tile<NP>& s, const T* __restrict__ src
 #pragma unroll
     for (int x = 0; x < kIt; ++x) {
       const int i = t + NT * x;
-      if (i < ROWS * 8) *reinterpret_cast<bf16x8*>(s.x + (i >> 3) * kTileRow + 8 * (i & 7)) = f[x].p[0];
+      if (i < ROWS * 8) *reinterpret_cast<bf16x8*>(s.x + tile_at(i >> 3, 8 * (i & 7))) = f[x].p[0];
     }
   } else {
 #pragma unroll
@@ -215,7 +218,7 @@ __device__ __forceinline__ void load_tile(Tile<NP>& s, const T* __restrict__ src
       if (i < ROWS * 8) {
         const Frag<NP> f = global_frag<NP>(src + r * stride + c, r < live && c < D);
 #pragma unroll
-        for (int e = 0; e < NP; ++e) *reinterpret_cast<bf16x8*>(s.x + e * kTileElems + r * kTileRow + c) = f.p[e];
+        for (int e = 0; e < NP; ++e) *reinterpret_cast<bf16x8*>(s.x + e * kTileElems + tile_at(r, c)) = f.p[e];
       }
     }
   }

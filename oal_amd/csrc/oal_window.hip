@@ -100,24 +100,21 @@ __device__ __forceinline__ bool sees_all(const WindowArgs& a, bool far, int i0, 
   return far ? j1 < a.sinks && i0 - j1 >= a.window : j1 <= i0 && i1 - j0 < a.window;
 }
 
-// 64 rows of a tensor in LDS as a block's 256 threads bring them there. bf16 rows
-// go there without passing registers, 16 bytes a lane in the order of the lanes: the 16-byte pieces of row r
-// stand at c ^ r % 8, so that reads of 8 rows meet all banks. Other types are split into parts on the way.
-// Rows past the last and columns past the width repeat others: what they meet is
-// masked or a zero of the other operand. Two barriers around bring(): all waves past their
-// reads before it, all rows there behind it (__syncthreads waits for the copies).
-template <typename T>
-struct Board {
-  static constexpr int NP = kPartsOf<T>;
-  Tile<NP> tile;
-  __device__ void bring(const T* src, int64_t stride, int D, int live, int t) {
-    load_rows(src, stride, D, live, t);
-  }
-  __device__ Frag<NP> rows(int r0, int t, int lane) const { return row_frag(tile, r0, t, lane); }
-  __device__ Frag<NP> columns(int c0, int t, int lane) const { return col_frag_perm(tile, c0, t, lane); }
-
- private:
-  __device__ void load_rows(const T* src, int64_t stride, int D, int live, int t) {
+// 64 rows of a tensor into an LDS tile by a block's 256 threads; bf16 rows go there
+// without passing registers, 16 bytes a lane in the order of the lanes. Rows past the last and columns
+// past the width repeat others: what they meet is masked or a zero of the other operand.
+// Two barriers around it: all waves past their reads before, all rows there behind
+// (__syncthreads waits for the copies).
+template <int NP, typename T>
+__device__ __forceinline__ void bring(Tile<NP>& s, const T* src, int64_t stride, int D, int live, int t) {
+  if constexpr (NP == 1) {
+    const int lane = t & 63, w = wave_of(t), c = 8 * ((lane & 7) ^ (lane >> 3));
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      const int r = 32 * n + 8 * w + (lane >> 3);
+      copy16_to_lds(src + (unsigned)(min(r, live - 1) * (int)stride + min(c, D - 8)), s.x + (32 * n + 8 * w) * 64);
+    }
+  } else {
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
       const int r = (t >> 3) + 32 * n, c = 8 * (t & 7);
@@ -125,31 +122,11 @@ struct Board {
       load_row8(x, src + (unsigned)(min(r, live - 1) * (int)stride + min(c, D - 8)));
       const Frag<NP> f = split<NP>(x);
 #pragma unroll
-      for (int e = 0; e < NP; ++e) *reinterpret_cast<bf16x8*>(tile.x + e * kTileElems + r * kTileRow + c) = f.p[e];
+      for (int e = 0; e < NP; ++e) *reinterpret_cast<bf16x8*>(s.x + e * kTileElems + tile_at(r, c)) = f.p[e];
     }
   }
-};
-template <>
-struct Board<uint16_t> {
-  alignas(16) __bf16 x[64 * 64];
-  __device__ void bring(const uint16_t* src, int64_t stride, int D, int live, int t) {
-    const int lane = t & 63, w = wave_of(t), c = 8 * ((lane & 7) ^ (lane >> 3));
-#pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      const int r = 32 * n + 8 * w + (lane >> 3);
-      copy16_to_lds(src + (unsigned)(min(r, live - 1) * (int)stride + min(c, D - 8)), x + (32 * n + 8 * w) * 64);
-    }
-  }
-  __device__ Frag<1> rows(int r0, int t, int lane) const {
-    const int r = lane & 15;
-    return {{*reinterpret_cast<const bf16x8*>(x + (r0 + r) * 64 + 8 * ((4 * t + (lane >> 4)) ^ (r & 7)))}};
-  }
-  __device__ Frag<1> columns(int c0, int t, int lane) const {
-    const int g = lane >> 4, i = lane & 15, r = 4 * g + (i >> 2);
-    const __bf16* p = x + (32 * t + r) * 64 + 8 * (((c0 >> 3) + ((i >> 1) & 1)) ^ (r & 7)) + 4 * (i & 1);
-    return {{tr_rows(p, p + 16 * 64)}};
-  }
-};
+}
+
 // What a block of the query side works on.
 struct Block {
   int b, hk, h, q0, i0, i1, first, last;
@@ -185,7 +162,7 @@ template <typename T>
 __global__ __launch_bounds__(256, kPartsOf<T> == 1 ? 4 : 1) void k_window_fwd(WindowArgs a, Shape sh, int qblocks, T* __restrict__ out,
                                                        float* __restrict__ lse) {
   constexpr int NP = kPartsOf<T>, CT = kColTiles<T>;
-  __shared__ Board<T> K, V;
+  __shared__ Tile<NP> K, V;
   const int t = threadIdx.x, lane = t & 63, w = wave_of(t), g = lane >> 4, c = lane & 15;
   const Block at = query_block<T>(a, sh, qblocks, w);
   const Keys keys(a, at.first, at.last);
@@ -225,7 +202,7 @@ __global__ __launch_bounds__(256, kPartsOf<T> == 1 ? 4 : 1) void k_window_fwd(Wi
     for (int m = 0; m < 2; ++m)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const Frag<NP> k = K.rows(32 * half + 16 * m, e, lane);
+        const Frag<NP> k = row_frag(K, 32 * half + 16 * m, e, lane);
 #pragma unroll
         for (int x = 0; x < CT; ++x) s[x][m] = mma(k, qf[x][e], s[x][m]);
       }
@@ -263,7 +240,7 @@ __global__ __launch_bounds__(256, kPartsOf<T> == 1 ? 4 : 1) void k_window_fwd(Wi
     }
 #pragma unroll
     for (int m = 0; m < 4; ++m) {
-      const Frag<NP> v = V.columns(16 * m, half, lane);
+      const Frag<NP> v = col_frag_perm(V, 16 * m, half, lane);
 #pragma unroll
       for (int x = 0; x < CT; ++x) acc[x][m] = mma(v, p[x], acc[x][m]);
     }
@@ -272,8 +249,8 @@ __global__ __launch_bounds__(256, kPartsOf<T> == 1 ? 4 : 1) void k_window_fwd(Wi
     const int j0 = keys.start(tile), live = min(64, at.last + 1 - j0);
     const bool far = tile < keys.far;
     if (tile) lds_sync();
-    K.bring(rows_at<T>(a.k, at.b, at.hk, j0), a.k.n, a.D, live, t);
-    V.bring(rows_at<T>(a.v, at.b, at.hk, j0), a.v.n, a.DV, live, t);
+    bring(K, rows_at<T>(a.k, at.b, at.hk, j0), a.k.n, a.D, live, t);
+    bring(V, rows_at<T>(a.v, at.b, at.hk, j0), a.v.n, a.DV, live, t);
     __syncthreads();
     if (!at.works) continue;
 #pragma nounroll
@@ -303,7 +280,7 @@ __global__ __launch_bounds__(256, kPartsOf<T> == 1 ? 3 : 1) void k_window_dq(Win
                                                       const float* __restrict__ lse, const T* __restrict__ dout,
                                                       float* __restrict__ delta, T* __restrict__ dq) {
   constexpr int NP = kPartsOf<T>, CT = kColTiles<T>;
-  __shared__ Board<T> K, V;
+  __shared__ Tile<NP> K, V;
   const int t = threadIdx.x, lane = t & 63, w = wave_of(t), g = lane >> 4, c = lane & 15;
   const Block at = query_block<T>(a, sh, qblocks, w);
   const Keys keys(a, at.first, at.last);
@@ -347,7 +324,7 @@ __global__ __launch_bounds__(256, kPartsOf<T> == 1 ? 3 : 1) void k_window_dq(Win
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const Frag<NP> k = K.rows(32 * half + 16 * m, e, lane), v = V.rows(32 * half + 16 * m, e, lane);
+        const Frag<NP> k = row_frag(K, 32 * half + 16 * m, e, lane), v = row_frag(V, 32 * half + 16 * m, e, lane);
 #pragma unroll
         for (int x = 0; x < CT; ++x) {
           s[x][m] = mma(k, qf[x][e], s[x][m]);
@@ -372,7 +349,7 @@ __global__ __launch_bounds__(256, kPartsOf<T> == 1 ? 3 : 1) void k_window_dq(Win
     }
 #pragma unroll
     for (int m = 0; m < 4; ++m) {
-      const Frag<NP> k = K.columns(16 * m, half, lane);
+      const Frag<NP> k = col_frag_perm(K, 16 * m, half, lane);
 #pragma unroll
       for (int x = 0; x < CT; ++x) acc[x][m] = mma(k, p[x], acc[x][m]);
     }
@@ -381,8 +358,8 @@ __global__ __launch_bounds__(256, kPartsOf<T> == 1 ? 3 : 1) void k_window_dq(Win
     const int j0 = keys.start(tile), live = min(64, at.last + 1 - j0);
     const bool far = tile < keys.far;
     if (tile) lds_sync();
-    K.bring(rows_at<T>(a.k, at.b, at.hk, j0), a.k.n, a.D, live, t);
-    V.bring(rows_at<T>(a.v, at.b, at.hk, j0), a.v.n, a.DV, live, t);
+    bring(K, rows_at<T>(a.k, at.b, at.hk, j0), a.k.n, a.D, live, t);
+    bring(V, rows_at<T>(a.v, at.b, at.hk, j0), a.v.n, a.DV, live, t);
     __syncthreads();
     if (!at.works) continue;
 #pragma nounroll
@@ -412,7 +389,7 @@ __global__ __launch_bounds__(256, kPartsOf<T> == 1 ? 3 : 1) void k_window_dkv(Wi
                                                        const float* __restrict__ delta, float* __restrict__ part,
                                                        float* __restrict__ farpart) {
   constexpr int NP = kPartsOf<T>, CT = kColTiles<T>, kKeys = 4 * kCols<T>;
-  __shared__ Board<T> Q, O;
+  __shared__ Tile<NP> Q, O;
   __shared__ alignas(16) float base[64], dot[64];
   const int t = threadIdx.x, lane = t & 63, w = wave_of(t), g = lane >> 4, c = lane & 15;
   const int R = a.Hq / a.Hk, off = a.Nk - a.Nq;
@@ -457,7 +434,7 @@ __global__ __launch_bounds__(256, kPartsOf<T> == 1 ? 3 : 1) void k_window_dkv(Wi
       for (int x = 0; x < CT; ++x) s[x][m] = f32x4{}, d[x][m] = dt;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const Frag<NP> q = Q.rows(32 * half + 16 * m, e, lane), o = O.rows(32 * half + 16 * m, e, lane);
+        const Frag<NP> q = row_frag(Q, 32 * half + 16 * m, e, lane), o = row_frag(O, 32 * half + 16 * m, e, lane);
 #pragma unroll
         for (int x = 0; x < CT; ++x) {
           s[x][m] = mma(q, kf[x][e], s[x][m]);
@@ -493,7 +470,7 @@ __global__ __launch_bounds__(256, kPartsOf<T> == 1 ? 3 : 1) void k_window_dkv(Wi
     }
 #pragma unroll
     for (int m = 0; m < 4; ++m) {
-      const Frag<NP> q = Q.columns(16 * m, half, lane), o = O.columns(16 * m, half, lane);
+      const Frag<NP> q = col_frag_perm(Q, 16 * m, half, lane), o = col_frag_perm(O, 16 * m, half, lane);
 #pragma unroll
       for (int x = 0; x < CT; ++x) {
         dk[x][m] = mma(q, z[x], dk[x][m]);
@@ -506,8 +483,8 @@ __global__ __launch_bounds__(256, kPartsOf<T> == 1 ? 3 : 1) void k_window_dkv(Wi
     if (++tile == tiles) tile = 0, ++r;
     const size_t at = ((size_t)b * a.Hq + h) * a.Nq + (i0 - off);
     if (step) lds_sync();
-    Q.bring(rows_at<T>(a.q, b, h, i0 - off), a.q.n, a.D, live, t);
-    O.bring(dout + at * a.DV, a.DV, a.DV, live, t);
+    bring(Q, rows_at<T>(a.q, b, h, i0 - off), a.q.n, a.D, live, t);
+    bring(O, dout + at * a.DV, a.DV, a.DV, live, t);
     if (t < 64) base[t] = lse[at + min(t, live - 1)];
     if (t >= 64 && t < 128) dot[t - 64] = -delta[at + min(t - 64, live - 1)];
     __syncthreads();
@@ -590,7 +567,8 @@ __device__ __forceinline__ Frag<NP> frag_of(const Row8<T>& r) {
 template <typename T>
 __global__ __launch_bounds__(256) void k_window_step(WindowStepArgs a) {
   constexpr int NP = kPartsOf<T>;
-  // 32 rows of V per wave; after the walk the waves' sums
+  // 32 rows of V per wave, 144 bytes each; after the walk the waves' sums
+  constexpr int kTileRow = 72;
   struct alignas(16) Rows {
     __bf16 x[NP * 32 * kTileRow];
   };
