@@ -251,7 +251,7 @@ struct Walk {
   const float* M;     // [units][maps][64][64]
   const float* D;
   const float* init;  // [rows][cols] state the walk starts from, by unit (segs == 1) or segment (null: zero)
-  float* each;        // [units][maps][64][64]: the state before each map (null: not wanted)
+  float* each;        // [units][maps][64][64]: the state before each map (with 4 column groups)
   float* end;         // the same: the state after the last map (null: not wanted)
   float* mend;        // with 8 column groups: the product of the segment's maps
   int maps, segs, len, units, rows, cols;
@@ -292,38 +292,43 @@ __global__ __launch_bounds__(kThr) void k_delta_walk(Walk a) {
       dd[q] = unit ? 0.f : a.D[at + (row + q) * 64 + col];
     }
   };
-#pragma unroll
-  for (int n = 0; n < kAhead; ++n) fetch(n, m[n], d[n]);
   f32x4 S;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     S[i] = unit ? (row + i == col ? 1.f : 0.f) : a.init && held(i) ? a.init[slot(i)] : 0.f;
-  for (int n0 = 0; n0 < count; n0 += kAhead) {
+  asm volatile("" : "+v"(S));  // here, not in the walk, is waited for it
 #pragma unroll
-    for (int x = 0; x < kAhead; ++x) {
-      const int n = n0 + x;
-      if (n >= count) break;
-      rows[x & 1][w][lane] = S;
-      if (a.each) {
-        const size_t at = base + (size_t)(a.back ? count - 1 - n : n) * kTile2;
+  for (int n = 0; n < kAhead; ++n) fetch(n, m[n], d[n]);
+  // the number of loads in flight is the same on every way to a step, so that it waits for its own
+  auto step = [&](int n, int x) {
+    rows[x & 1][w][lane] = S;
+    if constexpr (COLS == 4) {
+      const size_t at = base + (size_t)(a.back ? count - 1 - n : n) * kTile2;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) a.each[at + (row + i) * 64 + col] = S[i];
-      }
-      f32x4 next[4] = {{d[x][0], d[x][1], d[x][2], d[x][3]}};
-      float mm[16];
-#pragma unroll
-      for (int e = 0; e < 16; ++e) mm[e] = m[x][e];
-      fetch(n + kAhead, m[x], d[x]);
-      lds_sync();
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const f32x4 v = rows[x & 1][q][lane];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) next[q] = __builtin_amdgcn_mfma_f32_16x16x4f32(mm[4 * q + e], v[e], next[q], 0, 0, 0);
-      }
-      S = (next[0] + next[1]) + (next[2] + next[3]);
+      for (int i = 0; i < 4; ++i) a.each[at + (row + i) * 64 + col] = S[i];
     }
-  }
+    f32x4 next[4] = {{d[x][0], d[x][1], d[x][2], d[x][3]}};
+    lds_sync();
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const f32x4 v = rows[x & 1][q][lane];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        next[q] = __builtin_amdgcn_mfma_f32_16x16x4f32(m[x][4 * q + e], v[e], next[q], 0, 0, 0);
+    }
+    S = (next[0] + next[1]) + (next[2] + next[3]);
+    // behind the products, into the registers that they are done with: loaded before, the
+    // values would go through others and be waited for at once
+    __builtin_amdgcn_sched_barrier(0);
+    fetch(n + kAhead, m[x], d[x]);
+  };
+  int n = 0;
+  for (; n + kAhead <= count; n += kAhead)
+#pragma unroll
+    for (int x = 0; x < kAhead; ++x) step(n + x, x);
+#pragma unroll
+  for (int x = 0; x < kAhead - 1; ++x)
+    if (n + x < count) step(n + x, x);
   float* end = unit ? a.mend : a.end;
   if (!end) return;
 #pragma unroll
