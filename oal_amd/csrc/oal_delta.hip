@@ -35,13 +35,32 @@ constexpr int kTile2 = 64 * 64;
 // Smallest log-decay: exp of it is zero, and 64 of them leave the sums' differences exact.
 constexpr double kLeast = -1e4;
 
-struct Gates {
-  float hi[64], lo[64], beta[64];  // log2 of the decay up to and with token i, in two parts
-  __device__ float between(int i, int j) const {
-    return __builtin_amdgcn_exp2f((hi[i] - hi[j]) + (lo[i] - lo[j]));
-  }
-  __device__ float since(int i) const { return __builtin_amdgcn_exp2f(hi[i] + lo[i]); }
+// Of a chunk's tokens: log2 of the decay up to and with the token, in two parts; beta; the decay since
+// the chunk's start and until its end. Formed once, by k_delta_chunk.
+struct alignas(16) Gates {
+  float hi[64], lo[64], beta[64], since[64], until[64];
 };
+constexpr int kGates = sizeof(Gates) / sizeof(float);
+
+__device__ __forceinline__ f32x4 four(const float* p) { return *reinterpret_cast<const f32x4*>(p); }
+// Decays from token (hi, lo) to tokens r .. r + 3, and from those to it.
+__device__ __forceinline__ f32x4 decay_to(const Gates& s, int r, float hi, float lo) {
+  const f32x4 h = four(s.hi + r), l = four(s.lo + r);
+  f32x4 y;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y[i] = __builtin_amdgcn_exp2f((h[i] - hi) + (l[i] - lo));
+  return y;
+}
+__device__ __forceinline__ f32x4 decay_from(const Gates& s, int r, float hi, float lo) {
+  const f32x4 h = four(s.hi + r), l = four(s.lo + r);
+  f32x4 y;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y[i] = __builtin_amdgcn_exp2f((hi - h[i]) + (lo - l[i]));
+  return y;
+}
+__device__ __forceinline__ void fetch_gates(Gates& s, const float* __restrict__ src, int t) {
+  if (t < kGates / 4) reinterpret_cast<float4*>(&s)[t] = reinterpret_cast<const float4*>(src)[t];
+}
 
 template <typename T>
 __device__ __forceinline__ float beta_at(const DeltaArgs& a, int b, int h, int tok) {
@@ -51,7 +70,7 @@ __device__ __forceinline__ float beta_at(const DeltaArgs& a, int b, int h, int t
 
 // The first wave of the block; tokens past N decay nothing and write nothing.
 template <typename T>
-__device__ __forceinline__ void load_gates(Gates& s, const DeltaArgs& a, int b, int h, int tok0, int t) {
+__device__ __forceinline__ void form_gates(Gates& s, const DeltaArgs& a, int b, int h, int tok0, int t) {
   if (t >= 64) return;
   const int tok = tok0 + t;
   double x = 0;
@@ -66,29 +85,18 @@ __device__ __forceinline__ void load_gates(Gates& s, const DeltaArgs& a, int b, 
     const double y = __shfl_up(x, off, 64);
     if (t >= off) x += y;
   }
-  s.hi[t] = (float)x;
-  s.lo[t] = (float)(x - (double)(float)x);
+  const double end = __shfl(x, 63, 64);
+  const float hi = (float)x, lo = (float)(x - (double)hi);
+  s.hi[t] = hi;
+  s.lo[t] = lo;
   s.beta[t] = beta;
+  s.since[t] = __builtin_amdgcn_exp2f(hi + lo);
+  s.until[t] = __builtin_amdgcn_exp2f((float)(end - x));
 }
 
 template <typename T>
 __device__ __forceinline__ const T* rows_of(const Strided& s, int b, int h, int tok0) {
   return static_cast<const T*>(s.p) + b * s.b + h * s.h + (int64_t)tok0 * s.n;
-}
-
-// 64 x 64 fp32 values into NP parts.
-template <int NP>
-__device__ __forceinline__ void load_f32(Tile<NP>& s, const float* __restrict__ src, int t) {
-#pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    const int i = t + kThr * x;
-    float v[8];
-    load_row8(v, src + 8 * i);
-    const Frag<NP> f = split<NP>(v);
-#pragma unroll
-    for (int e = 0; e < NP; ++e)
-      *reinterpret_cast<bf16x8*>(s.x + e * kTileElems + tile_at(i >> 3, 8 * (i & 7))) = f.p[e];
-  }
 }
 
 // One wave: c[16][16] += a[16][K] b[K][16] of fp32 tiles in LDS (rows of 68) on the fp32 matrix cores.
@@ -121,8 +129,8 @@ __device__ __forceinline__ void put_parts(Tile<NP>& s, int row, int col, float x
 // the rule for two blocks, [L11 0; L21 L22]^-1 = [T11 0; -T22 L21 T11, T22], on the
 // fp32 matrix cores. In the products a wave owns 16 columns of M and of D.
 template <typename T>
-__global__ __launch_bounds__(kThr) void k_delta_chunk(DeltaArgs a, float* __restrict__ Tout, float* __restrict__ Mout,
-                                                      float* __restrict__ Dout) {
+__global__ __launch_bounds__(kThr) void k_delta_chunk(DeltaArgs a, float* __restrict__ Gout, float* __restrict__ Tout,
+                                                      float* __restrict__ Mout, float* __restrict__ Dout) {
   constexpr int NP = kPartsOf<T>;
   __shared__ Tile<NP> K, V;
   __shared__ Gates gate;
@@ -138,22 +146,32 @@ __global__ __launch_bounds__(kThr) void k_delta_chunk(DeltaArgs a, float* __rest
   const int ch = blockIdx.x % a.NC, u = blockIdx.x / a.NC, b = u / a.Hv, h = u % a.Hv;
   const int tok0 = 64 * ch, live = min(64, a.N - tok0);
   const size_t at = ((size_t)u * a.NC + ch) * kTile2;
-  load_tile<64, kThr>(K, rows_of<T>(a.k, b, h / (a.Hv / a.Hk), tok0), a.k.n, a.D, live, t);
-  load_tile<64, kThr>(V, rows_of<T>(a.v, b, h, tok0), a.v.n, a.DV, live, t);
-  load_gates<T>(gate, a, b, h, tok0, t);
-  __syncthreads();
-  for (int n = 0; n < 4; ++n) {
-    f32x4 kk = {};
-    if (n <= w)
-      for (int s = 0; s < 2; ++s) kk = mma(row_frag(K, 16 * w, s, lane), row_frag(K, 16 * n, s, lane), kk);
+  Incoming<NP, T> ki, vi;
+  ki.fetch(rows_of<T>(a.k, b, h / (a.Hv / a.Hk), tok0), a.k.n, a.D, live, t);
+  vi.fetch(rows_of<T>(a.v, b, h, tok0), a.v.n, a.DV, live, t);
+  form_gates<T>(gate, a, b, h, tok0, t);
+  ki.store(K, t);
+  vi.store(V, t);
+  lds_sync();
+  fetch_gates(*reinterpret_cast<Gates*>(Gout + ((size_t)u * a.NC + ch) * kGates), reinterpret_cast<const float*>(&gate), t);
+  {
+    const Frag<NP> k0 = row_frag(K, 16 * w, 0, lane), k1 = row_frag(K, 16 * w, 1, lane);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int i = 16 * w + 4 * g + r, j = 16 * n + c;
-      L[i * kRow32 + j] = j < i ? kk[r] * gate.between(i, j) * gate.beta[j] : 0.f;
-      S[i * kRow32 + j] = 0.f;
+    for (int n = 0; n < 4; ++n) {
+      const int j = 16 * n + c, row = 16 * w + 4 * g;
+      f32x4 kk = {};
+      if (n <= w) {
+        kk = mma(k0, row_frag(K, 16 * n, 0, lane), kk);
+        kk = mma(k1, row_frag(K, 16 * n, 1, lane), kk) * decay_to(gate, row, gate.hi[j], gate.lo[j]) * gate.beta[j];
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        L[(row + r) * kRow32 + j] = j < row + r ? kk[r] : 0.f;
+        S[(row + r) * kRow32 + j] = 0.f;
+      }
     }
   }
-  __syncthreads();
+  lds_sync();
   if (lane < 16) {
     const float* l = L + (16 * w) * kRow32 + 16 * w;
     float x[16];
@@ -166,7 +184,7 @@ __global__ __launch_bounds__(kThr) void k_delta_chunk(DeltaArgs a, float* __rest
       S[(16 * w + i) * kRow32 + 16 * w + c] = acc;
     }
   }
-  __syncthreads();
+  lds_sync();
   f32x4 y = {};
   if (w < 2) {
     const int o = 32 * w;
@@ -174,23 +192,23 @@ __global__ __launch_bounds__(kThr) void k_delta_chunk(DeltaArgs a, float* __rest
 #pragma unroll
     for (int r = 0; r < 4; ++r) Y[(16 * w + 4 * g + r) * kRow32 + c] = y[r];
   }
-  __syncthreads();
+  lds_sync();
   if (w < 2) {
     const int o = 32 * w;
     y = mma_f32<16>(S + (o + 16) * kRow32 + o + 16, Y + 16 * w * kRow32, f32x4{}, lane);
 #pragma unroll
     for (int r = 0; r < 4; ++r) S[(o + 16 + 4 * g + r) * kRow32 + o + c] = -y[r];
   }
-  __syncthreads();
+  lds_sync();
   const int m2 = 16 * (w >> 1), n2 = 16 * (w & 1);
   y = mma_f32<32>(L + (32 + m2) * kRow32, S + n2, f32x4{}, lane);
 #pragma unroll
   for (int r = 0; r < 4; ++r) Y[(m2 + 4 * g + r) * kRow32 + n2 + c] = y[r];
-  __syncthreads();
+  lds_sync();
   y = mma_f32<32>(S + (32 + m2) * kRow32 + 32, Y + n2, f32x4{}, lane);
 #pragma unroll
   for (int r = 0; r < 4; ++r) S[(32 + m2 + 4 * g + r) * kRow32 + n2 + c] = -y[r];
-  __syncthreads();
+  lds_sync();
   // twice: T's columns scaled by e^G times K, T times V; then what the chunk writes of it
 #pragma unroll
   for (int side = 0; side < 2; ++side) {
@@ -203,14 +221,15 @@ __global__ __launch_bounds__(kThr) void k_delta_chunk(DeltaArgs a, float* __rest
         float4* dst = reinterpret_cast<float4*>(Tout + at + 8 * i);
         dst[0] = make_float4(v[0], v[1], v[2], v[3]);
         dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+        const f32x4 g0 = four(gate.since + col), g1 = four(gate.since + col + 4);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] *= gate.since(col + e);
+        for (int e = 0; e < 8; ++e) v[e] *= e < 4 ? g0[e] : g1[e - 4];
       }
       const Frag<3> f = split<3>(v);
 #pragma unroll
       for (int e = 0; e < 3; ++e) *reinterpret_cast<bf16x8*>(P.x + e * kTileElems + tile_at(r, col)) = f.p[e];
     }
-    __syncthreads();
+    lds_sync();
     const Tile<NP>& B = side == 0 ? K : V;
     const Frag<NP> b0 = col_frag(B, 16 * w, 0, lane), b1 = col_frag(B, 16 * w, 1, lane);
     f32x4 z[4];
@@ -218,15 +237,11 @@ __global__ __launch_bounds__(kThr) void k_delta_chunk(DeltaArgs a, float* __rest
     for (int m = 0; m < 4; ++m) {
       z[m] = mma(row_frag(P, 16 * m, 0, lane), b0, f32x4{});
       if (m >= 2) z[m] = mma(row_frag(P, 16 * m, 1, lane), b1, z[m]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = 16 * m + 4 * g + i;
-        const float x = gate.beta[row] * gate.between(63, row);
-        z[m][i] *= side == 0 ? -x : x;
-      }
+      const f32x4 x = four(gate.beta + 16 * m + 4 * g) * four(gate.until + 16 * m + 4 * g);
+      z[m] *= side == 0 ? -x : x;
     }
     const Frag<3> z0 = acc_frag<3>(z[0], z[1]), z1 = acc_frag<3>(z[2], z[3]);
-    const float last = gate.since(63);
+    const float last = gate.since[63];
 #pragma unroll
     for (int m = 0; m < 4; ++m) {
       f32x4 x = mma(col_frag_perm(K, 16 * m, 0, lane), z0, f32x4{});
@@ -237,7 +252,7 @@ __global__ __launch_bounds__(kThr) void k_delta_chunk(DeltaArgs a, float* __rest
         (side == 0 ? Mout : Dout)[at + row * 64 + col] = side == 0 && row == col ? x[i] + last : x[i];
       }
     }
-    __syncthreads();
+    lds_sync();
   }
 }
 
@@ -342,9 +357,9 @@ __global__ __launch_bounds__(kThr) void k_delta_walk(Walk a) {
 // with U as they are. What goes on to the backward (KEEP) is exact to fp32; the outputs take
 // two parts per value for 16-bit tensors, twice their precision: one rounding is the output's own.
 template <typename T, bool KEEP>
-__global__ __launch_bounds__(kThr) void k_delta_out(DeltaArgs a, int each, const float* __restrict__ Tin,
-                                                    const float* __restrict__ Sin, float* __restrict__ Zout,
-                                                    T* __restrict__ out) {
+__global__ __launch_bounds__(kThr) void k_delta_out(DeltaArgs a, int each, const float* __restrict__ Gin,
+                                                    const float* __restrict__ Tin, const float* __restrict__ Sin,
+                                                    float* __restrict__ Zout, T* __restrict__ out) {
   constexpr int NP = kPartsOf<T>, NZ = KEEP || NP == 3 ? 3 : 2, NO = NP == 3 ? 3 : 2;
   __shared__ Tile<NP> K;
   __shared__ Tile<NZ> S, U;
@@ -355,9 +370,11 @@ __global__ __launch_bounds__(kThr) void k_delta_out(DeltaArgs a, int each, const
   const int b = u / a.Hv, h = u % a.Hv;
   const int tok0 = 64 * ch, live = min(64, a.N - tok0), own = 16 * w + c;
   const size_t at = ((size_t)u * a.NC + ch) * kTile2;
-  load_tile<64, kThr>(K, rows_of<T>(a.k, b, h / (a.Hv / a.Hk), tok0), a.k.n, a.D, live, t);
-  load_f32(S, Sin + at, t);
-  load_f32(U, Tin + at, t);
+  Incoming<NP, T> ki;
+  Incoming<NZ, float> si, ti;
+  ki.fetch(rows_of<T>(a.k, b, h / (a.Hv / a.Hk), tok0), a.k.n, a.D, live, t);
+  si.fetch(Sin + at, 64, 64, 64, t);
+  ti.fetch(Tin + at, 64, 64, 64, t);
   const T* v = rows_of<T>(a.v, b, h, tok0) + min(own, a.DV - 1);
   f32x4 z[4];
 #pragma unroll
@@ -368,16 +385,18 @@ __global__ __launch_bounds__(kThr) void k_delta_out(DeltaArgs a, int each, const
       z[m][i] = get(v + min(row, live - 1) * a.v.n);
       z[m][i] = row < live && own < a.DV ? z[m][i] : 0.f;
     }
-  load_gates<T>(gate, a, b, h, tok0, t);
-  __syncthreads();
+  fetch_gates(gate, Gin + at / kTile2 * kGates, t);
+  ki.store(K, t);
+  si.store(S, t);
+  ti.store(U, t);
+  lds_sync();
   {
     const Frag<NZ> s0 = col_frag(S, 16 * w, 0, lane), s1 = col_frag(S, 16 * w, 1, lane);
 #pragma unroll
     for (int m = 0; m < 4; ++m) {
       f32x4 x = mma(row_frag(K, 16 * m, 0, lane), s0, f32x4{});
       x = mma(row_frag(K, 16 * m, 1, lane), s1, x);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) z[m][i] -= gate.since(16 * m + 4 * g + i) * x[i];
+      z[m] -= four(gate.since + 16 * m + 4 * g) * x;
     }
   }
   {
@@ -388,17 +407,19 @@ __global__ __launch_bounds__(kThr) void k_delta_out(DeltaArgs a, int each, const
       if (m >= 2) z[m] = mma(row_frag_perm(U, 16 * m, 1, lane), r1, z[m]);
     }
   }
-  __syncthreads();
+  lds_sync();
 #pragma unroll
-  for (int m = 0; m < 4; ++m)
+  for (int m = 0; m < 4; ++m) {
+    const f32x4 u4 = four(gate.beta + 16 * m + 4 * g) * z[m];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int row = 16 * m + 4 * g + i;
       if (KEEP && part == 0) Zout[at + row * 64 + own] = z[m][i];
-      put_parts(U, row, own, gate.beta[row] * z[m][i]);
+      put_parts(U, row, own, u4[i]);
     }
-  __syncthreads();
-  const float since = a.scale * gate.since(own);
+  }
+  lds_sync();
+  const float since = a.scale * gate.since[own], hi = gate.hi[own], lo = gate.lo[own];
   for (int o = h * rep + part * each; o < min(h * rep + (part + 1) * each, (h + 1) * rep); ++o) {
     const T* q = rows_of<T>(a.q, b, o / (a.H / a.Hq), tok0) + own * a.q.n;
     Frag<NP> qf[2];
@@ -414,11 +435,9 @@ __global__ __launch_bounds__(kThr) void k_delta_out(DeltaArgs a, int each, const
       if (m > w) continue;
 #pragma unroll
       for (int s = 0; s < 2; ++s) p[m] = mma(row_frag(K, 16 * m, s, lane), qf[s], p[m]);
+      const f32x4 y = p[m] * a.scale * decay_from(gate, 16 * m + 4 * g, hi, lo);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int j = 16 * m + 4 * g + i;
-        p[m][i] = j <= own ? p[m][i] * a.scale * gate.between(own, j) : 0.f;
-      }
+      for (int i = 0; i < 4; ++i) p[m][i] = 16 * m + 4 * g + i <= own ? y[i] : 0.f;
     }
     const Frag<NO> p0 = acc_frag<NO>(p[0], p[1]), p1 = acc_frag<NO>(p[2], p[3]);
     T* dst = out + (((size_t)b * a.H + o) * a.N + tok0 + own) * a.DV;
@@ -441,8 +460,8 @@ __global__ __launch_bounds__(kThr) void k_delta_out(DeltaArgs a, int each, const
 // ---------------------------------------------------------------------------
 template <typename T>
 __global__ __launch_bounds__(kThr) void k_delta_bwd_local(DeltaArgs a, const T* __restrict__ dout,
-                                                          const float* __restrict__ Tin, float* __restrict__ E,
-                                                          float* __restrict__ F) {
+                                                          const float* __restrict__ Gin, const float* __restrict__ Tin,
+                                                          float* __restrict__ E, float* __restrict__ F) {
   constexpr int NP = kPartsOf<T>;
   __shared__ Tile<NP> K, Q, O;
   __shared__ Tile<3> P;
@@ -451,15 +470,28 @@ __global__ __launch_bounds__(kThr) void k_delta_bwd_local(DeltaArgs a, const T* 
   const int ch = blockIdx.x % a.NC, u = blockIdx.x / a.NC, b = u / a.Hv, h = u % a.Hv;
   const int tok0 = 64 * ch, live = min(64, a.N - tok0), own = 16 * w + c;
   const size_t at = ((size_t)u * a.NC + ch) * kTile2;
-  load_tile<64, kThr>(K, rows_of<T>(a.k, b, h / (a.Hv / a.Hk), tok0), a.k.n, a.D, live, t);
-  load_gates<T>(gate, a, b, h, tok0, t);
+  // the next head's rows are on their way while one is worked on, the solved triangle behind the last
+  Incoming<NP, T> ki, qi, oi;
+  Incoming<3, float> ti;
+  const int each = a.H / a.Hv, o1 = (h + 1) * each;
+  auto fetch = [&](int o) {
+    qi.fetch(rows_of<T>(a.q, b, o / (a.H / a.Hq), tok0), a.q.n, a.D, live, t);
+    oi.fetch(dout + (((size_t)b * a.H + o) * a.N + tok0) * a.DV, a.DV, a.DV, live, t);
+  };
+  ki.fetch(rows_of<T>(a.k, b, h / (a.Hv / a.Hk), tok0), a.k.n, a.D, live, t);
+  fetch(h * each);
+  fetch_gates(gate, Gin + at / kTile2 * kGates, t);
+  ki.store(K, t);
   f32x4 e[4] = {}, f[4] = {};
-  const int each = a.H / a.Hv;
-  for (int o = h * each; o < (h + 1) * each; ++o) {
-    if (o > h * each) __syncthreads();
-    load_tile<64, kThr>(Q, rows_of<T>(a.q, b, o / (a.H / a.Hq), tok0), a.q.n, a.D, live, t);
-    load_tile<64, kThr>(O, dout + (((size_t)b * a.H + o) * a.N + tok0) * a.DV, (int64_t)a.DV, a.DV, live, t);
-    __syncthreads();
+  for (int o = h * each; o < o1; ++o) {
+    if (o > h * each) lds_sync();
+    qi.store(Q, t);
+    oi.store(O, t);
+    lds_sync();
+    if (o + 1 < o1)
+      fetch(o + 1);
+    else
+      ti.fetch(Tin + at, 64, 64, 64, t);
     // the scores, queries by keys = own: to LDS with the queries along a row
 #pragma unroll
     for (int m = 0; m < 4; ++m) {
@@ -467,12 +499,10 @@ __global__ __launch_bounds__(kThr) void k_delta_bwd_local(DeltaArgs a, const T* 
       if (m >= w)
 #pragma unroll
         for (int s = 0; s < 2; ++s) p = mma(row_frag(Q, 16 * m, s, lane), row_frag(K, 16 * w, s, lane), p);
+      const f32x4 y = p * a.scale * decay_to(gate, 16 * m + 4 * g, gate.hi[own], gate.lo[own]);
       float v[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = 16 * m + 4 * g + i;
-        v[i] = own <= row ? p[i] * a.scale * gate.between(row, own) : 0.f;
-      }
+      for (int i = 0; i < 4; ++i) v[i] = own <= 16 * m + 4 * g + i ? y[i] : 0.f;
 #pragma unroll
       for (int x = 0; x < 3; ++x) {
         const bf16x4 y = __builtin_bit_cast(bf16x4, pack4(v));
@@ -487,16 +517,17 @@ __global__ __launch_bounds__(kThr) void k_delta_bwd_local(DeltaArgs a, const T* 
     for (int s = 0; s < 2; ++s) {
       of[s] = col_frag(O, 16 * w, s, lane);
       float v[8];
+      const f32x4 g0 = a.scale * four(gate.since + 32 * s + 8 * g), g1 = a.scale * four(gate.since + 32 * s + 8 * g + 4);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         v[j] = 0.f;
 #pragma unroll
         for (int x = NP - 1; x >= 0; --x) v[j] += static_cast<float>(of[s].p[x][j]);
-        v[j] *= a.scale * gate.since(32 * s + 8 * g + j);
+        v[j] *= j < 4 ? g0[j] : g1[j - 4];
       }
       og[s] = split<3>(v);
     }
-    __syncthreads();
+    lds_sync();
 #pragma unroll
     for (int m = 0; m < 4; ++m) {
       if (m < 2) e[m] = mma(row_frag(P, 16 * m, 0, lane), of[0], e[m]);
@@ -505,25 +536,22 @@ __global__ __launch_bounds__(kThr) void k_delta_bwd_local(DeltaArgs a, const T* 
       for (int s = 0; s < 2; ++s) f[m] = mma(col_frag(Q, 16 * m, s, lane), og[s], f[m]);
     }
   }
-  __syncthreads();
-  load_f32(P, Tin + at, t);
+  lds_sync();
+  ti.store(P, t);
   f32x4 z[4];
 #pragma unroll
-  for (int m = 0; m < 4; ++m)
+  for (int m = 0; m < 4; ++m) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = 16 * m + 4 * g + i;
-      E[at + row * 64 + own] = e[m][i];
-      e[m][i] *= gate.beta[row];
-    }
+    for (int i = 0; i < 4; ++i) E[at + (16 * m + 4 * g + i) * 64 + own] = e[m][i];
+    e[m] *= four(gate.beta + 16 * m + 4 * g);
+  }
   const Frag<3> e0 = acc_frag<3>(e[0], e[1]), e1 = acc_frag<3>(e[2], e[3]);
-  __syncthreads();
+  lds_sync();
 #pragma unroll
   for (int m = 0; m < 4; ++m) {
     z[m] = mma(col_frag_perm(P, 16 * m, 1, lane), e1, f32x4{});
     if (m < 2) z[m] = mma(col_frag_perm(P, 16 * m, 0, lane), e0, z[m]);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) z[m][i] *= -gate.since(16 * m + 4 * g + i);
+    z[m] *= -four(gate.since + 16 * m + 4 * g);
   }
   const Frag<3> z0 = acc_frag<3>(z[0], z[1]), z1 = acc_frag<3>(z[2], z[3]);
 #pragma unroll
@@ -557,8 +585,9 @@ __device__ __forceinline__ void own_row(Frag<3> (&f)[2], const float* row, int g
 // tokens are the columns.
 template <typename T>
 __global__ __launch_bounds__(kThr) void k_delta_bwd_out(DeltaArgs a, const T* __restrict__ dout,
-                                                        const float* __restrict__ Tin, const float* __restrict__ Sin,
-                                                        const float* __restrict__ Zin, const float* __restrict__ E,
+                                                        const float* __restrict__ Gin, const float* __restrict__ Tin,
+                                                        const float* __restrict__ Sin, const float* __restrict__ Zin,
+                                                        const float* __restrict__ E,
                                                         const float* __restrict__ dSin, T* __restrict__ dq,
                                                         float* __restrict__ dqh, T* __restrict__ dk,
                                                         float* __restrict__ dkh, T* __restrict__ dv,
@@ -573,9 +602,11 @@ __global__ __launch_bounds__(kThr) void k_delta_bwd_out(DeltaArgs a, const T* __
   const int tok0 = 64 * ch, live = min(64, a.N - tok0), own = 16 * w + c;
   const size_t at = ((size_t)u * a.NC + ch) * kTile2;
   const T* krows = rows_of<T>(a.k, b, h / (a.Hv / a.Hk), tok0);
-  load_tile<64, kThr>(K, krows, a.k.n, a.D, live, t);
-  load_f32(X, dSin + at, t);
-  load_f32(Z, Tin + at, t);
+  Incoming<NP, T> ki;
+  Incoming<3, float> xi, zi;
+  ki.fetch(krows, a.k.n, a.D, live, t);
+  xi.fetch(dSin + at, 64, 64, 64, t);
+  zi.fetch(Tin + at, 64, 64, 64, t);
   Frag<3> zf[2], dzf[2];
   own_row(zf, Zin + at + own * 64, g);
   f32x4 e[4];
@@ -591,16 +622,20 @@ __global__ __launch_bounds__(kThr) void k_delta_bwd_out(DeltaArgs a, const T* __
     const f32x4 s = load4(Sin + at + i), d = load4(dSin + at + i);
     ends += s[0] * d[0] + s[1] * d[1] + s[2] * d[2] + s[3] * d[3];
   }
-  load_gates<T>(gate, a, b, h, tok0, t);
-  __syncthreads();
-  ends *= gate.since(63);
-  const float beta = gate.beta[own];
+  fetch_gates(gate, Gin + at / kTile2 * kGates, t);
+  ki.store(K, t);
+  xi.store(X, t);
+  zi.store(Z, t);
+  lds_sync();
+  zi.fetch(Zin + at, 64, 64, 64, t);
+  ends *= gate.since[63];
+  const float beta = gate.beta[own], hi = gate.hi[own], lo = gate.lo[own];
   f32x4 reads[4] = {}, writes[4] = {};
   float dot = 0.f;    // of dbeta
   float decay = 0.f;  // of dG
   f32x4 kv[4];
   {
-    const float until = beta * gate.between(63, own);
+    const float until = beta * gate.until[own];
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
       kv[n] = f32x4{};
@@ -629,13 +664,10 @@ __global__ __launch_bounds__(kThr) void k_delta_bwd_out(DeltaArgs a, const T* __
     for (int m = 0; m < 4; ++m) {
       f32x4 x = mma(row_frag(K, 16 * m, 0, lane), s0, f32x4{});
       x = mma(row_frag(K, 16 * m, 1, lane), s1, x);
+      e[m] += four(gate.until + 16 * m + 4 * g) * x;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = 16 * m + 4 * g + i;
-        e[m][i] += gate.between(63, row) * x[i];
-        dots[4 * m + i] = e[m][i] * Zin[at + row * 64 + own];
-        e[m][i] *= gate.beta[row];
-      }
+      for (int i = 0; i < 4; ++i) dots[4 * m + i] = e[m][i] * Zin[at + (16 * m + 4 * g + i) * 64 + own];
+      e[m] *= four(gate.beta + 16 * m + 4 * g);
     }
     // sums over the 16 lanes of a row group; lane c ends with row 16 (c / 4) + 4 g + c % 4
 #pragma unroll
@@ -654,8 +686,8 @@ __global__ __launch_bounds__(kThr) void k_delta_bwd_out(DeltaArgs a, const T* __
       if (m < 2) e[m] = mma(col_frag_perm(Z, 16 * m, 0, lane), e0, e[m]);
     }
   }
-  __syncthreads();
-  load_f32(Z, Zin + at, t);
+  lds_sync();
+  zi.store(Z, t);
 #pragma unroll
   for (int m = 0; m < 4; ++m)
 #pragma unroll
@@ -664,7 +696,7 @@ __global__ __launch_bounds__(kThr) void k_delta_bwd_out(DeltaArgs a, const T* __
       put_parts(X, row, own, e[m][i]);
       if (row < live && own < a.DV) put(dv + ((size_t)u * a.N + tok0 + row) * a.DV + own, e[m][i]);
     }
-  __syncthreads();
+  lds_sync();
 #pragma unroll
   for (int s = 0; s < 2; ++s) dzf[s] = row_frag(X, 16 * w, s, lane);
   {
@@ -679,10 +711,10 @@ __global__ __launch_bounds__(kThr) void k_delta_bwd_out(DeltaArgs a, const T* __
         m[n] = mma(row_frag(Z, 16 * n, s, lane), dzf[s], m[n]);
         kk = mma(row_frag(K, 16 * n, s, lane), row_frag(K, 16 * w, s, lane), kk);
       }
+      const f32x4 y = -four(gate.beta + 16 * n + 4 * g) * decay_from(gate, 16 * n + 4 * g, hi, lo) * m[n];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int j = 16 * n + 4 * g + i;
-        m[n][i] = j < own ? -gate.beta[j] * gate.between(own, j) * m[n][i] : 0.f;
+        m[n][i] = 16 * n + 4 * g + i < own ? y[i] : 0.f;
         decay += m[n][i] * kk[i];
       }
     }
@@ -693,6 +725,7 @@ __global__ __launch_bounds__(kThr) void k_delta_bwd_out(DeltaArgs a, const T* __
       if (w >= 2) reads[n] = mma(col_frag_perm(K, 16 * n, 1, lane), m1, reads[n]);
     }
   }
+  xi.fetch(Sin + at, 64, 64, 64, t);
   {
     // M: rows i, columns j = own
     f32x4 m[4] = {};
@@ -705,10 +738,10 @@ __global__ __launch_bounds__(kThr) void k_delta_bwd_out(DeltaArgs a, const T* __
         m[n] = mma(row_frag(X, 16 * n, s, lane), zf[s], m[n]);
         kk = mma(row_frag(K, 16 * n, s, lane), row_frag(K, 16 * w, s, lane), kk);
       }
+      const f32x4 y = decay_to(gate, 16 * n + 4 * g, hi, lo) * m[n];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int row = 16 * n + 4 * g + i;
-        const float x = own < row ? gate.between(row, own) * m[n][i] : 0.f;
+        const float x = own < 16 * n + 4 * g + i ? y[i] : 0.f;
         dot -= x * kk[i];
         m[n][i] = -beta * x;
         decay -= m[n][i] * kk[i];
@@ -729,10 +762,17 @@ __global__ __launch_bounds__(kThr) void k_delta_bwd_out(DeltaArgs a, const T* __
     else
       put(static_cast<T*>(dbeta) + x, dot);
   }
-  __syncthreads();
-  load_f32(X, Sin + at, t);
-  __syncthreads();
-  const float since = gate.since(own);
+  lds_sync();
+  xi.store(X, t);
+  const int each = a.H / a.Hv, o1 = (h + 1) * each;
+  Incoming<NP, T> qi, oi;
+  auto fetch = [&](int o) {
+    qi.fetch(rows_of<T>(a.q, b, o / (a.H / a.Hq), tok0), a.q.n, a.D, live, t);
+    oi.fetch(dout + (((size_t)b * a.H + o) * a.N + tok0) * a.DV, a.DV, a.DV, live, t);
+  };
+  fetch(h * each);
+  lds_sync();
+  const float since = gate.since[own];
 #pragma unroll
   for (int n = 0; n < 4; ++n) {
     f32x4 x = {};
@@ -744,14 +784,14 @@ __global__ __launch_bounds__(kThr) void k_delta_bwd_out(DeltaArgs a, const T* __
       decay -= kv[n][i] * since * x[i];
     }
   }
-  const int each = a.H / a.Hv;
-  for (int o = h * each; o < (h + 1) * each; ++o) {
-    if (o > h * each) __syncthreads();
+  for (int o = h * each; o < o1; ++o) {
     const T* qrows = rows_of<T>(a.q, b, o / (a.H / a.Hq), tok0);
     const size_t orow = ((size_t)b * a.H + o) * a.N + tok0;
-    load_tile<64, kThr>(Q, qrows, a.q.n, a.D, live, t);
-    load_tile<64, kThr>(O, dout + orow * a.DV, (int64_t)a.DV, a.DV, live, t);
-    __syncthreads();
+    if (o > h * each) lds_sync();
+    qi.store(Q, t);
+    oi.store(O, t);
+    lds_sync();
+    if (o + 1 < o1) fetch(o + 1);
     Frag<NP> of[2];
 #pragma unroll
     for (int s = 0; s < 2; ++s) of[s] = row_frag(O, 16 * w, s, lane);
@@ -773,11 +813,12 @@ __global__ __launch_bounds__(kThr) void k_delta_bwd_out(DeltaArgs a, const T* __
         p[n] = mma(row_frag(Z, 16 * n, s, lane), of[s], p[n]);
         qk = mma(row_frag(K, 16 * n, s, lane), row_frag(Q, 16 * w, s, lane), qk);
       }
+      const f32x4 y = a.scale * four(gate.beta + 16 * n + 4 * g) * decay_from(gate, 16 * n + 4 * g, hi, lo) * p[n];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int j = 16 * n + 4 * g + i;
-        p[n][i] = j <= own ? a.scale * gate.beta[j] * gate.between(own, j) * p[n][i] : 0.f;
-        if (j < own) decay += p[n][i] * qk[i];
+        p[n][i] = j <= own ? y[i] : 0.f;
+        decay += j < own ? p[n][i] * qk[i] : 0.f;
       }
     }
     {
@@ -804,11 +845,12 @@ __global__ __launch_bounds__(kThr) void k_delta_bwd_out(DeltaArgs a, const T* __
         p[n] = mma(row_frag(O, 16 * n, s, lane), zf[s], p[n]);
         qk = mma(row_frag(Q, 16 * n, s, lane), row_frag(K, 16 * w, s, lane), qk);
       }
+      const f32x4 y = a.scale * beta * decay_to(gate, 16 * n + 4 * g, hi, lo) * p[n];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int row = 16 * n + 4 * g + i;
-        p[n][i] = own <= row ? a.scale * beta * gate.between(row, own) * p[n][i] : 0.f;
-        if (own < row) decay -= p[n][i] * qk[i];
+        p[n][i] = own <= row ? y[i] : 0.f;
+        decay -= own < row ? p[n][i] * qk[i] : 0.f;
       }
     }
     const Frag<3> p0 = acc_frag<3>(p[0], p[1]), p1 = acc_frag<3>(p[2], p[3]);
@@ -831,7 +873,7 @@ __global__ __launch_bounds__(kThr) void k_delta_bwd_out(DeltaArgs a, const T* __
   }
   decay = group_sum(decay);
   if (g == 0) dG[own] = decay;
-  __syncthreads();
+  lds_sync();
   if (w == 0) {
     double x = dG[lane];
     if (lane == 63) x += ((double)part[0] + part[1]) + ((double)part[2] + part[3]);
@@ -881,11 +923,11 @@ __global__ __launch_bounds__(kThr) void k_delta_step(DeltaStepArgs a) {
   auto over_rows = [&](float (&x)[4]) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) x[j] = group_sum(x[j]);
-    __syncthreads();
+    lds_sync();
     if (lane < 16)
 #pragma unroll
       for (int j = 0; j < 4; ++j) sum[w][c0 + j] = x[j];
-    __syncthreads();
+    lds_sync();
 #pragma unroll
     for (int j = 0; j < 4; ++j) x[j] = (sum[0][c0 + j] + sum[1][c0 + j]) + (sum[2][c0 + j] + sum[3][c0 + j]);
   };
@@ -1003,6 +1045,7 @@ DeltaSaved delta_saved_view(void* base, int U, int NC, bool keep) {
   DeltaSaved s;
   Room r{static_cast<char*>(base)};
   const size_t tiles = (size_t)U * NC * kTile2;
+  s.G = r.take((size_t)U * NC * kGates);
   s.T = r.take(tiles);
   s.M = r.take(tiles);
   s.S = r.take(tiles);
@@ -1035,16 +1078,16 @@ void launch_delta_forward(const DeltaArgs& a, const float* state, void* out, flo
   const int U = a.B * a.Hv, rep = a.H / a.Hv;
   const DeltaSaved s = delta_saved_view(saved, U, a.NC, keep);
   timed("k_delta_chunk", st,
-        [&] { hipLaunchKernelGGL(k_delta_chunk<T>, dim3(a.NC * U), dim3(kThr), 0, st, a, s.T, s.M, s.D); });
+        [&] { hipLaunchKernelGGL(k_delta_chunk<T>, dim3(a.NC * U), dim3(kThr), 0, st, a, s.G, s.T, s.M, s.D); });
   walk<false>(a, s.M, s.D, state, s.S, final_state, s.scratch, false, st, timed);
   // all heads of a state in one block, unless that leaves CUs without one
   const int parts = std::clamp((1024 + U * a.NC - 1) / (U * a.NC), 1, rep), each = (rep + parts - 1) / parts;
   const dim3 grid(U * a.NC * ((rep + each - 1) / each));
   timed("k_delta_out", st, [&] {
     if (keep)
-      hipLaunchKernelGGL((k_delta_out<T, true>), grid, dim3(kThr), 0, st, a, each, s.T, s.S, s.Z, static_cast<T*>(out));
+      hipLaunchKernelGGL((k_delta_out<T, true>), grid, dim3(kThr), 0, st, a, each, s.G, s.T, s.S, s.Z, static_cast<T*>(out));
     else
-      hipLaunchKernelGGL((k_delta_out<T, false>), grid, dim3(kThr), 0, st, a, each, s.T, s.S, s.Z, static_cast<T*>(out));
+      hipLaunchKernelGGL((k_delta_out<T, false>), grid, dim3(kThr), 0, st, a, each, s.G, s.T, s.S, s.Z, static_cast<T*>(out));
   });
 }
 
@@ -1057,11 +1100,11 @@ void launch_delta_backward(const DeltaArgs& a, const void* saved, const void* do
   const DeltaWork w = delta_work_view(work, a);
   const T* od = static_cast<const T*>(dout);
   timed("k_delta_bwd_local", st, [&] {
-    hipLaunchKernelGGL(k_delta_bwd_local<T>, dim3(a.NC * U), dim3(kThr), 0, st, a, od, s.T, w.E, w.F);
+    hipLaunchKernelGGL(k_delta_bwd_local<T>, dim3(a.NC * U), dim3(kThr), 0, st, a, od, s.G, s.T, w.E, w.F);
   });
   walk<true>(a, s.M, w.F, dfinal, w.dS, dstate, w.scratch, true, st, timed);
   timed("k_delta_bwd_out", st, [&] {
-    hipLaunchKernelGGL(k_delta_bwd_out<T>, dim3(a.NC * U), dim3(kThr), 0, st, a, od, s.T, s.S, s.Z, w.E, w.dS,
+    hipLaunchKernelGGL(k_delta_bwd_out<T>, dim3(a.NC * U), dim3(kThr), 0, st, a, od, s.G, s.T, s.S, s.Z, w.E, w.dS,
                        static_cast<T*>(dq), w.dqh, static_cast<T*>(dk), w.dkh, static_cast<T*>(dv), dg, dbeta);
   });
   auto sum = [&](const float* src, void* dst, int heads, int each) {

@@ -21,8 +21,9 @@ struct DeltaArgs {
   float scale;
 };
 
-// What the forward computes per unit u = b Hv + state head and chunk, and the backward reads (T to Z).
+// What the forward computes per unit u = b Hv + state head and chunk, and the backward reads (G to Z).
 struct DeltaSaved {
+  float* G;  // [U][NC][5][64] its tokens' decays and betas
   float* T;  // [U][NC][64][64] the chunk's solved triangle
   float* M;  // [U][NC][64][64] its map of the state, S' = M S + D
   float* S;  // [U][NC][64][64] state before the chunk

@@ -193,36 +193,43 @@ __device__ __forceinline__ Frag<NP> global_frag(const T* p, bool live) {
   return f;
 }
 
-// ROWS rows of D values, a multiple of 8 up to 64 (row stride in elements), into rows
-// 0 .. of an LDS tile, NT threads; rows at and past `live` and columns from D are zero. 16-byte aligned rows.
-template <int ROWS, int NT, int NP, typename T>
-__device__ __forceinline__ void load_tile(Tile<NP>& s, const T* __restrict__ src, int64_t stride, int D, int live, int t) {
-  constexpr int kIt = (ROWS * 8 + NT - 1) / NT;
-  if constexpr (NP == 1) {
-    // every load before the first store
-    Frag<1> f[kIt];
+// 64 rows of D values, a multiple of 8 up to 64 (row stride in elements, 16-byte aligned rows), on
+// their way to an LDS tile by 256 threads: fetch() has the loads of all that a kernel starts
+// with in flight together, store() waits for its own. Rows at and past `live` and columns from D are zero.
+template <int NP, typename T>
+struct Incoming {
+  Frag<1> raw[2];
+  float x[2][8];
+  __device__ __forceinline__ void fetch(const T* __restrict__ src, int64_t stride, int D, int live, int t) {
 #pragma unroll
-    for (int x = 0; x < kIt; ++x) {
-      const int i = t + NT * x, r = i >> 3, c = 8 * (i & 7);
-      f[x] = global_frag<1>(src + r * stride + c, r < live && c < D && i < ROWS * 8);
-    }
+    for (int n = 0; n < 2; ++n) {
+      const int r = (t >> 3) + 32 * n, c = 8 * (t & 7);
+      const bool in = r < live && c < D;
+      const T* p = src + (in ? r * stride + c : 0);
+      if constexpr (kPartsOf<T> == 1) {
+        raw[n] = global_frag<1>(p, true);
+        if (!in) raw[n] = Frag<1>{};
+      } else {
+        load_row8(x[n], p);
 #pragma unroll
-    for (int x = 0; x < kIt; ++x) {
-      const int i = t + NT * x;
-      if (i < ROWS * 8) *reinterpret_cast<bf16x8*>(s.x + tile_at(i >> 3, 8 * (i & 7))) = f[x].p[0];
-    }
-  } else {
-#pragma unroll
-    for (int x = 0; x < kIt; ++x) {
-      const int i = t + NT * x, r = i >> 3, c = 8 * (i & 7);
-      if (i < ROWS * 8) {
-        const Frag<NP> f = global_frag<NP>(src + r * stride + c, r < live && c < D);
-#pragma unroll
-        for (int e = 0; e < NP; ++e) *reinterpret_cast<bf16x8*>(s.x + e * kTileElems + tile_at(r, c)) = f.p[e];
+        for (int e = 0; e < 8; ++e) x[n][e] = in ? x[n][e] : 0.f;
       }
     }
   }
-}
+  __device__ __forceinline__ void store(Tile<NP>& s, int t) const {
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      __bf16* p = s.x + tile_at((t >> 3) + 32 * n, 8 * (t & 7));
+      if constexpr (kPartsOf<T> == 1) {
+        *reinterpret_cast<bf16x8*>(p) = raw[n].p[0];
+      } else {
+        const Frag<NP> f = split<NP>(x[n]);
+#pragma unroll
+        for (int e = 0; e < NP; ++e) *reinterpret_cast<bf16x8*>(p + e * kTileElems) = f.p[e];
+      }
+    }
+  }
+};
 
 // A thread's wave as a scalar: what depends on it branches once per wave.
 __device__ __forceinline__ int wave_of(int t) { return __builtin_amdgcn_readfirstlane(t >> 6); }

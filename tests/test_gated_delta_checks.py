@@ -69,8 +69,8 @@ def _lib():
 
 def test_c_entries_check_before_they_launch():
     lib = _lib()
-    assert lib.oal_gated_delta_saved_bytes(2, 2, 65, 1) == 4 * 2 * 5 * 4 * 4096
-    assert lib.oal_gated_delta_saved_bytes(2, 2, 65, 0) == 4 * 2 * 4 * 4 * 4096
+    assert lib.oal_gated_delta_saved_bytes(2, 2, 65, 1) == 4 * 2 * (5 * 4096 + 320) * 4
+    assert lib.oal_gated_delta_saved_bytes(2, 2, 65, 0) == 4 * 2 * (4 * 4096 + 320) * 4
     assert lib.oal_gated_delta_saved_bytes(0, 2, 65, 1) == 0 and b"positive" in lib.oal_last_error()
     assert lib.oal_gated_delta_workspace_bytes(1, 3, 2, 2, 64, 64) == 0 and b"divisible" in lib.oal_last_error()
     # shared heads need room for what is summed
