@@ -132,9 +132,13 @@ template <typename T>
 __global__ __launch_bounds__(kThr) void k_delta_chunk(DeltaArgs a, float* __restrict__ Gout, float* __restrict__ Tout,
                                                       float* __restrict__ Mout, float* __restrict__ Dout) {
   constexpr int NP = kPartsOf<T>;
-  __shared__ Tile<NP> K, V;
+  __shared__ Tile<NP> K;
   __shared__ Gates gate;
-  __shared__ alignas(16) float S[64 * kRow32];
+  // V takes the triangle's place when that is in parts: three blocks of bf16 rows fit a CU
+  constexpr int kRoomS = 64 * kRow32 * 4;
+  __shared__ alignas(16) char roomS[sizeof(Tile<NP>) > kRoomS ? sizeof(Tile<NP>) : kRoomS];
+  float* const S = reinterpret_cast<float*>(roomS);
+  Tile<NP>& V = *reinterpret_cast<Tile<NP>*>(roomS);
   struct Solve {
     float L[64 * kRow32], Y[32 * kRow32];
   };
@@ -151,7 +155,6 @@ __global__ __launch_bounds__(kThr) void k_delta_chunk(DeltaArgs a, float* __rest
   vi.fetch(rows_of<T>(a.v, b, h, tok0), a.v.n, a.DV, live, t);
   form_gates<T>(gate, a, b, h, tok0, t);
   ki.store(K, t);
-  vi.store(V, t);
   lds_sync();
   fetch_gates(*reinterpret_cast<Gates*>(Gout + ((size_t)u * a.NC + ch) * kGates), reinterpret_cast<const float*>(&gate), t);
   {
@@ -230,6 +233,10 @@ __global__ __launch_bounds__(kThr) void k_delta_chunk(DeltaArgs a, float* __rest
       for (int e = 0; e < 3; ++e) *reinterpret_cast<bf16x8*>(P.x + e * kTileElems + tile_at(r, col)) = f.p[e];
     }
     lds_sync();
+    if (side == 1) {
+      vi.store(V, t);
+      lds_sync();
+    }
     const Tile<NP>& B = side == 0 ? K : V;
     const Frag<NP> b0 = col_frag(B, 16 * w, 0, lane), b1 = col_frag(B, 16 * w, 1, lane);
     f32x4 z[4];
@@ -459,7 +466,7 @@ __global__ __launch_bounds__(kThr) void k_delta_out(DeltaArgs a, int each, const
 // Decays' gradients are sums of terms that cancel, so all of it is exact to fp32.
 // ---------------------------------------------------------------------------
 template <typename T>
-__global__ __launch_bounds__(kThr) void k_delta_bwd_local(DeltaArgs a, const T* __restrict__ dout,
+__global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 3 : 1) void k_delta_bwd_local(DeltaArgs a, const T* __restrict__ dout,
                                                           const float* __restrict__ Gin, const float* __restrict__ Tin,
                                                           float* __restrict__ E, float* __restrict__ F) {
   constexpr int NP = kPartsOf<T>;
@@ -592,7 +599,8 @@ __global__ __launch_bounds__(kThr) void k_delta_bwd_out(DeltaArgs a, const T* __
                                                         float* __restrict__ dqh, T* __restrict__ dk,
                                                         float* __restrict__ dkh, T* __restrict__ dv,
                                                         float* __restrict__ dg, void* __restrict__ dbeta) {
-  constexpr int NP = kPartsOf<T>;
+  // what goes into dq and dk alone takes two parts for 16-bit tensors
+  constexpr int NP = kPartsOf<T>, NO = NP == 3 ? 3 : 2;
   __shared__ Tile<NP> K, Q, O;
   __shared__ Tile<3> Z, X;
   __shared__ Gates gate;
@@ -718,7 +726,7 @@ __global__ __launch_bounds__(kThr) void k_delta_bwd_out(DeltaArgs a, const T* __
         decay += m[n][i] * kk[i];
       }
     }
-    const Frag<3> m0 = acc_frag<3>(m[0], m[1]), m1 = acc_frag<3>(m[2], m[3]);
+    const Frag<NO> m0 = acc_frag<NO>(m[0], m[1]), m1 = acc_frag<NO>(m[2], m[3]);
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
       reads[n] = mma(col_frag_perm(K, 16 * n, 0, lane), m0, reads[n]);
@@ -747,7 +755,7 @@ __global__ __launch_bounds__(kThr) void k_delta_bwd_out(DeltaArgs a, const T* __
         decay -= m[n][i] * kk[i];
       }
     }
-    const Frag<3> m0 = acc_frag<3>(m[0], m[1]), m1 = acc_frag<3>(m[2], m[3]);
+    const Frag<NO> m0 = acc_frag<NO>(m[0], m[1]), m1 = acc_frag<NO>(m[2], m[3]);
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
       if (w < 2) writes[n] = mma(col_frag_perm(K, 16 * n, 0, lane), m0, writes[n]);
@@ -822,7 +830,7 @@ __global__ __launch_bounds__(kThr) void k_delta_bwd_out(DeltaArgs a, const T* __
       }
     }
     {
-      const Frag<3> p0 = acc_frag<3>(p[0], p[1]), p1 = acc_frag<3>(p[2], p[3]);
+      const Frag<NO> p0 = acc_frag<NO>(p[0], p[1]), p1 = acc_frag<NO>(p[2], p[3]);
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
         acc[n] = mma(col_frag_perm(K, 16 * n, 0, lane), p0, acc[n]);
@@ -853,7 +861,7 @@ __global__ __launch_bounds__(kThr) void k_delta_bwd_out(DeltaArgs a, const T* __
         decay -= own < row ? p[n][i] * qk[i] : 0.f;
       }
     }
-    const Frag<3> p0 = acc_frag<3>(p[0], p[1]), p1 = acc_frag<3>(p[2], p[3]);
+    const Frag<NO> p0 = acc_frag<NO>(p[0], p[1]), p1 = acc_frag<NO>(p[2], p[3]);
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
       if (w < 2) writes[n] = mma(col_frag_perm(Q, 16 * n, 0, lane), p0, writes[n]);
@@ -910,12 +918,20 @@ __global__ __launch_bounds__(kThr) void k_delta_step(DeltaStepArgs a) {
   const int u = blockIdx.x, b = u / a.Hv, h = u % a.Hv;
   const int d0 = 4 * (t >> 4), c0 = 4 * (t & 15);
   float* state = a.state + (size_t)u * a.Dk * a.Dv;
+  const bool fours = a.Dv % 4 == 0 && reinterpret_cast<uintptr_t>(a.state) % 16 == 0;  // pieces of four are whole and aligned
   float s[4][4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      s[i][j] = d0 + i < a.Dk && c0 + j < a.Dv ? state[(d0 + i) * a.Dv + c0 + j] : 0.f;
+  for (int i = 0; i < 4; ++i) {
+    float4 v = make_float4(0, 0, 0, 0);
+    const float* p = state + (d0 + i) * a.Dv + c0;
+    if (d0 + i < a.Dk && c0 < a.Dv) {
+      if (fours)
+        v = *reinterpret_cast<const float4*>(p);
+      else
+        v = make_float4(p[0], c0 + 1 < a.Dv ? p[1] : 0.f, c0 + 2 < a.Dv ? p[2] : 0.f, c0 + 3 < a.Dv ? p[3] : 0.f);
+    }
+    s[i][0] = v.x, s[i][1] = v.y, s[i][2] = v.z, s[i][3] = v.w;
+  }
   const T* k = static_cast<const T*>(a.k.p) + b * a.k.b + (h / (a.Hv / a.Hk)) * a.k.h;
   const T* v = static_cast<const T*>(a.v.p) + b * a.v.b + h * a.v.h;
   const int each = a.H / a.Hv;
@@ -971,10 +987,17 @@ __global__ __launch_bounds__(kThr) void k_delta_step(DeltaStepArgs a) {
     }
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < 4; ++i) {
+    float* p = state + (d0 + i) * a.Dv + c0;
+    if (d0 + i >= a.Dk || c0 >= a.Dv) continue;
+    if (fours) {
+      *reinterpret_cast<float4*>(p) = make_float4(s[i][0], s[i][1], s[i][2], s[i][3]);
+    } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (d0 + i < a.Dk && c0 + j < a.Dv) state[(d0 + i) * a.Dv + c0 + j] = s[i][j];
+      for (int j = 0; j < 4; ++j)
+        if (c0 + j < a.Dv) p[j] = s[i][j];
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------
