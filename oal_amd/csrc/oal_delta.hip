@@ -273,27 +273,29 @@ struct Walk {
   const float* M;     // [units][maps][64][64]
   const float* D;
   const float* init;  // [rows][cols] state the walk starts from, by unit (segs == 1) or segment (null: zero)
-  float* each;        // [units][maps][64][64]: the state before each map (with 4 column groups)
+  float* each;        // [units][maps][64][64]: the state before each map (without MAPS)
   float* end;         // the same: the state after the last map (null: not wanted)
-  float* mend;        // with 8 column groups: the product of the segment's maps
+  float* mend;        // with MAPS: the product of the segment's maps
   int maps, segs, len, units, rows, cols;
   bool back;
 };
 
 constexpr int kAhead = 4;
 
-template <bool TR, int COLS>
+// With MAPS the block walks the same columns of the maps' product beside its own (from the
+// unit matrix, nothing added): twice the products from one load of the maps.
+template <bool TR, bool MAPS>
 __global__ __launch_bounds__(kThr) void k_delta_walk(Walk a) {
-  __shared__ f32x4 rows[2][4][64];
+  constexpr int SETS = MAPS ? 2 : 1;
+  __shared__ f32x4 rows[2][SETS][4][64];
   const int t = threadIdx.x, lane = t & 63, w = wave_of(t), g = lane >> 4, c = lane & 15;
   // a chain's column groups on one XCD (blocks go round the 8 of them): they share its maps
-  const int chains = a.units * a.segs, id = blockIdx.x, whole = chains / 8 * 8 * COLS;
-  const int chain = id < whole ? id % 8 + id / (8 * COLS) * 8 : chains / 8 * 8 + (id - whole) / COLS;
-  const int group = id < whole ? id / 8 % COLS : (id - whole) % COLS;
+  const int chains = a.units * a.segs, id = blockIdx.x, whole = chains / 8 * 32;
+  const int chain = id < whole ? id % 8 + id / 32 * 8 : chains / 8 * 8 + (id - whole) / 4;
+  const int group = id < whole ? id / 8 % 4 : (id - whole) % 4;
   const int u = chain / a.segs, seg = chain % a.segs;
-  const bool unit = group >= 4;  // columns of the maps' product: from the unit matrix, nothing added
   const int first = seg * a.len, count = min(a.len, a.maps - first);
-  const int col = 16 * (group & 3) + c, row = 16 * w + 4 * g;
+  const int col = 16 * group + c, row = 16 * w + 4 * g;
   const size_t base = ((size_t)u * a.maps + first) * kTile2;
   auto slot = [&](int i) { return ((size_t)chain * a.rows + row + i) * a.cols + col; };
   auto held = [&](int i) { return row + i < a.rows && col < a.cols; };
@@ -311,34 +313,40 @@ __global__ __launch_bounds__(kThr) void k_delta_walk(Walk a) {
         const float4 v = *reinterpret_cast<const float4*>(a.M + at + (16 * w + c) * 64 + k);
         mm[4 * q] = v.x, mm[4 * q + 1] = v.y, mm[4 * q + 2] = v.z, mm[4 * q + 3] = v.w;
       }
-      dd[q] = unit ? 0.f : a.D[at + (row + q) * 64 + col];
+      dd[q] = a.D[at + (row + q) * 64 + col];
     }
   };
-  f32x4 S;
+  f32x4 S[SETS];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    S[i] = unit ? (row + i == col ? 1.f : 0.f) : a.init && held(i) ? a.init[slot(i)] : 0.f;
-  asm volatile("" : "+v"(S));  // here, not in the walk, is waited for it
+  for (int i = 0; i < 4; ++i) {
+    S[0][i] = a.init && held(i) ? a.init[slot(i)] : 0.f;
+    if constexpr (MAPS) S[1][i] = row + i == col ? 1.f : 0.f;
+  }
+  asm volatile("" : "+v"(S[0]));  // here, not in the walk, is waited for it
 #pragma unroll
   for (int n = 0; n < kAhead; ++n) fetch(n, m[n], d[n]);
   // the number of loads in flight is the same on every way to a step, so that it waits for its own
   auto step = [&](int n, int x) {
-    rows[x & 1][w][lane] = S;
-    if constexpr (COLS == 4) {
+#pragma unroll
+    for (int p = 0; p < SETS; ++p) rows[x & 1][p][w][lane] = S[p];
+    if constexpr (!MAPS) {
       const size_t at = base + (size_t)(a.back ? count - 1 - n : n) * kTile2;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) a.each[at + (row + i) * 64 + col] = S[i];
+      for (int i = 0; i < 4; ++i) a.each[at + (row + i) * 64 + col] = S[0][i];
     }
-    f32x4 next[4] = {{d[x][0], d[x][1], d[x][2], d[x][3]}};
+    f32x4 next[SETS][4] = {{{d[x][0], d[x][1], d[x][2], d[x][3]}}};
     lds_sync();
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const f32x4 v = rows[x & 1][q][lane];
+    for (int q = 0; q < 4; ++q)
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        next[q] = __builtin_amdgcn_mfma_f32_16x16x4f32(m[x][4 * q + e], v[e], next[q], 0, 0, 0);
-    }
-    S = (next[0] + next[1]) + (next[2] + next[3]);
+      for (int p = 0; p < SETS; ++p) {
+        const f32x4 v = rows[x & 1][p][q][lane];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          next[p][q] = __builtin_amdgcn_mfma_f32_16x16x4f32(m[x][4 * q + e], v[e], next[p][q], 0, 0, 0);
+      }
+#pragma unroll
+    for (int p = 0; p < SETS; ++p) S[p] = (next[p][0] + next[p][1]) + (next[p][2] + next[p][3]);
     // behind the products, into the registers that they are done with: loaded before, the
     // values would go through others and be waited for at once
     __builtin_amdgcn_sched_barrier(0);
@@ -351,11 +359,12 @@ __global__ __launch_bounds__(kThr) void k_delta_walk(Walk a) {
 #pragma unroll
   for (int x = 0; x < kAhead - 1; ++x)
     if (n + x < count) step(n + x, x);
-  float* end = unit ? a.mend : a.end;
-  if (!end) return;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (held(i)) end[slot(i)] = S[i];
+  for (int i = 0; i < 4; ++i) {
+    if (!held(i)) continue;
+    if (a.end) a.end[slot(i)] = S[0][i];
+    if constexpr (MAPS) a.mend[slot(i)] = S[1][i];
+  }
 }
 
 // The outputs of one chunk for `each` output heads of a state head. First Z = T (V -
@@ -1014,10 +1023,12 @@ struct Room {
   }
 };
 
-// A chunk takes a walk about the same time whatever happens beside it, so long walks
-// of few chains are cut into segments: their maps' products at once (twice the
-// columns), a walk over those, then the segments from their own states. In units of a chunk's
-// time; a further launch costs about 10, and 512 blocks run at once.
+// A chunk takes a walk about the same time (0.85 us) whatever happens beside it, so long
+// walks of few chains are cut into segments: their maps' products at once (a chunk 1.6
+// times as long), a walk over those, then the segments from their own states. In units of a
+// chunk's time; two further launches cost about 20, and 512 blocks run at once. 32768
+// tokens of 14 states: 9 segments 205 us (4: 218, 18: 213; one walk 430); 1000 tokens of 4:
+// one walk 15 us (4 segments 26); 4 x 4096 tokens of 14: one walk 58 us (4 segments 104).
 struct Segments {
   int count, len;
 };
@@ -1027,7 +1038,7 @@ Segments segments(int U, int NC) {
   double least = NC * rounds(4LL * U);
   for (int len = 4; 2 * len <= NC; ++len) {
     const int n = (NC + len - 1) / len;
-    const double cost = len * (rounds(8LL * U * n) + rounds(4LL * U * n)) + n * rounds(4LL * U) + 20;
+    const double cost = 2.6 * len * rounds(4LL * U * n) + n * rounds(4LL * U) + 20;
     if (cost < least) least = cost, best = {n, len};
   }
   return best;
@@ -1038,25 +1049,23 @@ void walk(const DeltaArgs& g, const float* M, const float* D, const float* init,
           float* scratch, bool back, hipStream_t st, const Timer& timed) {
   const int U = g.B * g.Hv, NC = g.NC;
   const Segments sg = segments(U, NC);
-  auto launch = [&](const Walk& a, auto tr, int cols) {
+  auto launch = [&](const Walk& a, auto tr, auto maps) {
     timed("k_delta_walk", st, [&] {
-      if (cols == 8)
-        hipLaunchKernelGGL((k_delta_walk<decltype(tr)::value, 8>), dim3(a.units * a.segs * 8), dim3(kThr), 0, st, a);
-      else
-        hipLaunchKernelGGL((k_delta_walk<decltype(tr)::value, 4>), dim3(a.units * a.segs * 4), dim3(kThr), 0, st, a);
+      hipLaunchKernelGGL((k_delta_walk<decltype(tr)::value, decltype(maps)::value>), dim3(a.units * a.segs * 4),
+                         dim3(kThr), 0, st, a);
     });
   };
   using Tr = std::integral_constant<bool, TR>;
   if (sg.count == 1) {
-    launch({M, D, init, each, end, nullptr, NC, 1, NC, U, g.D, g.DV, back}, Tr{}, 4);
+    launch({M, D, init, each, end, nullptr, NC, 1, NC, U, g.D, g.DV, back}, Tr{}, std::false_type{});
     return;
   }
   const size_t part = (size_t)U * sg.count * kTile2;
   float *segM = scratch, *segD = scratch + part, *segS = scratch + 2 * part;
-  launch({M, D, nullptr, nullptr, segD, segM, NC, sg.count, sg.len, U, 64, 64, back}, Tr{}, 8);
+  launch({M, D, nullptr, nullptr, segD, segM, NC, sg.count, sg.len, U, 64, 64, back}, Tr{}, std::true_type{});
   // the products stand as they act, whichever way the walk goes
-  launch({segM, segD, init, segS, end, nullptr, sg.count, 1, sg.count, U, g.D, g.DV, back}, std::false_type{}, 4);
-  launch({M, D, segS, each, nullptr, nullptr, NC, sg.count, sg.len, U, 64, 64, back}, Tr{}, 4);
+  launch({segM, segD, init, segS, end, nullptr, sg.count, 1, sg.count, U, g.D, g.DV, back}, std::false_type{}, std::false_type{});
+  launch({M, D, segS, each, nullptr, nullptr, NC, sg.count, sg.len, U, 64, 64, back}, Tr{}, std::false_type{});
 }
 size_t walk_scratch(int U, int NC) {
   const Segments sg = segments(U, NC);
