@@ -279,7 +279,9 @@ template <typename T>
 __global__ __launch_bounds__(256, kPartsOf<T> == 1 ? 3 : 1) void k_window_dq(WindowArgs a, Shape sh, int qblocks, const T* __restrict__ out,
                                                       const float* __restrict__ lse, const T* __restrict__ dout,
                                                       float* __restrict__ delta, T* __restrict__ dq) {
-  constexpr int NP = kPartsOf<T>, CT = kColTiles<T>;
+  // dS takes two parts for bf16, as its sum has to be better than the one rounding of dq itself
+  // (one part: dq's relative error 2.5e-3 in place of 1.8e-3, and 135 us in place of 155 at 4 x 4096 tokens)
+  constexpr int NP = kPartsOf<T>, NS = NP == 1 ? 2 : NP, CT = kColTiles<T>;
   __shared__ Tile<NP> K, V;
   const int t = threadIdx.x, lane = t & 63, w = wave_of(t), g = lane >> 4, c = lane & 15;
   const Block at = query_block<T>(a, sh, qblocks, w);
@@ -332,7 +334,7 @@ __global__ __launch_bounds__(256, kPartsOf<T> == 1 ? 3 : 1) void k_window_dq(Win
         }
       }
     }
-    Frag<NP> p[CT];
+    Frag<NS> p[CT];
 #pragma unroll
     for (int x = 0; x < CT; ++x) {
       float y[8];
@@ -345,7 +347,7 @@ __global__ __launch_bounds__(256, kPartsOf<T> == 1 ? 3 : 1) void k_window_dq(Win
         for (int e = 0; e < 8; ++e)
           y[e] = sees(at.i0 + 16 * x + c, jh + 16 * (e >> 2) + 4 * g + (e & 3)) ? y[e] : 0.f;
       }
-      p[x] = split<NP>(y);
+      p[x] = split<NS>(y);
     }
 #pragma unroll
     for (int m = 0; m < 4; ++m) {
