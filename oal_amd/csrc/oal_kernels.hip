@@ -1617,13 +1617,14 @@ static int window_args(oal::WindowArgs* a, const char* what, const void* q, cons
     return fail("dtype must be OAL_DTYPE_F32, OAL_DTYPE_BF16 or OAL_DTYPE_F16");
   if (!q || !k || !v || !strides) return fail(std::string(what) + ": null pointer argument");
   *a = {strided(q, strides), strided(k, strides + 3), strided(v, strides + 6), batch, q_heads, kv_heads, query_len,
-        key_len, key_dim, value_dim, window, sinks, scale};
+        key_len, key_dim, value_dim, std::min(window, key_len), std::min(sinks, key_len), scale};
   if (!rows_aligned(a->q, dtype, batch, q_heads, query_len) || !rows_aligned(a->k, dtype, batch, kv_heads, key_len) ||
       !rows_aligned(a->v, dtype, batch, kv_heads, key_len))
     return fail(std::string(what) + ": rows must be 16-byte aligned");
   // 32-bit offsets inside a tile of 64 rows
-  for (const oal::Strided* s : {&a->q, &a->k, &a->v})
-    if (key_len > 1 && (s->n < 0 || s->n >= (1 << 24))) return fail(std::string(what) + ": rows are too far apart");
+  const auto near = [](const oal::Strided& s, int len) { return len <= 1 || (s.n >= 0 && s.n < (1 << 24)); };
+  if (!near(a->q, query_len) || !near(a->k, key_len) || !near(a->v, key_len))
+    return fail(std::string(what) + ": rows are too far apart");
   return 0;
 }
 

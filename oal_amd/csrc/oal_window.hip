@@ -25,7 +25,7 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNone = -__builtin_inff();
-constexpr float kFloor = -1e30f;  // before the first maximum: below every finite score
+constexpr float kFloor = -3.402823466e38f;  // before the first maximum: no finite score is below it
 
 template <typename T>
 __device__ __forceinline__ const T* rows_at(const Strided& s, int b, int h, int64_t row) {
@@ -719,13 +719,16 @@ __global__ __launch_bounds__(64) void k_window_step_join(WindowStepArgs a) {
 WindowPlan window_plan(int B, int Hq, int Hk, int Nq, int Nk, int window, int sinks, int keys) {
   WindowPlan p;
   const int R = Hq / Hk;
+  window = std::min(window, Nk), sinks = std::min(sinks, Nk);
   const int64_t blocks = (int64_t)B * Hk * ((Nk + keys - 1) / keys);
   // parts until every CU has a few blocks
   p.splits = (int)std::clamp<int64_t>((768 + blocks - 1) / blocks, 1, R);
   p.sink_rows = std::max(0, std::min(sinks, Nk - window));
   p.sink_blocks = (p.sink_rows + keys - 1) / keys;
-  const int64_t steps = (int64_t)R * ((std::min(Nq, Nk - std::min(window, Nk)) + 63) / 64);
-  p.chunks = p.sink_rows ? (int)std::clamp<int64_t>(steps / 8, 1, 64) : 0;
+  // the first keys' steps in pieces of 8 and more, up to 1024 blocks in all: each piece has sums of its own in memory
+  const int64_t steps = (int64_t)R * ((std::min(Nq, Nk - window) + 63) / 64);
+  const int64_t sums = (int64_t)B * Hk * p.sink_blocks;
+  p.chunks = p.sink_rows ? (int)std::clamp<int64_t>(std::min(steps / 8, 1024 / sums), 1, 64) : 0;
   return p;
 }
 

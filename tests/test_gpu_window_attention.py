@@ -96,6 +96,36 @@ def test_large_scores():
     assert float((got.double().cpu() - want).norm() / want.norm()) <= 64 * 800 * 2.0 ** -24
 
 
+def test_scores_below_any_that_a_sum_starts_from():
+    # all scores about -6e33 and equal: the weights are too
+    dev = _dev()
+    q, k, v, _ = (t.to(dev) for t in _qkv(1, (2, 1), 30, seed=4))
+    got = window_attention(torch.full_like(q, -1e16), torch.full_like(k, 1e16), v, window=7, scale=1.0)
+    want = dense(torch.zeros(1, 2, 30, 64), torch.zeros(1, 1, 30, 64), v.double().cpu(), window=7, sinks=0, scale=1.0)
+    _near(got, want, torch.float32)
+
+
+def test_one_query_far_from_its_heads():
+    # the stride of a dimension of one row does not matter
+    dev = _dev()
+    q, k, v, _ = (t.to(dev) for t in _qkv(1, (2, 1), 1, 30, seed=4))
+    far = q.as_strided(q.shape, (128, 64, 1 << 25, 1))
+    assert torch.equal(window_attention(far, k, v, window=7, sinks=2), window_attention(q, k, v, window=7, sinks=2))
+
+
+def test_widest_window_and_all_first_keys():
+    dev = _dev()
+    q, k, v, o = (t.to(dev) for t in _qkv(2, (4, 2), 150, dtype=torch.bfloat16, seed=6))
+    results = []
+    for window, sinks in ((150, 0), (150, 150), (1 << 30, 1 << 30)):
+        leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+        out = window_attention(*leaves, window=window, sinks=sinks)
+        results.append([out, *torch.autograd.grad(out, leaves, o)])
+    for result in results[1:]:
+        assert all(torch.equal(x, y) for x, y in zip(result, results[0]))
+    _check(_qkv(2, (4, 2), 150, dtype=torch.bfloat16, seed=6), 1, 1 << 30)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_strided_and_misaligned_rows(dtype):
     dev = _dev()
