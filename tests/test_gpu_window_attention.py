@@ -240,6 +240,21 @@ def test_step_without_a_token_leaves_its_caches():
     assert kc._version > version
 
 
+@pytest.mark.parametrize("batch,window,sinks", [(1, 65536, 0), (1, 40000, 7), (130, 300, 4), (2, 128, 0)])
+def test_step_in_as_many_pieces_as_the_cache_has(batch, window, sinks):
+    dev = _dev()
+    gen = torch.Generator().manual_seed(window)
+    q, k, v = (torch.randn(batch, h, 1, 64, generator=gen) for h in (4, 2, 2))
+    kc, vc = (torch.randn(batch, 2, window + sinks, 64, generator=gen) for _ in range(2))
+    at = sinks + 3 * window + 5
+    got = window_attention_step(*(t.to(dev) for t in (q, k, v)), kc.to(dev), vc.to(dev),
+                                torch.full((batch,), at, device=dev), window=window, sinks=sinks, scale=0.2)
+    kc[:, :, sinks + 5 % window], vc[:, :, sinks + 5 % window] = k[:, :, 0], v[:, :, 0]
+    score = 0.2 * q.double().view(batch, 2, 2, 64) @ kc.double().transpose(2, 3)
+    want = torch.softmax(score, -1) @ vc.double()
+    _near(got, want.view(batch, 4, 1, 64), torch.float32)
+
+
 def test_step_takes_slices_of_larger_caches():
     dev = _dev()
     gen = torch.Generator().manual_seed(6)
