@@ -282,8 +282,8 @@ int oal_check_outputs(int wide, int out_kind, const void* num, const void* den, 
 size_t oal_gated_delta_saved_bytes(int batch, int v_heads, int seq_len, int keep);
 int oal_gated_delta_forward(const void* q, const void* k, const void* v, const float* g, const void* beta,
                             const int64_t* strides, int beta_f32, int batch, int q_heads, int k_heads, int v_heads,
-                            int seq_len, int key_dim, int value_dim, int dtype, float scale, const float* state, void* out, float* final_state,
-                            void* saved, int keep, void* stream);
+                            int seq_len, int key_dim, int value_dim, int dtype, float scale, const float* state,
+                            void* out, float* final_state, void* saved, int keep, void* stream);
 
 /*
  * Its VJP: dout [B][H][N][value_dim] (dtype) and dfinal [B][Hv][key_dim][value_dim] f32 (may be NULL)
@@ -293,9 +293,9 @@ int oal_gated_delta_forward(const void* q, const void* k, const void* v, const f
 size_t oal_gated_delta_workspace_bytes(int batch, int q_heads, int k_heads, int v_heads, int seq_len, int key_dim);
 int oal_gated_delta_backward(const void* q, const void* k, const void* v, const float* g, const void* beta,
                              const int64_t* strides, int beta_f32, int batch, int q_heads, int k_heads, int v_heads,
-                             int seq_len, int key_dim, int value_dim, int dtype, float scale, const void* saved, const void* dout,
-                             const float* dfinal, void* dq, void* dk, void* dv, float* dg, void* dbeta, float* dstate,
-                             void* workspace, void* stream);
+                             int seq_len, int key_dim, int value_dim, int dtype, float scale, const void* saved,
+                             const void* dout, const float* dfinal, void* dq, void* dk, void* dv, float* dg,
+                             void* dbeta, float* dstate, void* workspace, void* stream);
 
 /*
  * The recurrence for a few tokens: state [B][Hv][key_dim][value_dim] f32 is updated
@@ -319,15 +319,17 @@ int oal_gated_delta_step(const void* q, const void* k, const void* v, const floa
  */
 int oal_window_attention_forward(const void* q, const void* k, const void* v, const int64_t* strides, int batch,
                                  int q_heads, int kv_heads, int query_len, int key_len, int key_dim,
-                                 int value_dim, int window, int sinks, int dtype, float scale, void* out, float* lse, void* stream);
+                                 int value_dim, int window, int sinks, int dtype, float scale, void* out,
+                                 float* lse, void* stream);
 
 /* Its VJP: out, lse and dout [B][Hq][query_len][value_dim] -> contiguous dq, dk, dv (dtype). */
 size_t oal_window_attention_workspace_bytes(int batch, int q_heads, int kv_heads, int query_len, int key_len,
                                             int window, int sinks, int dtype);
 int oal_window_attention_backward(const void* q, const void* k, const void* v, const int64_t* strides, int batch,
                                   int q_heads, int kv_heads, int query_len, int key_len, int key_dim,
-                                  int value_dim, int window, int sinks, int dtype, float scale, const void* out, const float* lse, const void* dout,
-                                  void* dq, void* dk, void* dv, void* workspace, void* stream);
+                                  int value_dim, int window, int sinks, int dtype, float scale, const void* out,
+                                  const float* lse, const void* dout, void* dq, void* dk, void* dv, void* workspace,
+                                  void* stream);
 
 /*
  * One token per sequence over ring caches [B][Hkv][sinks + window][D]: the token at

@@ -11,7 +11,12 @@
 // A chunk maps the state before it to M S + D, with M and D of its own tokens alone:
 // T, M and D are formed chunk by chunk at once, then S in a walk of one product per
 // chunk, then Z and O chunk by chunk at once. What makes the state is exact to fp32
-// whatever the tensors' type (oal_tile.hpp): a state is a sum over all tokens before it and is handed on in fp32.
+// whatever the tensors' type (oal_tile.hpp): a state is a sum over all tokens before it and is
+// handed on in fp32. T, M, D, S and Z pass through memory in fp32, 16 KB each per 64
+// tokens where q, k, v and out are 8 KB: they are what the chunked kernels move most of.
+//
+// Figures at the kernels: bfloat16, 4 x 4096 tokens of 14 heads and states (3584 chunks),
+// with the bytes that the kernel itself reads and writes; a copy reaches 5.2 TB/s.
 //
 // Decays enter as differences of sums, held in two floats (48 bits): a token that
 // forgets nearly everything leaves large sums whose differences still matter.
@@ -127,7 +132,9 @@ __device__ __forceinline__ void put_parts(Tile<NP>& s, int row, int col, float x
 //   M = e^(G_63) - (e^(G_63 - G) beta K)^T T e^G K,  D = (e^(G_63 - G) beta K)^T T V.
 // T's diagonal blocks of 16 rows by substitution (a lane per column), then twice
 // the rule for two blocks, [L11 0; L21 L22]^-1 = [T11 0; -T22 L21 T11, T22], on the
-// fp32 matrix cores. In the products a wave owns 16 columns of M and of D.
+// fp32 matrix cores. In the products a wave owns 16 columns of M and of D, V's tile in
+// the LDS that the triangle leaves: three blocks per CU (53 KB). 68 us, 240 MB: 3.5 TB/s, a
+// third of the time the inverse, whose steps wait for each other.
 template <typename T>
 __global__ __launch_bounds__(kThr) void k_delta_chunk(DeltaArgs a, float* __restrict__ Gout, float* __restrict__ Tout,
                                                       float* __restrict__ Mout, float* __restrict__ Dout) {
@@ -269,6 +276,8 @@ __global__ __launch_bounds__(kThr) void k_delta_chunk(DeltaArgs a, float* __rest
 // loaded kAhead maps before. On the fp32 matrix cores, whose operands are M and S as
 // they lie in registers and LDS (sum index 16 q + 4 g + e of instruction q, e): their
 // 16 instructions per map are slower than 12 of bf16 parts, but there is nothing to split.
+// 58 us for 64 maps, 0.9 us each: bound by the way of a state through LDS, 16
+// instructions and their sum, not by the 176 MB that it moves meanwhile (3.0 TB/s).
 struct Walk {
   const float* M;     // [units][maps][64][64]
   const float* D;
@@ -372,6 +381,7 @@ __global__ __launch_bounds__(kThr) void k_delta_walk(Walk a) {
 // wave's 16 queries are the columns, so the scores are an operand of the product
 // with U as they are. What goes on to the backward (KEEP) is exact to fp32; the outputs take
 // two parts per value for 16-bit tensors, twice their precision: one rounding is the output's own.
+// 80 us, 294 MB: 3.7 TB/s, with three blocks per CU (42 KB of LDS) where nothing is kept.
 template <typename T, bool KEEP>
 __global__ __launch_bounds__(kThr) void k_delta_out(DeltaArgs a, int each, const float* __restrict__ Gin,
                                                     const float* __restrict__ Tin, const float* __restrict__ Sin,
@@ -473,9 +483,11 @@ __global__ __launch_bounds__(kThr) void k_delta_out(DeltaArgs a, int each, const
 //   E = D^T dO,  F = scale (e^G Q)^T dO - (e^G K)^T T^T (beta E)
 //   dU = E + e^(G_63 - G) K dS',  dZ = dV = T^T (beta dU)
 // Decays' gradients are sums of terms that cancel, so all of it is exact to fp32.
+// k_delta_bwd_local: 60 us, 264 MB: 4.4 TB/s, three blocks per CU (two: 69 us).
 // ---------------------------------------------------------------------------
 template <typename T>
-__global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 3 : 1) void k_delta_bwd_local(DeltaArgs a, const T* __restrict__ dout,
+__global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 3 : 1)
+void k_delta_bwd_local(DeltaArgs a, const T* __restrict__ dout,
                                                           const float* __restrict__ Gin, const float* __restrict__ Tin,
                                                           float* __restrict__ E, float* __restrict__ F) {
   constexpr int NP = kPartsOf<T>;
@@ -533,7 +545,8 @@ __global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 3 : 1) void k_delta_bwd_lo
     for (int s = 0; s < 2; ++s) {
       of[s] = col_frag(O, 16 * w, s, lane);
       float v[8];
-      const f32x4 g0 = a.scale * four(gate.since + 32 * s + 8 * g), g1 = a.scale * four(gate.since + 32 * s + 8 * g + 4);
+      const f32x4 g0 = a.scale * four(gate.since + 32 * s + 8 * g);
+      const f32x4 g1 = a.scale * four(gate.since + 32 * s + 8 * g + 4);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         v[j] = 0.f;
@@ -598,7 +611,10 @@ __device__ __forceinline__ void own_row(Frag<3> (&f)[2], const float* row, int g
 // dg the sums of dG from each token to the chunk's end. Terms that do not decay (j = i,
 // the last token's write) are left out rather than cancelled: where all decay is
 // strong, dg is far smaller than they are. All products are transposed: a wave's 16
-// tokens are the columns.
+// tokens are the columns. What goes into dq and dk alone is cut to two bf16 parts
+// (16 bits) for 16-bit tensors, which then round once themselves; dg and dbeta see three.
+// 205 us, 470 MB: 2.3 TB/s. Two blocks per CU (76 KB of LDS, 251 registers) do not
+// cover its loads and its 13 products of 64 x 64 x 64 in 3 to 6 instructions each.
 template <typename T>
 __global__ __launch_bounds__(kThr) void k_delta_bwd_out(DeltaArgs a, const T* __restrict__ dout,
                                                         const float* __restrict__ Gin, const float* __restrict__ Tin,
@@ -918,7 +934,9 @@ __global__ __launch_bounds__(kThr) void k_delta_sum_heads(const float* __restric
 
 // ---------------------------------------------------------------------------
 // The recurrence itself, for single tokens: a block per state head holds the
-// state, 4 x 4 values per thread, for all N tokens and writes it back.
+// state, 4 x 4 values per thread, for all N tokens and writes it back. Bound by the state,
+// once there and back: 256 users of 14 states 29 us, 119 MB at 4.1 TB/s; one user 6.6 us, a
+// launch and its latencies.
 // ---------------------------------------------------------------------------
 template <typename T>
 __global__ __launch_bounds__(kThr) void k_delta_step(DeltaStepArgs a) {
@@ -927,7 +945,8 @@ __global__ __launch_bounds__(kThr) void k_delta_step(DeltaStepArgs a) {
   const int u = blockIdx.x, b = u / a.Hv, h = u % a.Hv;
   const int d0 = 4 * (t >> 4), c0 = 4 * (t & 15);
   float* state = a.state + (size_t)u * a.Dk * a.Dv;
-  const bool fours = a.Dv % 4 == 0 && reinterpret_cast<uintptr_t>(a.state) % 16 == 0;  // pieces of four are whole and aligned
+  // pieces of four are whole and aligned
+  const bool fours = a.Dv % 4 == 0 && reinterpret_cast<uintptr_t>(a.state) % 16 == 0;
   float s[4][4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -1064,7 +1083,8 @@ void walk(const DeltaArgs& g, const float* M, const float* D, const float* init,
   float *segM = scratch, *segD = scratch + part, *segS = scratch + 2 * part;
   launch({M, D, nullptr, nullptr, segD, segM, NC, sg.count, sg.len, U, 64, 64, back}, Tr{}, std::true_type{});
   // the products stand as they act, whichever way the walk goes
-  launch({segM, segD, init, segS, end, nullptr, sg.count, 1, sg.count, U, g.D, g.DV, back}, std::false_type{}, std::false_type{});
+  launch({segM, segD, init, segS, end, nullptr, sg.count, 1, sg.count, U, g.D, g.DV, back}, std::false_type{},
+         std::false_type{});
   launch({M, D, segS, each, nullptr, nullptr, NC, sg.count, sg.len, U, 64, 64, back}, Tr{}, std::false_type{});
 }
 size_t walk_scratch(int U, int NC) {
@@ -1117,9 +1137,11 @@ void launch_delta_forward(const DeltaArgs& a, const float* state, void* out, flo
   const dim3 grid(U * a.NC * ((rep + each - 1) / each));
   timed("k_delta_out", st, [&] {
     if (keep)
-      hipLaunchKernelGGL((k_delta_out<T, true>), grid, dim3(kThr), 0, st, a, each, s.G, s.T, s.S, s.Z, static_cast<T*>(out));
+      hipLaunchKernelGGL((k_delta_out<T, true>), grid, dim3(kThr), 0, st, a, each, s.G, s.T, s.S, s.Z,
+                         static_cast<T*>(out));
     else
-      hipLaunchKernelGGL((k_delta_out<T, false>), grid, dim3(kThr), 0, st, a, each, s.G, s.T, s.S, s.Z, static_cast<T*>(out));
+      hipLaunchKernelGGL((k_delta_out<T, false>), grid, dim3(kThr), 0, st, a, each, s.G, s.T, s.S, s.Z,
+                         static_cast<T*>(out));
   });
 }
 

@@ -19,8 +19,9 @@ query head o // (H / Hq) from state head o // (H / Hv).
 
 The rule is a stable memory for keys of length one (normalise them before the call)
 and beta up to 2. Sums over tokens do not depend on the type of q, k and v, which may be
-float32, bfloat16 or float16: states, decays and their gradients are exact to float32. A token with beta = 0 and g = 0 leaves the
-state as it is: pad batches of ragged lengths with such tokens. Values have to be
+float32, bfloat16 or float16: states, decays and their gradients are exact to float32.
+A token with beta = 0 and g = 0 leaves the state as it is: pad batches of ragged lengths
+with such tokens. Values have to be
 finite: a token that is not spoils the 64 tokens of its chunk.
 """
 
@@ -58,7 +59,8 @@ def _plain(q, k, v, g, beta, state) -> bool:
             and k.shape == (b, hk, n, d) and v.shape == (b, hv, n, dv) and g.shape == beta.shape == (b, hv, n)
             and b > 0 and hq > 0 and hk > 0 and hv > 0 and n > 0 and 0 < d <= HEAD_DIM and 0 < dv <= HEAD_DIM
             and hv % hk == 0 and (hq % hv == 0 or hv % hq == 0)
-            and (state is None or (state.dtype is torch.float32 and state.shape == (b, hv, d, dv) and state.device == dev))
+            and (state is None or (state.dtype is torch.float32 and state.shape == (b, hv, d, dv)
+                                   and state.device == dev))
         )
     except (AttributeError, ValueError, IndexError):
         return False

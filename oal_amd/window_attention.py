@@ -172,8 +172,8 @@ def window_attention_step(
     if size > _MOST:
         raise ValueError(f"the cache must have at most {_MOST} slots")
     for name, t, width in (("k_cache", k_cache, d), ("v_cache", v_cache, dv)):
-        if (isinstance(t, torch.Tensor) and t.dtype is q.dtype and t.device == q.device and t.shape == (b, hk, size, width)
-                and t.is_contiguous() and t.data_ptr() % 16 == 0):
+        if (isinstance(t, torch.Tensor) and t.dtype is q.dtype and t.device == q.device
+                and t.shape == (b, hk, size, width) and t.is_contiguous() and t.data_ptr() % 16 == 0):
             continue
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{name} must be a torch.Tensor")
