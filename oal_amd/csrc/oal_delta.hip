@@ -163,7 +163,8 @@ __global__ __launch_bounds__(kThr) void k_delta_chunk(DeltaArgs a, float* __rest
   form_gates<T>(gate, a, b, h, tok0, t);
   ki.store(K, t);
   lds_sync();
-  fetch_gates(*reinterpret_cast<Gates*>(Gout + ((size_t)u * a.NC + ch) * kGates), reinterpret_cast<const float*>(&gate), t);
+  float* gates = Gout + ((size_t)u * a.NC + ch) * kGates;
+  fetch_gates(*reinterpret_cast<Gates*>(gates), reinterpret_cast<const float*>(&gate), t);
   {
     const Frag<NP> k0 = row_frag(K, 16 * w, 0, lane), k1 = row_frag(K, 16 * w, 1, lane);
 #pragma unroll

@@ -11,9 +11,11 @@
 // ranges: the first keys that its window has left behind, and the window.
 //
 // Scores, maxima, sums and results are fp32. For bf16 tensors the weights p are
-// rounded to bf16 where they meet v or do, and ds where it meets q: each by at most half a
-// step (2^-8 of a weight), with independent signs over a row, beside the result's own
-// rounding. The sums of the weights are of the rounded ones, so they still average.
+// rounded to bf16 where they meet v or do: by at most half a step (2^-8 of a weight), with
+// independent signs over a row, beside the result's own rounding. The sums of the weights
+// are of the rounded ones, so they still average. ds takes two parts (16 bits): it has
+// both signs, and what cancels would leave the roundings (with one part dq and dk were off
+// by 2.5e-3 to 2.7e-3 of their norm in place of 1.8e-3 to 2.1e-3).
 //
 // Figures at the kernels: bfloat16, 4 x 4096 tokens of 14 query and 2 KV heads, window 1024.
 
@@ -285,13 +287,11 @@ void k_window_fwd(WindowArgs a, Shape sh, int qblocks, T* __restrict__ out, floa
 }
 
 // dq, and for the other side delta_i = do_i.o_i: the forward's walk again. Bound by the
-// matrix cores (36 % busy) and the exponentials together. 155 us, 509 TFLOP/s.
+// matrix cores (36 % busy) and the exponentials together. 155 us, 509 TFLOP/s (135 us with ds in one part).
 template <typename T>
 __global__ __launch_bounds__(256, kPartsOf<T> == 1 ? 3 : 1)
 void k_window_dq(WindowArgs a, Shape sh, int qblocks, const T* __restrict__ out, const float* __restrict__ lse,
                  const T* __restrict__ dout, float* __restrict__ delta, T* __restrict__ dq) {
-  // dS takes two parts for bf16, as its sum has to be better than the one rounding of dq itself
-  // (one part: dq's relative error 2.5e-3 in place of 1.8e-3, and 135 us in place of 155 at 4 x 4096 tokens)
   constexpr int NP = kPartsOf<T>, NS = NP == 1 ? 2 : NP, CT = kColTiles<T>;
   __shared__ Tile<NP> K, V;
   const int t = threadIdx.x, lane = t & 63, w = wave_of(t), g = lane >> 4, c = lane & 15;
@@ -398,13 +398,14 @@ void k_window_dq(WindowArgs a, Shape sh, int qblocks, const T* __restrict__ out,
 // 0 .. near - 1: through the window; the others: first keys seen from afar. A block's keys
 // stay in registers while the queries of all its heads pass, so heads that share keys are
 // summed there; parts of them where that leaves CUs empty, summed by k_window_sum in
-// order. 154 us, 685 TFLOP/s of the four products, 37 % of the matrix cores' cycles.
+// order. 185 us, 570 TFLOP/s of the four products (154 us with ds in one part; two
+// waves per SIMD, which holds all in registers, 198).
 template <typename T>
 __global__ __launch_bounds__(256, kPartsOf<T> == 1 ? 3 : 1)
 void k_window_dkv(WindowArgs a, WindowPlan plan, int kblocks, int near, const float* __restrict__ lse,
                   const T* __restrict__ dout, const float* __restrict__ delta, float* __restrict__ part,
                   float* __restrict__ farpart) {
-  constexpr int NP = kPartsOf<T>, CT = kColTiles<T>, kKeys = 4 * kCols<T>;
+  constexpr int NP = kPartsOf<T>, NS = NP == 1 ? 2 : NP, CT = kColTiles<T>, kKeys = 4 * kCols<T>;
   __shared__ Tile<NP> Q, O;
   __shared__ alignas(16) float base[64], dot[64];
   const int t = threadIdx.x, lane = t & 63, w = wave_of(t), g = lane >> 4, c = lane & 15;
@@ -458,7 +459,8 @@ void k_window_dkv(WindowArgs a, WindowPlan plan, int kblocks, int near, const fl
         }
       }
     }
-    Frag<NP> p[CT], z[CT];
+    Frag<NP> p[CT];
+    Frag<NS> z[CT];
 #pragma unroll
     for (int x = 0; x < CT; ++x) {
       float y[8], yd[8];
@@ -482,7 +484,7 @@ void k_window_dkv(WindowArgs a, WindowPlan plan, int kblocks, int near, const fl
         }
       }
       p[x] = split<NP>(y);
-      z[x] = split<NP>(yd);
+      z[x] = split<NS>(yd);
     }
 #pragma unroll
     for (int m = 0; m < 4; ++m) {
