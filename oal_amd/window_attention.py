@@ -15,9 +15,10 @@ the grouped quadratic operator. The token at position p is kept in slot p where 
 else in slot sinks + (p - sinks) % window: the filled slots are just what the token sees, so
 the caches never grow and nothing is masked.
 
-bfloat16 tensors run on the matrix cores as they are, with the softmax in
-float32; float32 and float16 tensors in three and two exact bfloat16 parts per value, so that
-results are exact to their type.
+bfloat16 tensors run on the matrix cores as they are, with the softmax and all sums in
+float32 and its weights rounded to bfloat16 for the product with v; float32 and float16
+tensors run in three and two exact bfloat16 parts per value, so that results are exact to
+their type.
 Padding at the end of a sequence changes nothing before it; its values have to be finite
 all the same, in k, v and the gradients (a masked weight of zero times infinity is not zero).
 """
