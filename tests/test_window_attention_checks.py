@@ -112,3 +112,17 @@ def test_c_entries_check_before_they_launch():
     assert step(p, p, p, p, p, rows, p, 1, 2, 2, 64, 64, 3, 0, 5, 0.1, p, p, None) and b"type" in lib.oal_last_error()
     assert step(p, p, p, p, odd, rows, p, 1, 2, 2, 64, 64, 3, 0, 1, 0.1, p, p, None) and b"16-byte" in lib.oal_last_error()
     assert step(p, p, p, p, p, rows, p, 1, 2, 2, 12, 64, 3, 0, 1, 0.1, p, p, None) and b"multiples of 8" in lib.oal_last_error()
+
+
+def test_workspace_follows_the_keys():
+    try:
+        lib = _native.load_library()
+    except RuntimeError:
+        pytest.skip("liboal_amd.so not built")
+    size = lib.oal_window_attention_workspace_bytes
+    most = (1 << 31) - 1
+    assert size(1, 14, 2, 100, 100, most, most, 1) == size(1, 14, 2, 100, 100, 100, 100, 1)
+    # pieces of the first keys' sums: fewer, the more first keys there are
+    without, few, many = (size(1, 14, 2, 32768, 32768, 1024, sinks, 1) for sinks in (0, 4, 16384))
+    assert few - without <= 64 * 2 * 2 * 64 * 64 * 4
+    assert many - without <= 4 * 2 * 2 * 16384 * 64 * 4 + 4096
