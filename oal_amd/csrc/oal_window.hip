@@ -767,7 +767,7 @@ WindowPlan window_plan(int B, int Hq, int Hk, int Nq, int Nk, int window, int si
   const int R = Hq / Hk;
   window = std::min(window, Nk), sinks = std::min(sinks, Nk);
   const int64_t blocks = (int64_t)B * Hk * ((Nk + keys - 1) / keys);
-  // parts until every CU has a few blocks
+  // parts until every CU has three blocks, as many as fit: 4 x 4096 tokens in 3 parts 169 us, in 2 195, in 4 200
   p.splits = (int)std::clamp<int64_t>((768 + blocks - 1) / blocks, 1, R);
   p.sink_rows = std::max(0, std::min(sinks, Nk - window));
   p.sink_blocks = (p.sink_rows + keys - 1) / keys;
