@@ -3,8 +3,8 @@
 //
 // A value in three bf16 parts (the value rounded, what that left, what that
 // left) carries 24 bits, so products of such parts that leave out only the terms below
-// 2^-24 are as exact as fp32, at 3 (one operand a bf16 value as it is) or 6 matrix
-// instructions in place of the 16 times slower fp32 ones. bf16 tensors enter as
+// 2^-24 are as exact as fp32, at 3 (one operand a bf16 value as it is), 4 (two operands of two parts)
+// to 6 matrix instructions in place of the 16 times slower fp32 ones. bf16 tensors enter as
 // one part, fp16 tensors as two, fp32 tensors and intermediate results that have to stay fp32 as three.
 //
 // An accumulator tile of v_mfma_f32_16x16x32_bf16 holds rows 4 g + i in lane group
@@ -51,18 +51,30 @@ __device__ __forceinline__ Frag<NP> split(const float (&v)[8]) {
   return f;
 }
 
-// c += a b without the terms of parts below fp32's last bit; small terms first.
-template <int NA, int NB>
-__device__ __forceinline__ f32x4 mma(const Frag<NA>& a, const Frag<NB>& b, f32x4 c) {
-  constexpr int kLast = (NA > NB ? NA : NB) - 1;
+// c += a b of the parts i + j <= LAST, small terms first.
+template <int LAST, int NA, int NB>
+__device__ __forceinline__ f32x4 mma_parts(const Frag<NA>& a, const Frag<NB>& b, f32x4 c) {
 #pragma unroll
-  for (int s = kLast; s >= 0; --s)
+  for (int s = LAST; s >= 0; --s)
 #pragma unroll
     for (int i = 0; i < NA; ++i) {
       const int j = s - i;
       if (j >= 0 && j < NB) c = mfma16(a.p[i], b.p[j], c);
     }
   return c;
+}
+// c += a b without the terms of parts below fp32's last bit: part i is at most 2^-8i of its value, so
+// those past i + j = 2. Two operands of two parts have all four terms.
+template <int NA, int NB>
+__device__ __forceinline__ f32x4 mma(const Frag<NA>& a, const Frag<NB>& b, f32x4 c) {
+  return mma_parts<(NA + NB - 2 < 2 ? NA + NB - 2 : 2)>(a, b, c);
+}
+// The same for a b that was itself cut to two parts: what the cut left is up to 2^-16 of a value, and
+// so is the product of the low parts, which is left out too (float16 window, 4 x 2048 tokens,
+// forward and backward: 457 us, with it 475).
+template <int NA, int NB>
+__device__ __forceinline__ f32x4 mma_cut(const Frag<NA>& a, const Frag<NB>& b, f32x4 c) {
+  return mma_parts<(NA > NB ? NA : NB) - 1>(a, b, c);
 }
 
 // LDS tile: NP parts of 64 rows of 64 bf16. The 16-byte piece c of row r stands at c ^ r % 8:

@@ -254,7 +254,7 @@ void k_window_fwd(WindowArgs a, Shape sh, int qblocks, T* __restrict__ out, floa
     for (int m = 0; m < 4; ++m) {
       const Frag<NP> v = col_frag_perm(V, 16 * m, half, lane);
 #pragma unroll
-      for (int x = 0; x < CT; ++x) acc[x][m] = mma(v, p[x], acc[x][m]);
+      for (int x = 0; x < CT; ++x) acc[x][m] = mma_cut(v, p[x], acc[x][m]);
     }
   };
   for (int tile = 0; tile < keys.tiles; ++tile) {
@@ -364,7 +364,7 @@ void k_window_dq(WindowArgs a, Shape sh, int qblocks, const T* __restrict__ out,
     for (int m = 0; m < 4; ++m) {
       const Frag<NP> k = col_frag_perm(K, 16 * m, half, lane);
 #pragma unroll
-      for (int x = 0; x < CT; ++x) acc[x][m] = mma(k, p[x], acc[x][m]);
+      for (int x = 0; x < CT; ++x) acc[x][m] = mma_cut(k, p[x], acc[x][m]);
     }
   };
   for (int tile = 0; tile < keys.tiles; ++tile) {
@@ -491,8 +491,8 @@ void k_window_dkv(WindowArgs a, WindowPlan plan, int kblocks, int near, const fl
       const Frag<NP> q = col_frag_perm(Q, 16 * m, half, lane), o = col_frag_perm(O, 16 * m, half, lane);
 #pragma unroll
       for (int x = 0; x < CT; ++x) {
-        dk[x][m] = mma(q, z[x], dk[x][m]);
-        dv[x][m] = mma(o, p[x], dv[x][m]);
+        dk[x][m] = mma_cut(q, z[x], dk[x][m]);
+        dv[x][m] = mma_cut(o, p[x], dv[x][m]);
       }
     }
   };
@@ -690,7 +690,7 @@ __global__ __launch_bounds__(256) void k_window_step(WindowStepArgs a) {
 #pragma unroll
       for (int e = 0; e < NP; ++e) v.p[e] = tr_rows(x + e * 32 * kTileRow, x + e * 32 * kTileRow + 16 * kTileRow);
       acc[m] *= keep;
-      acc[m] = mma(v, p, acc[m]);
+      acc[m] = mma_cut(v, p, acc[m]);
     }
     asm volatile("" ::: "memory");
     __builtin_amdgcn_wave_barrier();
