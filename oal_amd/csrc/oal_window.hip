@@ -628,8 +628,11 @@ __global__ __launch_bounds__(256) void k_window_step(WindowStepArgs a) {
   Frag<NP> qf[2];
 #pragma unroll
   for (int s = 0; s < 2; ++s) qf[s] = frag_of<T>(row8(q, 32 * s + 8 * g, a.D, r < R));
-  f32x4 acc[4] = {};
-  float top = kNone, sum = 0.f;
+  Frag<1> ones;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) ones.p[0][e] = static_cast<__bf16>(1.f);
+  f32x4 acc[4] = {}, sum = {};
+  float top = kNone;
   const float scale = a.scale * kLog2e;
   for (int j0 = begin + 32 * w; j0 < end; j0 += 128) {
     Row8<T> kr[2][2], vr[4];
@@ -663,16 +666,14 @@ __global__ __launch_bounds__(256) void k_window_step(WindowStepArgs a) {
     const float base = most == kNone ? 0.f : most;
     const float keep = __builtin_amdgcn_exp2f(top - base);
     top = most;
-    float part = 0.f;
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s[m][e] = __builtin_amdgcn_exp2f(s[m][e] - base);
-        part += s[m][e];
-      }
-    sum = sum * keep + part;
+      for (int e = 0; e < 4; ++e) s[m][e] = __builtin_amdgcn_exp2f(s[m][e] - base);
     const Frag<NP> p = acc_frag<NP>(s[0], s[1]);
+    // of the weights as the values meet them
+    sum *= keep;
+    sum = mma(ones, p, sum);
     // a wave's LDS accesses are in order: its own rows need no barrier
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
@@ -695,8 +696,7 @@ __global__ __launch_bounds__(256) void k_window_step(WindowStepArgs a) {
     asm volatile("" ::: "memory");
     __builtin_amdgcn_wave_barrier();
   }
-  sum = group_sum(sum);
-  if (g == 0) top4[w][c] = top, sum4[w][c] = sum;
+  if (g == 0) top4[w][c] = top, sum4[w][c] = sum[0];
 #pragma unroll
   for (int m = 0; m < 4; ++m) *reinterpret_cast<f32x4*>(&acc4[w][c][16 * m + 4 * g]) = acc[m];
   __syncthreads();

@@ -8,7 +8,7 @@ import torch
 
 from oal_amd import _native
 from oal_amd.gated_delta import gated_delta_attention
-from oal_amd.window_attention import window_attention
+from oal_amd.window_attention import window_attention, window_attention_step
 from oracle.delta_oracle import gated_delta
 from oracle.window_oracle import window_attention as dense
 
@@ -135,3 +135,18 @@ def test_float16_scores_are_exact():
                   for dtype in (torch.float16, torch.float32))
     print(f"lse: {err:.2e} {least:.2e}", flush=True)
     assert err <= 3 * least, f"{err:.3g}, as float32 {least:.3g}"
+
+
+@pytest.mark.parametrize("slots", [128, 2048])
+def test_weights_of_a_step_average(slots):
+    """The weights are summed as they meet the values: whatever their roundings, values that are all
+    one have the mean one. All but every 32nd weight here are 0.5018, which is 0.5 in bf16."""
+    dev = _dev()
+    k = torch.zeros(1, 1, slots, 8, device=dev, dtype=torch.bfloat16)
+    k[..., 0] = torch.where(torch.arange(slots, device=dev) % 32 == 0, 0.0, -1.0)
+    q = torch.zeros(1, 1, 1, 8, device=dev, dtype=torch.bfloat16)
+    q[..., 0] = 1.0
+    v = torch.ones_like(k)
+    at = torch.full((1,), 3 * slots, device=dev)
+    out = window_attention_step(q, k[:, :, :1].contiguous(), v[:, :, :1].contiguous(), k, v, at, window=slots, scale=0.68955)
+    assert torch.equal(out, torch.ones_like(out))
