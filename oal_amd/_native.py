@@ -166,6 +166,7 @@ def _scope(device: torch.device, name: str | None = None):
 
 
 _C = torch._C
+_forward_ad = torch.autograd.forward_ad
 _PLAIN_TYPES = (torch.Tensor, torch.nn.Parameter)
 _TRACERS = tuple(getattr(_C._TorchDispatchModeKey, name) for name in ("FAKE", "PROXY", "FUNCTIONAL"))
 
@@ -179,10 +180,31 @@ def ordinary(*tensors: torch.Tensor) -> bool:
         if type(t) not in _PLAIN_TYPES or not t.is_cuda:
             return False
     if (torch.compiler.is_compiling() or _C._is_tracing() or _C._are_functorch_transforms_active()
-            or torch.autograd.forward_ad._current_level >= 0):
+            or _forward_ad._current_level >= 0):
         return False
-    tracing = _C._len_torch_dispatch_stack() and any(_C._get_dispatch_mode(key) is not None for key in _TRACERS)
-    return torch.version.hip is not None and not tracing
+    return torch.version.hip is not None and not _dispatch_tracing()
+
+
+def _dispatch_tracing() -> bool:
+    return bool(_C._len_torch_dispatch_stack()) and any(_C._get_dispatch_mode(key) is not None for key in _TRACERS)
+
+
+def require_eager(name: str, *tensors: torch.Tensor | None) -> None:
+    """Refuses a call whose results would be missing what the kernels, which take pointers, do not
+    show: a trace would hold the outputs' memory alone, a transform or a tensor without memory of its own has
+    none, and a forward-mode tangent would be dropped. (Compiled code breaks its graph at
+    the library's call and runs it eagerly. Under 1 us: it is asked in every call.)"""
+    if torch.compiler.is_dynamo_compiling():
+        return
+    hidden = _C._is_tracing() or _C._are_functorch_transforms_active() or _dispatch_tracing()
+    for t in tensors:
+        if type(t) not in _PLAIN_TYPES and isinstance(t, torch.Tensor):
+            hidden = hidden or type(t).__torch_dispatch__ is not _C._disabled_torch_dispatch_impl
+    if hidden:
+        raise RuntimeError(f"{name} runs in eager calls alone: it can be neither traced nor transformed")
+    if _forward_ad._current_level >= 0 and any(
+            isinstance(t, torch.Tensor) and _forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{name} has no forward-mode derivative")
 
 
 def _aligned(t: torch.Tensor | None) -> torch.Tensor | None:

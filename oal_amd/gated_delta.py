@@ -23,6 +23,9 @@ float32, bfloat16 or float16: states, decays and their gradients are exact to fl
 A token with beta = 0 and g = 0 leaves the state as it is: pad batches of ragged lengths
 with such tokens. Values have to be
 finite: a token that is not spoils the 64 tokens of its chunk.
+
+Calls are eager: tracers, functorch's transforms and forward-mode derivatives are refused
+(compiled code runs the call between its graphs).
 """
 
 from __future__ import annotations
@@ -128,6 +131,7 @@ class _GatedDeltaFunction(torch.autograd.Function):
     def backward(ctx: Any, dout, dfinal):
         if torch.is_grad_enabled():
             raise RuntimeError("gated_delta_attention does not support double backward")
+        _native.require_eager("gated_delta_attention", dout, dfinal)
         q, k, v, g, beta, saved = ctx.saved_tensors
         dout, dfinal = (_native._aligned(t.contiguous()) for t in (dout, dfinal))
         grads = _native.delta_backward(q, k, v, g, beta, saved, dout, dfinal, scale=ctx.scale,
@@ -154,6 +158,7 @@ def gated_delta_attention(
     _validate(q, k, v, g, beta, initial_state, "initial_state")
     d, dv = q.shape[3], v.shape[3]
     scale = _validate_scale(scale, d)
+    _native.require_eager("gated_delta_attention", q, k, v, g, beta, initial_state)
     _native._require_device(q)
     if d % 8 == 0 and dv % 8 == 0:
         return _GatedDeltaFunction.apply(q, k, v, g, beta, initial_state, scale)
@@ -182,6 +187,7 @@ def gated_delta_step(
     if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, g, beta, state)):
         raise RuntimeError("gated_delta_step is not differentiable: call it under torch.no_grad()")
     scale = _validate_scale(scale, q.shape[3])
+    _native.require_eager("gated_delta_step", q, k, v, g, beta, state)
     _native._require_device(q)
     q, k, v = (t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous() for t in (q, k, v))
     out = _native.delta_step(q, k, v, g, beta, state, scale=scale)

@@ -21,6 +21,9 @@ tensors run in three and two exact bfloat16 parts per value, so that results are
 their type.
 Padding at the end of a sequence changes nothing before it; its values have to be finite
 all the same, in k, v and the gradients (a masked weight of zero times infinity is not zero).
+
+Calls of :func:`window_attention` and :func:`window_attention_step` are eager: tracers, functorch's
+transforms and forward-mode derivatives are refused (compiled code runs the call between its graphs).
 """
 
 from __future__ import annotations
@@ -93,6 +96,7 @@ class _WindowFunction(torch.autograd.Function):
             raise RuntimeError("window_attention does not support double backward")
         if dout is None:
             return (None,) * 6
+        _native.require_eager("window_attention", dout)
         q, k, v, out, lse = ctx.saved_tensors
         dout = _native._aligned(dout.contiguous())
         grads = _native.window_backward(q, k, v, out, lse, dout, **ctx.options)
@@ -114,6 +118,7 @@ def window_attention(
         raise ValueError("there must be a key for every query")
     d, dv = q.shape[3], v.shape[3]
     scale = _validate_scale(scale, d)
+    _native.require_eager("window_attention", q, k, v)
     _native._require_device(q)
     if d % 8 == 0 and dv % 8 == 0:
         return _WindowFunction.apply(q, k, v, window, sinks, scale)
@@ -164,6 +169,7 @@ def window_attention_step(
     """
     _validate(q, k, v)
     _validate_window(window, sinks)
+    _native.require_eager("window_attention_step", q, k, v, k_cache, v_cache)  # before addresses are looked at
     (b, hk, _, d), dv = k.shape, v.shape[3]
     if q.shape[2] != 1 or k.shape[2] != 1:
         raise ValueError("a step takes one token of each sequence")
