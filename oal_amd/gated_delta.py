@@ -153,7 +153,7 @@ def gated_delta_attention(
     q [B, Hq, N, D], k [B, Hk, N, D], v [B, Hv, N, DV] of one dtype, D and DV up to 64;
     g [B, Hv, N] float32; beta [B, Hv, N] float32 or q's dtype; initial_state
     [B, Hv, D, DV] float32 (None: zero). scale defaults to D^-1/2. Returns out
-    [B, max(Hq, Hv), N, DV] in q's dtype and the state after the last token.
+    [B, max(Hq, Hv), N, DV] in q's dtype and the state after the last token, contiguous.
     """
     _validate(q, k, v, g, beta, initial_state, "initial_state")
     d, dv = q.shape[3], v.shape[3]
@@ -166,7 +166,7 @@ def gated_delta_attention(
     if state is not None:
         state = torch.nn.functional.pad(state, (0, -dv % 8, 0, -d % 8))
     out, final = _GatedDeltaFunction.apply(_pad8(q), _pad8(k), _pad8(v), g, beta, state, scale)
-    return out[..., :dv], final[..., :d, :dv]
+    return out[..., :dv], final[..., :d, :dv].contiguous()  # as gated_delta_step takes it
 
 
 def gated_delta_step(
