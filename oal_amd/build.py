@@ -25,8 +25,9 @@ SOURCES = [os.path.join(PKG, "csrc", "oal_kernels.hip"), os.path.join(PKG, "csrc
 # Sources whose matrix-core accumulators the compiler would otherwise place in
 # the accumulation registers (AGPRs): there every VALU use of a group sum needs
 # a v_accvgpr_read copy first (256 of them per tile in the intra-chunk forward).
-# In VGPRs the VALU reads them directly; each kernel in these files stays
-# within 256 VGPRs without spilling.
+# In VGPRs the VALU reads them directly. The kernels of these files fit in 256 registers; some that are
+# bound to fewer for the sake of more waves spill a few (2 to 16; k_window_dkv in bf16 7), and
+# k_delta_bwd_out in fp32 keeps 10 values in AGPRs beside its 256.
 VGPR_FORM = {"oal_mfma_fwd.hip", "oal_mfma_local.hip", "oal_direct.hip", "oal_delta.hip", "oal_window.hip"}
 HEADERS = [os.path.join(PKG, "csrc", "oal_common.hpp"), os.path.join(ROOT, "include", "oal_amd.h")]
 OUTPUT = os.path.join(PKG, "liboal_amd.so")

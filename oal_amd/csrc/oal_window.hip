@@ -162,9 +162,10 @@ __device__ __forceinline__ Block query_block(const WindowArgs& a, const Shape& s
 
 }  // namespace
 
-// Bound by the exponentials: of the 6 issue slots per pair (a multiply-add, half a
-// maximum, an exponential of 4, half a conversion) they take 4, the two products 2.7 on
-// the matrix cores beside. The sums of the weights are a third product, with ones, of
+// A half tile (32 queries by 32 keys) takes a SIMD 930 cycles (740 in a long sequence): vector
+// instructions issue for 573 (504), 16 exponentials of 8 among them, and 18 matrix instructions run
+// for 288. Neither unit is full (62 to 68 % and 31 to 39 % busy), and waves wait 37 to 39 % of
+// their time: a tile is loaded, waited for and then used. The sums of the weights are a third product, with ones, of
 // the weights as the values meet them. A row's maximum is moved only when a score
 // exceeds it by 2^8, which float32 sums do not mind: else nothing is rescaled.
 // Four waves per SIMD (128 registers). 106 us, 498 TFLOP/s of the two products; one
@@ -286,8 +287,8 @@ void k_window_fwd(WindowArgs a, Shape sh, int qblocks, T* __restrict__ out, floa
   }
 }
 
-// dq, and for the other side delta_i = do_i.o_i: the forward's walk again. Bound by the
-// matrix cores (36 % busy) and the exponentials together. 155 us, 509 TFLOP/s (135 us with ds in one part).
+// dq, and for the other side delta_i = do_i.o_i: the forward's walk again. Matrix cores 36 %
+// busy, vector units 58 %, waves waiting 38 %, as in the forward. 155 us, 509 TFLOP/s (135 us with ds in one part).
 template <typename T>
 __global__ __launch_bounds__(256, kPartsOf<T> == 1 ? 3 : 1)
 void k_window_dq(WindowArgs a, Shape sh, int qblocks, const T* __restrict__ out, const float* __restrict__ lse,
@@ -398,8 +399,9 @@ void k_window_dq(WindowArgs a, Shape sh, int qblocks, const T* __restrict__ out,
 // 0 .. near - 1: through the window; the others: first keys seen from afar. A block's keys
 // stay in registers while the queries of all its heads pass, so heads that share keys are
 // summed there; parts of them where that leaves CUs empty, summed by k_window_sum in
-// order. 185 us, 570 TFLOP/s of the four products (154 us with ds in one part; two
-// waves per SIMD, which holds all in registers, 198).
+// order. 185 us, 570 TFLOP/s of the four products (154 us with ds in one part). Three waves per
+// SIMD cost bf16 7 spilled registers, loaded again in the loop over steps; two, which hold all, take
+// 198 us. Matrix cores 37 % busy, vector units 52 %, waves waiting 43 %.
 template <typename T>
 __global__ __launch_bounds__(256, kPartsOf<T> == 1 ? 3 : 1)
 void k_window_dkv(WindowArgs a, WindowPlan plan, int kblocks, int near, const float* __restrict__ lse,
@@ -555,7 +557,8 @@ __global__ __launch_bounds__(256) void k_window_sum(WindowArgs a, WindowPlan pla
 // are just what it sees, in any order. A wave takes 32 slots at a time; its 16
 // columns are query heads of one KV head. The slot's row comes from the token itself.
 // Bound by the caches' one reading: 128 users of 4100 slots, 2 KV heads, 40 us and the join 4,
-// 269 MB at 6.1 TB/s; one user of 1028 slots 5 us and the join 3.
+// 269 MB at 6.1 TB/s; one user of 1028 slots 5 us and the join 4. float16 takes twice as long (93 us): its
+// values are split, with two waves per SIMD.
 // ---------------------------------------------------------------------------
 namespace {
 

@@ -48,7 +48,8 @@ struct WindowStepArgs {
   void* out;    // [B][Hq][DV]
   float* part;  // [splits][B][Hq][DV + 2] (splits > 1)
 };
-// Keys per block and blocks per head group, from the cache's size alone.
+// Slots per block and blocks per head group: from the cache's size and how many head groups fill the chip, so
+// the same sequence may be summed in other pieces in another batch.
 void window_step_plan(int B, int Hq, int Hk, int64_t slots, int* splits, int* span);
 // kind: 0 float32, 1 bfloat16, 2 float16
 void launch_window_step(int kind, const WindowStepArgs& a, hipStream_t st, const Timer& timed);

@@ -22,7 +22,9 @@ and beta up to 2. Sums over tokens do not depend on the type of q, k and v, whic
 float32, bfloat16 or float16: states, decays and their gradients are exact to float32.
 A token with beta = 0 and g = 0 leaves the state as it is: pad batches of ragged lengths
 with such tokens. Values have to be
-finite: a token that is not spoils the 64 tokens of its chunk.
+finite: a token that is not spoils the 64 tokens of its chunk. Results repeat bit by bit from call to call;
+long sequences are cut by a rule on batch and heads, so that a sequence's last bits depend on how many others
+are in its batch.
 
 Calls are eager: tracers, functorch's transforms and forward-mode derivatives are refused
 (compiled code runs the call between its graphs).

@@ -22,6 +22,9 @@ their type.
 Padding at the end of a sequence changes nothing before it; its values have to be finite
 all the same, in k, v and the gradients (a masked weight of zero times infinity is not zero).
 
+Results repeat bit by bit from call to call. Long caches and the keys' gradients are summed in pieces
+whose number follows batch and heads, so that a sequence's last bits depend on how many others are in its batch.
+
 Calls of :func:`window_attention` and :func:`window_attention_step` are eager: tracers, functorch's
 transforms and forward-mode derivatives are refused (compiled code runs the call between its graphs).
 """
