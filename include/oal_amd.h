@@ -347,6 +347,77 @@ int oal_window_attention_step(const void* q, const void* k, const void* v, void*
                               int key_dim, int value_dim, int window, int sinks, int dtype, float scale, void* out,
                               void* workspace, void* stream);
 
+/*
+ * Linear attention with decays, per state head (exp, sums and state in fp32 or more):
+ *   S_t = e^(g_t) S_(t-1) + k_t v_t^T,  o_t = scale S_t^T q_t
+ * Operands, head counts and layouts as the gated delta rule's. g f32: strides (the last three of the twelve
+ * of q, k, v, g: batch, head, token) of zero where a head has one decay for all its tokens; a g of
+ * -inf forgets the state. per_head (backward): dg is [Hv], the sums over batch and tokens, and else
+ * [B][Hv][N]. saved (oal_decay_saved_bytes) is the forward's room and what the backward reads.
+ */
+size_t oal_decay_saved_bytes(int batch, int v_heads, int seq_len);
+int oal_decay_forward(const void* q, const void* k, const void* v, const float* g, const int64_t* strides, int batch,
+                      int q_heads, int k_heads, int v_heads, int seq_len, int key_dim, int value_dim, int dtype,
+                      float scale, const float* state, void* out, float* final_state, void* saved, void* stream);
+size_t oal_decay_workspace_bytes(int batch, int q_heads, int k_heads, int v_heads, int seq_len, int key_dim,
+                                 int per_head);
+int oal_decay_backward(const void* q, const void* k, const void* v, const float* g, const int64_t* strides,
+                       int per_head, int batch, int q_heads, int k_heads, int v_heads, int seq_len, int key_dim,
+                       int value_dim, int dtype, float scale, const void* saved, const void* dout,
+                       const float* dfinal, void* dq, void* dk, void* dv, float* dg, float* dstate, void* workspace,
+                       void* stream);
+
+/* The recurrence for a few tokens, as oal_gated_delta_step. */
+int oal_decay_step(const void* q, const void* k, const void* v, const float* g, const int64_t* strides, int batch,
+                   int q_heads, int k_heads, int v_heads, int seq_len, int key_dim, int value_dim, int dtype,
+                   float scale, float* state, void* out, void* stream);
+
+/*
+ * Projections q, k, v [B][N][heads][head_dim] (rows contiguous; strides: batch and token of q, k, v, in
+ * elements) to head-first [B][heads][N][head_dim]: q and k divided by the root of their mean square over a head
+ * (eps added to it), times q_weight, k_weight ([head_dim], or [heads][head_dim] with per_head; NULL: 1), and their
+ * first `rotary` dimensions turned by the rotate-half embedding of row position[b][n] of cosine, sine
+ * [table][rotary] (position NULL: n). A negative position means no token: zeros. One past the tables
+ * gives NaN. Weights are of dtype or (weight_f32) f32, tables of dtype or (table_f32) f32.
+ */
+int oal_norm_rotary_heads(const void* q, const void* k, const void* v, const int64_t* strides, const void* q_weight,
+                          const void* k_weight, int weight_f32, int per_head, const void* cosine, const void* sine,
+                          int table_f32, int table, int rotary, const int64_t* position, int batch, int q_heads,
+                          int kv_heads, int seq_len, int head_dim, int dtype, float eps, void* head_q, void* head_k,
+                          void* head_v, void* stream);
+
+/*
+ * Its VJP: gradients of head_q, head_k, head_v (contiguous; NULL: zero) -> contiguous dq, dk, dv
+ * [B][N][heads][head_dim] (NULL: not wanted) and, with a workspace, dq_weight and dk_weight (each may be NULL) in the weights' type.
+ * A weight's gradient needs dq or dk.
+ */
+size_t oal_norm_rotary_heads_workspace_bytes(int batch, int q_heads, int kv_heads, int seq_len, int head_dim,
+                                             int per_head);
+int oal_norm_rotary_heads_backward(const void* q, const void* k, const int64_t* strides, const void* q_weight,
+                                   const void* k_weight, int weight_f32, int per_head, const void* cosine,
+                                   const void* sine, int table_f32, int table, int rotary, const int64_t* position,
+                                   int batch, int q_heads, int kv_heads, int seq_len, int head_dim, int dtype,
+                                   float eps, const void* head_dq, const void* head_dk, const void* head_dv, void* dq,
+                                   void* dk, void* dv, void* dq_weight, void* dk_weight, void* workspace,
+                                   void* stream);
+
+/*
+ * Of logits [B][N][vocab] (dtype; strides: batch and row, in elements; a row is contiguous) and tokens [B][N]
+ * int64: log_probs [B][N] f32, the tokens' log probabilities (0 for a negative token, NaN for one past
+ * vocab); entropy [B][N] f32 (may be NULL) of each row's distribution; and for top in [1, 64], not more than vocab,
+ * top_log_probs [B][N][top] f32 and top_tokens [B][N][top] int64, the most likely tokens from the first, of
+ * equally likely ones the lowest before. saved [B][N][2] f32 (may be NULL) is what the backward reads.
+ */
+size_t oal_token_scores_workspace_bytes(int batch, int rows, int vocab, int top);
+int oal_token_scores(const void* logits, const int64_t* strides, const int64_t* tokens, int batch, int rows, int vocab,
+                     int dtype, int top, float* log_probs, float* entropy, float* top_log_probs, int64_t* top_tokens,
+                     float* saved, void* workspace, void* stream);
+
+/* Its VJP: dlog_probs and, with the forward's entropy, dentropy [B][N] f32 (each may be NULL) -> contiguous dlogits (dtype). */
+int oal_token_scores_backward(const void* logits, const int64_t* strides, const int64_t* tokens, int batch, int rows,
+                              int vocab, int dtype, const float* saved, const float* entropy, const float* dlog_probs,
+                              const float* dentropy, void* dlogits, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

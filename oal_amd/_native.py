@@ -88,6 +88,18 @@ _SIGNATURES = {
     "oal_window_attention_backward": ([_vp] * 4 + [_i] * 10 + [_f] + [_vp] * 8, _i),
     "oal_window_attention_step_workspace_bytes": ([_i] * 6, _sz),
     "oal_window_attention_step": ([_vp] * 7 + [_i] * 8 + [_f] + [_vp] * 3, _i),
+    "oal_decay_saved_bytes": ([_i] * 3, _sz),
+    "oal_decay_workspace_bytes": ([_i] * 7, _sz),
+    "oal_decay_forward": ([_vp] * 5 + [_i] * 8 + [_f] + [_vp] * 5, _i),
+    "oal_decay_backward": ([_vp] * 5 + [_i] * 9 + [_f] + [_vp] * 10, _i),
+    "oal_decay_step": ([_vp] * 5 + [_i] * 8 + [_f] + [_vp] * 3, _i),
+    "oal_norm_rotary_heads": ([_vp] * 6 + [_i] * 2 + [_vp] * 2 + [_i] * 3 + [_vp] + [_i] * 6 + [_f] + [_vp] * 4, _i),
+    "oal_norm_rotary_heads_workspace_bytes": ([_i] * 6, _sz),
+    "oal_norm_rotary_heads_backward": (
+        [_vp] * 5 + [_i] * 2 + [_vp] * 2 + [_i] * 3 + [_vp] + [_i] * 6 + [_f] + [_vp] * 10, _i),
+    "oal_token_scores_workspace_bytes": ([_i] * 4, _sz),
+    "oal_token_scores": ([_vp] * 3 + [_i] * 5 + [_vp] * 7, _i),
+    "oal_token_scores_backward": ([_vp] * 3 + [_i] * 4 + [_vp] * 6, _i),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
@@ -743,7 +755,8 @@ class Verdict:
 # are contiguous and 16-byte aligned, at any strides.
 # ---------------------------------------------------------------------------
 _DTYPES = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float16: 2}
-_Strides3, _Strides5 = ctypes.c_int64 * 9, ctypes.c_int64 * 15
+_Strides2, _Strides6 = ctypes.c_int64 * 2, ctypes.c_int64 * 6
+_Strides3, _Strides4, _Strides5 = ctypes.c_int64 * 9, ctypes.c_int64 * 12, ctypes.c_int64 * 15
 
 
 def row_tensor(t: torch.Tensor) -> torch.Tensor:
@@ -874,3 +887,158 @@ def window_step(q, k, v, k_cache, v_cache, positions, *, window: int, sinks: int
             work.data_ptr(), _stream(dev))
         _check(rc, lib, "oal_window_attention_step")
     return out
+
+
+# ---------------------------------------------------------------------------
+# Linear attention with decays (oal_decay.hip), head norms with rotary embedding
+# (oal_heads.hip) and token scores (oal_scores.hip). The callers (decay_attention.py,
+# norm_rotary.py, token_scores.py) have checked types, shapes and devices.
+# ---------------------------------------------------------------------------
+def _gate_strides(g: torch.Tensor) -> tuple[int, int, int]:
+    return (0, g.stride(0), 0) if g.ndim == 1 else g.stride()
+
+
+def decay_forward(q, k, v, g, state, *, scale: float):
+    """q, k [B, heads, N, D], v [B, Hv, N, DV], D and DV multiples of 8, rows as of :func:`row_tensor`; g float32 [Hv] or
+    [B, Hv, N], state contiguous float32 [B, Hv, D, DV] or None. Returns (out, final_state, saved)."""
+    lib = load_library()
+    b, hq, n, d = q.shape
+    hk, hv, dv, dev = k.shape[1], v.shape[1], v.shape[3], q.device
+    with _scope(dev, "oal_amd::decay_forward"):
+        nbytes = lib.oal_decay_saved_bytes(b, hv, n)
+        if nbytes == 0:
+            _check(1, lib, "oal_decay_saved_bytes")
+        out = q.new_empty((b, max(hq, hv), n, dv))
+        final = g.new_empty((b, hv, d, dv))
+        saved = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+        rc = lib.oal_decay_forward(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(),
+            _Strides4(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *_gate_strides(g)), b, hq, hk, hv, n, d, dv,
+            _DTYPES[q.dtype], scale, _ptr(state), out.data_ptr(), final.data_ptr(), saved.data_ptr(), _stream(dev))
+        _check(rc, lib, "oal_decay_forward")
+    return out, final, saved
+
+
+def decay_backward(q, k, v, g, saved, dout, dfinal, *, scale: float, need_state: bool):
+    """The VJP of :func:`decay_forward`: (dq, dk, dv, dg, dstate or None)."""
+    lib = load_library()
+    b, hq, n, d = q.shape
+    hk, hv, dv, dev = k.shape[1], v.shape[1], v.shape[3], q.device
+    with _scope(dev, "oal_amd::decay_backward"):
+        nbytes = lib.oal_decay_workspace_bytes(b, hq, hk, hv, n, d, g.ndim == 1)
+        if nbytes == 0:
+            _check(1, lib, "oal_decay_workspace_bytes")
+        work = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+        grads = [t.new_empty(t.shape) for t in (q, k, v, g)]
+        dstate = g.new_empty((b, hv, d, dv)) if need_state else None
+        rc = lib.oal_decay_backward(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(),
+            _Strides4(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *_gate_strides(g)), g.ndim == 1, b, hq, hk, hv, n,
+            d, dv, _DTYPES[q.dtype], scale, saved.data_ptr(), dout.data_ptr(), _ptr(dfinal),
+            *[t.data_ptr() for t in grads], _ptr(dstate), work.data_ptr(), _stream(dev))
+        _check(rc, lib, "oal_decay_backward")
+    return (*grads, dstate)
+
+
+def decay_step(q, k, v, g, state, *, scale: float) -> torch.Tensor:
+    """The recurrence over the N tokens of q, k, v [B, heads, N, D] (unit stride in a row, any
+    alignment); state [B, Hv, D, DV] contiguous float32 is updated in place."""
+    lib = load_library()
+    b, hq, n, d = q.shape
+    hk, hv, dv, dev = k.shape[1], v.shape[1], v.shape[3], q.device
+    with _scope(dev, "oal_amd::decay_step"):
+        out = q.new_empty((b, max(hq, hv), n, dv))
+        rc = lib.oal_decay_step(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(),
+            _Strides4(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *_gate_strides(g)), b, hq, hk, hv, n, d, dv,
+            _DTYPES[q.dtype], scale, state.data_ptr(), out.data_ptr(), _stream(dev))
+        _check(rc, lib, "oal_decay_step")
+    return out
+
+
+def norm_rotary_forward(q, k, v, q_weight, k_weight, cos, sin, positions, *, q_heads: int, kv_heads: int, eps: float):
+    """q, k, v [B, N, heads * D] of unit stride in a row; weights contiguous [D] or [heads, D] or None; cos and sin
+    contiguous [T, R]; positions contiguous int64 [B, N] or None. Returns head-first (q, k, v)."""
+    lib = load_library()
+    b, n, width = q.shape
+    d, dev = width // q_heads, q.device
+    weight = q_weight if q_weight is not None else k_weight
+    with _scope(dev, "oal_amd::norm_rotary_heads"):
+        outs = [q.new_empty((b, heads, n, d)) for heads in (q_heads, kv_heads, kv_heads)]
+        rc = lib.oal_norm_rotary_heads(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), _Strides6(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2]),
+            _ptr(q_weight), _ptr(k_weight), weight is None or weight.dtype is torch.float32,
+            weight is not None and weight.ndim == 2, cos.data_ptr(), sin.data_ptr(), cos.dtype is torch.float32,
+            cos.shape[0], cos.shape[1], _ptr(positions), b, q_heads, kv_heads, n, d, _DTYPES[q.dtype], eps,
+            *[t.data_ptr() for t in outs], _stream(dev))
+        _check(rc, lib, "oal_norm_rotary_heads")
+    return tuple(outs)
+
+
+def norm_rotary_backward(q, k, q_weight, k_weight, cos, sin, positions, ups, needs, *, q_heads: int, kv_heads: int,
+                         eps: float):
+    """The VJP of :func:`norm_rotary_forward`: gradients of (q, k, v, q_weight, k_weight), None where not needed. ups:
+    contiguous aligned gradients of its results, or None."""
+    lib = load_library()
+    b, n, width = q.shape
+    d, dev = width // q_heads, q.device
+    weight = q_weight if q_weight is not None else k_weight
+    per_head = weight is not None and weight.ndim == 2
+    with _scope(dev, "oal_amd::norm_rotary_heads_backward"):
+        dq = q.new_empty(q.shape) if needs[0] or needs[3] else None
+        dk = k.new_empty(k.shape) if needs[1] or needs[4] else None
+        dv = k.new_empty(k.shape) if needs[2] else None
+        dws = [w.new_empty(w.shape) if need else None for w, need in zip((q_weight, k_weight), needs[3:])]
+        work = None
+        if needs[3] or needs[4]:
+            nbytes = lib.oal_norm_rotary_heads_workspace_bytes(b, q_heads, kv_heads, n, d, per_head)
+            if nbytes == 0:
+                _check(1, lib, "oal_norm_rotary_heads_workspace_bytes")
+            work = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+        rc = lib.oal_norm_rotary_heads_backward(
+            q.data_ptr(), k.data_ptr(), (ctypes.c_int64 * 4)(*q.stride()[:2], *k.stride()[:2]), _ptr(q_weight),
+            _ptr(k_weight), weight is None or weight.dtype is torch.float32, per_head, cos.data_ptr(), sin.data_ptr(),
+            cos.dtype is torch.float32, cos.shape[0], cos.shape[1], _ptr(positions), b, q_heads, kv_heads, n, d,
+            _DTYPES[q.dtype], eps, *map(_ptr, ups), _ptr(dq), _ptr(dk), _ptr(dv), *map(_ptr, dws), _ptr(work),
+            _stream(dev))
+        _check(rc, lib, "oal_norm_rotary_heads_backward")
+    return dq, dk, dv, *dws
+
+
+def token_scores(logits, tokens, *, entropy: bool, top: int, keep: bool):
+    """logits [B, N, V] of unit stride in a row, tokens contiguous int64 [B, N]. Returns (log_probs, entropy or None,
+    top_log_probs or None, top_tokens or None, saved or None)."""
+    lib = load_library()
+    b, n, vocab = logits.shape
+    dev = logits.device
+    with _scope(dev, "oal_amd::token_scores"):
+        nbytes = lib.oal_token_scores_workspace_bytes(b, n, vocab, top)
+        if nbytes == 0:
+            _check(1, lib, "oal_token_scores_workspace_bytes")
+
+        def room(*shape, dtype=torch.float32):
+            return torch.empty(shape, dtype=dtype, device=dev)
+
+        work = room(nbytes, dtype=torch.uint8)
+        log_probs, entropies = room(b, n), room(b, n) if entropy else None
+        values, places = (room(b, n, top), room(b, n, top, dtype=torch.int64)) if top else (None, None)
+        saved = room(b, n, 2) if keep else None
+        rc = lib.oal_token_scores(
+            logits.data_ptr(), _Strides2(*logits.stride()[:2]), tokens.data_ptr(), b, n, vocab, _DTYPES[logits.dtype], top,
+            log_probs.data_ptr(), _ptr(entropies), _ptr(values), _ptr(places), _ptr(saved), work.data_ptr(), _stream(dev))
+        _check(rc, lib, "oal_token_scores")
+    return log_probs, entropies, values, places, saved
+
+
+def token_scores_backward(logits, tokens, saved, entropies, dlog, dentropy) -> torch.Tensor:
+    """The VJP of :func:`token_scores`: dlogits; dlog and dentropy contiguous float32 [B, N] or None."""
+    lib = load_library()
+    b, n, vocab = logits.shape
+    dev = logits.device
+    with _scope(dev, "oal_amd::token_scores_backward"):
+        grad = logits.new_empty((b, n, vocab))
+        rc = lib.oal_token_scores_backward(
+            logits.data_ptr(), _Strides2(*logits.stride()[:2]), tokens.data_ptr(), b, n, vocab, _DTYPES[logits.dtype],
+            saved.data_ptr(), _ptr(entropies), _ptr(dlog), _ptr(dentropy), grad.data_ptr(), _stream(dev))
+        _check(rc, lib, "oal_token_scores_backward")
+    return grad

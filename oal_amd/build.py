@@ -21,14 +21,15 @@ SOURCES = [os.path.join(PKG, "csrc", "oal_kernels.hip"), os.path.join(PKG, "csrc
            os.path.join(PKG, "csrc", "oal_mfma_pair.hip"), os.path.join(PKG, "csrc", "oal_f32_mma.hip"),
            os.path.join(PKG, "csrc", "oal_f64.hip"), os.path.join(PKG, "csrc", "oal_direct.hip"),
            os.path.join(PKG, "csrc", "oal_adapter.hip"), os.path.join(PKG, "csrc", "oal_delta.hip"),
-           os.path.join(PKG, "csrc", "oal_window.hip")]
+           os.path.join(PKG, "csrc", "oal_window.hip"), os.path.join(PKG, "csrc", "oal_decay.hip"),
+           os.path.join(PKG, "csrc", "oal_heads.hip"), os.path.join(PKG, "csrc", "oal_scores.hip")]
 # Sources whose matrix-core accumulators the compiler would otherwise place in
 # the accumulation registers (AGPRs): there every VALU use of a group sum needs
 # a v_accvgpr_read copy first (256 of them per tile in the intra-chunk forward).
 # In VGPRs the VALU reads them directly. The kernels of these files fit in 256 registers; some that are
 # bound to fewer for the sake of more waves spill a few (2 to 16; k_window_dkv in bf16 7), and
 # k_delta_bwd_out in fp32 keeps 10 values in AGPRs beside its 256.
-VGPR_FORM = {"oal_mfma_fwd.hip", "oal_mfma_local.hip", "oal_direct.hip", "oal_delta.hip", "oal_window.hip"}
+VGPR_FORM = {"oal_mfma_fwd.hip", "oal_mfma_local.hip", "oal_direct.hip", "oal_delta.hip", "oal_window.hip", "oal_decay.hip"}
 HEADERS = [os.path.join(PKG, "csrc", "oal_common.hpp"), os.path.join(ROOT, "include", "oal_amd.h")]
 OUTPUT = os.path.join(PKG, "liboal_amd.so")
 OBJDIR = os.path.join(PKG, "_build")

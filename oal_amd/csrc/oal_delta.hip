@@ -1126,6 +1126,16 @@ DeltaWork delta_work_view(void* base, const DeltaArgs& a) {
 }
 
 template <typename T>
+void launch_sum_heads(const float* src, T* dst, int B, int heads, int each, int64_t head, hipStream_t st,
+                      const Timer& timed) {
+  const int64_t total = (int64_t)B * heads * head;
+  timed("k_delta_sum_heads", st, [&] {
+    hipLaunchKernelGGL(k_delta_sum_heads<T>, dim3((unsigned)((total / 4 + kThr - 1) / kThr)), dim3(kThr), 0, st, src, dst,
+                       each, head, total);
+  });
+}
+
+template <typename T>
 void launch_delta_forward(const DeltaArgs& a, const float* state, void* out, float* final_state, void* saved, bool keep,
                           hipStream_t st, const Timer& timed) {
   const int U = a.B * a.Hv, rep = a.H / a.Hv;
@@ -1162,18 +1172,12 @@ void launch_delta_backward(const DeltaArgs& a, const void* saved, const void* do
     hipLaunchKernelGGL(k_delta_bwd_out<T>, dim3(a.NC * U), dim3(kThr), 0, st, a, od, s.G, s.T, s.S, s.Z, w.E, w.dS,
                        static_cast<T*>(dq), w.dqh, static_cast<T*>(dk), w.dkh, static_cast<T*>(dv), dg, dbeta);
   });
-  auto sum = [&](const float* src, void* dst, int heads, int each) {
-    const int64_t head = (int64_t)a.N * a.D, total = (int64_t)a.B * heads * head;
-    timed("k_delta_sum_heads", st, [&] {
-      hipLaunchKernelGGL(k_delta_sum_heads<T>, dim3((unsigned)((total / 4 + kThr - 1) / kThr)), dim3(kThr), 0, st, src,
-                         static_cast<T*>(dst), each, head, total);
-    });
-  };
-  if (w.dqh) sum(w.dqh, dq, a.Hq, a.H / a.Hq);
-  if (w.dkh) sum(w.dkh, dk, a.Hk, a.Hv / a.Hk);
+  if (w.dqh) launch_sum_heads(w.dqh, static_cast<T*>(dq), a.B, a.Hq, a.H / a.Hq, (int64_t)a.N * a.D, st, timed);
+  if (w.dkh) launch_sum_heads(w.dkh, static_cast<T*>(dk), a.B, a.Hk, a.Hv / a.Hk, (int64_t)a.N * a.D, st, timed);
 }
 
 #define OAL_DELTA(T)                                                                                                 \
+  template void launch_sum_heads<T>(const float*, T*, int, int, int, int64_t, hipStream_t, const Timer&);            \
   template void launch_delta_forward<T>(const DeltaArgs&, const float*, void*, float*, void*, bool, hipStream_t,     \
                                         const Timer&);                                                              \
   template void launch_delta_backward<T>(const DeltaArgs&, const void*, const void*, const float*, void*, void*,     \

@@ -55,6 +55,11 @@ void launch_delta_backward(const DeltaArgs& a, const void* saved, const void* do
                            void* dk, void* dv, float* dg, void* dbeta, float* dstate, void* work, hipStream_t st,
                            const Timer& timed);
 
+// dst [B][heads][head values] of src [B][heads each][head values]: sums over heads that one serves, in order.
+template <typename T>
+void launch_sum_heads(const float* src, T* dst, int B, int heads, int each, int64_t head, hipStream_t st,
+                      const Timer& timed);
+
 struct DeltaStepArgs {
   Strided q, k, v, g, beta;
   int B, Hq, Hk, Hv, H, N, Dk, Dv;

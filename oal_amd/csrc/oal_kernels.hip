@@ -30,9 +30,12 @@
 
 #include "oal_amd.h"
 #include "oal_common.hpp"
+#include "oal_decay.hpp"
 #include "oal_delta.hpp"
 #include "oal_direct.hpp"
+#include "oal_heads.hpp"
 #include "oal_internal.hpp"
+#include "oal_scores.hpp"
 #include "oal_window.hpp"
 
 namespace oal {
@@ -1720,6 +1723,245 @@ int oal_window_attention_step(const void* q, const void* k, const void* v, void*
   oal::window_step_plan(batch, q_heads, kv_heads, slots, &a.splits, &a.span);
   oal::launch_window_step(dtype, a, static_cast<hipStream_t>(stream), make_timer());
   return launch_status("oal_window_attention_step launch");
+}
+
+// ---------------------------------------------------------------------------
+// Linear attention with decays
+// ---------------------------------------------------------------------------
+static int decay_args(oal::DecayArgs* a, const char* what, const void* q, const void* k, const void* v, const float* g,
+                      const int64_t* strides, int per_head, int batch, int q_heads, int k_heads, int v_heads,
+                      int seq_len, int key_dim, int value_dim, int dtype, float scale) {
+  if (check_delta(batch, q_heads, k_heads, v_heads, seq_len)) return 1;
+  if (!dim_ok(key_dim) || !dim_ok(value_dim))
+    return fail(std::string(what) + ": dimensions must be multiples of 8 up to 64");
+  if (dtype < OAL_DTYPE_F32 || dtype > OAL_DTYPE_F16)
+    return fail("dtype must be OAL_DTYPE_F32, OAL_DTYPE_BF16 or OAL_DTYPE_F16");
+  if (!q || !k || !v || !g || !strides) return fail(std::string(what) + ": null pointer argument");
+  *a = {strided(q, strides), strided(k, strides + 3), strided(v, strides + 6), strided(g, strides + 9), batch, q_heads,
+        k_heads, v_heads, q_heads > v_heads ? q_heads : v_heads, seq_len, (seq_len + 63) / 64, key_dim, value_dim,
+        per_head != 0, scale};
+  if (!rows_aligned(a->q, dtype, batch, q_heads, seq_len) || !rows_aligned(a->k, dtype, batch, k_heads, seq_len) ||
+      !rows_aligned(a->v, dtype, batch, v_heads, seq_len))
+    return fail(std::string(what) + ": rows must be 16-byte aligned");
+  return 0;
+}
+
+size_t oal_decay_saved_bytes(int batch, int v_heads, int seq_len) {
+  if (check_delta(batch, v_heads, v_heads, v_heads, seq_len)) return 0;
+  return oal::decay_saved_view(nullptr, batch * v_heads, (seq_len + 63) / 64).bytes;
+}
+
+size_t oal_decay_workspace_bytes(int batch, int q_heads, int k_heads, int v_heads, int seq_len, int key_dim,
+                                 int per_head) {
+  if (check_delta(batch, q_heads, k_heads, v_heads, seq_len)) return 0;
+  if (!dim_ok(key_dim)) {
+    fail("oal_decay_workspace_bytes: dimensions must be multiples of 8 up to 64");
+    return 0;
+  }
+  oal::DecayArgs a{};
+  a.B = batch, a.Hq = q_heads, a.Hk = k_heads, a.Hv = v_heads, a.N = seq_len, a.D = key_dim;
+  a.H = q_heads > v_heads ? q_heads : v_heads, a.NC = (seq_len + 63) / 64, a.per_head = per_head != 0;
+  return oal::decay_work_view(nullptr, a).bytes;
+}
+
+int oal_decay_forward(const void* q, const void* k, const void* v, const float* g, const int64_t* strides, int batch,
+                      int q_heads, int k_heads, int v_heads, int seq_len, int key_dim, int value_dim, int dtype,
+                      float scale, const float* state, void* out, float* final_state, void* saved, void* stream) {
+  Range range("oal_decay_forward");
+  oal::DecayArgs a;
+  if (decay_args(&a, "oal_decay_forward", q, k, v, g, strides, 0, batch, q_heads, k_heads, v_heads, seq_len, key_dim,
+                 value_dim, dtype, scale))
+    return 1;
+  if (!out || !final_state || !saved) return fail("oal_decay_forward: null pointer argument");
+  const void* ptrs[] = {state, out, final_state, saved};
+  for (const void* p : ptrs)
+    if (!aligned16(p)) return fail("oal_decay_forward: tensor pointers must be 16-byte aligned");
+  const auto launch = dtype == OAL_DTYPE_F32    ? oal::launch_decay_forward<float>
+                      : dtype == OAL_DTYPE_BF16 ? oal::launch_decay_forward<uint16_t>
+                                                : oal::launch_decay_forward<_Float16>;
+  launch(a, state, out, final_state, saved, static_cast<hipStream_t>(stream), make_timer());
+  return launch_status("oal_decay_forward launch");
+}
+
+int oal_decay_backward(const void* q, const void* k, const void* v, const float* g, const int64_t* strides,
+                       int per_head, int batch, int q_heads, int k_heads, int v_heads, int seq_len, int key_dim,
+                       int value_dim, int dtype, float scale, const void* saved, const void* dout,
+                       const float* dfinal, void* dq, void* dk, void* dv, float* dg, float* dstate, void* workspace,
+                       void* stream) {
+  Range range("oal_decay_backward");
+  oal::DecayArgs a;
+  if (decay_args(&a, "oal_decay_backward", q, k, v, g, strides, per_head, batch, q_heads, k_heads, v_heads, seq_len,
+                 key_dim, value_dim, dtype, scale))
+    return 1;
+  if (!saved || !dout || !dq || !dk || !dv || !dg || !workspace)
+    return fail("oal_decay_backward: null pointer argument");
+  const void* ptrs[] = {saved, dout, dfinal, dq, dk, dv, dstate, workspace};
+  for (const void* p : ptrs)
+    if (!aligned16(p)) return fail("oal_decay_backward: tensor pointers must be 16-byte aligned");
+  const auto launch = dtype == OAL_DTYPE_F32    ? oal::launch_decay_backward<float>
+                      : dtype == OAL_DTYPE_BF16 ? oal::launch_decay_backward<uint16_t>
+                                                : oal::launch_decay_backward<_Float16>;
+  launch(a, saved, dout, dfinal, dq, dk, dv, dg, dstate, workspace, static_cast<hipStream_t>(stream), make_timer());
+  return launch_status("oal_decay_backward launch");
+}
+
+int oal_decay_step(const void* q, const void* k, const void* v, const float* g, const int64_t* strides, int batch,
+                   int q_heads, int k_heads, int v_heads, int seq_len, int key_dim, int value_dim, int dtype,
+                   float scale, float* state, void* out, void* stream) {
+  Range range("oal_decay_step");
+  if (check_delta(batch, q_heads, k_heads, v_heads, seq_len)) return 1;
+  if (key_dim < 1 || key_dim > 64 || value_dim < 1 || value_dim > 64)
+    return fail("oal_decay_step: dimensions must be in [1, 64]");
+  if (dtype < OAL_DTYPE_F32 || dtype > OAL_DTYPE_F16) return fail("oal_decay_step: unknown type");
+  if (!q || !k || !v || !g || !strides || !state || !out) return fail("oal_decay_step: null pointer argument");
+  const oal::DecayStepArgs a = {strided(q, strides), strided(k, strides + 3), strided(v, strides + 6),
+                                strided(g, strides + 9), batch, q_heads, k_heads, v_heads,
+                                q_heads > v_heads ? q_heads : v_heads, seq_len, key_dim, value_dim, scale, state, out};
+  oal::launch_decay_step(dtype, a, static_cast<hipStream_t>(stream), make_timer());
+  return launch_status("oal_decay_step launch");
+}
+
+// ---------------------------------------------------------------------------
+// Head norms with rotary embedding
+// ---------------------------------------------------------------------------
+static int heads_args(oal::HeadsArgs* a, const char* what, const void* q, const void* k, const void* v,
+                      const int64_t* strides, const void* q_weight, const void* k_weight, int weight_f32, int per_head,
+                      const void* cosine, const void* sine, int table_f32, int table, int rotary,
+                      const int64_t* position, int batch, int q_heads, int kv_heads, int seq_len, int head_dim,
+                      int dtype, float eps) {
+  if (batch <= 0 || q_heads <= 0 || kv_heads <= 0 || seq_len <= 0)
+    return fail("batch, head counts and sequence length must be positive");
+  if (dtype < OAL_DTYPE_F32 || dtype > OAL_DTYPE_F16)
+    return fail("dtype must be OAL_DTYPE_F32, OAL_DTYPE_BF16 or OAL_DTYPE_F16");
+  if (head_dim < 1 || head_dim > 64) return fail(std::string(what) + ": head_dim must be in [1, 64]");
+  if (rotary < 2 || rotary > head_dim || rotary % 2)
+    return fail(std::string(what) + ": the rotated dimensions must be an even number up to head_dim");
+  if (table < 1 || (!position && table < seq_len))
+    return fail(std::string(what) + ": the tables must have a row for every token");
+  if (int64_t(q_heads) + 2 * int64_t(kv_heads) > 65535 || int64_t(batch) > (int64_t(1) << 31) / seq_len)
+    return fail("batch, heads and sequence length are too large for one launch");
+  if (!q || !k || !v || !strides || !cosine || !sine) return fail(std::string(what) + ": null pointer argument");
+  *a = {q, k, v, strides[0], strides[1], strides[2], strides[3], strides[4], strides[5], q_weight, k_weight, cosine, sine,
+        position, batch, seq_len, q_heads, kv_heads, head_dim, rotary, table, weight_f32 != 0 || dtype == OAL_DTYPE_F32,
+        table_f32 != 0 || dtype == OAL_DTYPE_F32, per_head != 0, eps};
+  return 0;
+}
+
+int oal_norm_rotary_heads(const void* q, const void* k, const void* v, const int64_t* strides, const void* q_weight,
+                          const void* k_weight, int weight_f32, int per_head, const void* cosine, const void* sine,
+                          int table_f32, int table, int rotary, const int64_t* position, int batch, int q_heads,
+                          int kv_heads, int seq_len, int head_dim, int dtype, float eps, void* head_q, void* head_k,
+                          void* head_v, void* stream) {
+  Range range("oal_norm_rotary_heads");
+  oal::HeadsArgs a;
+  if (heads_args(&a, "oal_norm_rotary_heads", q, k, v, strides, q_weight, k_weight, weight_f32, per_head, cosine, sine,
+                 table_f32, table, rotary, position, batch, q_heads, kv_heads, seq_len, head_dim, dtype, eps))
+    return 1;
+  if (!head_q || !head_k || !head_v) return fail("oal_norm_rotary_heads: null pointer argument");
+  if (!aligned16(head_q) || !aligned16(head_k) || !aligned16(head_v))
+    return fail("oal_norm_rotary_heads: tensor pointers must be 16-byte aligned");
+  const auto launch = dtype == OAL_DTYPE_F32    ? oal::launch_heads_forward<float>
+                      : dtype == OAL_DTYPE_BF16 ? oal::launch_heads_forward<uint16_t>
+                                                : oal::launch_heads_forward<_Float16>;
+  launch(a, head_q, head_k, head_v, static_cast<hipStream_t>(stream), make_timer());
+  return launch_status("oal_norm_rotary_heads launch");
+}
+
+size_t oal_norm_rotary_heads_workspace_bytes(int batch, int q_heads, int kv_heads, int seq_len, int head_dim,
+                                             int per_head) {
+  oal::HeadsArgs a;
+  const int64_t none[6] = {};
+  if (heads_args(&a, "oal_norm_rotary_heads_workspace_bytes", none, none, none, none, nullptr, nullptr, 0, per_head, none,
+                 none, 0, 1, 2, none, batch, q_heads, kv_heads, seq_len, head_dim < 2 ? head_dim + 1 : head_dim, 0, 0.f))
+    return 0;
+  return (size_t)oal::heads_blocks(a) * (per_head ? q_heads + kv_heads : 2) * head_dim * sizeof(float);
+}
+
+int oal_norm_rotary_heads_backward(const void* q, const void* k, const int64_t* strides, const void* q_weight,
+                                   const void* k_weight, int weight_f32, int per_head, const void* cosine,
+                                   const void* sine, int table_f32, int table, int rotary, const int64_t* position,
+                                   int batch, int q_heads, int kv_heads, int seq_len, int head_dim, int dtype,
+                                   float eps, const void* head_dq, const void* head_dk, const void* head_dv, void* dq,
+                                   void* dk, void* dv, void* dq_weight, void* dk_weight, void* workspace,
+                                   void* stream) {
+  Range range("oal_norm_rotary_heads_backward");
+  oal::HeadsArgs a;
+  if (!strides) return fail("oal_norm_rotary_heads_backward: null pointer argument");
+  const int64_t all[6] = {strides[0], strides[1], strides[2], strides[3], 0, 0};
+  if (heads_args(&a, "oal_norm_rotary_heads_backward", q, k, q, all, q_weight, k_weight, weight_f32, per_head, cosine,
+                 sine, table_f32, table, rotary, position, batch, q_heads, kv_heads, seq_len, head_dim, dtype, eps))
+    return 1;
+  if ((dq_weight && !dq) || (dk_weight && !dk) || ((dq_weight || dk_weight) && !workspace))
+    return fail("oal_norm_rotary_heads_backward: a weight's gradient needs dq or dk and a workspace");
+  const void* ptrs[] = {head_dq, head_dk, head_dv, dq, dk, dv, workspace};
+  for (const void* p : ptrs)
+    if (!aligned16(p)) return fail("oal_norm_rotary_heads_backward: tensor pointers must be 16-byte aligned");
+  const auto launch = dtype == OAL_DTYPE_F32    ? oal::launch_heads_backward<float>
+                      : dtype == OAL_DTYPE_BF16 ? oal::launch_heads_backward<uint16_t>
+                                                : oal::launch_heads_backward<_Float16>;
+  launch(a, head_dq, head_dk, head_dv, dq, dk, dv, dq_weight, dk_weight,
+         dq_weight || dk_weight ? static_cast<float*>(workspace) : nullptr, static_cast<hipStream_t>(stream), make_timer());
+  return launch_status("oal_norm_rotary_heads_backward launch");
+}
+
+// ---------------------------------------------------------------------------
+// Token scores
+// ---------------------------------------------------------------------------
+static int score_args(oal::ScoreArgs* a, const char* what, const void* logits, const int64_t* strides,
+                      const int64_t* tokens, int batch, int rows, int vocab, int dtype, bool entropy, int top) {
+  if (batch <= 0 || rows <= 0 || vocab <= 0) return fail("batch, rows and vocab must be positive");
+  if (dtype < OAL_DTYPE_F32 || dtype > OAL_DTYPE_F16)
+    return fail("dtype must be OAL_DTYPE_F32, OAL_DTYPE_BF16 or OAL_DTYPE_F16");
+  if (top < 0 || top > oal::kMostTop || top > vocab)
+    return fail(std::string(what) + ": top must be in [0, 64] and not more than vocab");
+  if (vocab > (1 << 30) || int64_t(batch) > (int64_t(1) << 23) / rows)
+    return fail("batch, rows and vocab are too large for one launch");
+  if (!logits || !strides || !tokens) return fail(std::string(what) + ": null pointer argument");
+  if (reinterpret_cast<uintptr_t>(logits) % (dtype == OAL_DTYPE_F32 ? 4 : 2))
+    return fail(std::string(what) + ": logits must be aligned to their type");
+  *a = {logits, strides[0], strides[1], tokens, batch, rows, vocab, entropy, top};
+  return 0;
+}
+
+size_t oal_token_scores_workspace_bytes(int batch, int rows, int vocab, int top) {
+  oal::ScoreArgs a;
+  const int64_t none[2] = {};
+  if (score_args(&a, "oal_token_scores_workspace_bytes", none, none, none, batch, rows, vocab, 0, false, top)) return 0;
+  return std::max<size_t>(oal::score_work_bytes(a), 16);
+}
+
+int oal_token_scores(const void* logits, const int64_t* strides, const int64_t* tokens, int batch, int rows, int vocab,
+                     int dtype, int top, float* log_probs, float* entropy, float* top_log_probs, int64_t* top_tokens,
+                     float* saved, void* workspace, void* stream) {
+  Range range("oal_token_scores");
+  oal::ScoreArgs a;
+  if (score_args(&a, "oal_token_scores", logits, strides, tokens, batch, rows, vocab, dtype, entropy != nullptr, top))
+    return 1;
+  if (!log_probs || !workspace || (top && (!top_log_probs || !top_tokens)))
+    return fail("oal_token_scores: null pointer argument");
+  if (!aligned16(workspace)) return fail("oal_token_scores: the workspace must be 16-byte aligned");
+  const oal::ScoreOut out = {log_probs, entropy, top_log_probs, top_tokens, saved};
+  const auto launch = dtype == OAL_DTYPE_F32    ? oal::launch_scores<float>
+                      : dtype == OAL_DTYPE_BF16 ? oal::launch_scores<uint16_t>
+                                                : oal::launch_scores<_Float16>;
+  launch(a, out, workspace, static_cast<hipStream_t>(stream), make_timer());
+  return launch_status("oal_token_scores launch");
+}
+
+int oal_token_scores_backward(const void* logits, const int64_t* strides, const int64_t* tokens, int batch, int rows,
+                              int vocab, int dtype, const float* saved, const float* entropy, const float* dlog_probs,
+                              const float* dentropy, void* dlogits, void* stream) {
+  Range range("oal_token_scores_backward");
+  oal::ScoreArgs a;
+  if (score_args(&a, "oal_token_scores_backward", logits, strides, tokens, batch, rows, vocab, dtype, entropy != nullptr, 0))
+    return 1;
+  if (!saved || !dlogits || (dentropy && !entropy)) return fail("oal_token_scores_backward: null pointer argument");
+  if (!aligned16(dlogits)) return fail("oal_token_scores_backward: tensor pointers must be 16-byte aligned");
+  const auto launch = dtype == OAL_DTYPE_F32    ? oal::launch_scores_backward<float>
+                      : dtype == OAL_DTYPE_BF16 ? oal::launch_scores_backward<uint16_t>
+                                                : oal::launch_scores_backward<_Float16>;
+  launch(a, saved, entropy, dlog_probs, dentropy, dlogits, static_cast<hipStream_t>(stream), make_timer());
+  return launch_status("oal_token_scores_backward launch");
 }
 
 }  // extern "C"

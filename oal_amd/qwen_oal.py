@@ -39,6 +39,7 @@ from torch.utils.checkpoint import checkpoint
 
 from . import _native
 from .hd_block_gemm_adapters import prepare_grouped_hd_block_gemm, run_prepared_grouped_hd_block_gemm
+from .token_scores import TokenScores, token_log_probs
 
 
 @dataclass(frozen=True)
@@ -334,6 +335,20 @@ def causal_lm_loss(logits: torch.Tensor, tokens: torch.Tensor) -> torch.Tensor:
     return F.cross_entropy(logits[:, :-1].float().reshape(-1, logits.shape[-1]), tokens[:, 1:].reshape(-1))
 
 
+@torch.no_grad()
+def score_tokens(model: QwenOALModel, tokens: torch.Tensor, *, lengths: torch.Tensor | None = None, entropy: bool = False,
+                 top: int = 0) -> TokenScores:
+    """What the model makes of tokens [B, N], each from those before it: the log probabilities [B, N - 1] of
+    the second and later ones, with the entropy of the distributions that they are from and ``top``
+    alternatives if asked for (:func:`oal_amd.token_scores.token_log_probs`). lengths [B] (None: N each): the
+    tokens of each sequence of a batch padded at its end; behind them log probabilities are zero."""
+    targets = tokens[:, 1:]
+    if lengths is not None:
+        places = torch.arange(1, tokens.shape[1], device=tokens.device)
+        targets = torch.where(places < lengths[:, None], targets, -1)
+    return token_log_probs(model(tokens)[:, :-1], targets, entropy=entropy, top=top)
+
+
 def train_step(model: QwenOALModel, tokens: torch.Tensor, optimizer: torch.optim.Optimizer) -> torch.Tensor:
     """One LoRA training step: forward, loss, backward, optimizer update. Returns the loss."""
     optimizer.zero_grad(set_to_none=True)
@@ -343,4 +358,4 @@ def train_step(model: QwenOALModel, tokens: torch.Tensor, optimizer: torch.optim
     return loss.detach()
 
 
-__all__ = ("QwenOALConfig", "QwenOALModel", "causal_lm_loss", "train_step", "rotary_tables", "apply_rotary")
+__all__ = ("QwenOALConfig", "QwenOALModel", "causal_lm_loss", "score_tokens", "train_step", "rotary_tables", "apply_rotary")
