@@ -9,8 +9,9 @@
 //   dx = r w dy - x r^3 mean(x w dy),  dw = sum over tokens of x r dy
 //
 // Bound by memory: each value is read once and written once, four lanes to a head's
-// row, of which each takes 8 pairs of dimensions. A thread stays with one head, so that weights are read once and their
-// gradients' sums stay in registers; a block's go to memory, and a second kernel adds those up, in order.
+// row, of which each takes 8 pairs of dimensions. A thread stays with one token, whose row of the tables it reads once,
+// and goes over heads, the next one's values on their way. The weights' gradients stay in registers
+// until a weight row ends; a block's go to memory, and a second kernel adds those up, in order.
 // Arithmetic and sums are in fp32, one rounding to the tensors' type.
 
 #include <hip/hip_runtime.h>
@@ -27,100 +28,80 @@ namespace oal {
 namespace {
 
 constexpr int kThr = 256;
-constexpr int kRows = kThr / 4;  // a block's head rows at once
-constexpr int kBackBlocks = 512;
+constexpr int kTokens = kThr / 4;  // a block's tokens
+constexpr int kSumThr = 1024;
 
-__device__ __forceinline__ void store_row8(float* p, const float (&x)[8]) {
-  reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
-  reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ f32x8 load8(const float* p) {
+  const f32x4 a = load4(p), b = load4(p + 4);
+  return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
 }
-__device__ __forceinline__ void store_row8(uint16_t* p, const float (&x)[8]) {
-  *reinterpret_cast<bf16x8*>(p) = pack8(x);
+__device__ __forceinline__ f32x8 load8(const uint16_t* p) {
+  return __builtin_convertvector(*reinterpret_cast<const bf16x8*>(p), f32x8);
 }
-__device__ __forceinline__ void store_row8(_Float16* p, const float (&x)[8]) {
-  typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-  f16x8 v;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = static_cast<_Float16>(x[e]);
-  *reinterpret_cast<f16x8*>(p) = v;
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ f32x8 load8(const _Float16* p) {
+  return __builtin_convertvector(*reinterpret_cast<const f16x8*>(p), f32x8);
+}
+__device__ __forceinline__ void store8(float* p, const f32x8& x) {
+  store4(p, __builtin_shufflevector(x, x, 0, 1, 2, 3));
+  store4(p + 4, __builtin_shufflevector(x, x, 4, 5, 6, 7));
+}
+__device__ __forceinline__ void store8(uint16_t* p, const f32x8& x) {
+  *reinterpret_cast<bf16x8*>(p) = __builtin_convertvector(x, bf16x8);
+}
+__device__ __forceinline__ void store8(_Float16* p, const f32x8& x) {
+  *reinterpret_cast<f16x8*>(p) = __builtin_convertvector(x, f16x8);
 }
 
-// A lane's 8 pairs (lo, hi) of a row's D values: the first R / 2 pairs are those that the rotation
+struct Pair {
+  f32x8 lo, hi;
+};
+
+// Lane j's 8 pairs of a row's D values: the first R / 2 pairs are those that the rotation
 // turns, (p, p + R / 2), the others two of the rest. With WIDE a lane's lo and hi are 8 values in a row
 // each (R / 2 and (D - R) / 2 multiples of 8, rows 16-byte aligned).
 template <bool WIDE>
-struct Pairs {
-  int lo[WIDE ? 1 : 8], hi[WIDE ? 1 : 8];  // -1: none
-  bool turned[WIDE ? 1 : 8];
-  __device__ __forceinline__ Pairs(int D, int R, int j) {
-    const int half = R / 2;
+struct Place {
+  int D, R, j;
+  __device__ __forceinline__ bool turned(int e) const { return 8 * j + e < R / 2; }
+  __device__ __forceinline__ int lo(int e) const {
+    const int p = 8 * j + e;
+    return p < R / 2 ? p : R + 2 * (p - R / 2);
+  }
+  __device__ __forceinline__ int hi(int e) const { return lo(e) + (turned(e) ? R / 2 : WIDE ? 8 : 1); }
+  // fill: what a lane's places past D hold, and (angles) the places that are not turned
+  template <bool ANGLES = false, typename T>
+  __device__ __forceinline__ Pair load(const T* p, float fill = 0.f) const {
+    Pair x;
     if constexpr (WIDE) {
-      const int p = 8 * j;
-      turned[0] = p < half;
-      lo[0] = turned[0] ? p : R + 2 * (p - half);
-      hi[0] = turned[0] ? p + half : lo[0] + 8;
-      if (lo[0] >= D) lo[0] = hi[0] = -1;
+      const bool in = ANGLES ? turned(0) : lo(0) < D;
+      x.lo = x.hi = fill;
+      if (in) x.lo = load8(p + lo(0)), x.hi = load8(p + hi(0));
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const int p = 8 * j + e;
-        turned[e] = p < half;
-        lo[e] = turned[e] ? p : R + 2 * (p - half);
-        hi[e] = turned[e] ? p + half : lo[e] + 1;
-        if (lo[e] >= D) lo[e] = -1;
-        if (hi[e] >= D) hi[e] = -1;
+        const int l = lo(e), h = hi(e);
+        const bool a = ANGLES ? turned(e) : l < D, b = ANGLES ? turned(e) : h < D;
+        x.lo[e] = a ? get(p + (a ? l : 0)) : fill;
+        x.hi[e] = b ? get(p + (b ? h : 0)) : fill;
       }
     }
+    return x;
   }
   template <typename T>
-  __device__ __forceinline__ void load(const T* p, float (&x)[8], float (&y)[8], float none = 0.f) const {
+  __device__ __forceinline__ void store(T* p, const Pair& x) const {
     if constexpr (WIDE) {
-      if (lo[0] >= 0) {
-        load_row8(x, p + lo[0]);
-        load_row8(y, p + hi[0]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = y[e] = none;
+      if (lo(0) < D) {
+        store8(p + lo(0), x.lo);
+        store8(p + hi(0), x.hi);
       }
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        x[e] = lo[e] >= 0 ? get(p + lo[e]) : none;
-        y[e] = hi[e] >= 0 ? get(p + hi[e]) : none;
-      }
-    }
-  }
-  template <typename T>
-  __device__ __forceinline__ void store(T* p, const float (&x)[8], const float (&y)[8]) const {
-    if constexpr (WIDE) {
-      if (lo[0] >= 0) {
-        store_row8(p + lo[0], x);
-        store_row8(p + hi[0], y);
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if (lo[e] >= 0) put(p + lo[e], x[e]);
-        if (hi[e] >= 0) put(p + hi[e], y[e]);
-      }
-    }
-  }
-  // cos and sin of the pairs; those that are not turned by an angle of zero
-  template <typename T>
-  __device__ __forceinline__ void angles(const T* p, float (&x)[8], float (&y)[8], float none) const {
-    if constexpr (WIDE) {
-      if (turned[0] && lo[0] >= 0) {
-        load_row8(x, p + lo[0]);
-        load_row8(y, p + hi[0]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = y[e] = none;
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x[e] = turned[e] ? get(p + lo[e]) : none;
-        y[e] = turned[e] ? get(p + hi[e]) : none;
+        if (lo(e) < D) put(p + lo(e), x.lo[e]);
+        if (hi(e) < D) put(p + hi(e), x.hi[e]);
       }
     }
   }
@@ -131,174 +112,186 @@ __device__ __forceinline__ float row_sum(float x) {
   x += __shfl_xor(x, 1, 64);
   return x + __shfl_xor(x, 2, 64);
 }
+__device__ __forceinline__ float dot(const Pair& x, const Pair& y) {
+  float s = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) s += x.lo[e] * y.lo[e] + x.hi[e] * y.hi[e];
+  return s;
+}
+// The reciprocal root of a row's mean square.
+__device__ __forceinline__ float root(const Pair& x, const HeadsArgs& a) {
+  return 1.f / sqrtf(row_sum(dot(x, x)) / a.D + a.eps);
+}
 
-// The rows of a block: `tokens` tokens of `heads` heads at once, thread t's the row t / 4. Where there are
-// more heads than rows, blockIdx.y takes a part of them.
-struct Rows {
-  int heads, tokens, first;
-  __device__ __forceinline__ explicit Rows(int total) {
-    first = blockIdx.y * kRows;
-    heads = min(kRows, total - first);
-    tokens = kRows / heads;
+template <typename T, typename P>
+__device__ __forceinline__ Pair weight(const HeadsArgs& a, const P& at, const void* w, int h) {
+  const size_t from = a.per_head ? (size_t)h * a.D : 0;
+  if (!w) return {1.f, 1.f};
+  return a.w32 ? at.load(static_cast<const float*>(w) + from) : at.load(static_cast<const T*>(w) + from);
+}
+
+// A block's tokens and heads: 64 tokens, thread t's the token t / 4, and the heads [first, last) of all
+// of q, k and v. A thread keeps its token, whose row of the tables it reads once.
+struct Part {
+  int64_t token;
+  int b, n, first, last;
+  bool live;
+  int64_t pos;
+  __device__ __forceinline__ Part(const HeadsArgs& a, int each) {
+    const int64_t i = (int64_t)blockIdx.x * kTokens + (threadIdx.x >> 2), total = (int64_t)a.B * a.N;
+    live = i < total;
+    token = live ? i : total - 1;
+    b = (int)((uint32_t)token / (uint32_t)a.N);  // fewer than 2^31 tokens
+    n = (int)(token - (int64_t)b * a.N);
+    first = blockIdx.y * each;
+    last = min(first + each, a.Hq + 2 * a.Hk);
+    pos = a.position ? a.position[token] : n;
   }
 };
 
-template <typename T>
-__device__ __forceinline__ void weights(const HeadsArgs& a, const void* w, int h, const auto& at, float (&x)[8],
-                                        float (&y)[8]) {
-  const size_t from = a.per_head ? (size_t)h * a.D : 0;
-  if (!w) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = y[e] = 1.f;
-  } else if (a.w32) {
-    at.load(static_cast<const float*>(w) + from, x, y);
-  } else {
-    at.load(static_cast<const T*>(w) + from, x, y);
-  }
-}
-// cos and sin of a position, for the rotation or back. Positions past the tables give NaN.
-template <typename T>
-__device__ __forceinline__ void table_rows(const HeadsArgs& a, int64_t pos, const auto& at, float (&cl)[8], float (&ch)[8],
-                                           float (&sl)[8], float (&sh)[8]) {
-  const bool in = pos < a.table;
+// cos and sin of a position; past the tables NaN.
+template <typename T, typename P>
+__device__ __forceinline__ void angles(const HeadsArgs& a, const P& at, int64_t pos, Pair& cosine, Pair& sine) {
+  const bool in = pos >= 0 && pos < a.table;
   const size_t from = in ? (size_t)pos * a.R : 0;
   if (a.t32) {
-    at.angles(static_cast<const float*>(a.cosine) + from, cl, ch, 1.f);
-    at.angles(static_cast<const float*>(a.sine) + from, sl, sh, 0.f);
+    cosine = at.template load<true>(static_cast<const float*>(a.cosine) + from, 1.f);
+    sine = at.template load<true>(static_cast<const float*>(a.sine) + from, 0.f);
   } else {
-    at.angles(static_cast<const T*>(a.cosine) + from, cl, ch, 1.f);
-    at.angles(static_cast<const T*>(a.sine) + from, sl, sh, 0.f);
+    cosine = at.template load<true>(static_cast<const T*>(a.cosine) + from, 1.f);
+    sine = at.template load<true>(static_cast<const T*>(a.sine) + from, 0.f);
   }
-  if (!in) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) cl[e] = ch[e] = __builtin_nanf("");
-  }
+  if (pos >= a.table) cosine.lo = cosine.hi = __builtin_nanf("");
 }
 
 }  // namespace
 
 template <typename T, bool WIDE>
-__global__ __launch_bounds__(kThr) void k_heads(HeadsArgs a, T* __restrict__ hq, T* __restrict__ hk, T* __restrict__ hv) {
-  const Rows rows(a.Hq + 2 * a.Hk);
-  const int slot = threadIdx.x >> 2, hh = rows.first + slot % rows.heads;
-  if (slot >= rows.tokens * rows.heads) return;
-  const Pairs<WIDE> at(a.D, a.R, threadIdx.x & 3);
-  const bool is_q = hh < a.Hq, is_v = hh >= a.Hq + a.Hk;
-  const int h = is_q ? hh : is_v ? hh - a.Hq - a.Hk : hh - a.Hq, H = is_q ? a.Hq : a.Hk;
-  const T* src = static_cast<const T*>(is_q ? a.q : is_v ? a.v : a.k) + (size_t)h * a.D;
-  const int64_t sb = is_q ? a.qb : is_v ? a.vb : a.kb, sn = is_q ? a.qn : is_v ? a.vn : a.kn;
-  T* const dst = is_q ? hq : is_v ? hv : hk;
-  float wl[8], wh[8];
-  if (!is_v) weights<T>(a, is_q ? a.qw : a.kw, h, at, wl, wh);
-  const int64_t total = (int64_t)a.B * a.N;
-  for (int64_t i = (int64_t)blockIdx.x * rows.tokens + slot / rows.heads; i < total; i += (int64_t)gridDim.x * rows.tokens) {
-    const int64_t b = i / a.N, n = i % a.N;
-    const int64_t pos = a.position ? a.position[i] : n;
-    float lo[8], hi[8];
-    at.load(src + b * sb + n * sn, lo, hi);
+__global__ __launch_bounds__(kThr) void k_heads(HeadsArgs a, int each, T* __restrict__ hq, T* __restrict__ hk,
+                                                T* __restrict__ hv) {
+  const Part p(a, each);
+  if (!p.live) return;
+  const Place<WIDE> at{a.D, a.R, (int)(threadIdx.x & 3)};
+  auto fetch = [&](int h) {
+    const bool is_q = h < a.Hq, is_v = h >= a.Hq + a.Hk;
+    const int own = is_q ? h : is_v ? h - a.Hq - a.Hk : h - a.Hq;
+    return at.load(static_cast<const T*>(is_q ? a.q : is_v ? a.v : a.k) + p.b * (is_q ? a.qb : is_v ? a.vb : a.kb) +
+                   p.n * (is_q ? a.qn : is_v ? a.vn : a.kn) + own * a.D);
+  };
+  Pair next = fetch(p.first), cosine, sine, w;
+  angles<T>(a, at, p.pos, cosine, sine);
+  for (int h = p.first; h < p.last; ++h) {
+    Pair x = next;
+    if (h + 1 < p.last) next = fetch(h + 1);
+    const bool is_q = h < a.Hq, is_v = h >= a.Hq + a.Hk;
+    const int own = is_q ? h : is_v ? h - a.Hq - a.Hk : h - a.Hq;
     if (!is_v) {
-      float cl[8], ch[8], sl[8], sh[8], sum = 0.f;
-      table_rows<T>(a, pos < 0 ? 0 : pos, at, cl, ch, sl, sh);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) sum += lo[e] * lo[e] + hi[e] * hi[e];
-      const float r = 1.f / sqrtf(row_sum(sum) / a.D + a.eps);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float x = lo[e] * r * wl[e], y = hi[e] * r * wh[e];
-        lo[e] = x * cl[e] - y * sl[e];
-        hi[e] = y * ch[e] + x * sh[e];
-      }
+      if (h == p.first || h == a.Hq || a.per_head) w = weight<T>(a, at, is_q ? a.qw : a.kw, own);
+      const float r = root(x, a);
+      const f32x8 lo = x.lo * r * w.lo, hi = x.hi * r * w.hi;
+      x.lo = lo * cosine.lo - hi * sine.lo;
+      x.hi = hi * cosine.hi + lo * sine.hi;
     }
-    if (pos < 0) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) lo[e] = hi[e] = 0.f;
-    }
-    at.store(dst + ((b * H + h) * a.N + n) * a.D, lo, hi);
+    if (p.pos < 0) x.lo = x.hi = 0.f;
+    at.store((is_q ? hq : is_v ? hv : hk) + (((int64_t)p.b * (is_q ? a.Hq : a.Hk) + own) * a.N + p.n) * a.D, x);
   }
 }
 
 template <typename T, bool WIDE>
-__global__ __launch_bounds__(kThr) void k_heads_bwd(HeadsArgs a, const T* __restrict__ hq, const T* __restrict__ hk,
-                                                    const T* __restrict__ hv, T* __restrict__ dq, T* __restrict__ dk,
-                                                    T* __restrict__ dv, float* __restrict__ work) {
-  __shared__ alignas(16) float sums[kRows][68];
-  const Rows rows(a.Hq + 2 * a.Hk);
-  const int slot = threadIdx.x >> 2, hh = rows.first + slot % rows.heads;
-  const bool live = slot < rows.tokens * rows.heads;
-  const Pairs<WIDE> at(a.D, a.R, threadIdx.x & 3);
-  const bool is_q = hh < a.Hq, is_v = hh >= a.Hq + a.Hk;
-  const int h = is_q ? hh : is_v ? hh - a.Hq - a.Hk : hh - a.Hq, H = is_q ? a.Hq : a.Hk;
-  const T* up = is_q ? hq : is_v ? hv : hk;
-  T* const dst = is_q ? dq : is_v ? dv : dk;
-  const T* src = static_cast<const T*>(is_q ? a.q : a.k) + (size_t)h * a.D;
-  const int64_t sb = is_q ? a.qb : a.kb, sn = is_q ? a.qn : a.kn;
-  float wl[8], wh[8], gl[8] = {}, gh[8] = {};
-  if (!is_v) weights<T>(a, is_q ? a.qw : a.kw, h, at, wl, wh);
-  const int64_t total = live && dst ? (int64_t)a.B * a.N : 0;
-  for (int64_t i = (int64_t)blockIdx.x * rows.tokens + slot / rows.heads; i < total; i += (int64_t)gridDim.x * rows.tokens) {
-    const int64_t b = i / a.N, n = i % a.N;
-    const int64_t pos = a.position ? a.position[i] : n;
-    float lo[8] = {}, hi[8] = {};
-    if (up && pos >= 0) at.load(up + ((b * H + h) * a.N + n) * a.D, lo, hi);
-    if (!is_v) {
-      float cl[8], ch[8], sl[8], sh[8], xl[8], xh[8], sum = 0.f, dot = 0.f;
-      at.load(src + b * sb + n * sn, xl, xh);
-      table_rows<T>(a, pos < 0 ? 0 : pos, at, cl, ch, sl, sh);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float x = lo[e], y = hi[e];
-        lo[e] = x * cl[e] + y * sh[e];
-        hi[e] = y * ch[e] - x * sl[e];
-        sum += xl[e] * xl[e] + xh[e] * xh[e];
-      }
-      const float r = 1.f / sqrtf(row_sum(sum) / a.D + a.eps);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        xl[e] *= r, xh[e] *= r;
-        if (pos >= 0) gl[e] += xl[e] * lo[e], gh[e] += xh[e] * hi[e];
-        lo[e] *= wl[e], hi[e] *= wh[e];
-        dot += xl[e] * lo[e] + xh[e] * hi[e];
-      }
-      dot = row_sum(dot) / a.D;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        lo[e] = pos < 0 ? 0.f : r * (lo[e] - xl[e] * dot);
-        hi[e] = pos < 0 ? 0.f : r * (hi[e] - xh[e] * dot);
-      }
-    }
-    at.store(dst + ((int64_t)i * H + h) * a.D, lo, hi);
-  }
-  if (!work) return;
-  // the block's sums of each weight's gradient, rows in order
-  if (live && !is_v) at.store(sums[slot], gl, gh);
-  __syncthreads();
+__global__ __launch_bounds__(kThr) void k_heads_bwd(HeadsArgs a, int each, const T* __restrict__ hq,
+                                                    const T* __restrict__ hk, const T* __restrict__ hv,
+                                                    T* __restrict__ dq, T* __restrict__ dk, T* __restrict__ dv,
+                                                    float* __restrict__ work) {
+  __shared__ alignas(16) float sums[kTokens][68];
+  __shared__ float parts[kThr / 64][64];
+  const Part p(a, each);
+  const Place<WIDE> at{a.D, a.R, (int)(threadIdx.x & 3)};
+  // a place without a token asks for nothing
+  const bool there = p.live && p.pos >= 0;
+  Pair cosine, sine;
+  angles<T>(a, at, p.pos, cosine, sine);
   const int targets = a.per_head ? a.Hq + a.Hk : 2;
-  for (int x = threadIdx.x; x < targets * a.D; x += kThr) {
-    const int target = x / a.D, d = x % a.D;
-    float s = 0.f;
-    for (int i = 0; i < rows.tokens * rows.heads; ++i) {
-      const int head = rows.first + i % rows.heads;
-      if (head >= a.Hq + a.Hk) continue;
-      if ((a.per_head ? head : head >= a.Hq) == target) s += sums[i][d];
+  float* const rows = work + (a.per_head ? blockIdx.x : (size_t)blockIdx.y * gridDim.x + blockIdx.x) * targets * a.D;
+  // the part's heads of q or k: source x, gradients up and out, both from the projections' and the heads' first
+  auto norms = [&](const T* x0, int64_t xb, int64_t xn, const void* weights, const T* up0, T* out0, int H, int from,
+                   int to, int target) __attribute__((always_inline)) {
+    if (from >= to) {
+      if (work && !a.per_head && (int)threadIdx.x < a.D) rows[target * a.D + threadIdx.x] = 0.f;
+      return;
     }
-    work[((size_t)(blockIdx.y * gridDim.x + blockIdx.x) * targets + target) * a.D + d] = s;
+    const T* x1 = x0 + p.b * xb + p.n * xn;
+    const T* up1 = up0 + ((int64_t)p.b * H * a.N + p.n) * a.D;
+    T* out1 = out0 + p.token * H * a.D;
+    Pair w{}, g{}, x = at.load(x1 + from * a.D), up{};
+    if (up0 && there) up = at.load(up1 + (int64_t)from * a.N * a.D);
+    for (int h = from; h < to; ++h) {
+      Pair nx{}, nup{};
+      if (h + 1 < to) {
+        nx = at.load(x1 + (h + 1) * a.D);
+        if (up0 && there) nup = at.load(up1 + (int64_t)(h + 1) * a.N * a.D);
+      }
+      if (h == from || a.per_head) w = weight<T>(a, at, weights, h);
+      const float r = root(x, a);
+      Pair y;
+      y.lo = up.lo * cosine.lo + up.hi * sine.hi;
+      y.hi = up.hi * cosine.hi - up.lo * sine.lo;
+      x.lo *= r, x.hi *= r;
+      if (there) g.lo += x.lo * y.lo, g.hi += x.hi * y.hi;
+      y.lo *= w.lo, y.hi *= w.hi;
+      const float mean = row_sum(dot(x, y)) / a.D;
+      up.lo = r * (y.lo - x.lo * mean), up.hi = r * (y.hi - x.hi * mean);
+      if (!there) up = Pair{};
+      if (out0 && p.live) at.store(out1 + h * a.D, up);
+      x = nx, up = nup;
+      if (work && (a.per_head || h + 1 == to)) {
+        // the block's sum of a weight row's gradient, tokens in order
+        const int d = threadIdx.x & 63, part = threadIdx.x >> 6;
+        at.store(sums[threadIdx.x >> 2], g);
+        g = Pair{};
+        __syncthreads();
+        float s = 0.f;
+        if (d < a.D)
+          for (int i = 0; i < kTokens / 4; ++i) s += sums[part * (kTokens / 4) + i][d];
+        parts[part][d] = s;
+        __syncthreads();
+        if (part == 0 && d < a.D)
+          rows[(target + (a.per_head ? h : 0)) * a.D + d] = (parts[0][d] + parts[1][d]) + (parts[2][d] + parts[3][d]);
+      }
+    }
+  };
+  const int k0 = a.Hq, v0 = a.Hq + a.Hk;
+  norms(static_cast<const T*>(a.q), a.qb, a.qn, a.qw, hq, dq, a.Hq, p.first, min(p.last, k0), 0);
+  norms(static_cast<const T*>(a.k), a.kb, a.kn, a.kw, hk, dk, a.Hk, max(p.first, k0) - k0, min(p.last, v0) - k0,
+        a.per_head ? a.Hq : 1);
+  if (!dv || !p.live) return;
+  for (int h = max(p.first, v0) - v0; h < p.last - v0; ++h) {
+    Pair up{};
+    if (hv && there) up = at.load(hv + (((int64_t)p.b * a.Hk + h) * a.N + p.n) * a.D);
+    at.store(dv + (p.token * a.Hk + h) * a.D, up);
   }
 }
 
-// The weights' gradients: a block for each weight row adds up the blocks' sums, in fp64.
+// The weights' gradients: a block for 16 dimensions of each weight row adds up the blocks' sums, in fp64.
 template <typename W>
-__global__ __launch_bounds__(kThr) void k_heads_weights(const float* __restrict__ work, int blocks, int D, int split,
-                                                        W* __restrict__ dqw, W* __restrict__ dkw) {
-  __shared__ double sum[kThr / 64][64];
-  const int d = threadIdx.x & 63, part = threadIdx.x >> 6, target = blockIdx.x, targets = gridDim.x;
+__global__ __launch_bounds__(kSumThr) void k_heads_weights(const float* __restrict__ work, int rows, int D, int split,
+                                                           W* __restrict__ dqw, W* __restrict__ dkw) {
+  constexpr int kParts = kSumThr / 16;
+  __shared__ double sum[kParts][16];
+  const int c = threadIdx.x & 15, part = threadIdx.x >> 4, target = blockIdx.x, targets = gridDim.x, d = 16 * blockIdx.y + c;
   double s = 0;
-  if (d < D)
-    for (int i = part; i < blocks; i += kThr / 64) s += work[((size_t)i * targets + target) * D + d];
-  sum[part][d] = s;
+  if (d < D) {
+    const float* from = work + (size_t)target * D + d;
+#pragma unroll 8
+    for (int i = part; i < rows; i += kParts) s += from[(size_t)i * targets * D];
+  }
+  sum[part][c] = s;
   __syncthreads();
-  if (part || d >= D) return;
+  for (int n = kParts / 2; n > 0; n >>= 1) {
+    if (part < n) sum[part][c] += sum[part + n][c];
+    __syncthreads();
+  }
   W* const dst = target < split ? dqw : dkw;
-  if (dst) put(dst + (size_t)(target < split ? target : target - split) * D + d, (float)((sum[0][d] + sum[1][d]) + (sum[2][d] + sum[3][d])));
+  if (part == 0 && d < D && dst) put(dst + (size_t)(target < split ? target : target - split) * D + d, (float)sum[0][c]);
 }
 
 namespace {
@@ -311,24 +304,29 @@ bool wide(const HeadsArgs& a, int size) {
     if (s * size % 16) return false;
   return true;
 }
-dim3 heads_grid(const HeadsArgs& a, int most) {
-  const int heads = a.Hq + 2 * a.Hk, parts = (heads + kRows - 1) / kRows, tokens = kRows / std::min(heads, kRows);
-  const int64_t blocks = ((int64_t)a.B * a.N + tokens - 1) / tokens;
-  return dim3((unsigned)std::min<int64_t>(blocks, most), parts);
+// Blocks for all tokens, and as many parts of the heads that the GPU has four blocks a CU.
+struct Grid {
+  int blocks, parts, each;
+};
+Grid heads_grid(const HeadsArgs& a) {
+  const int heads = a.Hq + 2 * a.Hk, blocks = (int)(((int64_t)a.B * a.N + kTokens - 1) / kTokens);
+  const int each = std::max(1, (int)((int64_t)heads * blocks / 1024));
+  return {blocks, (heads + std::min(each, heads) - 1) / std::min(each, heads), std::min(each, heads)};
 }
 }  // namespace
 
 int heads_blocks(const HeadsArgs& a) {
-  const dim3 g = heads_grid(a, kBackBlocks);
-  return g.x * g.y;
+  const Grid g = heads_grid(a);
+  return a.per_head ? g.blocks : g.blocks * g.parts;
 }
 
 template <typename T>
 void launch_heads_forward(const HeadsArgs& a, void* hq, void* hk, void* hv, hipStream_t st, const Timer& timed) {
   const auto kernel = wide(a, sizeof(T)) ? k_heads<T, true> : k_heads<T, false>;
+  const Grid g = heads_grid(a);
   timed("k_heads", st, [&] {
-    hipLaunchKernelGGL(kernel, heads_grid(a, 4096), dim3(kThr), 0, st, a, static_cast<T*>(hq), static_cast<T*>(hk),
-                       static_cast<T*>(hv));
+    hipLaunchKernelGGL(kernel, dim3(g.blocks, g.parts), dim3(kThr), 0, st, a, g.each, static_cast<T*>(hq),
+                       static_cast<T*>(hk), static_cast<T*>(hv));
   });
 }
 
@@ -336,20 +334,22 @@ template <typename T>
 void launch_heads_backward(const HeadsArgs& a, const void* hq, const void* hk, const void* hv, void* dq, void* dk,
                            void* dv, void* dqw, void* dkw, float* work, hipStream_t st, const Timer& timed) {
   const auto kernel = wide(a, sizeof(T)) ? k_heads_bwd<T, true> : k_heads_bwd<T, false>;
-  const dim3 grid = heads_grid(a, kBackBlocks);
+  const Grid g = heads_grid(a);
   timed("k_heads_bwd", st, [&] {
-    hipLaunchKernelGGL(kernel, grid, dim3(kThr), 0, st, a, static_cast<const T*>(hq), static_cast<const T*>(hk),
-                       static_cast<const T*>(hv), static_cast<T*>(dq), static_cast<T*>(dk), static_cast<T*>(dv), work);
+    hipLaunchKernelGGL(kernel, dim3(g.blocks, g.parts), dim3(kThr), 0, st, a, g.each, static_cast<const T*>(hq),
+                       static_cast<const T*>(hk), static_cast<const T*>(hv), static_cast<T*>(dq), static_cast<T*>(dk),
+                       static_cast<T*>(dv), work);
   });
   if (!work) return;
   const int split = a.per_head ? a.Hq : 1, targets = a.per_head ? a.Hq + a.Hk : 2;
+  const dim3 grid(targets, (a.D + 15) / 16), block(kSumThr);
   timed("k_heads_weights", st, [&] {
     if (a.w32)
-      hipLaunchKernelGGL(k_heads_weights<float>, dim3(targets), dim3(kThr), 0, st, work, (int)(grid.x * grid.y), a.D,
-                         split, static_cast<float*>(dqw), static_cast<float*>(dkw));
+      hipLaunchKernelGGL(k_heads_weights<float>, grid, block, 0, st, work, heads_blocks(a), a.D, split,
+                         static_cast<float*>(dqw), static_cast<float*>(dkw));
     else
-      hipLaunchKernelGGL(k_heads_weights<T>, dim3(targets), dim3(kThr), 0, st, work, (int)(grid.x * grid.y), a.D, split,
-                         static_cast<T*>(dqw), static_cast<T*>(dkw));
+      hipLaunchKernelGGL(k_heads_weights<T>, grid, block, 0, st, work, heads_blocks(a), a.D, split, static_cast<T*>(dqw),
+                         static_cast<T*>(dkw));
   });
 }
 

@@ -20,7 +20,7 @@ struct HeadsArgs {
   float eps;
 };
 
-// Blocks of the backward: as many partial sums of each weight's gradient.
+// Partial sums of each weight row's gradient that the backward leaves.
 int heads_blocks(const HeadsArgs& a);
 
 // hq, hk, hv: [B][heads][N][D].

@@ -11,7 +11,8 @@
 //
 // The alternatives: a wave keeps the highest 64 of its values so far in order, one per lane, and
 // looks at a value only if it comes before the last that counts; of equal values the first. A row of random
-// order changes that list some K log(V / K) times.
+// order changes that list some K log(V / K) times. Where several lanes have such a value they are
+// sorted and merged with the list at once, as at the beginning; else they move up the list one by one.
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -57,12 +58,16 @@ __device__ __forceinline__ void join(Sums& a, Sums b) {
   a.t += b.t;
 }
 
-// Adds N values.
-template <int N, bool ENTROPY>
-__device__ __forceinline__ void add(Sums& a, const float (&x)[N]) {
+template <int N>
+__device__ __forceinline__ float most_of(const float (&x)[N]) {
   float most = x[0];
 #pragma unroll
   for (int e = 1; e < N; ++e) most = fmaxf(most, x[e]);
+  return most;
+}
+// Adds N values, the highest of them `most`.
+template <int N, bool ENTROPY>
+__device__ __forceinline__ void add(Sums& a, const float (&x)[N], float most) {
   if (most > a.m) move_to(a, most);
   const float m = a.m == -INFINITY ? 0.f : a.m;  // -inf values weigh nothing
 #pragma unroll
@@ -89,34 +94,63 @@ __device__ __forceinline__ float lane_f(float x, int l) {
 __device__ __forceinline__ uint32_t lane_u(uint32_t x, int l) { return __builtin_amdgcn_readlane(x, l); }
 
 // All lanes: value x of place i, which is the same in all, takes its place.
-__device__ __forceinline__ void insert(Best& b, float x, uint32_t i, int top, int lane) {
-  const bool behind = before(x, i, b.x, b.at);
-  const float px = __shfl_up(b.x, 1, 64);
-  const uint32_t pi = __shfl_up(b.at, 1, 64);
-  const bool prev = lane > 0 && before(x, i, px, pi);
-  if (behind) {
-    b.x = prev ? px : x;
-    b.at = prev ? pi : i;
-  }
-  b.last = lane_f(b.x, top - 1);
-  b.last_at = lane_u(b.at, top - 1);
+__device__ __forceinline__ void insert(Best& b, float x, uint32_t i) {
+  // from the lane before (wave_shr:1); lane 0 keeps what it had, which is behind nothing
+  const float px = __int_as_float(__builtin_amdgcn_update_dpp(0x7f800000, __float_as_int(b.x), 0x138, 0xf, 0xf, false));
+  const uint32_t pi = __builtin_amdgcn_update_dpp(0, b.at, 0x138, 0xf, 0xf, false);
+  const bool behind = before(x, i, b.x, b.at), prev = before(x, i, px, pi);
+  b.x = prev ? px : behind ? x : b.x;
+  b.at = prev ? pi : behind ? i : b.at;
 }
-// Each lane's N values of places i, i + 1, ...
+
+// One step of a sorting network: the lane keeps the earlier or the later of its own and its partner's.
+__device__ __forceinline__ void exchange(float& x, uint32_t& i, int with, bool earlier) {
+  const float y = __shfl_xor(x, with, 64);
+  const uint32_t j = __shfl_xor(i, with, 64);
+  if (before(y, j, x, i) == earlier) x = y, i = j;
+}
+// All lanes: each lane's value x of place i (or none: -inf, 0xffffffff) into the list. Sorted from the last to the
+// first, they and the list are a sequence that falls and rises, whose 64 highest six steps put in order. Values with
+// equal places are empty ones and change nothing, whichever is taken.
+__device__ __forceinline__ void merge(Best& b, float x, uint32_t i, int lane) {
+#pragma unroll
+  for (int k = 2; k <= 64; k <<= 1)
+#pragma unroll
+    for (int n = k >> 1; n > 0; n >>= 1) exchange(x, i, n, ((lane & n) == 0) != ((lane & k) == 0));
+  if (before(x, i, b.x, b.at)) b.x = x, b.at = i;
+#pragma unroll
+  for (int n = 32; n > 0; n >>= 1) exchange(b.x, b.at, n, (lane & n) == 0);
+}
+
+constexpr int kMerge = 6;  // lanes with a value to merge from which that is faster than one by one
+
+// Each lane's N values of places i, i + 1, ... (`in`: it has some); `most` is their maximum.
 template <int N>
-__device__ __forceinline__ void offer(Best& b, const float (&x)[N], uint32_t i, bool in, int top, int lane) {
-  float most = x[0];
-#pragma unroll
-  for (int e = 1; e < N; ++e) most = fmaxf(most, x[e]);
+__device__ __forceinline__ void offer(Best& b, float (&x)[N], float most, uint32_t i, bool in, int top, int lane) {
   if (!__ballot(in && before(most, i, b.last, b.last_at))) return;
+  // one value of each lane at a time, its highest; what has been looked at becomes NaN, which comes before nothing
+  for (;;) {
+    float v = -INFINITY;
+    uint32_t e = N;
 #pragma unroll
-  for (int e = 0; e < N; ++e) {
-    uint64_t who = __ballot(in && before(x[e], i + e, b.last, b.last_at));
-    while (who) {
-      const int l = __ffsll((unsigned long long)who) - 1;
-      insert(b, lane_f(x[e], l), lane_u(i + e, l), top, lane);
-      who &= who - 1;
-      who &= __ballot(in && before(x[e], i + e, b.last, b.last_at));
+    for (int n = 0; n < N; ++n)
+      if (x[n] > v || (x[n] == v && e == N)) v = x[n], e = n;
+    const bool take = in && e < N && before(v, i + e, b.last, b.last_at);
+    uint64_t who = __ballot(take);
+    if (!who) return;
+    if (__popcll(who) >= kMerge) {
+      merge(b, take ? v : -INFINITY, take ? i + e : 0xffffffffu, lane);
+    } else {
+      for (; who; who &= who - 1) {
+        const int l = __ffsll((unsigned long long)who) - 1;
+        insert(b, lane_f(v, l), lane_u(i + e, l));
+      }
     }
+    b.last = lane_f(b.x, top - 1);
+    b.last_at = lane_u(b.at, top - 1);
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+      if (take && n == (int)e) x[n] = __builtin_nanf("");
   }
 }
 
@@ -127,34 +161,97 @@ struct Part {
 
 template <typename T>
 constexpr int kPiece = 16 / sizeof(T);
+constexpr int kTurn = 4;  // pieces of a lane in flight at once
 
+// 16 bytes of a row, at any address of its type: rows of an odd vocabulary begin where they may.
 template <typename T>
-__device__ __forceinline__ void load_piece(float (&x)[kPiece<T>], const T* p) {
-  if constexpr (kPiece<T> == 8) {
-    load_row8(x, p);
-  } else {
-    const f32x4 v = load4(p);
+struct __attribute__((packed, aligned(sizeof(T)))) Raw {
+  uint32_t w[4];
+};
+template <typename T>
+__device__ __forceinline__ Raw<T> load_raw(const T* p) {
+  return *reinterpret_cast<const Raw<T>*>(p);
+}
+__device__ __forceinline__ void values(float (&x)[4], const Raw<float>& r) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = v[e];
+  for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(r.w[e]);
+}
+__device__ __forceinline__ void values(float (&x)[8], const Raw<uint16_t>& r) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    x[2 * e] = __uint_as_float(r.w[e] << 16);
+    x[2 * e + 1] = __uint_as_float(r.w[e] & 0xffff0000u);
   }
 }
+__device__ __forceinline__ void values(float (&x)[8], const Raw<_Float16>& r) {
+  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const f16x2 v = __builtin_bit_cast(f16x2, (uint32_t)r.w[e]);
+    x[2 * e] = static_cast<float>(v[0]);
+    x[2 * e + 1] = static_cast<float>(v[1]);
+  }
+}
+__device__ __forceinline__ void store_raw(float* p, const float (&x)[4]) {
+  Raw<float> r;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) r.w[e] = __float_as_uint(x[e]);
+  *reinterpret_cast<Raw<float>*>(p) = r;
+}
+__device__ __forceinline__ void store_raw(uint16_t* p, const float (&x)[8]) {
+  Raw<uint16_t> r;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) r.w[e] = pack_bf16x2(x[2 * e], x[2 * e + 1]);
+  *reinterpret_cast<Raw<uint16_t>*>(p) = r;
+}
+__device__ __forceinline__ void store_raw(_Float16* p, const float (&x)[8]) {
+  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+  Raw<_Float16> r;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const f16x2 v = {static_cast<_Float16>(x[2 * e]), static_cast<_Float16>(x[2 * e + 1])};
+    r.w[e] = __builtin_bit_cast(uint32_t, v);
+  }
+  *reinterpret_cast<Raw<_Float16>*>(p) = r;
+}
 
-// Where part p of `parts` of a row begins, in pieces from the row's first 16-byte boundary.
-__device__ __forceinline__ int64_t part_begin(int64_t pieces, int p, int parts) { return pieces * p / parts; }
+template <typename T>
+__device__ __forceinline__ const T* row_at(const ScoreArgs& a, int64_t row) {
+  return static_cast<const T*>(a.logits) + row / a.N * a.b + row % a.N * a.n;
+}
 
-}  // namespace
-
-// Merges the waves' lists of `count` places each in LDS: every entry counts those that come before it, and its
-// count is its place.
-__device__ __forceinline__ void place_best(const float* x, const uint32_t* at, int lists, int top, const auto& put_at) {
-  for (int i = threadIdx.x; i < lists * top; i += kThr) {
+// The waves' lists in LDS become one: every entry counts those that come before it, and its count is its
+// place. Empty entries are alike and come in the order that they stand in.
+__device__ __forceinline__ void place_best(const float* x, const uint32_t* at, int top, const auto& put_at) {
+  for (int i = threadIdx.x; i < kWaves * top; i += kThr) {
     const float v = x[i];
     const uint32_t j = at[i];
     int rank = 0;
-    for (int n = 0; n < lists * top; ++n) rank += before(x[n], at[n], v, j) || (at[n] == j && x[n] == v && n < i);
+    for (int n = 0; n < kWaves * top; ++n) rank += before(x[n], at[n], v, j) || (at[n] == j && n < i);
     if (rank < top) put_at(rank, v, j);
   }
 }
+
+// A row's results from its sums and the waves' lists.
+template <typename T, bool ENTROPY, bool TOP>
+__device__ __forceinline__ void finish(const ScoreArgs& a, const ScoreOut& out, int64_t row, const Sums& sum,
+                                       const float* bx, const uint32_t* bi) {
+  const float log = logf(sum.s);
+  if (threadIdx.x == 0) {
+    const int64_t token = a.tokens[row];
+    out.logp[row] = token < 0 ? 0.f : token < a.V ? get(row_at<T>(a, row) + token) - sum.m - log : __builtin_nanf("");
+    if (ENTROPY) out.entropy[row] = log - sum.t / sum.s;
+    if (out.saved) out.saved[2 * row] = sum.m, out.saved[2 * row + 1] = sum.s;
+  }
+  if constexpr (TOP) {
+    place_best(bx, bi, a.top, [&](int rank, float v, uint32_t j) {
+      out.top[row * a.top + rank] = v - sum.m - log;
+      out.place[row * a.top + rank] = j == 0xffffffffu ? -1 : (int64_t)j;
+    });
+  }
+}
+
+}  // namespace
 
 // One part of one row. With parts == 1 it writes the row's results.
 template <typename T, bool ENTROPY, bool TOP>
@@ -167,34 +264,38 @@ __global__ __launch_bounds__(kThr) void k_scores(ScoreArgs a, ScoreOut out, int 
   const int t = threadIdx.x, lane = t & 63, w = wave_of(t);
   const int64_t row = blockIdx.x / parts;
   const int part = blockIdx.x % parts;
-  const T* x = static_cast<const T*>(a.logits) + row / a.N * a.b + row % a.N * a.n;
-  // values before the first boundary, whole pieces, values behind the last
-  const int lead = min((int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (int)sizeof(T), a.V);
-  const int64_t pieces = (a.V - lead) / P;
-  const int tail = lead + (int)pieces * P;
-  const int64_t first = part_begin(pieces, part, parts), end = part_begin(pieces, part + 1, parts);
+  const T* x = row_at<T>(a, row);
+  const int64_t pieces = a.V / P, first = pieces * part / parts, end = pieces * (part + 1) / parts;
   Sums mine = kNothing;
   Best b;
   auto take = [&](auto& v, uint32_t i, bool in) {
     constexpr int N = sizeof(v) / sizeof(v[0]);
-    if (in) add<N, ENTROPY>(mine, v);
-    if constexpr (TOP) offer<N>(b, v, i, in, a.top, lane);
+    const float most = most_of(v);
+    add<N, ENTROPY>(mine, v, most);
+    if constexpr (TOP) offer<N>(b, v, most, i, in, a.top, lane);
   };
-  if (part == 0 && w == 0) {
-    float v[1] = {t < lead ? get(x + t) : -INFINITY};
-    take(v, t, t < lead);
+  // whole waves, whose lanes past the end have nothing: a list belongs to all lanes
+  for (int64_t i = first + 64 * w; i < end; i += kTurn * kThr) {
+    Raw<T> raw[kTurn];
+#pragma unroll
+    for (int n = 0; n < kTurn; ++n) raw[n] = load_raw(x + min(i + n * kThr + lane, end - 1) * P);
+#pragma unroll
+    for (int n = 0; n < kTurn; ++n) {
+      const int64_t p = i + n * kThr + lane;
+      if (p - lane >= end) break;
+      float v[P];
+      values(v, raw[n]);
+      if (p >= end)
+#pragma unroll
+        for (int e = 0; e < P; ++e) v[e] = -INFINITY;
+      take(v, (uint32_t)(p * P), p < end);
+    }
   }
-  // whole waves: a list belongs to all lanes
-  for (int64_t i = first; i < end; i += kThr) {
-    const int64_t p = i + t;
-    const bool in = p < end;
-    float v[P];
-    load_piece<T>(v, x + lead + (in ? p : first) * P);
-    take(v, (uint32_t)(lead + p * P), in);
-  }
-  if (part == parts - 1 && w == kWaves - 1) {
-    float v[1] = {tail + lane < a.V ? get(x + tail + lane) : -INFINITY};
-    take(v, tail + lane, tail + lane < a.V);
+  // values behind the last whole piece
+  if (part == parts - 1 && w == kWaves - 1 && pieces * P < a.V) {
+    const int p = (int)pieces * P + lane;
+    float v[1] = {p < a.V ? get(x + p) : -INFINITY};
+    take(v, p, p < a.V);
   }
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) {
@@ -209,63 +310,53 @@ __global__ __launch_bounds__(kThr) void k_scores(ScoreArgs a, ScoreOut out, int 
   mine = shared[0];
 #pragma unroll
   for (int n = 1; n < kWaves; ++n) join(mine, shared[n]);
-  if (parts > 1) {
-    if (t == 0) sums[blockIdx.x] = {mine.m, mine.s, mine.t, 0.f};
-    if constexpr (TOP) {
-      place_best(bx, bi, kWaves, a.top, [&](int rank, float v, uint32_t j) {
-        best[(size_t)blockIdx.x * a.top + rank] = v;
-        best_at[(size_t)blockIdx.x * a.top + rank] = j;
-      });
-    }
+  if (parts == 1) {
+    finish<T, ENTROPY, TOP>(a, out, row, mine, bx, bi);
     return;
   }
-  const float log = logf(mine.s);
-  if (t == 0) {
-    const int64_t token = a.tokens[row];
-    out.logp[row] = token < 0 ? 0.f : token < a.V ? get(x + token) - mine.m - log : __builtin_nanf("");
-    if (ENTROPY) out.entropy[row] = log - mine.t / mine.s;
-    if (out.saved) out.saved[2 * row] = mine.m, out.saved[2 * row + 1] = mine.s;
-  }
+  if (t == 0) sums[blockIdx.x] = {mine.m, mine.s, mine.t, 0.f};
   if constexpr (TOP) {
-    place_best(bx, bi, kWaves, a.top, [&](int rank, float v, uint32_t j) {
-      out.top[row * a.top + rank] = v - mine.m - log;
-      out.place[row * a.top + rank] = j == 0xffffffffu ? -1 : (int64_t)j;
-    });
+    // the waves' lists as they are: the join puts them in order
+    for (int i = t; i < kWaves * a.top; i += kThr) {
+      best[(size_t)blockIdx.x * kWaves * a.top + i] = bx[i];
+      best_at[(size_t)blockIdx.x * kWaves * a.top + i] = bi[i];
+    }
   }
 }
 
-// The parts of one row, joined.
+// The parts of one row, joined: a wave's list takes a quarter of theirs, 64 entries at once.
 template <typename T, bool ENTROPY, bool TOP>
 __global__ __launch_bounds__(kThr) void k_scores_join(ScoreArgs a, ScoreOut out, int parts, const Part* __restrict__ sums,
                                                       const float* __restrict__ best,
                                                       const uint32_t* __restrict__ best_at) {
-  extern __shared__ char room[];
-  const int t = threadIdx.x;
+  __shared__ float bx[TOP ? kWaves * kMostTop : 1];
+  __shared__ uint32_t bi[TOP ? kWaves * kMostTop : 1];
+  const int t = threadIdx.x, lane = t & 63, w = wave_of(t);
   const int64_t row = blockIdx.x;
+  // every wave has all sums, of at most 64 parts
   Sums mine = kNothing;
-  for (int p = 0; p < parts; ++p) {
-    const Part x = sums[row * parts + p];
-    join(mine, {x.m, x.s, x.t});
+  if (lane < parts) {
+    const Part x = sums[row * parts + lane];
+    mine = {x.m, x.s, x.t};
   }
-  const float log = logf(mine.s);
-  if (t == 0) {
-    const T* x = static_cast<const T*>(a.logits) + row / a.N * a.b + row % a.N * a.n;
-    const int64_t token = a.tokens[row];
-    out.logp[row] = token < 0 ? 0.f : token < a.V ? get(x + token) - mine.m - log : __builtin_nanf("");
-    if (ENTROPY) out.entropy[row] = log - mine.t / mine.s;
-    if (out.saved) out.saved[2 * row] = mine.m, out.saved[2 * row + 1] = mine.s;
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) {
+    const Sums other = {__shfl_xor(mine.m, off, 64), __shfl_xor(mine.s, off, 64), __shfl_xor(mine.t, off, 64)};
+    join(mine, other);
   }
   if constexpr (TOP) {
-    const int count = parts * a.top;
-    float* bx = reinterpret_cast<float*>(room);
-    uint32_t* bi = reinterpret_cast<uint32_t*>(bx + count);
-    for (int i = t; i < count; i += kThr) bx[i] = best[row * count + i], bi[i] = best_at[row * count + i];
+    const int count = parts * kWaves * a.top;
+    Best b;
+    for (int i = 64 * w; i < count; i += kThr) {
+      float v[1] = {-INFINITY};
+      uint32_t j = 0xffffffffu;
+      if (i + lane < count) v[0] = best[row * count + i + lane], j = best_at[row * count + i + lane];
+      offer<1>(b, v, v[0], j, j != 0xffffffffu, a.top, lane);
+    }
+    if (lane < a.top) bx[w * a.top + lane] = b.x, bi[w * a.top + lane] = b.at;
     __syncthreads();
-    place_best(bx, bi, parts, a.top, [&](int rank, float v, uint32_t j) {
-      out.top[row * a.top + rank] = v - mine.m - log;
-      out.place[row * a.top + rank] = j == 0xffffffffu ? -1 : (int64_t)j;
-    });
   }
+  finish<T, ENTROPY, TOP>(a, out, row, mine, bx, bi);
 }
 
 // The gradient of one part of one row.
@@ -273,28 +364,49 @@ template <typename T>
 __global__ __launch_bounds__(kThr) void k_scores_bwd(ScoreArgs a, int parts, const float* __restrict__ saved,
                                                      const float* __restrict__ entropy, const float* __restrict__ dlog,
                                                      const float* __restrict__ dentropy, T* __restrict__ dlogits) {
+  constexpr int P = kPiece<T>;
   const int t = threadIdx.x;
   const int64_t row = blockIdx.x / parts;
   const int part = blockIdx.x % parts;
-  const T* x = static_cast<const T*>(a.logits) + row / a.N * a.b + row % a.N * a.n;
+  const T* x = row_at<T>(a, row);
   T* dx = dlogits + row * a.V;
   const int64_t token = a.tokens[row];
-  const float m = saved[2 * row], s = saved[2 * row + 1], log = logf(s), inv = 1.f / s;
+  const float m = saved[2 * row], s = saved[2 * row + 1], inv = 1.f / s;
   float dl = dlog && token >= 0 ? dlog[row] : 0.f;
   if (token >= a.V) dl *= __builtin_nanf("");
-  const float dh = dentropy ? dentropy[row] : 0.f, base = dentropy ? entropy[row] - log : 0.f;
-  const int from = (int)((int64_t)a.V * part / parts), to = (int)((int64_t)a.V * (part + 1) / parts);
-  for (int v = from + t; v < to; v += kThr) {
-    const float z = get(x + v) - m, p = exp_of(z) * inv;
-    put(dx + v, (v == token ? dl : 0.f) - p * (dl + dh * (fmaxf(z, -1e30f) + base)));
+  // -p (dl + dh (log p + H)), log p + H = z + base
+  const float dh = dentropy ? dentropy[row] : 0.f, base = dentropy ? entropy[row] - logf(s) : 0.f;
+  const float flat = -inv * (dl + dh * base), slope = -inv * dh;
+  auto grad = [&](float v, int64_t i) {
+    const float z = v - m;
+    const float d = exp_of(z) * fmaf(slope, fmaxf(z, -1e30f), flat);  // where p is zero it is
+    return i == token ? d + dl : d;
+  };
+  const int64_t pieces = a.V / P, first = pieces * part / parts, end = pieces * (part + 1) / parts;
+  for (int64_t i = first + t; i < end; i += kTurn * kThr) {
+    Raw<T> raw[kTurn];
+#pragma unroll
+    for (int n = 0; n < kTurn; ++n) raw[n] = load_raw(x + min(i + n * kThr, end - 1) * P);
+#pragma unroll
+    for (int n = 0; n < kTurn; ++n) {
+      const int64_t p = i + n * kThr;
+      if (p >= end) break;
+      float v[P];
+      values(v, raw[n]);
+#pragma unroll
+      for (int e = 0; e < P; ++e) v[e] = grad(v[e], p * P + e);
+      store_raw(dx + p * P, v);
+    }
   }
+  const int64_t tail = pieces * P + t;
+  if (part == parts - 1 && tail < a.V) put(dx + tail, grad(get(x + tail), tail));
 }
 
 namespace {
 int score_parts(const ScoreArgs& a) {
   const int64_t rows = (int64_t)a.B * a.N;
-  // a part has two turns of the block's 16-byte pieces or more
-  const int64_t most = std::max(1, a.V / (kThr * 16));
+  // a part has a turn of the block's pieces or more, and a wave joins 64 parts at most
+  const int64_t most = std::max(1, a.V / (kThr * kTurn * 4));
   return (int)std::clamp<int64_t>((1024 + rows - 1) / rows, 1, std::min<int64_t>(most, 64));
 }
 }  // namespace
@@ -302,7 +414,7 @@ int score_parts(const ScoreArgs& a) {
 size_t score_work_bytes(const ScoreArgs& a) {
   const int parts = score_parts(a);
   if (parts == 1) return 0;
-  return (size_t)a.B * a.N * parts * (sizeof(Part) + 8 * a.top);
+  return (size_t)a.B * a.N * parts * (sizeof(Part) + 8 * kWaves * a.top);
 }
 
 template <typename T>
@@ -311,15 +423,14 @@ void launch_scores(const ScoreArgs& a, const ScoreOut& out, void* work, hipStrea
   const int64_t rows = (int64_t)a.B * a.N;
   Part* sums = static_cast<Part*>(work);
   float* best = reinterpret_cast<float*>(sums + rows * parts);
-  uint32_t* best_at = reinterpret_cast<uint32_t*>(best + rows * parts * a.top);
+  uint32_t* best_at = reinterpret_cast<uint32_t*>(best + rows * parts * kWaves * a.top);
   auto launch = [&](auto kernel, auto second) {
     timed("k_scores", st, [&] {
       hipLaunchKernelGGL(kernel, dim3((unsigned)(rows * parts)), dim3(kThr), 0, st, a, out, parts, sums, best, best_at);
     });
     if (parts > 1)
       timed("k_scores_join", st, [&] {
-        hipLaunchKernelGGL(second, dim3((unsigned)rows), dim3(kThr), (size_t)8 * parts * a.top, st, a, out, parts, sums,
-                           best, best_at);
+        hipLaunchKernelGGL(second, dim3((unsigned)rows), dim3(kThr), 0, st, a, out, parts, sums, best, best_at);
       });
   };
   if (a.top && a.entropy)

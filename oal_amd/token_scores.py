@@ -9,8 +9,8 @@ numbers for each row beside them.
 
 Logits are float32, bfloat16 or float16; sums and results are float32. A logit of -inf is a token
 that cannot be; a row of such logits alone, and one with NaN or +inf, has NaN scores, as log_softmax has. Results repeat bit
-by bit from call to call; few rows are cut into parts by a rule on their number, and a row is read from
-its first 16-byte boundary, so that last bits depend on how many others are in the call and on its address.
+by bit from call to call; few rows are cut into parts by a rule on their number, so that last bits
+depend on how many others are in the call.
 
 Calls are eager: tracers, functorch's transforms and forward-mode derivatives are refused
 (compiled code runs the call between its graphs).
