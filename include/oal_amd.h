@@ -353,12 +353,14 @@ int oal_window_attention_step(const void* q, const void* k, const void* v, void*
  * Operands, head counts and layouts as the gated delta rule's. g f32: strides (the last three of the twelve
  * of q, k, v, g: batch, head, token) of zero where a head has one decay for all its tokens; a g of
  * -inf forgets the state. per_head (backward): dg is [Hv], the sums over batch and tokens, and else
- * [B][Hv][N]. saved (oal_decay_saved_bytes) is the forward's room and what the backward reads.
+ * [B][Hv][N]. saved (oal_decay_saved_bytes) is the forward's room and, with keep, what the backward reads. Rows of a
+ * tensor are less than 2^24 elements apart.
  */
-size_t oal_decay_saved_bytes(int batch, int v_heads, int seq_len);
+size_t oal_decay_saved_bytes(int batch, int v_heads, int seq_len, int keep);
 int oal_decay_forward(const void* q, const void* k, const void* v, const float* g, const int64_t* strides, int batch,
                       int q_heads, int k_heads, int v_heads, int seq_len, int key_dim, int value_dim, int dtype,
-                      float scale, const float* state, void* out, float* final_state, void* saved, void* stream);
+                      float scale, const float* state, void* out, float* final_state, void* saved, int keep,
+                      void* stream);
 size_t oal_decay_workspace_bytes(int batch, int q_heads, int k_heads, int v_heads, int seq_len, int key_dim,
                                  int per_head);
 int oal_decay_backward(const void* q, const void* k, const void* v, const float* g, const int64_t* strides,

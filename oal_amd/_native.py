@@ -88,9 +88,9 @@ _SIGNATURES = {
     "oal_window_attention_backward": ([_vp] * 4 + [_i] * 10 + [_f] + [_vp] * 8, _i),
     "oal_window_attention_step_workspace_bytes": ([_i] * 6, _sz),
     "oal_window_attention_step": ([_vp] * 7 + [_i] * 8 + [_f] + [_vp] * 3, _i),
-    "oal_decay_saved_bytes": ([_i] * 3, _sz),
+    "oal_decay_saved_bytes": ([_i] * 4, _sz),
     "oal_decay_workspace_bytes": ([_i] * 7, _sz),
-    "oal_decay_forward": ([_vp] * 5 + [_i] * 8 + [_f] + [_vp] * 5, _i),
+    "oal_decay_forward": ([_vp] * 5 + [_i] * 8 + [_f] + [_vp] * 4 + [_i, _vp], _i),
     "oal_decay_backward": ([_vp] * 5 + [_i] * 9 + [_f] + [_vp] * 10, _i),
     "oal_decay_step": ([_vp] * 5 + [_i] * 8 + [_f] + [_vp] * 3, _i),
     "oal_norm_rotary_heads": ([_vp] * 6 + [_i] * 2 + [_vp] * 2 + [_i] * 3 + [_vp] + [_i] * 6 + [_f] + [_vp] * 4, _i),
@@ -898,14 +898,15 @@ def _gate_strides(g: torch.Tensor) -> tuple[int, int, int]:
     return (0, g.stride(0), 0) if g.ndim == 1 else g.stride()
 
 
-def decay_forward(q, k, v, g, state, *, scale: float):
+def decay_forward(q, k, v, g, state, *, scale: float, keep: bool):
     """q, k [B, heads, N, D], v [B, Hv, N, DV], D and DV multiples of 8, rows as of :func:`row_tensor`; g float32 [Hv] or
-    [B, Hv, N], state contiguous float32 [B, Hv, D, DV] or None. Returns (out, final_state, saved)."""
+    [B, Hv, N], state contiguous float32 [B, Hv, D, DV] or None. Returns (out, final_state, saved); saved serves
+    the backward if kept."""
     lib = load_library()
     b, hq, n, d = q.shape
     hk, hv, dv, dev = k.shape[1], v.shape[1], v.shape[3], q.device
     with _scope(dev, "oal_amd::decay_forward"):
-        nbytes = lib.oal_decay_saved_bytes(b, hv, n)
+        nbytes = lib.oal_decay_saved_bytes(b, hv, n, keep)
         if nbytes == 0:
             _check(1, lib, "oal_decay_saved_bytes")
         out = q.new_empty((b, max(hq, hv), n, dv))
@@ -914,7 +915,7 @@ def decay_forward(q, k, v, g, state, *, scale: float):
         rc = lib.oal_decay_forward(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(),
             _Strides4(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *_gate_strides(g)), b, hq, hk, hv, n, d, dv,
-            _DTYPES[q.dtype], scale, _ptr(state), out.data_ptr(), final.data_ptr(), saved.data_ptr(), _stream(dev))
+            _DTYPES[q.dtype], scale, _ptr(state), out.data_ptr(), final.data_ptr(), saved.data_ptr(), keep, _stream(dev))
         _check(rc, lib, "oal_decay_forward")
     return out, final, saved
 

@@ -9,7 +9,9 @@
 // and back, dS' the gradient of the state after the chunk:
 //   dS = e^(G_63) dS' + scale (e^G Q)^T dO
 //   dQ = scale (e^G dO S^T + (exp(G_i - G_j) dO_i.v_j)_(j <= i) K), dK and dV alike from dS'.
-// What makes the state and the decays' gradients is exact to fp32 whatever the tensors'
+// A block walks a segment of chunks with the state in its accumulators; where there are too few
+// units (batch and state heads) for the GPU, sequences are cut into segments, whose sums and a scan over them give the
+// states that they start from. What makes the state and the decays' gradients is exact to fp32 whatever the tensors'
 // type (oal_tile.hpp): a state is a sum over all tokens before it and is handed on in fp32.
 //
 // Decays enter as differences of sums, held in two floats (48 bits): a token that
@@ -37,70 +39,224 @@ constexpr double kLeast = -1e4;
 constexpr float kNothingKept = -104.f;
 
 // Of a chunk's tokens: log2 of the decay up to and with the token, in two parts; the decay since
-// the chunk's start and until its end. end: the chunk's decay, in two parts.
+// the chunk's start and until its end, and since and until those of its tile of 16 tokens. end: the chunk's decay in two
+// parts, and its log2.
 struct alignas(16) Decays {
-  float hi[64], lo[64], since[64], until[64], end[4];
+  float hi[64], lo[64], since[64], until[64], head[64], tail[64], end[2];
+  double log_end;
 };
-constexpr int kDecays = sizeof(Decays) / sizeof(float);
+constexpr int kSlots = 4;  // chunks whose decays a block forms at once, a wave each
 
 __device__ __forceinline__ f32x4 four(const float* p) { return *reinterpret_cast<const f32x4*>(p); }
-// Decays from token (hi, lo) to tokens r .. r + 3, and from those to it.
-__device__ __forceinline__ f32x4 decay_to(const Decays& s, int r, float hi, float lo) {
-  const f32x4 h = four(s.hi + r), l = four(s.lo + r);
+// The decays of a tile: from tokens r .. r + 3 to token (hi, lo), or with TO from it to them. Between tiles they
+// are products of the tokens' own and one between the tiles' borders, an exponential where there would be four.
+template <bool TO>
+__device__ __forceinline__ f32x4 decays(const Decays& s, int r, int tile, bool same, float hi, float lo) {
   f32x4 y;
+  if (same) {
+    const f32x4 h = four(s.hi + r), l = four(s.lo + r);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) y[i] = __builtin_amdgcn_exp2f((h[i] - hi) + (l[i] - lo));
+    for (int i = 0; i < 4; ++i)
+      y[i] = __builtin_amdgcn_exp2f(TO ? (h[i] - hi) + (l[i] - lo) : (hi - h[i]) + (lo - l[i]));
+  } else if constexpr (TO) {
+    y = four(s.head + r) * __builtin_amdgcn_exp2f((s.hi[tile - 1] - hi) + (s.lo[tile - 1] - lo));
+  } else {
+    y = four(s.tail + r) * __builtin_amdgcn_exp2f((hi - s.hi[tile + 15]) + (lo - s.lo[tile + 15]));
+  }
   return y;
 }
-__device__ __forceinline__ f32x4 decay_from(const Decays& s, int r, float hi, float lo) {
-  const f32x4 h = four(s.hi + r), l = four(s.lo + r);
-  f32x4 y;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) y[i] = __builtin_amdgcn_exp2f((hi - h[i]) + (lo - l[i]));
-  return y;
+// A number's parts: it is their sum to 48 bits.
+__device__ __forceinline__ void in_two(double x, float (&y)[2]) {
+  y[0] = (float)x;
+  y[1] = (float)(x - (double)y[0]);
 }
-__device__ __forceinline__ void copy_decays(Decays& s, const Decays& src, int t) {
-  if (t < kDecays / 4) reinterpret_cast<float4*>(&s)[t] = reinterpret_cast<const float4*>(&src)[t];
-}
+// y = e x + d, e in two parts: slow decays multiply for many chunks.
+__device__ __forceinline__ float carry(const float (&e)[2], float x, float d) { return fmaf(e[0], x, fmaf(e[1], x, d)); }
 
 __device__ __forceinline__ float gate_at(const DecayArgs& a, int b, int h, int tok) {
   return static_cast<const float*>(a.g.p)[b * a.g.b + h * a.g.h + tok * a.g.n];
 }
 
-// The first wave of the block; tokens past N decay nothing.
-__device__ __forceinline__ void form_decays(Decays& s, const DecayArgs& a, int b, int h, int tok0, int t) {
-  if (t >= 64) return;
-  const int tok = tok0 + t;
-  double x = 0;
-  if (tok < a.N) {
-    x = gate_at(a, b, h, tok);
-    x = (x < kLeast ? kLeast : x) * 1.4426950408889634;
-  }
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const double y = __shfl_up(x, off, 64);
-    if (t >= off) x += y;
-  }
-  const double end = __shfl(x, 63, 64);
-  const float hi = (float)x, lo = (float)(x - (double)hi);
-  s.hi[t] = hi;
-  s.lo[t] = lo;
-  s.since[t] = __builtin_amdgcn_exp2f(hi + lo);
-  s.until[t] = __builtin_amdgcn_exp2f((float)(end - x));
-  // slow decays stay for many chunks: their chunks' factors multiply
-  const double whole = exp2(end);
-  const float first = (float)whole;
-  if (t < 4) s.end[t] = t == 0 ? first : t == 1 ? (float)(whole - (double)first) : 0.f;
+// A wave's running sums, the lane's own value with it: within rows of 16 lanes, then from rows to the rows behind.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double from_lanes(double x) {
+  const uint64_t v = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (uint32_t)v, CTRL, ROWS, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (uint32_t)(v >> 32), CTRL, ROWS, 0xf, false);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
+__device__ __forceinline__ double running_sum(double x) {
+  x += from_lanes<0x111, 0xf>(x);  // row_shr:1, 2, 4, 8
+  x += from_lanes<0x112, 0xf>(x);
+  x += from_lanes<0x114, 0xf>(x);
+  x += from_lanes<0x118, 0xf>(x);
+  x += from_lanes<0x142, 0xa>(x);  // row_bcast:15 into rows 1 and 3
+  x += from_lanes<0x143, 0xc>(x);  // row_bcast:31 into rows 2 and 3
+  return x;
+}
+__device__ __forceinline__ double lane_of(double x, int lane) {
+  const uint64_t v = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)v, lane), hi = __builtin_amdgcn_readlane((uint32_t)(v >> 32), lane);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
+// A wave: the decays of 64 tokens with log-decays gate.
+__device__ __forceinline__ void form_decays(Decays& s, float gate, int lane) {
+  const double x = running_sum((gate < kLeast ? kLeast : (double)gate) * 1.4426950408889634);
+  const double end = lane_of(x, 63);
+  float y[2];
+  in_two(x, y);
+  s.hi[lane] = y[0];
+  s.lo[lane] = y[1];
+  s.since[lane] = __builtin_amdgcn_exp2f(y[0] + y[1]);
+  s.until[lane] = __builtin_amdgcn_exp2f((float)(end - x));
+  // the last tokens of the tile before and of the own one
+  const double b0 = lane_of(x, 15), b1 = lane_of(x, 31), b2 = lane_of(x, 47);
+  const double before = lane < 16 ? 0.0 : lane < 32 ? b0 : lane < 48 ? b1 : b2;
+  const double last = lane < 16 ? b0 : lane < 32 ? b1 : lane < 48 ? b2 : end;
+  s.head[lane] = __builtin_amdgcn_exp2f((float)(x - before));
+  s.tail[lane] = __builtin_amdgcn_exp2f((float)(last - x));
+  if (lane == 0) {
+    in_two(exp2(end), s.end);
+    s.log_end = end;
+  }
+}
+
+// A block's part of the walk: unit u = (b, h), chunks [first, last) of its segment, one after another or back.
+struct Course {
+  int u, b, h, seg, first, last;
+  __device__ __forceinline__ Course(const DecayArgs& a, const DecaySegments& sg, int id) {
+    seg = id % sg.count;
+    u = id / sg.count;
+    b = u / a.Hv;
+    h = u % a.Hv;
+    first = seg * sg.len;
+    last = min(first + sg.len, a.NC);
+  }
+};
+// Every kSlots chunks each wave forms the decays of one of the chunks that follow; their gates are on their way
+// since the last time. Tokens past N decay nothing.
+struct Gates {
+  float next;
+  __device__ __forceinline__ void fetch(const DecayArgs& a, const Course& x, int n, int step, int w, int lane) {
+    const int ch = (step > 0 ? x.first : x.last - 1) + step * (n + w), tok = 64 * ch + lane;
+    next = ch >= x.first && ch < x.last && tok < a.N ? gate_at(a, x.b, x.h, tok) : 0.f;
+  }
+  __device__ __forceinline__ void form(Decays (&dec)[kSlots], const DecayArgs& a, const Course& x, int n, int step, int w,
+                                       int lane) {
+    if (n % kSlots) return;
+    if (n + w < x.last - x.first) form_decays(dec[w], next, lane);
+    fetch(a, x, n + kSlots, step, w, lane);
+  }
+};
 
 template <typename T>
 __device__ __forceinline__ const T* rows_of(const Strided& s, int b, int h, int tok0) {
   return static_cast<const T*>(s.p) + b * s.b + h * s.h + (int64_t)tok0 * s.n;
 }
 
-// The column x of a tile of 64 rows, read by rows 32 s + 8 g + j, each row scaled: operand exact to fp32.
+// Element `at` from a base that the block shares: 32 bits of offset (rows are less than 2^24 elements apart).
+template <typename T>
+__device__ __forceinline__ const T* shared_at(const T* base, uint32_t at) {
+  return reinterpret_cast<const T*>(reinterpret_cast<const char*>(base) + at * (uint32_t)sizeof(T));
+}
+template <typename T>
+__device__ __forceinline__ T* shared_at(T* base, uint32_t at) {
+  return reinterpret_cast<T*>(reinterpret_cast<char*>(base) + at * (uint32_t)sizeof(T));
+}
+
+// 64 rows of D values on their way to an LDS tile, by 256 threads. Rows at and past `live` and columns from D, which
+// only the last chunk and narrow heads have, are read from places that there are, and stored as zeros.
+template <int NP, typename T>
+struct Coming {
+  uint4 raw[2];
+  float x[2][8];
+  __device__ __forceinline__ void fetch(const T* base, uint32_t stride, int D, int live, int t) {
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      const int r = min((t >> 3) + 32 * n, live - 1), c = 8 * (t & 7);
+      const T* p = shared_at(base, __umul24(r, stride) + (c < D ? c : 0));
+      if constexpr (NP == 1)
+        raw[n] = *reinterpret_cast<const uint4*>(p);
+      else
+        load_row8(x[n], p);
+    }
+  }
+  __device__ __forceinline__ void store(Tile<NP>& s, int D, int live, int t) const {
+    const bool edge = live < 64 || D < 64;
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      const int r = (t >> 3) + 32 * n, c = 8 * (t & 7);
+      const bool in = !edge || (r < live && c < D);
+      __bf16* p = s.x + tile_at(r, c);
+      Frag<NP> f;
+      if constexpr (NP == 1)
+        f.p[0] = __builtin_bit_cast(bf16x8, raw[n]);
+      else
+        f = split<NP>(x[n]);
+      if (edge && !in) f = Frag<NP>{};
+#pragma unroll
+      for (int e = 0; e < NP; ++e) *reinterpret_cast<bf16x8*>(p + e * kTileElems) = f.p[e];
+    }
+  }
+};
+
+// A token's row as operands of sums over its D values: 32 k + 8 g + j, zero from D on. Columns of a product
+// that belong to rows past the last are not used, so that any row serves for them.
+template <int NP, typename T>
+__device__ __forceinline__ void own_row(Frag<NP> (&f)[2], const T* base, uint32_t stride, int D, int row, int g) {
+  const uint32_t at = __umul24(row, stride) + 8 * g;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const T* p = shared_at(base, at + 32 * k);
+    if (D == 64)
+      f[k] = global_frag<NP>(p, true);
+    else
+      f[k] = global_frag<NP>(p, 32 * k + 8 * g < D);
+  }
+}
+// Row `row` of a tile as the accumulators of a product with it have it: values 16 m + 4 g + i.
 template <int NP>
-__device__ __forceinline__ Frag<3> scaled_col(const Tile<NP>& s, int c0, int half, int lane, const float* by, float scale) {
+__device__ __forceinline__ f32x4 own_values(const Tile<NP>& s, int row, int m, int lane) {
+  f32x4 x = {};
+#pragma unroll
+  for (int e = NP - 1; e >= 0; --e)
+    x += __builtin_convertvector(
+        *reinterpret_cast<const bf16x4*>(s.x + e * kTileElems + tile_at(row, 16 * m + 4 * (lane >> 4))), f32x4);
+  return x;
+}
+
+// An accumulator tile in parts: two of them are the operand of a sum over their 32 rows (perm order).
+template <int N>
+struct Half {
+  bf16x4 p[N];
+};
+template <int N>
+__device__ __forceinline__ Half<N> half_of(const f32x4& x) {
+  Half<N> h;
+  float v[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    h.p[e] = __builtin_bit_cast(bf16x4, pack4(v));
+    if (e + 1 < N) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] -= static_cast<float>(h.p[e][i]);
+    }
+  }
+  return h;
+}
+template <int N>
+__device__ __forceinline__ Frag<N> both(const Half<N>& a, const Half<N>& b) {
+  Frag<N> f;
+#pragma unroll
+  for (int e = 0; e < N; ++e) f.p[e] = __builtin_shufflevector(a.p[e], b.p[e], 0, 1, 2, 3, 4, 5, 6, 7);
+  return f;
+}
+
+// Columns c0 .. of a tile of 64 rows, read by rows 32 s + 8 g + j, each row scaled: an operand of UP parts, exact to fp32
+// if three.
+template <int UP, int NP>
+__device__ __forceinline__ Frag<UP> scaled_col(const Tile<NP>& s, int c0, int half, int lane, const float* by, float scale) {
   const Frag<NP> f = col_frag(s, c0, half, lane);
   const int g = lane >> 4;
   const f32x4 b0 = scale * four(by + 32 * half + 8 * g), b1 = scale * four(by + 32 * half + 8 * g + 4);
@@ -112,363 +268,506 @@ __device__ __forceinline__ Frag<3> scaled_col(const Tile<NP>& s, int c0, int hal
     for (int x = NP - 1; x >= 0; --x) v[j] += static_cast<float>(f.p[x][j]);
     v[j] *= j < 4 ? b0[j] : b1[j - 4];
   }
-  return split<3>(v);
+  return split<UP>(v);
 }
+
+// Nothing moves over it: operands of later products, loaded early, would not fit the registers.
+__device__ __forceinline__ void phase() { __builtin_amdgcn_sched_barrier(0); }
+
+// What follows from it is computed here: kept from before a loop, all the addresses in LDS would not fit either.
+__device__ __forceinline__ int here(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
+// A state in accumulators, four tiles of a wave's 16 columns: S[m][i] is row 16 m + 4 g + i of column 16 w + c.
+typedef f32x4 State[4];
+// x += A^T (by B) over the rows of two tiles, A's columns the rows of x and B's 16 w .. the wave's columns.
+template <int UP, int NP>
+__device__ __forceinline__ void add_outer(State& x, const Tile<NP>& A, const Tile<NP>& B, const float* by, float scale,
+                                          int w, int lane) {
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    phase();
+    const Frag<UP> b = scaled_col<UP>(B, 16 * w, s, lane, by, scale);
+#pragma unroll
+    for (int m = 0; m < 4; ++m) x[m] = mma(col_frag(A, 16 * m, s, lane), b, x[m]);
+  }
+  phase();
+}
+// Over a few chunks one part of their decays does (2^-25 each); over many two.
+__device__ __forceinline__ void decay_state(State& x, const float (&end)[2], const DecaySegments& sg) {
+#pragma unroll
+  for (int m = 0; m < 4; ++m) x[m] *= end[0] + (sg.len > 8 ? 0.f : end[1]);
+  if (sg.len > 8) {
+    const float more = end[0] == 0.f ? 0.f : end[1] / end[0];
+#pragma unroll
+    for (int m = 0; m < 4; ++m)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[m][i] = fmaf(more, x[m][i], x[m][i]);
+  }
+}
+// The state's columns as rows of a tile: four consecutive rows of the state at once.
+template <int NP>
+__device__ __forceinline__ void put_state(Tile<NP>& s, const State& x, int w, int lane) {
+#pragma unroll
+  for (int m = 0; m < 4; ++m) {
+    const Half<NP> h = half_of<NP>(x[m]);
+#pragma unroll
+    for (int e = 0; e < NP; ++e)
+      *reinterpret_cast<bf16x4*>(s.x + e * kTileElems + tile_at(16 * w + (lane & 15), 16 * m + 4 * (lane >> 4))) = h.p[e];
+  }
+}
+// A state [rows][cols] in memory: TURNED where the accumulators' rows are its columns. Past its edges zero.
+template <bool TURNED>
+__device__ __forceinline__ void load_state(State& x, const float* p, int rows, int cols, int w, int lane) {
+  const int own = 16 * w + (lane & 15);
+#pragma unroll
+  for (int m = 0; m < 4; ++m) {
+    const int r = 16 * m + 4 * (lane >> 4);
+    x[m] = f32x4{};
+    if (!p) continue;
+    if constexpr (TURNED) {
+      if (own < rows && r < cols) x[m] = load4(p + own * cols + r);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (r + i < rows && own < cols) x[m][i] = p[(r + i) * cols + own];
+    }
+  }
+}
+template <bool TURNED>
+__device__ __forceinline__ void store_state(const State& x, float* p, int rows, int cols, int w, int lane) {
+  const int own = 16 * w + (lane & 15);
+#pragma unroll
+  for (int m = 0; m < 4; ++m) {
+    const int r = 16 * m + 4 * (lane >> 4);
+    if constexpr (TURNED) {
+      if (own < rows && r < cols) store4(p + own * cols + r, x[m]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (r + i < rows && own < cols) p[(r + i) * cols + own] = x[m][i];
+    }
+  }
+}
+// What a segment starts from: the states of the scan, or the call's own where there is but one segment.
+struct From {
+  const float* p;
+  int rows, cols;
+  __device__ __forceinline__ const float* of(const DecaySegments& sg, const Course& x) const {
+    return p ? p + ((size_t)x.u * sg.count + x.seg) * rows * cols : nullptr;
+  }
+};
 
 }  // namespace
 
-// What a chunk adds to the state, D = K^T (e^(G_63 - G) V); its decays. A wave per 16 columns.
-template <typename T>
-__global__ __launch_bounds__(kThr) void k_decay_sum(DecayArgs a, Decays* __restrict__ G, float* __restrict__ D) {
+// What a segment adds to the state, or (BACK) what its outputs ask of the state before it, over a state's
+// output heads: k, v or q, dO of its chunks, one after another; and its decay.
+template <typename T, bool BACK>
+__global__ __launch_bounds__(kThr) void k_decay_sum(DecayArgs a, DecaySegments sg, const T* __restrict__ dout,
+                                                    float* __restrict__ G, float* __restrict__ D) {
   constexpr int NP = kPartsOf<T>;
-  __shared__ Tile<NP> K, V;
-  __shared__ Decays dec;
-  const int t = threadIdx.x, lane = t & 63, w = wave_of(t), g = lane >> 4, c = lane & 15;
-  const int ch = blockIdx.x % a.NC, u = blockIdx.x / a.NC, b = u / a.Hv, h = u % a.Hv;
-  const int tok0 = 64 * ch, live = min(64, a.N - tok0);
-  const size_t at = ((size_t)u * a.NC + ch) * kTile2;
-  Incoming<NP, T> ki, vi;
-  ki.fetch(rows_of<T>(a.k, b, h / (a.Hv / a.Hk), tok0), a.k.n, a.D, live, t);
-  vi.fetch(rows_of<T>(a.v, b, h, tok0), a.v.n, a.DV, live, t);
-  form_decays(dec, a, b, h, tok0, t);
-  ki.store(K, t);
-  vi.store(V, t);
-  lds_sync();
-  copy_decays(G[(size_t)u * a.NC + ch], dec, t);
-  const Frag<3> v0 = scaled_col(V, 16 * w, 0, lane, dec.until, 1.f), v1 = scaled_col(V, 16 * w, 1, lane, dec.until, 1.f);
-#pragma unroll
-  for (int m = 0; m < 4; ++m) {
-    f32x4 x = mma(col_frag(K, 16 * m, 0, lane), v0, f32x4{});
-    x = mma(col_frag(K, 16 * m, 1, lane), v1, x);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) D[at + (16 * m + 4 * g + i) * 64 + 16 * w + c] = x[i];
+  __shared__ Tile<NP> A, B;
+  __shared__ Decays dec[kSlots];
+  const int t = threadIdx.x, lane = t & 63, w = wave_of(t);
+  const Course x(a, sg, blockIdx.x);
+  const int each = BACK ? a.H / a.Hv : 1, o0 = x.h * each, count = (x.last - x.first) * each;
+  Coming<NP, T> ai, bi;
+  auto fetch = [&](int i) {
+    const int n = i / each, o = o0 + i % each, ch = BACK ? x.last - 1 - n : x.first + n;
+    const int tok0 = 64 * ch, live = min(64, a.N - tok0);
+    if constexpr (BACK) {
+      ai.fetch(rows_of<T>(a.q, x.b, o / (a.H / a.Hq), tok0), a.q.n, a.D, live, t);
+      bi.fetch(dout + (((size_t)x.b * a.H + o) * a.N + tok0) * a.DV, a.DV, a.DV, live, t);
+    } else {
+      ai.fetch(rows_of<T>(a.k, x.b, x.h / (a.Hv / a.Hk), tok0), a.k.n, a.D, live, t);
+      bi.fetch(rows_of<T>(a.v, x.b, x.h, tok0), a.v.n, a.DV, live, t);
+    }
+  };
+  State s = {};
+  double log = 0;
+  Gates gates;
+  gates.fetch(a, x, 0, BACK ? -1 : 1, w, lane);
+  fetch(0);
+  for (int i = 0; i < count; ++i) {
+    const int n = i / each, ch = BACK ? x.last - 1 - n : x.first + n;
+    if (i) lds_sync();
+    if (i % each == 0) gates.form(dec, a, x, n, BACK ? -1 : 1, w, lane);
+    const int live = min(64, a.N - 64 * ch);
+    ai.store(A, a.D, live, t);
+    bi.store(B, a.DV, live, t);
+    lds_sync();
+    if (i + 1 < count) fetch(i + 1);
+    const Decays& d = dec[n % kSlots];
+    if (i % each == 0) {
+      decay_state(s, d.end, sg);
+      log += d.log_end;
+    }
+    add_outer<3>(s, A, B, BACK ? d.since : d.until, BACK ? a.scale : 1.f, w, lane);
   }
+  store_state<false>(s, D + (size_t)blockIdx.x * kTile2, 64, 64, w, lane);
+  float y[2];
+  in_two(exp2(log), y);
+  if (t == 0) G[2 * blockIdx.x] = y[0], G[2 * blockIdx.x + 1] = y[1];
 }
 
-// S' = e S + D over the chunks, or back over them; what a chunk adds is replaced by the state
-// that it starts from (back: whose gradient it takes). Four values per thread.
+// S' = e S + D over the segments, or back over them; what a segment adds is replaced by the state
+// that it starts from (back: whose gradient it takes). A value per thread, the next ones on their way.
 struct Scan {
-  const Decays* G;
-  float* S;           // [U][NC][64][64]
+  const float* G;
+  float* S;           // [U][segments][64][64]
   const float* init;  // [U][rows][cols] (null: zero)
-  float* end;         // the same (null: not wanted)
-  int NC, rows, cols;
+  float* end;         // the same: the state after the last (null: not wanted)
+  int count, rows, cols;
   bool back;
 };
+constexpr int kAhead = 8;
 __global__ __launch_bounds__(kThr) void k_decay_scan(Scan a) {
-  const int x = blockIdx.x * kThr + threadIdx.x, u = x >> 10, i = 4 * (x & 1023), row = i >> 6, col = i & 63;
+  const int x = blockIdx.x * kThr + threadIdx.x, u = x / kTile2, i = x % kTile2, row = i / 64, col = i % 64;
+  float s = 0.f;
   const bool held = row < a.rows && col < a.cols;
   const size_t slot = ((size_t)u * a.rows + row) * a.cols + col;
-  f32x4 s = {};
-  if (a.init && held) s = load4(a.init + slot);
-  for (int n = 0; n < a.NC; ++n) {
-    const size_t at = (size_t)u * a.NC + (a.back ? a.NC - 1 - n : n);
-    float* p = a.S + at * kTile2 + i;
-    const f32x4 d = load4(p);
-    const float hi = a.G[at].end[0], lo = a.G[at].end[1];
-    store4(p, s);
+  if (a.init && held) s = a.init[slot];
+  for (int n0 = 0; n0 < a.count; n0 += kAhead) {
+    float d[kAhead], e[kAhead][2];
+    auto at = [&](int n) { return (size_t)u * a.count + (a.back ? a.count - 1 - n : n); };
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s[e] = fmaf(hi, s[e], fmaf(lo, s[e], d[e]));
-  }
-  if (a.end && held) store4(a.end + slot, s);
-}
-
-// The outputs of one chunk for `each` output heads of a state head, transposed: a wave's 16 queries
-// are the columns, so the scores are an operand of the product with V as they are. 16-bit tensors take
-// two parts per value, twice their precision: one rounding is the output's own.
-template <typename T>
-__global__ __launch_bounds__(kThr) void k_decay_out(DecayArgs a, int each, const Decays* __restrict__ G,
-                                                    const float* __restrict__ Sin, T* __restrict__ out) {
-  constexpr int NP = kPartsOf<T>, NO = NP == 3 ? 3 : 2;
-  __shared__ Tile<NP> K, V;
-  __shared__ Tile<NO> S;
-  __shared__ Decays dec;
-  const int t = threadIdx.x, lane = t & 63, w = wave_of(t), g = lane >> 4, c = lane & 15;
-  const int rep = a.H / a.Hv, parts = (rep + each - 1) / each;
-  const int part = blockIdx.x % parts, ch = blockIdx.x / parts % a.NC, u = blockIdx.x / parts / a.NC;
-  const int b = u / a.Hv, h = u % a.Hv;
-  const int tok0 = 64 * ch, live = min(64, a.N - tok0), own = 16 * w + c;
-  Incoming<NP, T> ki, vi;
-  Incoming<NO, float> si;
-  ki.fetch(rows_of<T>(a.k, b, h / (a.Hv / a.Hk), tok0), a.k.n, a.D, live, t);
-  vi.fetch(rows_of<T>(a.v, b, h, tok0), a.v.n, a.DV, live, t);
-  si.fetch(Sin + ((size_t)u * a.NC + ch) * kTile2, 64, 64, 64, t);
-  copy_decays(dec, G[(size_t)u * a.NC + ch], t);
-  ki.store(K, t);
-  vi.store(V, t);
-  si.store(S, t);
-  lds_sync();
-  const float since = a.scale * dec.since[own], hi = dec.hi[own], lo = dec.lo[own];
-  for (int o = h * rep + part * each; o < min(h * rep + (part + 1) * each, (h + 1) * rep); ++o) {
-    const T* q = rows_of<T>(a.q, b, o / (a.H / a.Hq), tok0) + own * a.q.n;
-    Frag<NP> qf[2];
-#pragma unroll
-    for (int s = 0; s < 2; ++s) qf[s] = global_frag<NP>(q + 32 * s + 8 * g, own < live && 32 * s + 8 * g < a.D);
-    f32x4 acc[4] = {}, p[4] = {};
-#pragma unroll
-    for (int m = 0; m < 4; ++m) {
-#pragma unroll
-      for (int s = 0; s < 2; ++s) acc[m] = mma(col_frag<NO>(S, 16 * m, s, lane), qf[s], acc[m]);
-      acc[m] *= since;
-      if (m > w) continue;
-#pragma unroll
-      for (int s = 0; s < 2; ++s) p[m] = mma(row_frag(K, 16 * m, s, lane), qf[s], p[m]);
-      const f32x4 y = p[m] * a.scale * decay_from(dec, 16 * m + 4 * g, hi, lo);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) p[m][i] = 16 * m + 4 * g + i <= own ? y[i] : 0.f;
+    for (int n = 0; n < kAhead; ++n) {
+      const size_t k = at(min(n0 + n, a.count - 1));
+      d[n] = a.S[k * kTile2 + i];
+      e[n][0] = a.G[2 * k], e[n][1] = a.G[2 * k + 1];
     }
-    const Frag<NO> p0 = acc_frag<NO>(p[0], p[1]), p1 = acc_frag<NO>(p[2], p[3]);
-    T* dst = out + (((size_t)b * a.H + o) * a.N + tok0 + own) * a.DV;
 #pragma unroll
-    for (int m = 0; m < 4; ++m) {
-      acc[m] = mma(col_frag_perm(V, 16 * m, 0, lane), p0, acc[m]);
-      if (w >= 2) acc[m] = mma(col_frag_perm(V, 16 * m, 1, lane), p1, acc[m]);
-      if (own < live && 16 * m + 4 * g < a.DV) store4(dst + 16 * m + 4 * g, acc[m]);
+    for (int n = 0; n < kAhead; ++n) {
+      if (n0 + n >= a.count) break;
+      a.S[at(n0 + n) * kTile2 + i] = s;
+      s = carry(e[n], s, d[n]);
     }
   }
+  if (a.end && held) a.end[slot] = s;
 }
 
-// What a chunk's outputs ask of the state before it, F = scale (e^G Q)^T dO, over a state's output heads.
-template <typename T>
-__global__ __launch_bounds__(kThr) void k_decay_bwd_sum(DecayArgs a, const T* __restrict__ dout,
-                                                        const Decays* __restrict__ G, float* __restrict__ F) {
+// The outputs of one segment for `each` output heads of a state head, chunk by chunk, with the state in
+// accumulators and, as bf16 parts, in LDS. Outputs are transposed: a wave's 16 queries
+// are the columns, so the scores are an operand of the product with V as they are. bf16 tensors take
+// scores and states as they round to bf16, as the output itself rounds; fp16 tensors take them in two parts.
+// UP: parts of what the state takes on, three where it goes on to the caller or (states: kept before every
+// chunk) to the backward, two where no further than the segment's own outputs.
+template <typename T, int UP>
+__global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 4 : 2) void k_decay_out(DecayArgs a, DecaySegments sg, int each,
+                                                                              From from, T* __restrict__ out,
+                                                                              float* __restrict__ final_state,
+                                                                              float* __restrict__ states) {
   constexpr int NP = kPartsOf<T>;
-  __shared__ Tile<NP> Q, O;
-  __shared__ Decays dec;
-  const int t = threadIdx.x, lane = t & 63, w = wave_of(t), g = lane >> 4, c = lane & 15;
-  const int ch = blockIdx.x % a.NC, u = blockIdx.x / a.NC, b = u / a.Hv, h = u % a.Hv;
-  const int tok0 = 64 * ch, live = min(64, a.N - tok0);
-  const int each = a.H / a.Hv, o1 = (h + 1) * each;
-  Incoming<NP, T> qi, oi;
-  auto fetch = [&](int o) {
-    qi.fetch(rows_of<T>(a.q, b, o / (a.H / a.Hq), tok0), a.q.n, a.D, live, t);
-    oi.fetch(dout + (((size_t)b * a.H + o) * a.N + tok0) * a.DV, a.DV, a.DV, live, t);
+  __shared__ Tile<NP> K, V;
+  __shared__ Tile<NP> S;  // rows: values
+  __shared__ Decays dec[kSlots];
+  int t = threadIdx.x, lane = t & 63;
+  const int w = wave_of(t), g = lane >> 4, c = lane & 15, own = 16 * w + c;
+  const int rep = a.H / a.Hv, parts = (rep + each - 1) / each, part = blockIdx.x % parts;
+  const Course x(a, sg, blockIdx.x / parts);
+  const int o0 = x.h * rep + part * each, o1 = min(o0 + each, (x.h + 1) * rep);
+  State s;
+  load_state<false>(s, from.of(sg, x), from.rows, from.cols, w, lane);
+  Coming<NP, T> ki, vi;
+  Frag<NP> next[2];
+  auto fetch = [&](int ch) {
+    const int tok0 = 64 * ch, live = min(64, a.N - tok0);
+    ki.fetch(rows_of<T>(a.k, x.b, x.h / (a.Hv / a.Hk), tok0), a.k.n, a.D, live, t);
+    vi.fetch(rows_of<T>(a.v, x.b, x.h, tok0), a.v.n, a.DV, live, t);
   };
-  fetch(h * each);
-  copy_decays(dec, G[(size_t)u * a.NC + ch], t);
-  f32x4 f[4] = {};
-  for (int o = h * each; o < o1; ++o) {
-    if (o > h * each) lds_sync();
-    qi.store(Q, t);
-    oi.store(O, t);
+  auto fetch_q = [&](int ch, int o) {
+    own_row(next, rows_of<T>(a.q, x.b, o / (a.H / a.Hq), 64 * ch), a.q.n, a.D, min(own, a.N - 64 * ch - 1), g);
+  };
+  Gates gates;
+  gates.fetch(a, x, 0, 1, w, lane);
+  fetch(x.first);
+  fetch_q(x.first, o0);
+  for (int ch = x.first; ch < x.last; ++ch) {
+    const int n = ch - x.first, tok0 = 64 * ch, live = min(64, a.N - tok0);
+    lane = here(lane), t = here(t);
+    if (n) lds_sync();
+    gates.form(dec, a, x, n, 1, w, lane);
+    ki.store(K, a.D, live, t);
+    vi.store(V, a.DV, live, t);
+    put_state(S, s, w, lane);
+    if (states && part == 0) store_state<false>(s, states + ((size_t)x.u * a.NC + ch) * kTile2, 64, 64, w, lane);
     lds_sync();
-    if (o + 1 < o1) fetch(o + 1);
+    if (ch + 1 < x.last) fetch(ch + 1);
+    const Decays& d = dec[n % kSlots];
+    const float since = a.scale * d.since[own], hi = d.hi[own], lo = d.lo[own];
+    for (int o = o0; o < o1; ++o) {
+      lane = here(lane);
+      const Frag<NP> qf[2] = {next[0], next[1]};
+      if (o + 1 < o1)
+        fetch_q(ch, o + 1);
+      else if (ch + 1 < x.last)
+        fetch_q(ch + 1, o0);
+      Half<NP> p[4] = {};
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const Frag<3> of = scaled_col(O, 16 * w, s, lane, dec.since, a.scale);
+      for (int m = 0; m < 4; ++m) {
+        if (m > w) continue;
+        f32x4 y = {};
 #pragma unroll
-      for (int m = 0; m < 4; ++m) f[m] = mma(col_frag(Q, 16 * m, s, lane), of, f[m]);
+        for (int k = 0; k < 2; ++k) y = mma(row_frag(K, 16 * m, k, lane), qf[k], y);
+        y *= a.scale * decays<false>(d, 16 * m + 4 * g, 16 * m, m == w, hi, lo);
+        if (m == w)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) y[i] = 4 * g + i <= c ? y[i] : 0.f;
+        p[m] = half_of<NP>(y);
+      }
+      phase();
+      const Frag<NP> p0 = both(p[0], p[1]), p1 = both(p[2], p[3]);
+      T* dst = out + (((size_t)x.b * a.H + o) * a.N + tok0) * a.DV;
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+        f32x4 y = {};
+#pragma unroll
+        for (int k = 0; k < 2; ++k) y = mma(row_frag(S, 16 * m, k, lane), qf[k], y);
+        y *= since;
+        y = mma(col_frag_perm(V, 16 * m, 0, lane), p0, y);
+        if (w >= 2) y = mma(col_frag_perm(V, 16 * m, 1, lane), p1, y);
+        if (own < live && 16 * m + 4 * g < a.DV) store4(shared_at(dst, __umul24(own, a.DV) + 16 * m + 4 * g), y);
+      }
+    }
+    if (ch + 1 < x.last || UP == 3) {
+      decay_state(s, d.end, sg);
+      add_outer<UP>(s, K, V, d.until, 1.f, w, lane);
     }
   }
-  const size_t at = ((size_t)u * a.NC + ch) * kTile2;
-#pragma unroll
-  for (int m = 0; m < 4; ++m)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) F[at + (16 * m + 4 * g + i) * 64 + 16 * w + c] = f[m][i];
+  if (UP == 3 && final_state && x.last == a.NC && part == 0)
+    store_state<false>(s, final_state + (size_t)x.u * a.D * a.DV, a.D, a.DV, w, lane);
 }
 
-// All gradients of one chunk and state head, with D_ij = scale exp(G_i - G_j) (j <= i):
+// ---------------------------------------------------------------------------
+// Backward, with D_ij = scale exp(G_i - G_j) (j <= i) in a chunk, S before it and dS' behind it:
 //   dq_i = scale e^(G_i) S dO_i + sum_j D_ij (dO_i.v_j) k_j     (per output head)
 //   dk_j = e^(G_63 - G_j) dS' v_j + sum_i D_ij (dO_i.v_j) q_i
 //   dv_j = e^(G_63 - G_j) dS'^T k_j + sum_i D_ij (q_i.k_j) dO_i
-//   dG_i = sum_(j < i) D_ij (q_i.k_j) (dO_i.v_j) - sum_(j > i) D_ji (q_j.k_i) (dO_j.v_i)
-//          + scale e^(G_i) q_i.(S dO_i) - e^(G_63 - G_i) k_i.(dS' v_i),
-//   and at the chunk's end e^(G_63) <S, dS'> + sum_j e^(G_63 - G_j) k_j.(dS' v_j);
-// dg the sums of dG from each token to the chunk's end. Terms that do not decay (j = i,
-// the last token's write) are left out rather than cancelled: where all decay is
-// strong, dg is far smaller than they are. All products are transposed: a wave's 16
-// tokens are the columns. What goes into dq, dk and dv alone is cut to two bf16 parts
-// (16 bits) for 16-bit tensors, which then round once themselves; dg sees three.
+//   dg_t = sum over all pairs j < t <= i of what passes from j to i: with M_ij = D_ij (q_i.k_j) (dO_i.v_j),
+//     r_i = sum_(j < i) M_ij + scale e^(G_i) q_i.(S dO_i), c_j = sum_(i > j) M_ij, s_j = e^(G_63 - G_j) k_j.(dS' v_j),
+//     dg_t = sum_(i >= t) (r_i - c_i) + sum_(j < t) s_j + e^(G_63) <S, dS'>
+// A block walks back with dS' in its accumulators; S the forward has kept. Both take turns in one tile of LDS. All
+// products are transposed: a wave's 16 tokens are the columns. What goes into dq, dk and dv alone rounds
+// to bf16 for bf16 tensors, as these do themselves, and to two parts for fp16; dg sees all 24 bits.
+// ---------------------------------------------------------------------------
 template <typename T>
-__global__ __launch_bounds__(kThr) void k_decay_bwd(DecayArgs a, const T* __restrict__ dout, const Decays* __restrict__ G,
-                                                    const float* __restrict__ Sin, const float* __restrict__ dSin,
-                                                    T* __restrict__ dq, float* __restrict__ dqh, T* __restrict__ dk,
-                                                    float* __restrict__ dkh, T* __restrict__ dv, float* __restrict__ dg,
-                                                    double* __restrict__ dgsum) {
-  constexpr int NP = kPartsOf<T>, NO = NP == 3 ? 3 : 2;
+__global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 2 : 1) void k_decay_bwd(
+    DecayArgs a, DecaySegments sg, From from, const T* __restrict__ dout, const float* __restrict__ states,
+    T* __restrict__ dq, float* __restrict__ dqh, T* __restrict__ dk, float* __restrict__ dkh, T* __restrict__ dv,
+    float* __restrict__ dg, double* __restrict__ dgsum, float* __restrict__ dstate) {
+  constexpr int NP = kPartsOf<T>;
   __shared__ Tile<NP> K, V, Q, O;
-  __shared__ Tile<3> X;
-  __shared__ Decays dec;
-  __shared__ float dG[64], part[4];
-  const int t = threadIdx.x, lane = t & 63, w = wave_of(t), g = lane >> 4, c = lane & 15;
-  const int ch = blockIdx.x % a.NC, u = blockIdx.x / a.NC, b = u / a.Hv, h = u % a.Hv;
-  const int tok0 = 64 * ch, live = min(64, a.N - tok0), own = 16 * w + c;
-  const size_t at = ((size_t)u * a.NC + ch) * kTile2;
-  const T* krows = rows_of<T>(a.k, b, h / (a.Hv / a.Hk), tok0);
-  Incoming<NP, T> ki, vi, qi, oi;
-  Incoming<3, float> xi;
-  ki.fetch(krows, a.k.n, a.D, live, t);
-  vi.fetch(rows_of<T>(a.v, b, h, tok0), a.v.n, a.DV, live, t);
-  xi.fetch(dSin + at, 64, 64, 64, t);
-  // <S, dS'>
-  float ends = 0.f;
-#pragma unroll
-  for (int x = 0; x < 4; ++x) {
-    const int i = 4 * (t + kThr * x);
-    const f32x4 s = load4(Sin + at + i), d = load4(dSin + at + i);
-    ends += s[0] * d[0] + s[1] * d[1] + s[2] * d[2] + s[3] * d[3];
-  }
-  copy_decays(dec, G[(size_t)u * a.NC + ch], t);
-  ki.store(K, t);
-  vi.store(V, t);
-  xi.store(X, t);
-  lds_sync();
-  xi.fetch(Sin + at, 64, 64, 64, t);
-  const int each = a.H / a.Hv, o1 = (h + 1) * each;
-  auto fetch = [&](int o) {
-    qi.fetch(rows_of<T>(a.q, b, o / (a.H / a.Hq), tok0), a.q.n, a.D, live, t);
-    oi.fetch(dout + (((size_t)b * a.H + o) * a.N + tok0) * a.DV, a.DV, a.DV, live, t);
+  __shared__ Tile<3> X;  // rows: keys' dimensions
+  __shared__ Decays dec[kSlots];
+  __shared__ float dG[2][64], ss[2][64], ends[2][4];
+  int t = threadIdx.x, lane = t & 63;
+  const int w = wave_of(t), g = lane >> 4, c = lane & 15, own = 16 * w + c;
+  const Course x(a, sg, blockIdx.x);
+  const int each = a.H / a.Hv, o0 = x.h * each;
+  State s;  // the gradient of the state; rows: values, columns: keys' dimensions
+  load_state<true>(s, from.of(sg, x), from.rows, from.cols, w, lane);
+  Coming<NP, T> ki, vi, qi, oi;
+  auto krows = [&](int ch) { return rows_of<T>(a.k, x.b, x.h / (a.Hv / a.Hk), 64 * ch); };
+  auto qrows = [&](int ch, int o) { return rows_of<T>(a.q, x.b, o / (a.H / a.Hq), 64 * ch); };
+  auto fetch = [&](int ch, int o) {
+    const int tok0 = 64 * ch, live = min(64, a.N - tok0);
+    qi.fetch(qrows(ch, o), a.q.n, a.D, live, t);
+    oi.fetch(dout + (((size_t)x.b * a.H + o) * a.N + tok0) * a.DV, a.DV, a.DV, live, t);
   };
-  fetch(h * each);
-  ends *= dec.since[63];
-  const float hi = dec.hi[own], lo = dec.lo[own];
-  Frag<NP> kf[2], vf[2];
-#pragma unroll
-  for (int s = 0; s < 2; ++s) kf[s] = row_frag(K, 16 * w, s, lane), vf[s] = row_frag(V, 16 * w, s, lane);
-  f32x4 wk[4], wv[4];  // dk and dv
-  float decay = 0.f;   // of dG
-  {
-    const float until = dec.until[own];
-#pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      f32x4 kv = {}, x = {}, y = {};
-      if (own < live && 16 * n + 4 * g < a.D) kv = load4(krows + own * a.k.n + 16 * n + 4 * g);
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        x = mma(row_frag(X, 16 * n, s, lane), vf[s], x);
-        y = mma(col_frag<NO>(X, 16 * n, s, lane), kf[s], y);
-      }
-      wk[n] = until * x;
-      wv[n] = until * y;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        // what the last token writes does not decay
-        const float z = own < live - 1 ? kv[i] * wk[n][i] : 0.f;
-        ends += z;
-        decay -= z;
-      }
-    }
-  }
-  ends = wave_sum(ends);
-  if (lane == 0) part[w] = ends;
-  lds_sync();
-  xi.store(X, t);
-  const float since = a.scale * dec.since[own];
-  for (int o = h * each; o < o1; ++o) {
-    const T* qrows = rows_of<T>(a.q, b, o / (a.H / a.Hq), tok0);
-    const size_t orow = ((size_t)b * a.H + o) * a.N + tok0;
-    if (o > h * each) lds_sync();
-    qi.store(Q, t);
-    oi.store(O, t);
+  auto fetch_k = [&](int ch) {
+    const int live = min(64, a.N - 64 * ch);
+    ki.fetch(krows(ch), a.k.n, a.D, live, t);
+    vi.fetch(rows_of<T>(a.v, x.b, x.h, 64 * ch), a.v.n, a.DV, live, t);
+  };
+  State before;
+  auto fetch_state = [&](int ch) {
+    load_state<true>(before, states + ((size_t)x.u * a.NC + ch) * kTile2, 64, 64, w, lane);
+  };
+  Gates gates;
+  gates.fetch(a, x, 0, -1, w, lane);
+  fetch_k(x.last - 1);
+  fetch(x.last - 1, o0);
+  fetch_state(x.last - 1);
+  for (int ch = x.last - 1; ch >= x.first; --ch) {
+    const int n = x.last - 1 - ch, tok0 = 64 * ch, live = min(64, a.N - tok0), turn = n & 1;
+    lane = here(lane), t = here(t);
+    gates.form(dec, a, x, n, -1, w, lane);
+    ki.store(K, a.D, live, t);
+    vi.store(V, a.DV, live, t);
+    qi.store(Q, a.D, live, t);
+    oi.store(O, a.DV, live, t);
+    put_state(X, s, w, lane);
     lds_sync();
-    if (o + 1 < o1) fetch(o + 1);
-    Frag<NP> of[2], qf[2];
+    if (ch > x.first) fetch_k(ch - 1);
+    const Decays& d = dec[n % kSlots];
+    const float hi = d.hi[own], lo = d.lo[own], since = a.scale * d.since[own];
+    f32x4 wk[4], wv[4];
+    float passed = 0.f, decay = 0.f;  // s_j and r_j - c_j
+    {
+      const Frag<NP> kf[2] = {row_frag(K, 16 * w, 0, lane), row_frag(K, 16 * w, 1, lane)};
+      const Frag<NP> vf[2] = {row_frag(V, 16 * w, 0, lane), row_frag(V, 16 * w, 1, lane)};
+      const float until = d.until[own];
 #pragma unroll
-    for (int s = 0; s < 2; ++s) of[s] = row_frag(O, 16 * w, s, lane), qf[s] = row_frag(Q, 16 * w, s, lane);
-    f32x4 acc[4], p[4] = {};
+      for (int m = 0; m < 4; ++m) {
+        f32x4 y = {}, z = {};
 #pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      f32x4 x = {}, qk = {}, qv = {};
-      if (own < live && 16 * n + 4 * g < a.D) qv = load4(qrows + own * a.q.n + 16 * n + 4 * g);
+        for (int i = 0; i < 2; ++i) {
+          y = mma(row_frag(X, 16 * m, i, lane), vf[i], y);
+          z = mma(col_frag<NP>(X, 16 * m, i, lane), kf[i], z);
+        }
+        wk[m] = until * y;
+        wv[m] = until * z;
+        const f32x4 k = own_values(K, own, m, lane);
 #pragma unroll
-      for (int s = 0; s < 2; ++s) x = mma(row_frag(X, 16 * n, s, lane), of[s], x);
-      acc[n] = since * x;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) decay += qv[i] * acc[n][i];
-      if (n > w) continue;
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        p[n] = mma(row_frag(V, 16 * n, s, lane), of[s], p[n]);
-        qk = mma(row_frag(K, 16 * n, s, lane), qf[s], qk);
-      }
-      const f32x4 y = a.scale * decay_from(dec, 16 * n + 4 * g, hi, lo) * p[n];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int j = 16 * n + 4 * g + i;
-        p[n][i] = j <= own ? y[i] : 0.f;
-        decay += j < own ? p[n][i] * qk[i] : 0.f;
+        for (int i = 0; i < 4; ++i) passed += k[i] * wk[m][i];
       }
     }
-    {
-      const Frag<NO> p0 = acc_frag<NO>(p[0], p[1]), p1 = acc_frag<NO>(p[2], p[3]);
+    // the gradient of the state before the chunk, and what passes the whole chunk
+    decay_state(s, d.end, sg);
+    float through = 0.f;
 #pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        acc[n] = mma(col_frag_perm(K, 16 * n, 0, lane), p0, acc[n]);
-        if (w >= 2) acc[n] = mma(col_frag_perm(K, 16 * n, 1, lane), p1, acc[n]);
-        if (own < live && 16 * n + 4 * g < a.D) {
-          if (dqh)
-            store4(dqh + (orow + own) * a.D + 16 * n + 4 * g, acc[n]);
-          else
-            store4(dq + (orow + own) * a.D + 16 * n + 4 * g, acc[n]);
+    for (int m = 0; m < 4; ++m)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) through += before[m][i] * s[m][i];
+    through = wave_sum(through);
+    lds_sync();
+    put_state(X, before, w, lane);
+    if (ch > x.first) fetch_state(ch - 1);
+    for (int o = o0; o < o0 + each; ++o) {
+      lane = here(lane), t = here(t);
+      if (o > o0) {
+        lds_sync();
+        qi.store(Q, a.D, live, t);
+        oi.store(O, a.DV, live, t);
+      }
+      lds_sync();
+      if (o + 1 < o0 + each)
+        fetch(ch, o + 1);
+      else if (ch > x.first)
+        fetch(ch - 1, o0);
+      {
+        // queries: own
+        const Frag<NP> qf[2] = {row_frag(Q, 16 * w, 0, lane), row_frag(Q, 16 * w, 1, lane)};
+        const Frag<NP> of[2] = {row_frag(O, 16 * w, 0, lane), row_frag(O, 16 * w, 1, lane)};
+        Half<NP> p[4] = {};
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          if (m > w) continue;
+          f32x4 y = {}, qk = {};
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            y = mma(row_frag(V, 16 * m, i, lane), of[i], y);
+            qk = mma(row_frag(K, 16 * m, i, lane), qf[i], qk);
+          }
+          y *= a.scale * decays<false>(d, 16 * m + 4 * g, 16 * m, m == w, hi, lo);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (m == w) {
+              decay += 4 * g + i < c ? y[i] * qk[i] : 0.f;
+              y[i] = 4 * g + i <= c ? y[i] : 0.f;
+            } else {
+              decay += y[i] * qk[i];
+            }
+          }
+          p[m] = half_of<NP>(y);
+        }
+        const Frag<NP> p0 = both(p[0], p[1]), p1 = both(p[2], p[3]);
+        const size_t at = (((size_t)x.b * a.H + o) * a.N + tok0) * a.D;
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          f32x4 y = {};
+#pragma unroll
+          for (int i = 0; i < 2; ++i) y = mma(row_frag(X, 16 * m, i, lane), of[i], y);
+          y *= since;
+          const f32x4 q = own_values(Q, own, m, lane);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) decay += q[i] * y[i];
+          y = mma(col_frag_perm(K, 16 * m, 0, lane), p0, y);
+          if (w >= 2) y = mma(col_frag_perm(K, 16 * m, 1, lane), p1, y);
+          if (own < live && 16 * m + 4 * g < a.D) {
+            const uint32_t to = __umul24(own, a.D) + 16 * m + 4 * g;
+            if (dqh)
+              store4(shared_at(dqh + at, to), y);
+            else
+              store4(shared_at(dq + at, to), y);
+          }
         }
       }
+      phase();
+      {
+        // keys: own
+        const Frag<NP> kf[2] = {row_frag(K, 16 * w, 0, lane), row_frag(K, 16 * w, 1, lane)};
+        const Frag<NP> vf[2] = {row_frag(V, 16 * w, 0, lane), row_frag(V, 16 * w, 1, lane)};
+        Half<NP> p[4] = {}, r[4] = {};
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          if (m < w) continue;
+          f32x4 qk = {}, ov = {};
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            ov = mma(row_frag(O, 16 * m, i, lane), vf[i], ov);
+            qk = mma(row_frag(Q, 16 * m, i, lane), kf[i], qk);
+          }
+          f32x4 e = a.scale * decays<true>(d, 16 * m + 4 * g, 16 * m, m == w, hi, lo);
+          if (m == w)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) e[i] = c <= 4 * g + i ? e[i] : 0.f;
+          ov *= e;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) decay -= m > w || c < 4 * g + i ? ov[i] * qk[i] : 0.f;
+          p[m] = half_of<NP>(ov);
+          r[m] = half_of<NP>(e * qk);
+        }
+        const Frag<NP> p0 = both(p[0], p[1]), p1 = both(p[2], p[3]), r0 = both(r[0], r[1]), r1 = both(r[2], r[3]);
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          if (w < 2) {
+            wk[m] = mma(col_frag_perm(Q, 16 * m, 0, lane), p0, wk[m]);
+            wv[m] = mma(col_frag_perm(O, 16 * m, 0, lane), r0, wv[m]);
+          }
+          wk[m] = mma(col_frag_perm(Q, 16 * m, 1, lane), p1, wk[m]);
+          wv[m] = mma(col_frag_perm(O, 16 * m, 1, lane), r1, wv[m]);
+        }
+      }
+      if (ch > x.first || (dstate && sg.count == 1)) add_outer<3>(s, O, Q, d.since, a.scale, w, lane);
     }
-    f32x4 r[4] = {};
+    const size_t at = (size_t)x.u * a.N + tok0;
 #pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      p[n] = f32x4{};
-      if (n < w) continue;
-      f32x4 qk = {}, ov = {};
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        ov = mma(row_frag(O, 16 * n, s, lane), vf[s], ov);
-        qk = mma(row_frag(Q, 16 * n, s, lane), kf[s], qk);
+    for (int m = 0; m < 4; ++m) {
+      const int e = 16 * m + 4 * g;
+      if (own < live && e < a.D) {
+        if (dkh)
+          store4(shared_at(dkh + at * a.D, __umul24(own, a.D) + e), wk[m]);
+        else
+          store4(shared_at(dk + at * a.D, __umul24(own, a.D) + e), wk[m]);
       }
-      const f32x4 y = a.scale * decay_to(dec, 16 * n + 4 * g, hi, lo);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = 16 * n + 4 * g + i;
-        const float e = own <= row ? y[i] : 0.f;
-        p[n][i] = e * ov[i];
-        r[n][i] = e * qk[i];
-        decay -= own < row ? p[n][i] * qk[i] : 0.f;
-      }
+      if (own < live && e < a.DV) store4(shared_at(dv + at * a.DV, __umul24(own, a.DV) + e), wv[m]);
     }
-    const Frag<NO> p0 = acc_frag<NO>(p[0], p[1]), p1 = acc_frag<NO>(p[2], p[3]);
-    const Frag<NO> r0 = acc_frag<NO>(r[0], r[1]), r1 = acc_frag<NO>(r[2], r[3]);
+    decay = group_sum(decay);
+    passed = group_sum(passed);
+    if (g == 0) dG[turn][own] = decay, ss[turn][own] = passed;
+    if (lane == 0) ends[turn][w] = through;
+    lds_sync();
+    // one wave, another for each chunk; the next but one chunk writes these places again, behind a barrier
+    if (w == n % 4) {
+      // dg_t = sum of all r_i - c_i, and of s_j - (r_j - c_j) over j < t
+      const double mine = dG[turn][lane], past = lane ? (double)ss[turn][lane - 1] - (double)dG[turn][lane - 1] : 0.0;
+      const double all = lane_of(running_sum(mine), 63);
+      double y = all + running_sum(past) + (((double)ends[turn][0] + ends[turn][1]) + ((double)ends[turn][2] + ends[turn][3]));
+      // where nothing is kept nothing depends on g; the sums' roundings do not cancel
+      if (lane >= live || gate_at(a, x.b, x.h, tok0 + lane) < kNothingKept) y = 0;
+      if (dgsum) {
 #pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      if (w < 2) {
-        wk[n] = mma(col_frag_perm(Q, 16 * n, 0, lane), p0, wk[n]);
-        wv[n] = mma(col_frag_perm(O, 16 * n, 0, lane), r0, wv[n]);
+        for (int off = 32; off > 0; off >>= 1) y += __shfl_xor(y, off, 64);
+        if (lane == 0) dgsum[(size_t)x.u * a.NC + ch] = y;
+      } else if (lane < live) {
+        dg[(size_t)x.u * a.N + tok0 + lane] = (float)y;
       }
-      wk[n] = mma(col_frag_perm(Q, 16 * n, 1, lane), p1, wk[n]);
-      wv[n] = mma(col_frag_perm(O, 16 * n, 1, lane), r1, wv[n]);
     }
   }
-  const size_t row = (size_t)u * a.N + tok0 + own;
-#pragma unroll
-  for (int n = 0; n < 4; ++n) {
-    const int d = 16 * n + 4 * g;
-    if (own < live && d < a.D) {
-      if (dkh)
-        store4(dkh + row * a.D + d, wk[n]);
-      else
-        store4(dk + row * a.D + d, wk[n]);
-    }
-    if (own < live && d < a.DV) store4(dv + row * a.DV + d, wv[n]);
-  }
-  decay = group_sum(decay);
-  if (g == 0) dG[own] = decay;
-  lds_sync();
-  if (w == 0) {
-    double x = dG[lane];
-    if (lane == 63) x += ((double)part[0] + part[1]) + ((double)part[2] + part[3]);
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const double y = __shfl_down(x, off, 64);
-      if (lane + off < 64) x += y;
-    }
-    // where nothing is kept nothing depends on g; the sums' roundings do not cancel
-    if (lane >= live || gate_at(a, b, h, tok0 + lane) < kNothingKept) x = 0;
-    if (dgsum) {
-#pragma unroll
-      for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
-      if (lane == 0) dgsum[(size_t)u * a.NC + ch] = x;
-    } else if (lane < live) {
-      dg[(size_t)u * a.N + tok0 + lane] = (float)x;
-    }
-  }
+  if (dstate && sg.count == 1) store_state<true>(s, dstate + (size_t)x.u * a.D * a.DV, a.D, a.DV, w, lane);
 }
 
 // The gradient of a head's one decay: its chunks' sums over the batch, a block per head.
@@ -578,18 +877,36 @@ struct Room {
   }
 };
 
-void scan(const DecayArgs& a, const float* G, float* S, const float* init, float* end, bool back, hipStream_t st,
-          const Timer& timed) {
-  const Scan s = {reinterpret_cast<const Decays*>(G), S, init, end, a.NC, a.D, a.DV, back};
-  timed("k_decay_scan", st, [&] { hipLaunchKernelGGL(k_decay_scan, dim3(4 * a.B * a.Hv), dim3(kThr), 0, st, s); });
+void scan(const DecayArgs& a, const DecaySegments& sg, const float* G, float* S, const float* init, float* end,
+          bool back, hipStream_t st, const Timer& timed) {
+  const Scan s = {G, S, init, end, sg.count, a.D, a.DV, back};
+  timed("k_decay_scan", st,
+        [&] { hipLaunchKernelGGL(k_decay_scan, dim3(a.B * a.Hv * (kTile2 / kThr)), dim3(kThr), 0, st, s); });
 }
+
+// Heads of a state that one block of the forward takes: all, unless that leaves CUs without a block.
+int heads_each(const DecayArgs& a, const DecaySegments& sg) {
+  const int rep = a.H / a.Hv, blocks = a.B * a.Hv * sg.count, parts = std::clamp(1024 / blocks, 1, rep);
+  return (rep + parts - 1) / parts;
+}
+// Segments so that `blocks` blocks have one each, the GPU's at once.
+DecaySegments segments(int U, int NC, int blocks) {
+  const int count = std::clamp(blocks / U, 1, NC), len = (NC + count - 1) / count;
+  return {(NC + len - 1) / len, len};
+}
+DecaySegments forward_segments(int U, int NC) { return segments(U, NC, 1024); }
+DecaySegments backward_segments(int U, int NC) { return segments(U, NC, 512); }
 }  // namespace
 
-DecaySaved decay_saved_view(void* base, int U, int NC) {
+DecaySaved decay_saved_view(void* base, int U, int NC, bool keep) {
   DecaySaved s;
   Room r{static_cast<char*>(base)};
-  s.G = r.take<float>((size_t)U * NC * kDecays);
-  s.S = r.take<float>((size_t)U * NC * kTile2);
+  const DecaySegments sg = forward_segments(U, NC);
+  const size_t segs = sg.count > 1 ? (size_t)U * sg.count : 0;
+  s.S = keep ? r.take<float>((size_t)U * NC * kTile2) : nullptr;
+  // needed by the forward alone: after what the backward reads
+  s.G = r.take<float>(2 * segs + 1);
+  s.D = r.take<float>(segs * kTile2);
   s.bytes = r.off;
   return s;
 }
@@ -597,29 +914,37 @@ DecaySaved decay_saved_view(void* base, int U, int NC) {
 DecayWork decay_work_view(void* base, const DecayArgs& a) {
   DecayWork w;
   Room r{static_cast<char*>(base)};
-  const size_t chunks = (size_t)a.B * a.Hv * a.NC;
-  w.dS = r.take<float>(chunks * kTile2);
+  const int U = a.B * a.Hv;
+  const DecaySegments sg = backward_segments(U, a.NC);
+  const size_t segs = sg.count > 1 ? (size_t)U * sg.count : 0;
+  w.G = r.take<float>(2 * segs + 1);
+  w.dS = r.take<float>(segs * kTile2);
   w.dqh = a.H != a.Hq ? r.take<float>((size_t)a.B * a.H * a.N * a.D) : nullptr;
   w.dkh = a.Hv != a.Hk ? r.take<float>((size_t)a.B * a.Hv * a.N * a.D) : nullptr;
-  w.sum = a.per_head ? r.take<double>(chunks) : nullptr;
+  w.sum = a.per_head ? r.take<double>((size_t)U * a.NC) : nullptr;
   w.bytes = r.off;
   return w;
 }
 
 template <typename T>
-void launch_decay_forward(const DecayArgs& a, const float* state, void* out, float* final_state, void* saved,
+void launch_decay_forward(const DecayArgs& a, const float* state, void* out, float* final_state, void* saved, bool keep,
                           hipStream_t st, const Timer& timed) {
   const int U = a.B * a.Hv, rep = a.H / a.Hv;
-  const DecaySaved s = decay_saved_view(saved, U, a.NC);
-  Decays* G = reinterpret_cast<Decays*>(s.G);
-  timed("k_decay_sum", st,
-        [&] { hipLaunchKernelGGL(k_decay_sum<T>, dim3(a.NC * U), dim3(kThr), 0, st, a, G, s.S); });
-  scan(a, s.G, s.S, state, final_state, false, st, timed);
-  // all heads of a state in one block, unless that leaves CUs without one
-  const int parts = std::clamp((1024 + U * a.NC - 1) / (U * a.NC), 1, rep), each = (rep + parts - 1) / parts;
+  const DecaySegments sg = forward_segments(U, a.NC);
+  const DecaySaved s = decay_saved_view(saved, U, a.NC, keep);
+  From from = {state, a.D, a.DV};
+  if (sg.count > 1) {
+    timed("k_decay_sum", st, [&] {
+      hipLaunchKernelGGL((k_decay_sum<T, false>), dim3(U * sg.count), dim3(kThr), 0, st, a, sg, nullptr, s.G, s.D);
+    });
+    scan(a, sg, s.G, s.D, state, final_state, false, st, timed);
+    from = {s.D, 64, 64};
+  }
+  const auto kernel = sg.count > 1 && !keep && kPartsOf<T> < 3 ? k_decay_out<T, 2> : k_decay_out<T, 3>;
+  const int each = heads_each(a, sg);
   timed("k_decay_out", st, [&] {
-    hipLaunchKernelGGL(k_decay_out<T>, dim3(U * a.NC * ((rep + each - 1) / each)), dim3(kThr), 0, st, a, each, G, s.S,
-                       static_cast<T*>(out));
+    hipLaunchKernelGGL(kernel, dim3(U * sg.count * ((rep + each - 1) / each)), dim3(kThr), 0, st, a, sg, each, from,
+                       static_cast<T*>(out), sg.count > 1 ? nullptr : final_state, s.S);
   });
 }
 
@@ -628,16 +953,21 @@ void launch_decay_backward(const DecayArgs& a, const void* saved, const void* do
                            void* dk, void* dv, float* dg, float* dstate, void* work, hipStream_t st,
                            const Timer& timed) {
   const int U = a.B * a.Hv;
-  const DecaySaved s = decay_saved_view(const_cast<void*>(saved), U, a.NC);
+  const DecaySegments sg = backward_segments(U, a.NC);
+  const DecaySaved s = decay_saved_view(const_cast<void*>(saved), U, a.NC, true);
   const DecayWork w = decay_work_view(work, a);
-  const Decays* G = reinterpret_cast<const Decays*>(s.G);
   const T* od = static_cast<const T*>(dout);
-  timed("k_decay_bwd_sum", st,
-        [&] { hipLaunchKernelGGL(k_decay_bwd_sum<T>, dim3(a.NC * U), dim3(kThr), 0, st, a, od, G, w.dS); });
-  scan(a, s.G, w.dS, dfinal, dstate, true, st, timed);
+  From from = {dfinal, a.D, a.DV};
+  if (sg.count > 1) {
+    timed("k_decay_sum_back", st, [&] {
+      hipLaunchKernelGGL((k_decay_sum<T, true>), dim3(U * sg.count), dim3(kThr), 0, st, a, sg, od, w.G, w.dS);
+    });
+    scan(a, sg, w.G, w.dS, dfinal, dstate, true, st, timed);
+    from = {w.dS, 64, 64};
+  }
   timed("k_decay_bwd", st, [&] {
-    hipLaunchKernelGGL(k_decay_bwd<T>, dim3(a.NC * U), dim3(kThr), 0, st, a, od, G, s.S, w.dS, static_cast<T*>(dq),
-                       w.dqh, static_cast<T*>(dk), w.dkh, static_cast<T*>(dv), dg, w.sum);
+    hipLaunchKernelGGL(k_decay_bwd<T>, dim3(U * sg.count), dim3(kThr), 0, st, a, sg, from, od, s.S,
+                       static_cast<T*>(dq), w.dqh, static_cast<T*>(dk), w.dkh, static_cast<T*>(dv), dg, w.sum, dstate);
   });
   if (w.sum)
     timed("k_decay_gate_sum", st, [&] {
@@ -648,7 +978,7 @@ void launch_decay_backward(const DecayArgs& a, const void* saved, const void* do
 }
 
 #define OAL_DECAY(T)                                                                                               \
-  template void launch_decay_forward<T>(const DecayArgs&, const float*, void*, float*, void*, hipStream_t,         \
+  template void launch_decay_forward<T>(const DecayArgs&, const float*, void*, float*, void*, bool, hipStream_t,   \
                                         const Timer&);                                                            \
   template void launch_decay_backward<T>(const DecayArgs&, const void*, const void*, const float*, void*, void*,   \
                                          void*, float*, float*, void*, hipStream_t, const Timer&);

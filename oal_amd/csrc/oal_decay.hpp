@@ -16,16 +16,23 @@ struct DecayArgs {
   float scale;
 };
 
-// What the forward computes per unit u = b Hv + state head and chunk, and the backward reads.
+// Chunks are walked in segments of `len`.
+struct DecaySegments {
+  int count, len;
+};
+
+// What the forward computes per unit u = b Hv + state head and chunk, and the backward reads (S).
 struct DecaySaved {
-  float* G;  // [U][NC] decays of the chunk's tokens
-  float* S;  // [U][NC][64][64] state before the chunk
+  float* S;  // [U][NC][64][64] state before the chunk (null: not kept)
+  float* G;  // [U][segments][2] the segment's decay, in two parts (nothing for a single one)
+  float* D;  // [U][segments][64][64] what it adds to the state, then the state before it
   size_t bytes;
 };
-DecaySaved decay_saved_view(void* base, int U, int NC);
+DecaySaved decay_saved_view(void* base, int U, int NC, bool keep);
 
 struct DecayWork {
-  float* dS;    // [U][NC][64][64] gradient of the state after the chunk
+  float* G;     // [U][segments][2]
+  float* dS;    // [U][segments][64][64] gradient of the state after the segment
   float* dqh;   // [B][H][N][D] dq of every output head (null: heads are not shared)
   float* dkh;   // [B][Hv][N][D] dk of every state head (null: heads are not shared)
   double* sum;  // [U][NC] sums of dg over the chunk (null: g is per token)
@@ -33,8 +40,9 @@ struct DecayWork {
 };
 DecayWork decay_work_view(void* base, const DecayArgs& a);
 
+// keep: for a backward
 template <typename T>
-void launch_decay_forward(const DecayArgs& a, const float* state, void* out, float* final_state, void* saved,
+void launch_decay_forward(const DecayArgs& a, const float* state, void* out, float* final_state, void* saved, bool keep,
                           hipStream_t st, const Timer& timed);
 // dout [B][H][N][DV]; dfinal [U][D][DV] may be null (no gradient).
 template <typename T>

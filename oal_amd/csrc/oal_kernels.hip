@@ -1743,12 +1743,15 @@ static int decay_args(oal::DecayArgs* a, const char* what, const void* q, const 
   if (!rows_aligned(a->q, dtype, batch, q_heads, seq_len) || !rows_aligned(a->k, dtype, batch, k_heads, seq_len) ||
       !rows_aligned(a->v, dtype, batch, v_heads, seq_len))
     return fail(std::string(what) + ": rows must be 16-byte aligned");
+  // 32-bit offsets inside a tile of 64 rows
+  for (const oal::Strided* r : {&a->q, &a->k, &a->v})
+    if (seq_len > 1 && (r->n < 0 || r->n >= (1 << 24))) return fail(std::string(what) + ": rows are too far apart");
   return 0;
 }
 
-size_t oal_decay_saved_bytes(int batch, int v_heads, int seq_len) {
+size_t oal_decay_saved_bytes(int batch, int v_heads, int seq_len, int keep) {
   if (check_delta(batch, v_heads, v_heads, v_heads, seq_len)) return 0;
-  return oal::decay_saved_view(nullptr, batch * v_heads, (seq_len + 63) / 64).bytes;
+  return oal::decay_saved_view(nullptr, batch * v_heads, (seq_len + 63) / 64, keep != 0).bytes;
 }
 
 size_t oal_decay_workspace_bytes(int batch, int q_heads, int k_heads, int v_heads, int seq_len, int key_dim,
@@ -1766,7 +1769,8 @@ size_t oal_decay_workspace_bytes(int batch, int q_heads, int k_heads, int v_head
 
 int oal_decay_forward(const void* q, const void* k, const void* v, const float* g, const int64_t* strides, int batch,
                       int q_heads, int k_heads, int v_heads, int seq_len, int key_dim, int value_dim, int dtype,
-                      float scale, const float* state, void* out, float* final_state, void* saved, void* stream) {
+                      float scale, const float* state, void* out, float* final_state, void* saved, int keep,
+                      void* stream) {
   Range range("oal_decay_forward");
   oal::DecayArgs a;
   if (decay_args(&a, "oal_decay_forward", q, k, v, g, strides, 0, batch, q_heads, k_heads, v_heads, seq_len, key_dim,
@@ -1779,7 +1783,7 @@ int oal_decay_forward(const void* q, const void* k, const void* v, const float* 
   const auto launch = dtype == OAL_DTYPE_F32    ? oal::launch_decay_forward<float>
                       : dtype == OAL_DTYPE_BF16 ? oal::launch_decay_forward<uint16_t>
                                                 : oal::launch_decay_forward<_Float16>;
-  launch(a, state, out, final_state, saved, static_cast<hipStream_t>(stream), make_timer());
+  launch(a, state, out, final_state, saved, keep != 0, static_cast<hipStream_t>(stream), make_timer());
   return launch_status("oal_decay_forward launch");
 }
 

@@ -22,7 +22,8 @@ query head o // (H / Hq) from state head o // (H / Hv).
 
 Sums over tokens do not depend on the type of q, k and v, which may be
 float32, bfloat16 or float16: states, decays and their gradients are exact to float32.
-Values have to be finite: a token that is not spoils the 64 tokens of its chunk. Results repeat bit by bit from call to call.
+Values have to be finite: a token that is not spoils the 64 tokens of its chunk. Results repeat bit by bit from call to call;
+sequences are cut into segments by a rule on batch, heads and length, so that last bits depend on those.
 
 Calls are eager: tracers, functorch's transforms and forward-mode derivatives are refused
 (compiled code runs the call between its graphs).
@@ -106,8 +107,9 @@ class _DecayFunction(torch.autograd.Function):
     def forward(ctx: Any, q, k, v, g, state, scale: float):
         q, k, v = map(_native.row_tensor, (q, k, v))
         start = None if state is None else _native._aligned(state.contiguous())
-        out, final, saved = _native.decay_forward(q, k, v, g, start, scale=scale)
-        if any(ctx.needs_input_grad):
+        keep = any(ctx.needs_input_grad)
+        out, final, saved = _native.decay_forward(q, k, v, g, start, scale=scale, keep=keep)
+        if keep:
             ctx.save_for_backward(q, k, v, g, saved)
             ctx.scale = scale
         return out, final

@@ -71,9 +71,9 @@ def _lib():
 
 def test_c_entries_check_before_they_launch():
     lib = _lib()
-    assert lib.oal_decay_saved_bytes(2, 2, 65) >= 4 * 2 * 4096 * 4
-    assert lib.oal_decay_saved_bytes(0, 2, 65) == 0 and b"positive" in lib.oal_last_error()
-    assert lib.oal_decay_saved_bytes(1 << 20, 64, 1 << 20) == 0 and b"too large" in lib.oal_last_error()
+    assert lib.oal_decay_saved_bytes(2, 2, 65, 0) > 0 and lib.oal_decay_saved_bytes(2, 2, 65, 1) >= 4 * 2 * 4096 * 4
+    assert lib.oal_decay_saved_bytes(0, 2, 65, 1) == 0 and b"positive" in lib.oal_last_error()
+    assert lib.oal_decay_saved_bytes(1 << 20, 64, 1 << 20, 1) == 0 and b"too large" in lib.oal_last_error()
     assert lib.oal_decay_workspace_bytes(1, 3, 2, 2, 64, 64, 0) == 0 and b"divisible" in lib.oal_last_error()
     assert lib.oal_decay_workspace_bytes(1, 2, 2, 2, 64, 12, 0) == 0 and b"multiples of 8" in lib.oal_last_error()
     # shared heads need room for what is summed
@@ -82,7 +82,7 @@ def test_c_entries_check_before_they_launch():
     rows = (ctypes.c_int64 * 12)(*[64] * 12)
 
     def forward(q=p, strides=rows, dtype=1, out=p, dim=64):
-        return lib.oal_decay_forward(q, p, p, p, strides, 1, 2, 2, 2, 64, dim, 64, dtype, 0.1, None, out, p, p, None)
+        return lib.oal_decay_forward(q, p, p, p, strides, 1, 2, 2, 2, 64, dim, 64, dtype, 0.1, None, out, p, p, 1, None)
 
     assert forward(q=None) and b"null" in lib.oal_last_error()
     assert forward(strides=None) and b"null" in lib.oal_last_error()
@@ -91,6 +91,7 @@ def test_c_entries_check_before_they_launch():
     assert forward(q=odd) and b"16-byte" in lib.oal_last_error()
     assert forward(strides=(ctypes.c_int64 * 12)(*[63] * 12)) and b"16-byte" in lib.oal_last_error()
     assert forward(out=odd) and b"16-byte" in lib.oal_last_error()
+    assert forward(strides=(ctypes.c_int64 * 12)(*[1 << 24] * 12)) and b"too far apart" in lib.oal_last_error()
     rc = lib.oal_decay_backward(p, p, p, p, rows, 0, 1, 2, 2, 2, 64, 64, 64, 1, 0.1, p, None, None, p, p, p, p, None, p, None)
     assert rc and b"null" in lib.oal_last_error()
     rc = lib.oal_decay_backward(p, p, p, p, rows, 0, 1, 2, 2, 2, 64, 64, 64, 1, 0.1, p, odd, None, p, p, p, p, None, p, None)
