@@ -354,7 +354,7 @@ int oal_window_attention_step(const void* q, const void* k, const void* v, void*
  * of q, k, v, g: batch, head, token) of zero where a head has one decay for all its tokens; a g of
  * -inf forgets the state. per_head (backward): dg is [Hv], the sums over batch and tokens, and else
  * [B][Hv][N]. saved (oal_decay_saved_bytes) is the forward's room and, with keep, what the backward reads. Rows of a
- * tensor are less than 2^24 elements apart.
+ * tensor are less than 2^23 elements apart.
  */
 size_t oal_decay_saved_bytes(int batch, int v_heads, int seq_len, int keep);
 int oal_decay_forward(const void* q, const void* k, const void* v, const float* g, const int64_t* strides, int batch,

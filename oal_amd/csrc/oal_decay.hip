@@ -138,14 +138,16 @@ struct Course {
 // since the last time. Tokens past N decay nothing.
 struct Gates {
   float next;
+  __device__ __forceinline__ int token(const Course& x, int n, int step, int w, int lane) const {
+    return 64 * ((step > 0 ? x.first : x.last - 1) + step * (n + w)) + lane;
+  }
   __device__ __forceinline__ void fetch(const DecayArgs& a, const Course& x, int n, int step, int w, int lane) {
-    const int ch = (step > 0 ? x.first : x.last - 1) + step * (n + w), tok = 64 * ch + lane;
-    next = ch >= x.first && ch < x.last && tok < a.N ? gate_at(a, x.b, x.h, tok) : 0.f;
+    next = gate_at(a, x.b, x.h, min(max(token(x, n, step, w, lane), 0), a.N - 1));
   }
   __device__ __forceinline__ void form(Decays (&dec)[kSlots], const DecayArgs& a, const Course& x, int n, int step, int w,
                                        int lane) {
     if (n % kSlots) return;
-    if (n + w < x.last - x.first) form_decays(dec[w], next, lane);
+    if (n + w < x.last - x.first) form_decays(dec[w], token(x, n, step, w, lane) < a.N ? next : 0.f, lane);
     fetch(a, x, n + kSlots, step, w, lane);
   }
 };
@@ -155,66 +157,98 @@ __device__ __forceinline__ const T* rows_of(const Strided& s, int b, int h, int 
   return static_cast<const T*>(s.p) + b * s.b + h * s.h + (int64_t)tok0 * s.n;
 }
 
-// Element `at` from a base that the block shares: 32 bits of offset (rows are less than 2^24 elements apart).
-template <typename T>
-__device__ __forceinline__ const T* shared_at(const T* base, uint32_t at) {
-  return reinterpret_cast<const T*>(reinterpret_cast<const char*>(base) + at * (uint32_t)sizeof(T));
+// A window of memory from a base that the block shares, with 32-bit offsets (rows are less than 2^23 elements
+// apart). What lies at kNowhere is read as zero and not written: loads and stores of rows past the last or columns
+// past the width are none that a lane could skip, so that the ones in flight can be counted on every way.
+constexpr uint32_t kNowhere = 0x80000000u;
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+struct Window {
+  __amdgpu_buffer_rsrc_t r;
+  __device__ __forceinline__ explicit Window(const void* p)
+      : r(__builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)(kNowhere - 16), 0x00027000)) {}
+  __device__ __forceinline__ u32x4 load(uint32_t at) const { return __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 0); }
+  __device__ __forceinline__ void store(uint32_t at, const u32x4& x) const {
+    __builtin_amdgcn_raw_buffer_store_b128(x, r, at, 0, 0);
+  }
+  __device__ __forceinline__ void store(uint32_t at, const u32x2& x) const {
+    __builtin_amdgcn_raw_buffer_store_b64(x, r, at, 0, 0);
+  }
+};
+// Four values to element `at`, or nowhere.
+__device__ __forceinline__ void put4(const Window& w, const float*, bool in, uint32_t at, const f32x4& x) {
+  w.store(in ? 4 * at : kNowhere, __builtin_bit_cast(u32x4, x));
 }
-template <typename T>
-__device__ __forceinline__ T* shared_at(T* base, uint32_t at) {
-  return reinterpret_cast<T*>(reinterpret_cast<char*>(base) + at * (uint32_t)sizeof(T));
+__device__ __forceinline__ void put4(const Window& w, const uint16_t*, bool in, uint32_t at, const f32x4& x) {
+  w.store(in ? 2 * at : kNowhere, u32x2{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])});
 }
+__device__ __forceinline__ void put4(const Window& w, const _Float16*, bool in, uint32_t at, const f32x4& x) {
+  w.store(in ? 2 * at : kNowhere, __builtin_bit_cast(u32x2, __builtin_convertvector(x, f16x4)));
+}
+// Eight values of a row, or zeros, as they come.
+template <typename T>
+struct Eight {
+  u32x4 w[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const Window& from, bool in, uint32_t at) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = from.load(in ? at * (uint32_t)sizeof(T) + 16 * i : kNowhere);
+  }
+  template <int NP>
+  __device__ __forceinline__ Frag<NP> parts() const {
+    Frag<NP> f;
+    if constexpr (NP == 1) {
+      f.p[0] = __builtin_bit_cast(bf16x8, w[0]);
+    } else {
+      float x[8];
+      if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(w[e / 4][e % 4]);
+      } else {
+        typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+        const f16x8 v = __builtin_bit_cast(f16x8, w[0]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = static_cast<float>(v[e]);
+      }
+      f = split<NP>(x);
+    }
+    return f;
+  }
+};
 
-// 64 rows of D values on their way to an LDS tile, by 256 threads. Rows at and past `live` and columns from D, which
-// only the last chunk and narrow heads have, are read from places that there are, and stored as zeros.
+// 64 rows of D values on their way to an LDS tile, by 256 threads; zeros for rows at and past `live` and columns from D.
 template <int NP, typename T>
 struct Coming {
-  uint4 raw[2];
-  float x[2][8];
+  Eight<T> x[2];
   __device__ __forceinline__ void fetch(const T* base, uint32_t stride, int D, int live, int t) {
-#pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      const int r = min((t >> 3) + 32 * n, live - 1), c = 8 * (t & 7);
-      const T* p = shared_at(base, __umul24(r, stride) + (c < D ? c : 0));
-      if constexpr (NP == 1)
-        raw[n] = *reinterpret_cast<const uint4*>(p);
-      else
-        load_row8(x[n], p);
-    }
-  }
-  __device__ __forceinline__ void store(Tile<NP>& s, int D, int live, int t) const {
-    const bool edge = live < 64 || D < 64;
+    const Window from(base);
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
       const int r = (t >> 3) + 32 * n, c = 8 * (t & 7);
-      const bool in = !edge || (r < live && c < D);
-      __bf16* p = s.x + tile_at(r, c);
-      Frag<NP> f;
-      if constexpr (NP == 1)
-        f.p[0] = __builtin_bit_cast(bf16x8, raw[n]);
-      else
-        f = split<NP>(x[n]);
-      if (edge && !in) f = Frag<NP>{};
+      x[n].load(from, r < live && c < D, __umul24(r, stride) + c);
+    }
+  }
+  __device__ __forceinline__ void store(Tile<NP>& s, int t) const {
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      const Frag<NP> f = x[n].template parts<NP>();
+      __bf16* p = s.x + tile_at((t >> 3) + 32 * n, 8 * (t & 7));
 #pragma unroll
       for (int e = 0; e < NP; ++e) *reinterpret_cast<bf16x8*>(p + e * kTileElems) = f.p[e];
     }
   }
 };
-
-// A token's row as operands of sums over its D values: 32 k + 8 g + j, zero from D on. Columns of a product
-// that belong to rows past the last are not used, so that any row serves for them.
-template <int NP, typename T>
-__device__ __forceinline__ void own_row(Frag<NP> (&f)[2], const T* base, uint32_t stride, int D, int row, int g) {
-  const uint32_t at = __umul24(row, stride) + 8 * g;
+// A token's row as operands of sums over its D values: 32 k + 8 g + j, on its way.
+template <typename T>
+struct ComingRow {
+  Eight<T> x[2];
+  __device__ __forceinline__ void fetch(const T* base, uint32_t stride, int D, int live, int row, int g) {
+    const Window from(base);
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const T* p = shared_at(base, at + 32 * k);
-    if (D == 64)
-      f[k] = global_frag<NP>(p, true);
-    else
-      f[k] = global_frag<NP>(p, 32 * k + 8 * g < D);
+    for (int k = 0; k < 2; ++k)
+      x[k].load(from, row < live && 32 * k + 8 * g < D, __umul24(row, stride) + 32 * k + 8 * g);
   }
-}
+};
+
 // Row `row` of a tile as the accumulators of a product with it have it: values 16 m + 4 g + i.
 template <int NP>
 __device__ __forceinline__ f32x4 own_values(const Tile<NP>& s, int row, int m, int lane) {
@@ -351,6 +385,17 @@ __device__ __forceinline__ void store_state(const State& x, float* p, int rows, 
     }
   }
 }
+// A whole state in memory, its columns the accumulators' rows.
+__device__ __forceinline__ void load_tile(State& x, const float* p, int w, int lane) {
+#pragma unroll
+  for (int m = 0; m < 4; ++m) x[m] = load4(p + (16 * w + (lane & 15)) * 64 + 16 * m + 4 * (lane >> 4));
+}
+__device__ __forceinline__ void store_tile(const State& x, float* p, int w, int lane) {
+#pragma unroll
+  for (int m = 0; m < 4; ++m)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[(16 * m + 4 * (lane >> 4) + i) * 64 + 16 * w + (lane & 15)] = x[m][i];
+}
 // What a segment starts from: the states of the scan, or the call's own where there is but one segment.
 struct From {
   const float* p;
@@ -394,11 +439,10 @@ __global__ __launch_bounds__(kThr) void k_decay_sum(DecayArgs a, DecaySegments s
     const int n = i / each, ch = BACK ? x.last - 1 - n : x.first + n;
     if (i) lds_sync();
     if (i % each == 0) gates.form(dec, a, x, n, BACK ? -1 : 1, w, lane);
-    const int live = min(64, a.N - 64 * ch);
-    ai.store(A, a.D, live, t);
-    bi.store(B, a.DV, live, t);
+    ai.store(A, t);
+    bi.store(B, t);
     lds_sync();
-    if (i + 1 < count) fetch(i + 1);
+    fetch(min(i + 1, count - 1));
     const Decays& d = dec[n % kSlots];
     if (i % each == 0) {
       decay_state(s, d.end, sg);
@@ -406,7 +450,7 @@ __global__ __launch_bounds__(kThr) void k_decay_sum(DecayArgs a, DecaySegments s
     }
     add_outer<3>(s, A, B, BACK ? d.since : d.until, BACK ? a.scale : 1.f, w, lane);
   }
-  store_state<false>(s, D + (size_t)blockIdx.x * kTile2, 64, 64, w, lane);
+  store_tile(s, D + (size_t)blockIdx.x * kTile2, w, lane);
   float y[2];
   in_two(exp2(log), y);
   if (t == 0) G[2 * blockIdx.x] = y[0], G[2 * blockIdx.x + 1] = y[1];
@@ -471,14 +515,14 @@ __global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 4 : 2) void k_decay_out(De
   State s;
   load_state<false>(s, from.of(sg, x), from.rows, from.cols, w, lane);
   Coming<NP, T> ki, vi;
-  Frag<NP> next[2];
+  ComingRow<T> next;
   auto fetch = [&](int ch) {
     const int tok0 = 64 * ch, live = min(64, a.N - tok0);
     ki.fetch(rows_of<T>(a.k, x.b, x.h / (a.Hv / a.Hk), tok0), a.k.n, a.D, live, t);
     vi.fetch(rows_of<T>(a.v, x.b, x.h, tok0), a.v.n, a.DV, live, t);
   };
   auto fetch_q = [&](int ch, int o) {
-    own_row(next, rows_of<T>(a.q, x.b, o / (a.H / a.Hq), 64 * ch), a.q.n, a.D, min(own, a.N - 64 * ch - 1), g);
+    next.fetch(rows_of<T>(a.q, x.b, o / (a.H / a.Hq), 64 * ch), a.q.n, a.D, a.N - 64 * ch, own, g);
   };
   Gates gates;
   gates.fetch(a, x, 0, 1, w, lane);
@@ -489,21 +533,19 @@ __global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 4 : 2) void k_decay_out(De
     lane = here(lane), t = here(t);
     if (n) lds_sync();
     gates.form(dec, a, x, n, 1, w, lane);
-    ki.store(K, a.D, live, t);
-    vi.store(V, a.DV, live, t);
+    ki.store(K, t);
+    vi.store(V, t);
     put_state(S, s, w, lane);
-    if (states && part == 0) store_state<false>(s, states + ((size_t)x.u * a.NC + ch) * kTile2, 64, 64, w, lane);
+    if (states && part == 0) store_tile(s, states + ((size_t)x.u * a.NC + ch) * kTile2, w, lane);
     lds_sync();
-    if (ch + 1 < x.last) fetch(ch + 1);
+    fetch(min(ch + 1, x.last - 1));
     const Decays& d = dec[n % kSlots];
     const float since = a.scale * d.since[own], hi = d.hi[own], lo = d.lo[own];
-    for (int o = o0; o < o1; ++o) {
+    int o = o0;
+    do {  // once at least: what is in flight behind it can be counted
       lane = here(lane);
-      const Frag<NP> qf[2] = {next[0], next[1]};
-      if (o + 1 < o1)
-        fetch_q(ch, o + 1);
-      else if (ch + 1 < x.last)
-        fetch_q(ch + 1, o0);
+      const Frag<NP> qf[2] = {next.x[0].template parts<NP>(), next.x[1].template parts<NP>()};
+      fetch_q(o + 1 < o1 ? ch : min(ch + 1, x.last - 1), o + 1 < o1 ? o + 1 : o0);
       Half<NP> p[4] = {};
 #pragma unroll
       for (int m = 0; m < 4; ++m) {
@@ -519,7 +561,7 @@ __global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 4 : 2) void k_decay_out(De
       }
       phase();
       const Frag<NP> p0 = both(p[0], p[1]), p1 = both(p[2], p[3]);
-      T* dst = out + (((size_t)x.b * a.H + o) * a.N + tok0) * a.DV;
+      const Window dst(out + (((size_t)x.b * a.H + o) * a.N + tok0) * a.DV);
 #pragma unroll
       for (int m = 0; m < 4; ++m) {
         f32x4 y = {};
@@ -528,9 +570,9 @@ __global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 4 : 2) void k_decay_out(De
         y *= since;
         y = mma(col_frag_perm(V, 16 * m, 0, lane), p0, y);
         if (w >= 2) y = mma(col_frag_perm(V, 16 * m, 1, lane), p1, y);
-        if (own < live && 16 * m + 4 * g < a.DV) store4(shared_at(dst, __umul24(own, a.DV) + 16 * m + 4 * g), y);
+        put4(dst, out, own < live && 16 * m + 4 * g < a.DV, __umul24(own, a.DV) + 16 * m + 4 * g, y);
       }
-    }
+    } while (++o < o1);
     if (ch + 1 < x.last || UP == 3) {
       decay_state(s, d.end, sg);
       add_outer<UP>(s, K, V, d.until, 1.f, w, lane);
@@ -583,7 +625,7 @@ __global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 2 : 1) void k_decay_bwd(
   };
   State before;
   auto fetch_state = [&](int ch) {
-    load_state<true>(before, states + ((size_t)x.u * a.NC + ch) * kTile2, 64, 64, w, lane);
+    load_tile(before, states + ((size_t)x.u * a.NC + ch) * kTile2, w, lane);
   };
   Gates gates;
   gates.fetch(a, x, 0, -1, w, lane);
@@ -594,13 +636,13 @@ __global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 2 : 1) void k_decay_bwd(
     const int n = x.last - 1 - ch, tok0 = 64 * ch, live = min(64, a.N - tok0), turn = n & 1;
     lane = here(lane), t = here(t);
     gates.form(dec, a, x, n, -1, w, lane);
-    ki.store(K, a.D, live, t);
-    vi.store(V, a.DV, live, t);
-    qi.store(Q, a.D, live, t);
-    oi.store(O, a.DV, live, t);
+    ki.store(K, t);
+    vi.store(V, t);
+    qi.store(Q, t);
+    oi.store(O, t);
     put_state(X, s, w, lane);
     lds_sync();
-    if (ch > x.first) fetch_k(ch - 1);
+    fetch_k(max(ch - 1, x.first));
     const Decays& d = dec[n % kSlots];
     const float hi = d.hi[own], lo = d.lo[own], since = a.scale * d.since[own];
     f32x4 wk[4], wv[4];
@@ -634,19 +676,17 @@ __global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 2 : 1) void k_decay_bwd(
     through = wave_sum(through);
     lds_sync();
     put_state(X, before, w, lane);
-    if (ch > x.first) fetch_state(ch - 1);
-    for (int o = o0; o < o0 + each; ++o) {
+    fetch_state(max(ch - 1, x.first));
+    int o = o0;
+    do {
       lane = here(lane), t = here(t);
       if (o > o0) {
         lds_sync();
-        qi.store(Q, a.D, live, t);
-        oi.store(O, a.DV, live, t);
+        qi.store(Q, t);
+        oi.store(O, t);
       }
       lds_sync();
-      if (o + 1 < o0 + each)
-        fetch(ch, o + 1);
-      else if (ch > x.first)
-        fetch(ch - 1, o0);
+      fetch(o + 1 < o0 + each ? ch : max(ch - 1, x.first), o + 1 < o0 + each ? o + 1 : o0);
       {
         // queries: own
         const Frag<NP> qf[2] = {row_frag(Q, 16 * w, 0, lane), row_frag(Q, 16 * w, 1, lane)};
@@ -686,13 +726,12 @@ __global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 2 : 1) void k_decay_bwd(
           for (int i = 0; i < 4; ++i) decay += q[i] * y[i];
           y = mma(col_frag_perm(K, 16 * m, 0, lane), p0, y);
           if (w >= 2) y = mma(col_frag_perm(K, 16 * m, 1, lane), p1, y);
-          if (own < live && 16 * m + 4 * g < a.D) {
-            const uint32_t to = __umul24(own, a.D) + 16 * m + 4 * g;
-            if (dqh)
-              store4(shared_at(dqh + at, to), y);
-            else
-              store4(shared_at(dq + at, to), y);
-          }
+          const bool in = own < live && 16 * m + 4 * g < a.D;
+          const uint32_t to = __umul24(own, a.D) + 16 * m + 4 * g;
+          if (dqh)
+            put4(Window(dqh + at), dqh, in, to, y);
+          else
+            put4(Window(dq + at), dq, in, to, y);
         }
       }
       phase();
@@ -732,18 +771,17 @@ __global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 2 : 1) void k_decay_bwd(
         }
       }
       if (ch > x.first || (dstate && sg.count == 1)) add_outer<3>(s, O, Q, d.since, a.scale, w, lane);
-    }
+    } while (++o < o0 + each);
     const size_t at = (size_t)x.u * a.N + tok0;
 #pragma unroll
     for (int m = 0; m < 4; ++m) {
       const int e = 16 * m + 4 * g;
-      if (own < live && e < a.D) {
-        if (dkh)
-          store4(shared_at(dkh + at * a.D, __umul24(own, a.D) + e), wk[m]);
-        else
-          store4(shared_at(dk + at * a.D, __umul24(own, a.D) + e), wk[m]);
-      }
-      if (own < live && e < a.DV) store4(shared_at(dv + at * a.DV, __umul24(own, a.DV) + e), wv[m]);
+      const uint32_t to = __umul24(own, a.D) + e;
+      if (dkh)
+        put4(Window(dkh + at * a.D), dkh, own < live && e < a.D, to, wk[m]);
+      else
+        put4(Window(dk + at * a.D), dk, own < live && e < a.D, to, wk[m]);
+      put4(Window(dv + at * a.DV), dv, own < live && e < a.DV, __umul24(own, a.DV) + e, wv[m]);
     }
     decay = group_sum(decay);
     passed = group_sum(passed);

@@ -1745,7 +1745,7 @@ static int decay_args(oal::DecayArgs* a, const char* what, const void* q, const 
     return fail(std::string(what) + ": rows must be 16-byte aligned");
   // 32-bit offsets inside a tile of 64 rows
   for (const oal::Strided* r : {&a->q, &a->k, &a->v})
-    if (seq_len > 1 && (r->n < 0 || r->n >= (1 << 24))) return fail(std::string(what) + ": rows are too far apart");
+    if (seq_len > 1 && (r->n < 0 || r->n >= (1 << 23))) return fail(std::string(what) + ": rows are too far apart");
   return 0;
 }
 

@@ -100,12 +100,18 @@ def _validate(q, k, v, g, state, name: str) -> None:
             raise ValueError(f"{name} must be on the same device as q")
 
 
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """t as the kernels read it; rows that lie very far apart are copied together."""
+    t = _native.row_tensor(t)
+    return t if t.stride(2) < 1 << 23 or t.shape[2] == 1 else t.contiguous()
+
+
 class _DecayFunction(torch.autograd.Function):
     """(q, k, v, g, state or None, scale) -> (out, final state); dimensions multiples of 8, on one ROCm device."""
 
     @staticmethod
     def forward(ctx: Any, q, k, v, g, state, scale: float):
-        q, k, v = map(_native.row_tensor, (q, k, v))
+        q, k, v = map(_rows, (q, k, v))
         start = None if state is None else _native._aligned(state.contiguous())
         keep = any(ctx.needs_input_grad)
         out, final, saved = _native.decay_forward(q, k, v, g, start, scale=scale, keep=keep)

@@ -91,7 +91,7 @@ def test_c_entries_check_before_they_launch():
     assert forward(q=odd) and b"16-byte" in lib.oal_last_error()
     assert forward(strides=(ctypes.c_int64 * 12)(*[63] * 12)) and b"16-byte" in lib.oal_last_error()
     assert forward(out=odd) and b"16-byte" in lib.oal_last_error()
-    assert forward(strides=(ctypes.c_int64 * 12)(*[1 << 24] * 12)) and b"too far apart" in lib.oal_last_error()
+    assert forward(strides=(ctypes.c_int64 * 12)(*[1 << 23] * 12)) and b"too far apart" in lib.oal_last_error()
     rc = lib.oal_decay_backward(p, p, p, p, rows, 0, 1, 2, 2, 2, 64, 64, 64, 1, 0.1, p, None, None, p, p, p, p, None, p, None)
     assert rc and b"null" in lib.oal_last_error()
     rc = lib.oal_decay_backward(p, p, p, p, rows, 0, 1, 2, 2, 2, 64, 64, 64, 1, 0.1, p, odd, None, p, p, p, p, None, p, None)
