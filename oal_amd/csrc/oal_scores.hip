@@ -103,26 +103,62 @@ __device__ __forceinline__ void insert(Best& b, float x, uint32_t i) {
   b.at = prev ? pi : behind ? i : b.at;
 }
 
+// The value of the lane `WITH` away (lane ^ WITH), by lane moves alone: through LDS a step of the network below would
+// wait for its answer.
+template <int WITH>
+__device__ __forceinline__ uint32_t partner(uint32_t x, int lane) {
+  auto move = [](uint32_t v, auto how) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(how)::value, 0xf, 0xf, true);
+  };
+  if constexpr (WITH == 1)
+    return move(x, std::integral_constant<int, 0xb1>());  // quad_perm:[1,0,3,2]
+  else if constexpr (WITH == 2)
+    return move(x, std::integral_constant<int, 0x4e>());  // quad_perm:[2,3,0,1]
+  else if constexpr (WITH == 4)  // lane ^ 7 (row_half_mirror), then ^ 3 (quad_perm:[3,2,1,0])
+    return move(move(x, std::integral_constant<int, 0x141>()), std::integral_constant<int, 0x1b>());
+  else if constexpr (WITH == 8)
+    return move(x, std::integral_constant<int, 0x128>());  // row_ror:8
+  else if constexpr (WITH == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    return lane & 16 ? r[0] : r[1];
+  } else {
+    const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return lane & 32 ? r[0] : r[1];
+  }
+}
 // One step of a sorting network: the lane keeps the earlier or the later of its own and its partner's.
-__device__ __forceinline__ void exchange(float& x, uint32_t& i, int with, bool earlier) {
-  const float y = __shfl_xor(x, with, 64);
-  const uint32_t j = __shfl_xor(i, with, 64);
+template <int WITH>
+__device__ __forceinline__ void exchange(float& x, uint32_t& i, bool earlier, int lane) {
+  const float y = __uint_as_float(partner<WITH>(__float_as_uint(x), lane));
+  const uint32_t j = partner<WITH>(i, lane);
   if (before(y, j, x, i) == earlier) x = y, i = j;
 }
-// All lanes: each lane's value x of place i (or none: -inf, 0xffffffff) into the list. Sorted from the last to the
-// first, they and the list are a sequence that falls and rises, whose 64 highest six steps put in order. Values with
-// equal places are empty ones and change nothing, whichever is taken.
-__device__ __forceinline__ void merge(Best& b, float x, uint32_t i, int lane) {
-#pragma unroll
-  for (int k = 2; k <= 64; k <<= 1)
-#pragma unroll
-    for (int n = k >> 1; n > 0; n >>= 1) exchange(x, i, n, ((lane & n) == 0) != ((lane & k) == 0));
+// Steps of WITH, WITH / 2, ... 1 lanes, towards earlier in the lower lanes where `down`.
+template <int WITH>
+__device__ __forceinline__ void settle(float& x, uint32_t& i, bool down, int lane) {
+  exchange<WITH>(x, i, ((lane & WITH) == 0) == down, lane);
+  if constexpr (WITH > 1) settle<WITH / 2>(x, i, down, lane);
+}
+// All lanes: values x of places i (or none: -inf, 0xffffffff), sorted from the last to the first, into the list. They
+// and the list are a sequence that falls and rises, whose 64 highest six steps put in order. Values with equal places
+// are empty ones and change nothing, whichever is taken.
+__device__ __forceinline__ void merge_sorted(Best& b, float x, uint32_t i, int lane) {
   if (before(x, i, b.x, b.at)) b.x = x, b.at = i;
-#pragma unroll
-  for (int n = 32; n > 0; n >>= 1) exchange(b.x, b.at, n, (lane & n) == 0);
+  settle<32>(b.x, b.at, true, lane);
+}
+// The same, in any order.
+__device__ __forceinline__ void merge(Best& b, float x, uint32_t i, int lane) {
+  settle<1>(x, i, lane & 2, lane);
+  settle<2>(x, i, lane & 4, lane);
+  settle<4>(x, i, lane & 8, lane);
+  settle<8>(x, i, lane & 16, lane);
+  settle<16>(x, i, lane & 32, lane);
+  settle<32>(x, i, false, lane);
+  merge_sorted(b, x, i, lane);
 }
 
-constexpr int kMerge = 6;  // lanes with a value to merge from which that is faster than one by one
+constexpr int kJoin = 16;  // waves that join the parts' lists
+constexpr int kMerge = 12;  // lanes with a value to merge from which that is faster than one by one
 
 // Each lane's N values of places i, i + 1, ... (`in`: it has some); `most` is their maximum.
 template <int N>
@@ -148,7 +184,6 @@ __device__ __forceinline__ void offer(Best& b, float (&x)[N], float most, uint32
     }
     b.last = lane_f(b.x, top - 1);
     b.last_at = lane_u(b.at, top - 1);
-#pragma unroll
     for (int n = 0; n < N; ++n)
       if (take && n == (int)e) x[n] = __builtin_nanf("");
   }
@@ -161,7 +196,7 @@ struct Part {
 
 template <typename T>
 constexpr int kPiece = 16 / sizeof(T);
-constexpr int kTurn = 4;  // pieces of a lane in flight at once
+constexpr int kTurn = 3;  // pieces of a lane in flight at once
 
 // 16 bytes of a row, at any address of its type: rows of an odd vocabulary begin where they may.
 template <typename T>
@@ -220,34 +255,35 @@ __device__ __forceinline__ const T* row_at(const ScoreArgs& a, int64_t row) {
   return static_cast<const T*>(a.logits) + row / a.N * a.b + row % a.N * a.n;
 }
 
-// The waves' lists in LDS become one: every entry counts those that come before it, and its count is its
-// place. Empty entries are alike and come in the order that they stand in.
-__device__ __forceinline__ void place_best(const float* x, const uint32_t* at, int top, const auto& put_at) {
-  for (int i = threadIdx.x; i < kWaves * top; i += kThr) {
-    const float v = x[i];
-    const uint32_t j = at[i];
-    int rank = 0;
-    for (int n = 0; n < kWaves * top; ++n) rank += before(x[n], at[n], v, j) || (at[n] == j && n < i);
-    if (rank < top) put_at(rank, v, j);
-  }
+// The lists of a block's W waves become the first wave's, half of them into the other half at a time.
+template <int W>
+struct Lists {
+  float x[W][64];
+  uint32_t at[W][64];
+};
+template <int W, int HALF = W / 2>
+__device__ __forceinline__ void join_lists(Best& b, Lists<W>& lists, int w, int lane) {
+  if (w >= HALF && w < 2 * HALF) lists.x[w][lane] = b.x, lists.at[w][lane] = b.at;
+  __syncthreads();
+  if (w < HALF) merge_sorted(b, lists.x[w + HALF][63 - lane], lists.at[w + HALF][63 - lane], lane);
+  if constexpr (HALF > 1) join_lists<W, HALF / 2>(b, lists, w, lane);
 }
 
-// A row's results from its sums and the waves' lists.
+// A row's results from its sums and the first wave's list.
 template <typename T, bool ENTROPY, bool TOP>
 __device__ __forceinline__ void finish(const ScoreArgs& a, const ScoreOut& out, int64_t row, const Sums& sum,
-                                       const float* bx, const uint32_t* bi) {
+                                       const Best& b) {
+  const int t = threadIdx.x;
   const float log = logf(sum.s);
-  if (threadIdx.x == 0) {
+  if (t == 0) {
     const int64_t token = a.tokens[row];
     out.logp[row] = token < 0 ? 0.f : token < a.V ? get(row_at<T>(a, row) + token) - sum.m - log : __builtin_nanf("");
     if (ENTROPY) out.entropy[row] = log - sum.t / sum.s;
     if (out.saved) out.saved[2 * row] = sum.m, out.saved[2 * row + 1] = sum.s;
   }
-  if constexpr (TOP) {
-    place_best(bx, bi, a.top, [&](int rank, float v, uint32_t j) {
-      out.top[row * a.top + rank] = v - sum.m - log;
-      out.place[row * a.top + rank] = j == 0xffffffffu ? -1 : (int64_t)j;
-    });
+  if (TOP && t < a.top) {
+    out.top[row * a.top + t] = b.x - sum.m - log;
+    out.place[row * a.top + t] = b.at == 0xffffffffu ? -1 : (int64_t)b.at;
   }
 }
 
@@ -259,8 +295,7 @@ __global__ __launch_bounds__(kThr) void k_scores(ScoreArgs a, ScoreOut out, int 
                                                  float* __restrict__ best, uint32_t* __restrict__ best_at) {
   constexpr int P = kPiece<T>;
   __shared__ Sums shared[kWaves];
-  __shared__ float bx[TOP ? kWaves * kMostTop : 1];
-  __shared__ uint32_t bi[TOP ? kWaves * kMostTop : 1];
+  __shared__ Lists<TOP ? kWaves : 1> lists;
   const int t = threadIdx.x, lane = t & 63, w = wave_of(t);
   const int64_t row = blockIdx.x / parts;
   const int part = blockIdx.x % parts;
@@ -282,13 +317,14 @@ __global__ __launch_bounds__(kThr) void k_scores(ScoreArgs a, ScoreOut out, int 
 #pragma unroll
     for (int n = 0; n < kTurn; ++n) {
       const int64_t p = i + n * kThr + lane;
-      if (p - lane >= end) break;
-      float v[P];
-      values(v, raw[n]);
-      if (p >= end)
+      if (p - lane < end) {
+        float v[P];
+        values(v, raw[n]);
+        if (p >= end)
 #pragma unroll
-        for (int e = 0; e < P; ++e) v[e] = -INFINITY;
-      take(v, (uint32_t)(p * P), p < end);
+          for (int e = 0; e < P; ++e) v[e] = -INFINITY;
+        take(v, (uint32_t)(p * P), p < end);
+      }
     }
   }
   // values behind the last whole piece
@@ -303,37 +339,46 @@ __global__ __launch_bounds__(kThr) void k_scores(ScoreArgs a, ScoreOut out, int 
     join(mine, other);
   }
   if (lane == 0) shared[w] = mine;
-  if constexpr (TOP) {
-    if (lane < a.top) bx[w * a.top + lane] = b.x, bi[w * a.top + lane] = b.at;
-  }
-  __syncthreads();
+  if constexpr (TOP) join_lists(b, lists, w, lane);
+  else __syncthreads();
+  if (w) return;
   mine = shared[0];
 #pragma unroll
   for (int n = 1; n < kWaves; ++n) join(mine, shared[n]);
   if (parts == 1) {
-    finish<T, ENTROPY, TOP>(a, out, row, mine, bx, bi);
+    finish<T, ENTROPY, TOP>(a, out, row, mine, b);
     return;
   }
   if (t == 0) sums[blockIdx.x] = {mine.m, mine.s, mine.t, 0.f};
-  if constexpr (TOP) {
-    // the waves' lists as they are: the join puts them in order
-    for (int i = t; i < kWaves * a.top; i += kThr) {
-      best[(size_t)blockIdx.x * kWaves * a.top + i] = bx[i];
-      best_at[(size_t)blockIdx.x * kWaves * a.top + i] = bi[i];
-    }
+  if (TOP && t < a.top) {
+    best[(size_t)blockIdx.x * a.top + t] = b.x;
+    best_at[(size_t)blockIdx.x * a.top + t] = b.at;
   }
 }
 
-// The parts of one row, joined: a wave's list takes a quarter of theirs, 64 entries at once.
+// The parts of one row, joined. A wave takes every kJoin-th part's list; without lists one wave is enough.
 template <typename T, bool ENTROPY, bool TOP>
-__global__ __launch_bounds__(kThr) void k_scores_join(ScoreArgs a, ScoreOut out, int parts, const Part* __restrict__ sums,
-                                                      const float* __restrict__ best,
-                                                      const uint32_t* __restrict__ best_at) {
-  __shared__ float bx[TOP ? kWaves * kMostTop : 1];
-  __shared__ uint32_t bi[TOP ? kWaves * kMostTop : 1];
+__global__ __launch_bounds__(64 * kJoin) void k_scores_join(ScoreArgs a, ScoreOut out, int parts,
+                                                            const Part* __restrict__ sums,
+                                                            const float* __restrict__ best,
+                                                            const uint32_t* __restrict__ best_at) {
+  __shared__ Lists<TOP ? kJoin : 1> lists;
   const int t = threadIdx.x, lane = t & 63, w = wave_of(t);
   const int64_t row = blockIdx.x;
-  // every wave has all sums, of at most 64 parts
+  Best b;
+  if constexpr (TOP) {
+    for (int part = w; part < parts; part += kJoin) {
+      const int n = 63 - lane;
+      const int64_t at = (row * parts + part) * a.top + n;
+      float x = -INFINITY;
+      uint32_t i = 0xffffffffu;
+      if (n < a.top) x = best[at], i = best_at[at];
+      merge_sorted(b, x, i, lane);
+    }
+    join_lists(b, lists, w, lane);
+  }
+  if (w) return;
+  // of at most 64 parts
   Sums mine = kNothing;
   if (lane < parts) {
     const Part x = sums[row * parts + lane];
@@ -344,19 +389,7 @@ __global__ __launch_bounds__(kThr) void k_scores_join(ScoreArgs a, ScoreOut out,
     const Sums other = {__shfl_xor(mine.m, off, 64), __shfl_xor(mine.s, off, 64), __shfl_xor(mine.t, off, 64)};
     join(mine, other);
   }
-  if constexpr (TOP) {
-    const int count = parts * kWaves * a.top;
-    Best b;
-    for (int i = 64 * w; i < count; i += kThr) {
-      float v[1] = {-INFINITY};
-      uint32_t j = 0xffffffffu;
-      if (i + lane < count) v[0] = best[row * count + i + lane], j = best_at[row * count + i + lane];
-      offer<1>(b, v, v[0], j, j != 0xffffffffu, a.top, lane);
-    }
-    if (lane < a.top) bx[w * a.top + lane] = b.x, bi[w * a.top + lane] = b.at;
-    __syncthreads();
-  }
-  finish<T, ENTROPY, TOP>(a, out, row, mine, bx, bi);
+  finish<T, ENTROPY, TOP>(a, out, row, mine, b);
 }
 
 // The gradient of one part of one row.
@@ -414,7 +447,7 @@ int score_parts(const ScoreArgs& a) {
 size_t score_work_bytes(const ScoreArgs& a) {
   const int parts = score_parts(a);
   if (parts == 1) return 0;
-  return (size_t)a.B * a.N * parts * (sizeof(Part) + 8 * kWaves * a.top);
+  return (size_t)a.B * a.N * parts * (sizeof(Part) + 8 * a.top);
 }
 
 template <typename T>
@@ -423,14 +456,15 @@ void launch_scores(const ScoreArgs& a, const ScoreOut& out, void* work, hipStrea
   const int64_t rows = (int64_t)a.B * a.N;
   Part* sums = static_cast<Part*>(work);
   float* best = reinterpret_cast<float*>(sums + rows * parts);
-  uint32_t* best_at = reinterpret_cast<uint32_t*>(best + rows * parts * kWaves * a.top);
+  uint32_t* best_at = reinterpret_cast<uint32_t*>(best + rows * parts * a.top);
   auto launch = [&](auto kernel, auto second) {
     timed("k_scores", st, [&] {
       hipLaunchKernelGGL(kernel, dim3((unsigned)(rows * parts)), dim3(kThr), 0, st, a, out, parts, sums, best, best_at);
     });
     if (parts > 1)
       timed("k_scores_join", st, [&] {
-        hipLaunchKernelGGL(second, dim3((unsigned)rows), dim3(kThr), 0, st, a, out, parts, sums, best, best_at);
+        hipLaunchKernelGGL(second, dim3((unsigned)rows), dim3(a.top ? 64 * kJoin : 64), 0, st, a, out, parts, sums, best,
+                           best_at);
       });
   };
   if (a.top && a.entropy)
