@@ -97,19 +97,21 @@ def _unit_rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
 
 
+def _ready(q, k, v, q_weight, k_weight, cos, sin, positions):
+    """The operands as the kernels read them."""
+    return (*map(_unit_rows, (q, k, v)), *(None if w is None else w.contiguous() for w in (q_weight, k_weight)),
+            cos.contiguous(), sin.contiguous(), None if positions is None else positions.to(torch.int64).contiguous())
+
+
 class _NormRotaryFunction(torch.autograd.Function):
     """(q, k, v, q_weight, k_weight, cos, sin, positions, options) -> head-first (q, k, v), on one ROCm device."""
 
     @staticmethod
     def forward(ctx: Any, q, k, v, q_weight, k_weight, cos, sin, positions, options: dict):
         ctx.set_materialize_grads(False)
-        q, k, v = map(_unit_rows, (q, k, v))
-        q_weight, k_weight = (None if w is None else w.contiguous() for w in (q_weight, k_weight))
-        cos, sin = cos.contiguous(), sin.contiguous()
-        if positions is not None:
-            positions = positions.to(torch.int64).contiguous()
-        outs = _native.norm_rotary_forward(q, k, v, q_weight, k_weight, cos, sin, positions, **options)
-        ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, positions)
+        operands = _ready(q, k, v, q_weight, k_weight, cos, sin, positions)
+        outs = _native.norm_rotary_forward(*operands, **options)
+        ctx.save_for_backward(*operands[:2], *operands[3:])
         ctx.options = options
         return outs
 
@@ -145,7 +147,10 @@ def norm_rotary_heads(
     _native.require_eager("norm_rotary_heads", q, k, v, q_weight, k_weight, cos, sin, positions)
     _native._require_device(q)
     options = dict(q_heads=q_heads, kv_heads=kv_heads, eps=float(eps))
-    return _NormRotaryFunction.apply(q, k, v, q_weight, k_weight, cos, sin, positions, options)
+    operands = (q, k, v, q_weight, k_weight, cos, sin, positions)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in operands[:5]):
+        return _NormRotaryFunction.apply(*operands, options)
+    return _native.norm_rotary_forward(*_ready(*operands), **options)  # a step's host time is most of it
 
 
 __all__ = ("norm_rotary_heads",)

@@ -108,7 +108,11 @@ def token_log_probs(
     rows = logits if logits.ndim == 3 else logits[None] if logits.ndim == 2 else logits.reshape(1, -1, vocab)
     if rows.stride(2) != 1 and vocab > 1:
         rows = rows.contiguous()
-    scores = _TokenScoresFunction.apply(rows, tokens.reshape(rows.shape[:2]).to(torch.int64).contiguous(), entropy, top)
+    tokens = tokens.reshape(rows.shape[:2]).to(torch.int64).contiguous()
+    if torch.is_grad_enabled() and rows.requires_grad:
+        scores = _TokenScoresFunction.apply(rows, tokens, entropy, top)
+    else:  # a short call's host time is most of it
+        scores = _native.token_scores(rows, tokens, entropy=entropy, top=top, keep=False)[:4]
     return TokenScores(*(None if t is None else t.reshape((*shape, *t.shape[2:])) for t in scores))
 
 
