@@ -1842,8 +1842,8 @@ static int heads_args(oal::HeadsArgs* a, const char* what, const void* q, const 
     return fail(std::string(what) + ": the rotated dimensions must be an even number up to head_dim");
   if (table < 1 || (!position && table < seq_len))
     return fail(std::string(what) + ": the tables must have a row for every token");
-  // a grid's second dimension; tokens in 31 bits; a row's values
-  if (int64_t(q_heads) + 2 * int64_t(kv_heads) > 65535 || int64_t(batch) > ((int64_t(1) << 31) - 64) / seq_len)
+  // a grid's second dimension; its first one's threads, four to a token, in 32 bits
+  if (int64_t(q_heads) + 2 * int64_t(kv_heads) > 65535 || int64_t(batch) > ((int64_t(1) << 30) - 64) / seq_len)
     return fail("batch, heads and sequence length are too large for one launch");
   if (!q || !k || !v || !strides || !cosine || !sine) return fail(std::string(what) + ": null pointer argument");
   *a = {q, k, v, strides[0], strides[1], strides[2], strides[3], strides[4], strides[5], q_weight, k_weight, cosine, sine,

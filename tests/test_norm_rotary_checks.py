@@ -86,5 +86,6 @@ def test_c_entries_check_before_they_launch():
                          (dict(up=odd), b"16-byte")):
         assert backward(**change) and text in lib.oal_last_error(), change
     size = lib.oal_norm_rotary_heads_workspace_bytes
-    assert size(2, 4, 2, 5, 8, 0) > 0 and size(2, 4, 2, 5, 8, 1) == 3 * size(2, 4, 2, 5, 8, 0) and size(1, 1, 1, 1, 1, 0) > 0
+    # a float for each dimension of each weight row at least
+    assert size(2, 4, 2, 5, 8, 0) >= 2 * 8 * 4 and size(2, 4, 2, 5, 8, 1) >= 6 * 8 * 4 and size(1, 1, 1, 1, 1, 0) > 0
     assert size(2, 0, 2, 5, 8, 0) == 0 and b"positive" in lib.oal_last_error()
