@@ -314,6 +314,12 @@ __device__ __forceinline__ int here(int x) {
   return x;
 }
 
+// Parts of the scores inside a chunk. bf16 ones in two, off by 2^-16, as float16 ones: results are then off by their own
+// rounding and the states' (1.0 to 1.07 of it over 1 to 500 tokens; with scores of one part 1.4), in the same time:
+// 4 x 4096 tokens, forward and backward, 197 us either way.
+template <typename T>
+constexpr int kScoreParts = kPartsOf<T> == 1 ? 2 : kPartsOf<T>;
+
 // A state in accumulators, four tiles of a wave's 16 columns: S[m][i] is row 16 m + 4 g + i of column 16 w + c.
 typedef f32x4 State[4];
 // x += A^T (by B) over the rows of two tiles, A's columns the rows of x and B's 16 w .. the wave's columns.
@@ -494,8 +500,9 @@ __global__ __launch_bounds__(kThr) void k_decay_scan(Scan a) {
 
 // The outputs of one segment for `each` output heads of a state head, chunk by chunk, with the state in
 // accumulators and, as bf16 parts, in LDS. Outputs are transposed: a wave's 16 queries
-// are the columns, so the scores are an operand of the product with V as they are. bf16 tensors take
-// scores and states as they round to bf16, as the output itself rounds; fp16 tensors take them in two parts.
+// are the columns, so the scores are an operand of the product with V as they are. Of bf16 tensors
+// the state's part of an output takes the state as it rounds to bf16, as the output itself rounds; fp16 tensors
+// take it in two parts.
 // UP: parts of what the state takes on, three where it goes on to the caller or (states: kept before every
 // chunk) to the backward, two where no further than the segment's own outputs.
 template <typename T, int UP>
@@ -503,7 +510,7 @@ __global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 4 : 2) void k_decay_out(De
                                                                               From from, T* __restrict__ out,
                                                                               float* __restrict__ final_state,
                                                                               float* __restrict__ states) {
-  constexpr int NP = kPartsOf<T>;
+  constexpr int NP = kPartsOf<T>, SP = kScoreParts<T>;
   __shared__ Tile<NP> K, V;
   __shared__ Tile<NP> S;  // rows: values
   __shared__ Decays dec[kSlots];
@@ -546,7 +553,7 @@ __global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 4 : 2) void k_decay_out(De
       lane = here(lane);
       const Frag<NP> qf[2] = {next.x[0].template parts<NP>(), next.x[1].template parts<NP>()};
       fetch_q(o + 1 < o1 ? ch : min(ch + 1, x.last - 1), o + 1 < o1 ? o + 1 : o0);
-      Half<NP> p[4] = {};
+      Half<SP> p[4] = {};
 #pragma unroll
       for (int m = 0; m < 4; ++m) {
         if (m > w) continue;
@@ -557,10 +564,10 @@ __global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 4 : 2) void k_decay_out(De
         if (m == w)
 #pragma unroll
           for (int i = 0; i < 4; ++i) y[i] = 4 * g + i <= c ? y[i] : 0.f;
-        p[m] = half_of<NP>(y);
+        p[m] = half_of<SP>(y);
       }
       phase();
-      const Frag<NP> p0 = both(p[0], p[1]), p1 = both(p[2], p[3]);
+      const Frag<SP> p0 = both(p[0], p[1]), p1 = both(p[2], p[3]);
       const Window dst(out + (((size_t)x.b * a.H + o) * a.N + tok0) * a.DV);
 #pragma unroll
       for (int m = 0; m < 4; ++m) {
@@ -591,19 +598,20 @@ __global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 4 : 2) void k_decay_out(De
 //     r_i = sum_(j < i) M_ij + scale e^(G_i) q_i.(S dO_i), c_j = sum_(i > j) M_ij, s_j = e^(G_63 - G_j) k_j.(dS' v_j),
 //     dg_t = sum_(i >= t) (r_i - c_i) + sum_(j < t) s_j + e^(G_63) <S, dS'>
 // A block walks back with dS' in its accumulators; S the forward has kept. Both take turns in one tile of LDS. All
-// products are transposed: a wave's 16 tokens are the columns. What goes into dq, dk and dv alone rounds
-// to bf16 for bf16 tensors, as these do themselves, and to two parts for fp16; dg sees all 24 bits.
+// products are transposed: a wave's 16 tokens are the columns. dg is a difference of large
+// sums and sees all 24 bits of the states, in three parts of X; dq, dk and dv take what is there.
 // ---------------------------------------------------------------------------
 template <typename T>
 __global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 2 : 1) void k_decay_bwd(
     DecayArgs a, DecaySegments sg, From from, const T* __restrict__ dout, const float* __restrict__ states,
     T* __restrict__ dq, float* __restrict__ dqh, T* __restrict__ dk, float* __restrict__ dkh, T* __restrict__ dv,
     float* __restrict__ dg, double* __restrict__ dgsum, float* __restrict__ dstate) {
-  constexpr int NP = kPartsOf<T>;
+  constexpr int NP = kPartsOf<T>, SP = kScoreParts<T>;
   __shared__ Tile<NP> K, V, Q, O;
   __shared__ Tile<3> X;  // rows: keys' dimensions
   __shared__ Decays dec[kSlots];
-  __shared__ float dG[2][64], ss[2][64], ends[2][4];
+  __shared__ float ss[2][64], ends[2][4];
+  __shared__ double dG[2][64];
   int t = threadIdx.x, lane = t & 63;
   const int w = wave_of(t), g = lane >> 4, c = lane & 15, own = 16 * w + c;
   const Course x(a, sg, blockIdx.x);
@@ -646,7 +654,7 @@ __global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 2 : 1) void k_decay_bwd(
     const Decays& d = dec[n % kSlots];
     const float hi = d.hi[own], lo = d.lo[own], since = a.scale * d.since[own];
     f32x4 wk[4], wv[4];
-    float passed = 0.f, decay = 0.f;  // s_j and r_j - c_j
+    float passed = 0.f;  // s_j
     {
       const Frag<NP> kf[2] = {row_frag(K, 16 * w, 0, lane), row_frag(K, 16 * w, 1, lane)};
       const Frag<NP> vf[2] = {row_frag(V, 16 * w, 0, lane), row_frag(V, 16 * w, 1, lane)};
@@ -687,11 +695,12 @@ __global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 2 : 1) void k_decay_bwd(
       }
       lds_sync();
       fetch(o + 1 < o0 + each ? ch : max(ch - 1, x.first), o + 1 < o0 + each ? o + 1 : o0);
+      float share = 0.f;  // r_j - c_j of a head
       {
         // queries: own
         const Frag<NP> qf[2] = {row_frag(Q, 16 * w, 0, lane), row_frag(Q, 16 * w, 1, lane)};
         const Frag<NP> of[2] = {row_frag(O, 16 * w, 0, lane), row_frag(O, 16 * w, 1, lane)};
-        Half<NP> p[4] = {};
+        Half<SP> p[4] = {};
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
           if (m > w) continue;
@@ -705,15 +714,15 @@ __global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 2 : 1) void k_decay_bwd(
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             if (m == w) {
-              decay += 4 * g + i < c ? y[i] * qk[i] : 0.f;
+              share += 4 * g + i < c ? y[i] * qk[i] : 0.f;
               y[i] = 4 * g + i <= c ? y[i] : 0.f;
             } else {
-              decay += y[i] * qk[i];
+              share += y[i] * qk[i];
             }
           }
-          p[m] = half_of<NP>(y);
+          p[m] = half_of<SP>(y);
         }
-        const Frag<NP> p0 = both(p[0], p[1]), p1 = both(p[2], p[3]);
+        const Frag<SP> p0 = both(p[0], p[1]), p1 = both(p[2], p[3]);
         const size_t at = (((size_t)x.b * a.H + o) * a.N + tok0) * a.D;
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
@@ -723,7 +732,7 @@ __global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 2 : 1) void k_decay_bwd(
           y *= since;
           const f32x4 q = own_values(Q, own, m, lane);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) decay += q[i] * y[i];
+          for (int i = 0; i < 4; ++i) share += q[i] * y[i];
           y = mma(col_frag_perm(K, 16 * m, 0, lane), p0, y);
           if (w >= 2) y = mma(col_frag_perm(K, 16 * m, 1, lane), p1, y);
           const bool in = own < live && 16 * m + 4 * g < a.D;
@@ -739,7 +748,7 @@ __global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 2 : 1) void k_decay_bwd(
         // keys: own
         const Frag<NP> kf[2] = {row_frag(K, 16 * w, 0, lane), row_frag(K, 16 * w, 1, lane)};
         const Frag<NP> vf[2] = {row_frag(V, 16 * w, 0, lane), row_frag(V, 16 * w, 1, lane)};
-        Half<NP> p[4] = {}, r[4] = {};
+        Half<SP> p[4] = {}, r[4] = {};
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
           if (m < w) continue;
@@ -755,11 +764,11 @@ __global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 2 : 1) void k_decay_bwd(
             for (int i = 0; i < 4; ++i) e[i] = c <= 4 * g + i ? e[i] : 0.f;
           ov *= e;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) decay -= m > w || c < 4 * g + i ? ov[i] * qk[i] : 0.f;
-          p[m] = half_of<NP>(ov);
-          r[m] = half_of<NP>(e * qk);
+          for (int i = 0; i < 4; ++i) share -= m > w || c < 4 * g + i ? ov[i] * qk[i] : 0.f;
+          p[m] = half_of<SP>(ov);
+          r[m] = half_of<SP>(e * qk);
         }
-        const Frag<NP> p0 = both(p[0], p[1]), p1 = both(p[2], p[3]), r0 = both(r[0], r[1]), r1 = both(r[2], r[3]);
+        const Frag<SP> p0 = both(p[0], p[1]), p1 = both(p[2], p[3]), r0 = both(r[0], r[1]), r1 = both(r[2], r[3]);
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
           if (w < 2) {
@@ -770,6 +779,9 @@ __global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 2 : 1) void k_decay_bwd(
           wv[m] = mma(col_frag_perm(O, 16 * m, 1, lane), r1, wv[m]);
         }
       }
+      // their sums over heads in 64 bits: in 32 dg is off by 8e-7 after seven heads, so by 3e-7
+      share = group_sum(share);
+      if (g == 0) dG[turn][own] = share + (o > o0 ? dG[turn][own] : 0.0);
       if (ch > x.first || (dstate && sg.count == 1)) add_outer<3>(s, O, Q, d.since, a.scale, w, lane);
     } while (++o < o0 + each);
     const size_t at = (size_t)x.u * a.N + tok0;
@@ -783,15 +795,14 @@ __global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 2 : 1) void k_decay_bwd(
         put4(Window(dk + at * a.D), dk, own < live && e < a.D, to, wk[m]);
       put4(Window(dv + at * a.DV), dv, own < live && e < a.DV, __umul24(own, a.DV) + e, wv[m]);
     }
-    decay = group_sum(decay);
     passed = group_sum(passed);
-    if (g == 0) dG[turn][own] = decay, ss[turn][own] = passed;
+    if (g == 0) ss[turn][own] = passed;
     if (lane == 0) ends[turn][w] = through;
     lds_sync();
     // one wave, another for each chunk; the next but one chunk writes these places again, behind a barrier
     if (w == n % 4) {
       // dg_t = sum of all r_i - c_i, and of s_j - (r_j - c_j) over j < t
-      const double mine = dG[turn][lane], past = lane ? (double)ss[turn][lane - 1] - (double)dG[turn][lane - 1] : 0.0;
+      const double mine = dG[turn][lane], past = lane ? (double)ss[turn][lane - 1] - dG[turn][lane - 1] : 0.0;
       const double all = lane_of(running_sum(mine), 63);
       double y = all + running_sum(past) + (((double)ends[turn][0] + ends[turn][1]) + ((double)ends[turn][2] + ends[turn][3]));
       // where nothing is kept nothing depends on g; the sums' roundings do not cancel

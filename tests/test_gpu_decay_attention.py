@@ -2,9 +2,10 @@
 
 Tolerances, as the norm of the error over the norm of the result, are counted in
 roundings. float32 results pass chains of two products of 64 terms each, 128
-roundings of at most 2^-24. A bf16 result is rounded once, by at most 2^-8, and its terms are
-bf16 values in two parts, off by at most 2^-16 each; a float16 one by at most
-2^-11, on top of the float32 chain and of terms in two parts."""
+roundings of at most 2^-24. A bf16 result is rounded once, by at most 2^-8, and so is the state that its
+share is taken from: both in the norm by 2^-8 / sqrt(3) at most, where values are spread over a step, together
+0.82 2^-8; its scores are in two parts, off by at most 2^-16 each. A float16 result is off by at most 2^-11, on top
+of the float32 chain and of scores and states in two parts."""
 
 import pytest
 import torch
