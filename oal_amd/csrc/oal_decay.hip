@@ -16,6 +16,12 @@
 //
 // Decays enter as differences of sums, held in two floats (48 bits): a token that
 // forgets everything (g of -inf, the first of a new text) leaves large sums whose differences still matter.
+//
+// 4 x 4096 tokens of 14/14/14 heads of 64, bf16, forward and backward: 191 us of kernels, of which the gradients are 98,
+// the outputs 39, both sums 35, both scans 14. What has to be read and written takes 47 us at the rate of a large copy. What
+// bounds it is the vector unit's work on operands (decays, splits into parts, fragments from LDS), some 1500
+// instructions a wave and chunk in the backward, and waiting for LDS between phases that depend on one another; the
+// matrix units are busy for less than a tenth. A prompt of 32768 tokens, 7/7/14 heads: 85 us, copied in 35.
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -414,7 +420,9 @@ struct From {
 }  // namespace
 
 // What a segment adds to the state, or (BACK) what its outputs ask of the state before it, over a state's
-// output heads: k, v or q, dO of its chunks, one after another; and its decay.
+// output heads: k, v or q, dO of its chunks, one after another; and its decay. 17 us over 4 x 4096 tokens (59 MB). The next
+// chunk is on its way while one is worked on; with the next two there the registers leave three waves a SIMD for
+// four, and training takes 187 us for 185.
 template <typename T, bool BACK>
 __global__ __launch_bounds__(kThr) void k_decay_sum(DecayArgs a, DecaySegments sg, const T* __restrict__ dout,
                                                     float* __restrict__ G, float* __restrict__ D) {
@@ -463,7 +471,8 @@ __global__ __launch_bounds__(kThr) void k_decay_sum(DecayArgs a, DecaySegments s
 }
 
 // S' = e S + D over the segments, or back over them; what a segment adds is replaced by the state
-// that it starts from (back: whose gradient it takes). A value per thread, the next ones on their way.
+// that it starts from (back: whose gradient it takes). A value per thread, the next ones on their way: 14 us
+// for both scans over 4 x 4096 tokens, 16 and 8 segments of 56 states (15 and 7 MB in and out again).
 struct Scan {
   const float* G;
   float* S;           // [U][segments][64][64]
@@ -504,7 +513,8 @@ __global__ __launch_bounds__(kThr) void k_decay_scan(Scan a) {
 // the state's part of an output takes the state as it rounds to bf16, as the output itself rounds; fp16 tensors
 // take it in two parts.
 // UP: parts of what the state takes on, three where it goes on to the caller or (states: kept before every
-// chunk) to the backward, two where no further than the segment's own outputs.
+// chunk) to the backward, two where no further than the segment's own outputs (32768 tokens: 51 us for 56).
+// In training 39 us over 4 x 4096 tokens, 117 MB of heads and 59 MB of states (4.5 TB/s).
 template <typename T, int UP>
 __global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 4 : 2) void k_decay_out(DecayArgs a, DecaySegments sg, int each,
                                                                               From from, T* __restrict__ out,
@@ -600,6 +610,7 @@ __global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 4 : 2) void k_decay_out(De
 // A block walks back with dS' in its accumulators; S the forward has kept. Both take turns in one tile of LDS. All
 // products are transposed: a wave's 16 tokens are the columns. dg is a difference of large
 // sums and sees all 24 bits of the states, in three parts of X; dq, dk and dv take what is there.
+// 98 us over 4 x 4096 tokens, 512 blocks at two a CU with all their registers (bf16: ten of them in scratch).
 // ---------------------------------------------------------------------------
 template <typename T>
 __global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 2 : 1) void k_decay_bwd(
@@ -933,12 +944,15 @@ void scan(const DecayArgs& a, const DecaySegments& sg, const float* G, float* S,
         [&] { hipLaunchKernelGGL(k_decay_scan, dim3(a.B * a.Hv * (kTile2 / kThr)), dim3(kThr), 0, st, s); });
 }
 
-// Heads of a state that one block of the forward takes: all, unless that leaves CUs without a block.
+// Heads of a state that one block of the forward takes: all, unless that leaves CUs without a block. The block's work on
+// the state is done for each part of the heads again.
 int heads_each(const DecayArgs& a, const DecaySegments& sg) {
   const int rep = a.H / a.Hv, blocks = a.B * a.Hv * sg.count, parts = std::clamp(1024 / blocks, 1, rep);
   return (rep + parts - 1) / parts;
 }
-// Segments so that `blocks` blocks have one each, the GPU's at once.
+// Segments so that `blocks` blocks have one each, those that the GPU holds at once: four a CU in the forward, two in the
+// backward. Forward with 512, 1024 and 2048 blocks: 98, 85 and 90 us for 32768 tokens, 189, 191 and 203 for training over
+// 4 x 4096; backward with 256, 512 and 1024: 241, 191 and 190.
 DecaySegments segments(int U, int NC, int blocks) {
   const int count = std::clamp(blocks / U, 1, NC), len = (NC + count - 1) / count;
   return {(NC + len - 1) / len, len};

@@ -13,6 +13,9 @@
 // and goes over heads, the next one's values on their way. The weights' gradients stay in registers
 // until a weight row ends; a block's go to memory, and a second kernel adds those up, in order.
 // Arithmetic and sums are in fp32, one rounding to the tensors' type.
+//
+// 4 x 4096 tokens, 14 query and 2 key heads of 64, bf16: forward 15 us (75 MB in and out, 5.1 TB/s), backward 22 and the
+// weights' sums 3 (109 MB, 4.3 TB/s). One token: 3.5 us, a launch and two waits for memory.
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -141,7 +144,7 @@ struct Part {
     const int64_t i = (int64_t)blockIdx.x * kTokens + (threadIdx.x >> 2), total = (int64_t)a.B * a.N;
     live = i < total;
     token = live ? i : total - 1;
-    b = (int)((uint32_t)token / (uint32_t)a.N);  // fewer than 2^31 tokens
+    b = (int)((uint32_t)token / (uint32_t)a.N);  // fewer than 2^30 tokens
     n = (int)(token - (int64_t)b * a.N);
     first = blockIdx.y * each;
     last = min(first + each, a.Hq + 2 * a.Hk);
@@ -295,7 +298,7 @@ __global__ __launch_bounds__(kSumThr) void k_heads_weights(const float* __restri
 }
 
 namespace {
-// Rows of 16-byte pieces: lanes move 8 values at once.
+// Rows of 16-byte pieces: lanes move 8 values at once. Value by value the sizes above take 87 and 120 us.
 bool wide(const HeadsArgs& a, int size) {
   if ((a.R / 2) % 8 || (a.D - a.R) % 16) return false;
   for (const void* p : {a.q, a.k, a.v, a.qw, a.kw, a.cosine, a.sine})
@@ -304,26 +307,29 @@ bool wide(const HeadsArgs& a, int size) {
     if (s * size % 16) return false;
   return true;
 }
-// Blocks for all tokens, and as many parts of the heads that the GPU has four blocks a CU.
+// Blocks for all tokens, and parts of the heads so that there are about `most` blocks: more parts read the tables
+// again, fewer leave CUs waiting. At the sizes above the forward takes 17 us with 512 or 2048, 15 with 1024;
+// the backward, whose parts leave sums behind, 22 and 3 with 512, 24 and 4 with 1024, 28 and 6 with 2048.
 struct Grid {
   int blocks, parts, each;
 };
-Grid heads_grid(const HeadsArgs& a) {
+Grid heads_grid(const HeadsArgs& a, int most) {
   const int heads = a.Hq + 2 * a.Hk, blocks = (int)(((int64_t)a.B * a.N + kTokens - 1) / kTokens);
-  const int each = std::max(1, (int)((int64_t)heads * blocks / 1024));
-  return {blocks, (heads + std::min(each, heads) - 1) / std::min(each, heads), std::min(each, heads)};
+  const int each = (int)std::clamp<int64_t>((int64_t)heads * blocks / most, 1, heads);
+  return {blocks, (heads + each - 1) / each, each};
 }
+constexpr int kForward = 1024, kBackward = 512;
 }  // namespace
 
 int heads_blocks(const HeadsArgs& a) {
-  const Grid g = heads_grid(a);
+  const Grid g = heads_grid(a, kBackward);
   return a.per_head ? g.blocks : g.blocks * g.parts;
 }
 
 template <typename T>
 void launch_heads_forward(const HeadsArgs& a, void* hq, void* hk, void* hv, hipStream_t st, const Timer& timed) {
   const auto kernel = wide(a, sizeof(T)) ? k_heads<T, true> : k_heads<T, false>;
-  const Grid g = heads_grid(a);
+  const Grid g = heads_grid(a, kForward);
   timed("k_heads", st, [&] {
     hipLaunchKernelGGL(kernel, dim3(g.blocks, g.parts), dim3(kThr), 0, st, a, g.each, static_cast<T*>(hq),
                        static_cast<T*>(hk), static_cast<T*>(hv));
@@ -334,7 +340,7 @@ template <typename T>
 void launch_heads_backward(const HeadsArgs& a, const void* hq, const void* hk, const void* hv, void* dq, void* dk,
                            void* dv, void* dqw, void* dkw, float* work, hipStream_t st, const Timer& timed) {
   const auto kernel = wide(a, sizeof(T)) ? k_heads_bwd<T, true> : k_heads_bwd<T, false>;
-  const Grid g = heads_grid(a);
+  const Grid g = heads_grid(a, kBackward);
   timed("k_heads_bwd", st, [&] {
     hipLaunchKernelGGL(kernel, dim3(g.blocks, g.parts), dim3(kThr), 0, st, a, g.each, static_cast<const T*>(hq),
                        static_cast<const T*>(hk), static_cast<const T*>(hv), static_cast<T*>(dq), static_cast<T*>(dk),

@@ -7,11 +7,16 @@
 //
 // Bound by memory: a row is read once, 16 bytes per lane, with running maxima and sums per lane that
 // are joined at the end. Rows are cut into parts where there are fewer than fill the GPU, and a
-// second kernel joins those. All of it is in fp32: differences to the maximum are exact for 16-bit logits.
+// second kernel joins those. All of it is in fp32: a difference to the maximum is one rounding, an exponential two more.
+//
+// 2 x 1000 rows of 151936 bf16 logits with the entropy: forward 157 us (608 MB, 3.9 TB/s), gradient 229 us (1216 MB,
+// 5.3 TB/s). 4096 rows with five alternatives: 290 us (1245 MB, 4.3 TB/s); beside the loads a value costs about ten
+// instructions. One row with 20 alternatives: 12 us in 49 parts and 6 to join them, most of it the lists' beginnings;
+// 48 rows of 32003 fp32 logits in 10 parts each: 16 and 5.
 //
 // The alternatives: a wave keeps the highest 64 of its values so far in order, one per lane, and
 // looks at a value only if it comes before the last that counts; of equal values the first. A row of random
-// order changes that list some K log(V / K) times. Where several lanes have such a value they are
+// order changes that list some K log(V / K) times. Where many lanes have such a value they are
 // sorted and merged with the list at once, as at the beginning; else they move up the list one by one.
 
 #include <hip/hip_runtime.h>
@@ -157,8 +162,11 @@ __device__ __forceinline__ void merge(Best& b, float x, uint32_t i, int lane) {
   merge_sorted(b, x, i, lane);
 }
 
-constexpr int kJoin = 16;  // waves that join the parts' lists
-constexpr int kMerge = 12;  // lanes with a value to merge from which that is faster than one by one
+// Lanes with a value to merge from which that is faster than one by one: 4096 rows with five alternatives take 306 us with
+// 3, 294 with 6, 293 with 12 and 292 with 20.
+constexpr int kMerge = 12;
+// Waves that join the parts' lists, 4 to a wave at most: 6 us for one row; four waves, sorting them anew, took 17.
+constexpr int kJoin = 16;
 
 // Each lane's N values of places i, i + 1, ... (`in`: it has some); `most` is their maximum.
 template <int N>
@@ -196,7 +204,9 @@ struct Part {
 
 template <typename T>
 constexpr int kPiece = 16 / sizeof(T);
-constexpr int kTurn = 3;  // pieces of a lane in flight at once
+// Pieces of a lane in flight at once: with 1, 2, 3 and 4 the 4096 rows take 332, 298, 294 and 287 us, 2 x 1000 rows forward
+// and back 388, 388, 388 and 412.
+constexpr int kTurn = 3;
 
 // 16 bytes of a row, at any address of its type: rows of an odd vocabulary begin where they may.
 template <typename T>
@@ -392,7 +402,8 @@ __global__ __launch_bounds__(64 * kJoin) void k_scores_join(ScoreArgs a, ScoreOu
   finish<T, ENTROPY, TOP>(a, out, row, mine, b);
 }
 
-// The gradient of one part of one row.
+// The gradient of one part of one row: the logits once more, with the row's maximum and sum from the forward, and as many
+// bytes out; nothing else is kept from the forward, so that a loss takes no memory of the logits' size before it.
 template <typename T>
 __global__ __launch_bounds__(kThr) void k_scores_bwd(ScoreArgs a, int parts, const float* __restrict__ saved,
                                                      const float* __restrict__ entropy, const float* __restrict__ dlog,
@@ -438,7 +449,9 @@ __global__ __launch_bounds__(kThr) void k_scores_bwd(ScoreArgs a, int parts, con
 namespace {
 int score_parts(const ScoreArgs& a) {
   const int64_t rows = (int64_t)a.B * a.N;
-  // a part has a turn of the block's pieces or more, and a wave joins 64 parts at most
+  // Parts fill the GPU's 256 CUs four times; a part has a turn of the block's pieces or more, and a wave joins 64 parts at
+  // most. With twice or half as many blocks one row, 48 and 2000 take the same within 1%: 2000 rows in two parts
+  // each 383 us, whole 387.
   const int64_t most = std::max(1, a.V / (kThr * kTurn * 4));
   return (int)std::clamp<int64_t>((1024 + rows - 1) / rows, 1, std::min<int64_t>(most, 64));
 }
