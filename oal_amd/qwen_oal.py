@@ -342,6 +342,10 @@ def score_tokens(model: QwenOALModel, tokens: torch.Tensor, *, lengths: torch.Te
     the second and later ones, with the entropy of the distributions that they are from and ``top``
     alternatives if asked for (:func:`oal_amd.token_scores.token_log_probs`). lengths [B] (None: N each): the
     tokens of each sequence of a batch padded at its end; behind them log probabilities are zero."""
+    if tokens.ndim != 2:
+        raise ValueError("tokens must be [B, N]")
+    if lengths is not None and (lengths.shape != tokens.shape[:1] or lengths.is_floating_point()):
+        raise ValueError("lengths must be integers [B]")
     targets = tokens[:, 1:]
     if lengths is not None:
         places = torch.arange(1, tokens.shape[1], device=tokens.device)

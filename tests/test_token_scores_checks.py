@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from oal_amd import _native
+from oal_amd.qwen_oal import score_tokens
 from oal_amd.token_scores import token_log_probs
 
 _z = torch.zeros
@@ -65,3 +66,14 @@ def test_c_entries_check_before_they_launch():
         assert backward(**change) and text in lib.oal_last_error(), change
     assert lib.oal_token_scores_workspace_bytes(2, 5, 64, 2) > 0
     assert lib.oal_token_scores_workspace_bytes(2, 0, 64, 2) == 0 and b"positive" in lib.oal_last_error()
+
+
+@pytest.mark.parametrize("tokens,lengths", [
+    (torch.zeros(5, dtype=torch.int64), None),
+    (torch.zeros(2, 5, dtype=torch.int64), torch.tensor([3])),
+    (torch.zeros(2, 5, dtype=torch.int64), torch.tensor([[3, 4]])),
+    (torch.zeros(2, 5, dtype=torch.int64), torch.tensor([3.0, 4.0])),
+])
+def test_the_model_scores_batches_of_tokens(tokens, lengths):
+    with pytest.raises(ValueError, match=r"\[B"):
+        score_tokens(None, tokens, lengths=lengths)
