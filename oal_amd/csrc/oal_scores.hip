@@ -9,9 +9,9 @@
 // are joined at the end. Rows are cut into parts where there are fewer than fill the GPU, and a
 // second kernel joins those. All of it is in fp32: a difference to the maximum is one rounding, an exponential two more.
 //
-// 2 x 1000 rows of 151936 bf16 logits with the entropy: forward 157 us (608 MB, 3.9 TB/s), gradient 229 us (1216 MB,
-// 5.3 TB/s). 4096 rows with five alternatives: 290 us (1245 MB, 4.3 TB/s); beside the loads a value costs about ten
-// instructions. One row with 20 alternatives: 12 us in 49 parts and 6 to join them, most of it the lists' beginnings;
+// 2 x 1000 rows of 151936 bf16 logits with the entropy: forward 150 us (608 MB, 4.1 TB/s), gradient 229 us (1216 MB,
+// 5.3 TB/s). 4096 rows with five alternatives: 261 us (1245 MB, 4.8 TB/s). Beside the loads a value costs about ten
+// instructions, an exponential of four times the price among them. One row with 20 alternatives: 12 us in 49 parts and 6 to join them, most of it the lists' beginnings;
 // 48 rows of 32003 fp32 logits in 10 parts each: 16 and 5.
 //
 // The alternatives: a wave keeps the highest 64 of its values so far in order, one per lane, and
@@ -70,10 +70,13 @@ __device__ __forceinline__ float most_of(const float (&x)[N]) {
   for (int e = 1; e < N; ++e) most = fmaxf(most, x[e]);
   return most;
 }
-// Adds N values, the highest of them `most`.
+// Adds N values, the highest of them `most`. What they are taken relative to follows the maximum only where it is passed
+// by more than e^8: so it hardly ever does (276 us for 286 over 4096 rows), and sums of less than e^8 2^30 are as
+// exact as of less than 2^30.
+constexpr float kBeyond = 8.f;
 template <int N, bool ENTROPY>
 __device__ __forceinline__ void add(Sums& a, const float (&x)[N], float most) {
-  if (most > a.m) move_to(a, most);
+  if (most > a.m + kBeyond) move_to(a, most);
   const float m = a.m == -INFINITY ? 0.f : a.m;  // -inf values weigh nothing
 #pragma unroll
   for (int e = 0; e < N; ++e) {
@@ -162,16 +165,18 @@ __device__ __forceinline__ void merge(Best& b, float x, uint32_t i, int lane) {
   merge_sorted(b, x, i, lane);
 }
 
-// Lanes with a value to merge from which that is faster than one by one: 4096 rows with five alternatives take 306 us with
-// 3, 294 with 6, 293 with 12 and 292 with 20.
+// Lanes with a value to merge from which that is faster than one by one: 4096 rows with five alternatives took 306 us with
+// 3, 294 with 6, 293 with 12 and 292 with 20 before the other steps here.
 constexpr int kMerge = 12;
 // Waves that join the parts' lists, 4 to a wave at most: 6 us for one row; four waves, sorting them anew, took 17.
 constexpr int kJoin = 16;
 
-// Each lane's N values of places i, i + 1, ... (`in`: it has some); `most` is their maximum.
+// Each lane's N values of places i, i + 1, ... (`in`: it has some); `most` is their maximum. Another wave of the
+// row has as many values as count that are not below `limit`.
 template <int N>
-__device__ __forceinline__ void offer(Best& b, float (&x)[N], float most, uint32_t i, bool in, int top, int lane) {
-  if (!__ballot(in && before(most, i, b.last, b.last_at))) return;
+__device__ __forceinline__ void offer(Best& b, float (&x)[N], float most, uint32_t i, bool in, float limit, int top,
+                                      int lane) {
+  if (!__ballot(in && most >= limit && before(most, i, b.last, b.last_at))) return;
   // one value of each lane at a time, its highest; what has been looked at becomes NaN, which comes before nothing
   for (;;) {
     float v = -INFINITY;
@@ -179,7 +184,7 @@ __device__ __forceinline__ void offer(Best& b, float (&x)[N], float most, uint32
 #pragma unroll
     for (int n = 0; n < N; ++n)
       if (x[n] > v || (x[n] == v && e == N)) v = x[n], e = n;
-    const bool take = in && e < N && before(v, i + e, b.last, b.last_at);
+    const bool take = in && e < N && v >= limit && before(v, i + e, b.last, b.last_at);
     uint64_t who = __ballot(take);
     if (!who) return;
     if (__popcll(who) >= kMerge) {
@@ -204,8 +209,9 @@ struct Part {
 
 template <typename T>
 constexpr int kPiece = 16 / sizeof(T);
-// Pieces of a lane in flight at once: with 1, 2, 3 and 4 the 4096 rows take 332, 298, 294 and 287 us, 2 x 1000 rows forward
-// and back 388, 388, 388 and 412.
+// Pieces of a lane in flight at once, in the forward with as many of the next turn: with 2, 3 and 4 the 4096 rows take 254,
+// 261 and 258 us, 2 x 1000 rows forward 152, 150 and 145, back 230, 229 and 256, 48 short rows 20, 20 and 23. Without the
+// next turn on its way the forward takes 276 and 152.
 constexpr int kTurn = 3;
 
 // 16 bytes of a row, at any address of its type: rows of an odd vocabulary begin where they may.
@@ -310,36 +316,71 @@ __global__ __launch_bounds__(kThr) void k_scores(ScoreArgs a, ScoreOut out, int 
   const int64_t row = blockIdx.x / parts;
   const int part = blockIdx.x % parts;
   const T* x = row_at<T>(a, row);
-  const int64_t pieces = a.V / P, first = pieces * part / parts, end = pieces * (part + 1) / parts;
+  const int pieces = a.V / P, first = (int)((int64_t)pieces * part / parts), end = (int)((int64_t)pieces * (part + 1) / parts);
   Sums mine = kNothing;
   Best b;
+  // The waves tell one another the last value that counts, when they come to it: late news lets more through, no less
+  // (286 us for 303 over 4096 rows).
+  __shared__ float lasts[kWaves];
+  if constexpr (TOP) {
+    if (lane == 0) lasts[w] = -INFINITY;
+    __syncthreads();
+  }
+  float limit = -INFINITY;
+  auto hear = [&]() {
+    __hip_atomic_store(&lasts[w], b.last, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+#pragma unroll
+    for (int n = 0; n < kWaves; ++n)
+      limit = fmaxf(limit, __hip_atomic_load(&lasts[n], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP));
+  };
   auto take = [&](auto& v, uint32_t i, bool in) {
     constexpr int N = sizeof(v) / sizeof(v[0]);
     const float most = most_of(v);
     add<N, ENTROPY>(mine, v, most);
-    if constexpr (TOP) offer<N>(b, v, most, i, in, a.top, lane);
+    if constexpr (TOP) offer<N>(b, v, most, i, in, limit, a.top, lane);
   };
-  // whole waves, whose lanes past the end have nothing: a list belongs to all lanes
-  for (int64_t i = first + 64 * w; i < end; i += kTurn * kThr) {
-    Raw<T> raw[kTurn];
+  // A wave's turns: whole ones, of which the next is on its way, then piece by piece, with lanes past the end that have
+  // nothing: a list belongs to all lanes.
+  int i = first + 64 * w;
+  auto load = [&](Raw<T>(&raw)[kTurn], int from) {
 #pragma unroll
-    for (int n = 0; n < kTurn; ++n) raw[n] = load_raw(x + min(i + n * kThr + lane, end - 1) * P);
+    for (int n = 0; n < kTurn; ++n) raw[n] = load_raw(x + (int64_t)(from + n * kThr + lane) * P);
+  };
+  constexpr int kWhole = (kTurn - 1) * kThr + 64;
+  if (i + kWhole <= end) {
+    Raw<T> next[kTurn];
+    load(next, i);
+    do {
+      Raw<T> raw[kTurn];
 #pragma unroll
-    for (int n = 0; n < kTurn; ++n) {
-      const int64_t p = i + n * kThr + lane;
-      if (p - lane < end) {
+      for (int n = 0; n < kTurn; ++n) raw[n] = next[n];
+      const int after = i + kTurn * kThr;
+      load(next, after + kWhole <= end ? after : i);
+      if constexpr (TOP) hear();
+#pragma unroll
+      for (int n = 0; n < kTurn; ++n) {
         float v[P];
         values(v, raw[n]);
-        if (p >= end)
-#pragma unroll
-          for (int e = 0; e < P; ++e) v[e] = -INFINITY;
-        take(v, (uint32_t)(p * P), p < end);
+        take(v, (uint32_t)(i + n * kThr + lane) * P, true);
       }
-    }
+      i = after;
+    } while (i + kWhole <= end);
+  }
+#pragma unroll 1
+  for (; i < end; i += kThr) {
+    const int p = i + lane;
+    const Raw<T> raw = load_raw(x + (int64_t)min(p, end - 1) * P);
+    float v[P];
+    values(v, raw);
+    if (p >= end)
+#pragma unroll
+      for (int e = 0; e < P; ++e) v[e] = -INFINITY;
+    if constexpr (TOP) hear();
+    take(v, (uint32_t)p * P, p < end);
   }
   // values behind the last whole piece
   if (part == parts - 1 && w == kWaves - 1 && pieces * P < a.V) {
-    const int p = (int)pieces * P + lane;
+    const int p = pieces * P + lane;
     float v[1] = {p < a.V ? get(x + p) : -INFINITY};
     take(v, p, p < a.V);
   }
@@ -450,8 +491,7 @@ namespace {
 int score_parts(const ScoreArgs& a) {
   const int64_t rows = (int64_t)a.B * a.N;
   // Parts fill the GPU's 256 CUs four times; a part has a turn of the block's pieces or more, and a wave joins 64 parts at
-  // most. With twice or half as many blocks one row, 48 and 2000 take the same within 1%: 2000 rows in two parts
-  // each 383 us, whole 387.
+  // most. With twice or half as many blocks one row, 48 and 2000 take the same within 1%.
   const int64_t most = std::max(1, a.V / (kThr * kTurn * 4));
   return (int)std::clamp<int64_t>((1024 + rows - 1) / rows, 1, std::min<int64_t>(most, 64));
 }
