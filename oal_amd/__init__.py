@@ -12,7 +12,13 @@ Drop-in for the reference ``oal_attention`` operator surface:
 Beside it, for whole sequences and token by token:
 
 * ``oal_amd.gated_delta.gated_delta_attention`` / ``gated_delta_step``
+* ``oal_amd.decay_attention.decay_attention`` / ``decay_step``
 * ``oal_amd.window_attention.window_attention`` / ``window_attention_step`` / ``window_cache``
+
+Around them:
+
+* ``oal_amd.norm_rotary.norm_rotary_heads``
+* ``oal_amd.token_scores.token_log_probs``
 
 The arithmetic runs in ``liboal_amd.so`` (hand-written HIP kernels behind the
 C ABI in ``include/oal_amd.h``); PyTorch supplies device memory and streams.
