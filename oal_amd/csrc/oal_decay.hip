@@ -325,6 +325,11 @@ __device__ __forceinline__ int here(int x) {
 // 4 x 4096 tokens, forward and backward, 197 us either way.
 template <typename T>
 constexpr int kScoreParts = kPartsOf<T> == 1 ? 2 : kPartsOf<T>;
+// Parts of the states that 16-bit results read: two too, off by 2^-17, so that a result is rounded once, to its own
+// type. In one part bf16 outputs were 1.9e-3 off where a rounding is 1.7e-3 (32768 tokens, k_decay_out 51 us for 56);
+// three parts leave room for three blocks a CU in place of four (69 us).
+template <typename T>
+constexpr int kStateParts = kPartsOf<T> == 1 ? 2 : kPartsOf<T>;
 
 // A state in accumulators, four tiles of a wave's 16 columns: S[m][i] is row 16 m + 4 g + i of column 16 w + c.
 typedef f32x4 State[4];
@@ -508,10 +513,8 @@ __global__ __launch_bounds__(kThr) void k_decay_scan(Scan a) {
 }
 
 // The outputs of one segment for `each` output heads of a state head, chunk by chunk, with the state in
-// accumulators and, as bf16 parts, in LDS. Outputs are transposed: a wave's 16 queries
-// are the columns, so the scores are an operand of the product with V as they are. Of bf16 tensors
-// the state's part of an output takes the state as it rounds to bf16, as the output itself rounds; fp16 tensors
-// take it in two parts.
+// accumulators and, as bf16 parts (kStateParts), in LDS. Outputs are transposed: a wave's 16 queries
+// are the columns, so the scores are an operand of the product with V as they are.
 // UP: parts of what the state takes on, three where it goes on to the caller or (states: kept before every
 // chunk) to the backward, two where no further than the segment's own outputs (32768 tokens: 51 us for 56).
 // In training 39 us over 4 x 4096 tokens, 117 MB of heads and 59 MB of states (4.5 TB/s).
@@ -522,7 +525,7 @@ __global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 4 : 2) void k_decay_out(De
                                                                               float* __restrict__ states) {
   constexpr int NP = kPartsOf<T>, SP = kScoreParts<T>;
   __shared__ Tile<NP> K, V;
-  __shared__ Tile<NP> S;  // rows: values
+  __shared__ Tile<kStateParts<T>> S;  // rows: values
   __shared__ Decays dec[kSlots];
   int t = threadIdx.x, lane = t & 63;
   const int w = wave_of(t), g = lane >> 4, c = lane & 15, own = 16 * w + c;
@@ -609,7 +612,7 @@ __global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 4 : 2) void k_decay_out(De
 //     dg_t = sum_(i >= t) (r_i - c_i) + sum_(j < t) s_j + e^(G_63) <S, dS'>
 // A block walks back with dS' in its accumulators; S the forward has kept. Both take turns in one tile of LDS. All
 // products are transposed: a wave's 16 tokens are the columns. dg is a difference of large
-// sums and sees all 24 bits of the states, in three parts of X; dq, dk and dv take what is there.
+// sums and sees all 24 bits of the states, in three parts of X; so do dq and dk, and dv kStateParts.
 // 98 us over 4 x 4096 tokens, 512 blocks at two a CU with all their registers (bf16: ten of them in scratch).
 // ---------------------------------------------------------------------------
 template <typename T>
@@ -676,7 +679,7 @@ __global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 2 : 1) void k_decay_bwd(
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           y = mma(row_frag(X, 16 * m, i, lane), vf[i], y);
-          z = mma(col_frag<NP>(X, 16 * m, i, lane), kf[i], z);
+          z = mma(col_frag<kStateParts<T>>(X, 16 * m, i, lane), kf[i], z);
         }
         wk[m] = until * y;
         wv[m] = until * z;
