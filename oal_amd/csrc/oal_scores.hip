@@ -458,7 +458,8 @@ __global__ __launch_bounds__(kThr) void k_scores_bwd(ScoreArgs a, int parts, con
   const int64_t token = a.tokens[row];
   const float m = saved[2 * row], s = saved[2 * row + 1], inv = 1.f / s;
   float dl = dlog && token >= 0 ? dlog[row] : 0.f;
-  if (token >= a.V) dl *= __builtin_nanf("");
+  // what nobody asks about a token that there is not is no gradient, and the entropy does not depend on the token
+  if (token >= a.V && dl != 0.f) dl = __builtin_nanf("");
   // -p (dl + dh (log p + H)), log p + H = z + base
   const float dh = dentropy ? dentropy[row] : 0.f, base = dentropy ? entropy[row] - logf(s) : 0.f;
   const float flat = -inv * (dl + dh * base), slope = -inv * dh;

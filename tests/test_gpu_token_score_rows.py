@@ -1,0 +1,51 @@
+"""Gradients of token scores' rows that something is wrong with: a token past the vocabulary, no
+token, no distribution. What does not depend on it stays as it is.
+
+Tolerances as for ordinary rows: 200 roundings of 2^-24 of the norm, and of one for numbers of order one."""
+
+import math
+
+import pytest
+import torch
+
+from oal_amd.token_scores import token_log_probs
+from oracle.heads_oracle import token_scores
+
+pytestmark = pytest.mark.gpu
+
+_SUM = 200 * 2.0 ** -24
+
+
+def _dev():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    return torch.device("cuda:0")
+
+
+def _inputs(rows, vocab, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    return (2 * torch.randn(rows, vocab, generator=gen), torch.randint(0, vocab, (rows,), generator=gen),
+            torch.randn(rows, generator=gen))
+
+
+@pytest.mark.parametrize("rows,vocab", [(4, 50), (3, 40001), (1100, 700)])
+def test_the_entropys_gradient_does_not_depend_on_the_token(rows, vocab):
+    dev = _dev()
+    logits, tokens, up = _inputs(rows, vocab)
+    leaf = logits.double().requires_grad_()
+    want, = torch.autograd.grad(token_scores(leaf, tokens)[1], leaf, up.double())
+    tokens[0], tokens[1 % rows] = vocab, 2 ** 40
+    mine = logits.to(dev).requires_grad_()
+    got = token_log_probs(mine, tokens.to(dev), entropy=True)
+    assert torch.isnan(got.log_probs[0].detach()) and torch.isfinite(got.entropy).all()
+    grad, = torch.autograd.grad(got.entropy, mine, up.to(dev))
+    assert float((grad.cpu().double() - want).norm()) <= _SUM * float(want.norm())
+    # nor does it where the other rows' log probabilities have gradients beside it
+    got = token_log_probs(mine, tokens.to(dev), entropy=True)
+    none = torch.zeros(rows, device=dev)
+    both, = torch.autograd.grad((got.log_probs, got.entropy), mine, (none, up.to(dev)))
+    assert torch.equal(both, grad)
+    # one that is asked for is NaN
+    none[0] = 1.0
+    grad, = torch.autograd.grad(token_log_probs(mine, tokens.to(dev)).log_probs, mine, none)
+    assert torch.isnan(grad[0]).all() and not grad[1:].any()
