@@ -463,7 +463,10 @@ __global__ __launch_bounds__(kThr) void k_scores_bwd(ScoreArgs a, int parts, con
   // -p (dl + dh (log p + H)), log p + H = z + base
   const float dh = dentropy ? dentropy[row] : 0.f, base = dentropy ? entropy[row] - logf(s) : 0.f;
   const float flat = -inv * (dl + dh * base), slope = -inv * dh;
+  // rows that nothing is asked about have no gradient, also those without a distribution (padding, say)
+  const bool asked = dl != 0.f || dh != 0.f;
   auto grad = [&](float v, int64_t i) {
+    if (!asked) return 0.f;
     const float z = v - m;
     const float d = exp_of(z) * fmaf(slope, fmaxf(z, -1e30f), flat);  // where p is zero it is
     return i == token ? d + dl : d;

@@ -49,3 +49,29 @@ def test_the_entropys_gradient_does_not_depend_on_the_token(rows, vocab):
     none[0] = 1.0
     grad, = torch.autograd.grad(token_log_probs(mine, tokens.to(dev)).log_probs, mine, none)
     assert torch.isnan(grad[0]).all() and not grad[1:].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,vocab", [(6, 57), (5, 40001), (1100, 700)])
+def test_rows_that_nothing_is_asked_about_have_no_gradient(rows, vocab, dtype):
+    """Places without a token, as a padded batch has them, whose logits are whatever is there: the others' gradients are
+    those of the others alone."""
+    dev = _dev()
+    logits, tokens, up = _inputs(rows, vocab, seed=3)
+    logits = logits.to(dtype)
+    clean = logits.to(dev).requires_grad_()
+    tokens[:4] = torch.tensor([-1, -100, -1, -2])
+    outs = token_log_probs(clean, tokens.to(dev), entropy=True)
+    up = up.to(dev)
+    live = torch.zeros(rows, device=dev)
+    live[4:] = 1.0
+    want, = torch.autograd.grad(outs[:2], clean, (up, up * live))
+    logits[0], logits[1, 5], logits[2, -1] = -math.inf, math.nan, math.inf
+    logits[3, vocab // 2:] = -math.inf
+    leaf = logits.to(dev).requires_grad_()
+    outs = token_log_probs(leaf, tokens.to(dev), entropy=True)
+    assert not outs.log_probs[:4].any() and torch.isfinite(outs.log_probs).all()
+    grad, = torch.autograd.grad(outs[:2], leaf, (up, up * live))
+    assert not grad[:4].any() and torch.equal(grad, want)
+    grad, = torch.autograd.grad(token_log_probs(leaf, tokens.to(dev)).log_probs, leaf, up)
+    assert not grad[:4].any() and torch.isfinite(grad).all() and grad[4:].any()
