@@ -41,8 +41,6 @@ constexpr int kThr = 256;
 constexpr int kTile2 = 64 * 64;
 // Smallest log-decay: exp of it is zero, and 64 of them leave the sums' differences exact.
 constexpr double kLeast = -1e4;
-// exp of less is zero in fp32.
-constexpr float kNothingKept = -104.f;
 
 // Of a chunk's tokens: log2 of the decay up to and with the token, in two parts; the decay since
 // the chunk's start and until its end, and since and until those of its tile of 16 tokens. end: the chunk's decay in two
@@ -91,11 +89,14 @@ __device__ __forceinline__ double from_lanes(double x) {
   const uint32_t hi = __builtin_amdgcn_update_dpp(0, (uint32_t)(v >> 32), CTRL, ROWS, 0xf, false);
   return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
-__device__ __forceinline__ double running_sum(double x) {
+__device__ __forceinline__ double running_sum_of_16(double x) {
   x += from_lanes<0x111, 0xf>(x);  // row_shr:1, 2, 4, 8
   x += from_lanes<0x112, 0xf>(x);
   x += from_lanes<0x114, 0xf>(x);
-  x += from_lanes<0x118, 0xf>(x);
+  return x + from_lanes<0x118, 0xf>(x);
+}
+__device__ __forceinline__ double running_sum(double x) {
+  x = running_sum_of_16(x);
   x += from_lanes<0x142, 0xa>(x);  // row_bcast:15 into rows 1 and 3
   x += from_lanes<0x143, 0xc>(x);  // row_bcast:31 into rows 2 and 3
   return x;
@@ -309,6 +310,31 @@ __device__ __forceinline__ Frag<UP> scaled_col(const Tile<NP>& s, int c0, int ha
     v[j] *= j < 4 ? b0[j] : b1[j - 4];
   }
   return split<UP>(v);
+}
+
+// Sums over a row of 16 lanes, in all of them.
+__device__ __forceinline__ float sum_of_16(float x) {
+  auto add = [&](auto how) {
+    x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), decltype(how)::value, 0xf, 0xf, true));
+  };
+  add(std::integral_constant<int, 0x128>());  // row_ror:8, 4, 2, 1
+  add(std::integral_constant<int, 0x124>());
+  add(std::integral_constant<int, 0x122>());
+  add(std::integral_constant<int, 0x121>());
+  return x;
+}
+// The sum of what the lane groups before have in this column.
+__device__ __forceinline__ float groups_before(float x, int g) {
+  const float up = __shfl_up(x, 16, 64), a = g >= 1 ? up : 0.f;
+  const float next = __shfl_up(a, 16, 64), b = a + (g >= 2 ? next : 0.f);
+  const float last = __shfl_up(a, 32, 64);
+  return b + (g == 3 ? last : 0.f);
+}
+// Sums over the lane groups of one column: of a in group 0, b in 1, c in 2, d in 3.
+__device__ __forceinline__ float group_sums(float a, float b, float c, float d, int g) {
+  const bool high = g & 2, odd = g & 1;
+  const float x = (high ? c : a) + __shfl_xor(high ? a : c, 32, 64), y = (high ? d : b) + __shfl_xor(high ? b : d, 32, 64);
+  return (odd ? y : x) + __shfl_xor(odd ? x : y, 16, 64);
 }
 
 // Nothing moves over it: operands of later products, loaded early, would not fit the registers.
@@ -608,12 +634,16 @@ __global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 4 : 2) void k_decay_out(De
 //   dk_j = e^(G_63 - G_j) dS' v_j + sum_i D_ij (dO_i.v_j) q_i
 //   dv_j = e^(G_63 - G_j) dS'^T k_j + sum_i D_ij (q_i.k_j) dO_i
 //   dg_t = sum over all pairs j < t <= i of what passes from j to i: with M_ij = D_ij (q_i.k_j) (dO_i.v_j),
-//     r_i = sum_(j < i) M_ij + scale e^(G_i) q_i.(S dO_i), c_j = sum_(i > j) M_ij, s_j = e^(G_63 - G_j) k_j.(dS' v_j),
-//     dg_t = sum_(i >= t) (r_i - c_i) + sum_(j < t) s_j + e^(G_63) <S, dS'>
+//     a_i = scale e^(G_i) q_i.(S dO_i), s_j = e^(G_63 - G_j) k_j.(dS' v_j),
+//     dg_t = sum_(j < t <= i) M_ij + sum_(i >= t) a_i + sum_(j < t) s_j + e^(G_63) <S, dS'>
+//   and no pair that t is not between: where its decay is strong, those are larger than what is asked for by any factor.
+//   So of the pairs of the tiles m <= w of 16 tokens, t in tile T, those with m < T = w are summed over j by query, from t
+//   on; those with m = T < w over i by key, up to t; those of m < T < w whole; those of m = T = w one by one.
 // A block walks back with dS' in its accumulators; S the forward has kept. Both take turns in one tile of LDS. All
-// products are transposed: a wave's 16 tokens are the columns. dg is a difference of large
-// sums and sees all 24 bits of the states, in three parts of X; so do dq and dk, and dv kStateParts.
-// 98 us over 4 x 4096 tokens, 512 blocks at two a CU with all their registers (bf16: ten of them in scratch).
+// products are transposed: a wave's 16 tokens are the columns. dg
+// sees all 24 bits of the states, in three parts of X, and so do dq and dk; dv takes kStateParts.
+// 105 us over 4 x 4096 tokens, 448 blocks at two a CU with all their registers (bf16: twenty of them in scratch): 64 CUs have
+// but one. dg as a difference of sums over all pairs took 96 us and left noise of 1e-7 of the largest sum.
 // ---------------------------------------------------------------------------
 template <typename T>
 __global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 2 : 1) void k_decay_bwd(
@@ -625,7 +655,9 @@ __global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 2 : 1) void k_decay_bwd(
   __shared__ Tile<3> X;  // rows: keys' dimensions
   __shared__ Decays dec[kSlots];
   __shared__ float ss[2][64], ends[2][4];
-  __shared__ double dG[2][64];
+  // a_i; M of a query with the keys of the tiles before its own, of the first, of the first two; of a key with the queries
+  // of the tiles behind its own; of the pairs around a token in its tile
+  __shared__ double ofq[2][4][64], ofk[2][64], ofd[2][64];
   int t = threadIdx.x, lane = t & 63;
   const int w = wave_of(t), g = lane >> 4, c = lane & 15, own = 16 * w + c;
   const Course x(a, sg, blockIdx.x);
@@ -709,8 +741,10 @@ __global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 2 : 1) void k_decay_bwd(
       }
       lds_sync();
       fetch(o + 1 < o0 + each ? ch : max(ch - 1, x.first), o + 1 < o0 + each ? o + 1 : o0);
-      float share = 0.f;  // r_j - c_j of a head
+      // of the head; their sums over heads are in 64 bits
+      auto add = [&](double& sum, float x) { sum = x + (o > o0 ? sum : 0.0); };
       {
+        float a_i = 0.f, near = 0.f, first = 0.f, two = 0.f;
         // queries: own
         const Frag<NP> qf[2] = {row_frag(Q, 16 * w, 0, lane), row_frag(Q, 16 * w, 1, lane)};
         const Frag<NP> of[2] = {row_frag(O, 16 * w, 0, lane), row_frag(O, 16 * w, 1, lane)};
@@ -725,14 +759,26 @@ __global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 2 : 1) void k_decay_bwd(
             qk = mma(row_frag(K, 16 * m, i, lane), qf[i], qk);
           }
           y *= a.scale * decays<false>(d, 16 * m + 4 * g, 16 * m, m == w, hi, lo);
+          if (m == w) {
+            // pairs (j, own query) summed over the keys before 4 g + i, then over the queries from there on
+            float x[4], before[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (m == w) {
-              share += 4 * g + i < c ? y[i] * qk[i] : 0.f;
+            for (int i = 0; i < 4; ++i) {
+              x[i] = 4 * g + i < c ? y[i] * qk[i] : 0.f;
               y[i] = 4 * g + i <= c ? y[i] : 0.f;
-            } else {
-              share += y[i] * qk[i];
+              before[i] = i ? before[i - 1] + x[i - 1] : 0.f;
             }
+            const float less = groups_before(before[3] + x[3], g);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = sum_of_16(4 * g + i <= c ? less + before[i] : 0.f);
+            if (c < 4) add(ofd[turn][16 * w + 4 * g + c], c == 0 ? x[0] : c == 1 ? x[1] : c == 2 ? x[2] : x[3]);
+          } else {
+            float x = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x += y[i] * qk[i];
+            near += x;
+            if (m == 0 && w >= 2) first += x;
+            if (m <= 1 && w == 3) two += x;
           }
           p[m] = half_of<SP>(y);
         }
@@ -746,7 +792,7 @@ __global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 2 : 1) void k_decay_bwd(
           y *= since;
           const f32x4 q = own_values(Q, own, m, lane);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) share += q[i] * y[i];
+          for (int i = 0; i < 4; ++i) a_i += q[i] * y[i];
           y = mma(col_frag_perm(K, 16 * m, 0, lane), p0, y);
           if (w >= 2) y = mma(col_frag_perm(K, 16 * m, 1, lane), p1, y);
           const bool in = own < live && 16 * m + 4 * g < a.D;
@@ -756,10 +802,13 @@ __global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 2 : 1) void k_decay_bwd(
           else
             put4(Window(dq + at), dq, in, to, y);
         }
+        // each lane group has the sum of another one
+        add(ofq[turn][g][own], group_sums(a_i, near, first, two, g));
       }
       phase();
       {
         // keys: own
+        float behind = 0.f;
         const Frag<NP> kf[2] = {row_frag(K, 16 * w, 0, lane), row_frag(K, 16 * w, 1, lane)};
         const Frag<NP> vf[2] = {row_frag(V, 16 * w, 0, lane), row_frag(V, 16 * w, 1, lane)};
         Half<SP> p[4] = {}, r[4] = {};
@@ -778,7 +827,7 @@ __global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 2 : 1) void k_decay_bwd(
             for (int i = 0; i < 4; ++i) e[i] = c <= 4 * g + i ? e[i] : 0.f;
           ov *= e;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) share -= m > w || c < 4 * g + i ? ov[i] * qk[i] : 0.f;
+          for (int i = 0; i < 4; ++i) behind += m > w ? ov[i] * qk[i] : 0.f;
           p[m] = half_of<SP>(ov);
           r[m] = half_of<SP>(e * qk);
         }
@@ -792,10 +841,9 @@ __global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 2 : 1) void k_decay_bwd(
           wk[m] = mma(col_frag_perm(Q, 16 * m, 1, lane), p1, wk[m]);
           wv[m] = mma(col_frag_perm(O, 16 * m, 1, lane), r1, wv[m]);
         }
+        behind = group_sum(behind);
+        if (g == 0) add(ofk[turn][own], behind);
       }
-      // their sums over heads in 64 bits: in 32 dg is off by 8e-7 after seven heads, so by 3e-7
-      share = group_sum(share);
-      if (g == 0) dG[turn][own] = share + (o > o0 ? dG[turn][own] : 0.0);
       if (ch > x.first || (dstate && sg.count == 1)) add_outer<3>(s, O, Q, d.since, a.scale, w, lane);
     } while (++o < o0 + each);
     const size_t at = (size_t)x.u * a.N + tok0;
@@ -815,12 +863,16 @@ __global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 2 : 1) void k_decay_bwd(
     lds_sync();
     // one wave, another for each chunk; the next but one chunk writes these places again, behind a barrier
     if (w == n % 4) {
-      // dg_t = sum of all r_i - c_i, and of s_j - (r_j - c_j) over j < t
-      const double mine = dG[turn][lane], past = lane ? (double)ss[turn][lane - 1] - dG[turn][lane - 1] : 0.0;
-      const double all = lane_of(running_sum(mine), 63);
-      double y = all + running_sum(past) + (((double)ends[turn][0] + ends[turn][1]) + ((double)ends[turn][2] + ends[turn][3]));
-      // where nothing is kept nothing depends on g; the sums' roundings do not cancel
-      if (lane >= live || gate_at(a, x.b, x.h, tok0 + lane) < kNothingKept) y = 0;
+      // sums from a token on are running sums from the last one back
+      const int back = 63 - lane;
+      const double from = running_sum(ofq[turn][0][back]) + running_sum_of_16(ofq[turn][1][back]);
+      const double until = running_sum(lane ? (double)ss[turn][lane - 1] : 0.0) +
+                           running_sum_of_16(c ? ofk[turn][lane - 1] : 0.0);
+      // over a whole tile; those that none passes have zeros
+      const float over1 = wave_sum((float)ofq[turn][2][lane]), over2 = wave_sum((float)ofq[turn][3][lane]);
+      double y = __shfl(from, back, 64) + until + ofd[turn][lane] + (g == 1 ? over1 : g == 2 ? over2 : 0.f) +
+                 (((double)ends[turn][0] + ends[turn][1]) + ((double)ends[turn][2] + ends[turn][3]));
+      if (lane >= live) y = 0;
       if (dgsum) {
 #pragma unroll
         for (int off = 32; off > 0; off >>= 1) y += __shfl_xor(y, off, 64);
