@@ -74,8 +74,12 @@ __device__ __forceinline__ void in_two(double x, float (&y)[2]) {
   y[0] = (float)x;
   y[1] = (float)(x - (double)y[0]);
 }
+// What is forgotten is gone, NaN and infinities too: a decay of zero is no factor.
+__device__ __forceinline__ f32x4 decayed(float by, const f32x4& x) { return by == 0.f ? f32x4{} : by * x; }
 // y = e x + d, e in two parts: slow decays multiply for many chunks.
-__device__ __forceinline__ float carry(const float (&e)[2], float x, float d) { return fmaf(e[0], x, fmaf(e[1], x, d)); }
+__device__ __forceinline__ float carry(const float (&e)[2], float x, float d) {
+  return e[0] == 0.f ? d : fmaf(e[0], x, fmaf(e[1], x, d));
+}
 
 __device__ __forceinline__ float gate_at(const DecayArgs& a, int b, int h, int tok) {
   return static_cast<const float*>(a.g.p)[b * a.g.b + h * a.g.h + tok * a.g.n];
@@ -375,7 +379,7 @@ __device__ __forceinline__ void add_outer(State& x, const Tile<NP>& A, const Til
 // Over a few chunks one part of their decays does (2^-25 each); over many two.
 __device__ __forceinline__ void decay_state(State& x, const float (&end)[2], const DecaySegments& sg) {
 #pragma unroll
-  for (int m = 0; m < 4; ++m) x[m] *= end[0] + (sg.len > 8 ? 0.f : end[1]);
+  for (int m = 0; m < 4; ++m) x[m] = decayed(end[0] + (sg.len > 8 ? 0.f : end[1]), x[m]);
   if (sg.len > 8) {
     const float more = end[0] == 0.f ? 0.f : end[1] / end[0];
 #pragma unroll
@@ -613,7 +617,7 @@ __global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 4 : 2) void k_decay_out(De
         f32x4 y = {};
 #pragma unroll
         for (int k = 0; k < 2; ++k) y = mma(row_frag(S, 16 * m, k, lane), qf[k], y);
-        y *= since;
+        y = decayed(since, y);
         y = mma(col_frag_perm(V, 16 * m, 0, lane), p0, y);
         if (w >= 2) y = mma(col_frag_perm(V, 16 * m, 1, lane), p1, y);
         put4(dst, out, own < live && 16 * m + 4 * g < a.DV, __umul24(own, a.DV) + 16 * m + 4 * g, y);
@@ -713,8 +717,8 @@ __global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 2 : 1) void k_decay_bwd(
           y = mma(row_frag(X, 16 * m, i, lane), vf[i], y);
           z = mma(col_frag<kStateParts<T>>(X, 16 * m, i, lane), kf[i], z);
         }
-        wk[m] = until * y;
-        wv[m] = until * z;
+        wk[m] = decayed(until, y);
+        wv[m] = decayed(until, z);
         const f32x4 k = own_values(K, own, m, lane);
 #pragma unroll
         for (int i = 0; i < 4; ++i) passed += k[i] * wk[m][i];
@@ -727,7 +731,7 @@ __global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 2 : 1) void k_decay_bwd(
     for (int m = 0; m < 4; ++m)
 #pragma unroll
       for (int i = 0; i < 4; ++i) through += before[m][i] * s[m][i];
-    through = wave_sum(through);
+    through = d.end[0] == 0.f ? 0.f : wave_sum(through);
     lds_sync();
     put_state(X, before, w, lane);
     fetch_state(max(ch - 1, x.first));
@@ -789,7 +793,7 @@ __global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 2 : 1) void k_decay_bwd(
           f32x4 y = {};
 #pragma unroll
           for (int i = 0; i < 2; ++i) y = mma(row_frag(X, 16 * m, i, lane), of[i], y);
-          y *= since;
+          y = decayed(since, y);
           const f32x4 q = own_values(Q, own, m, lane);
 #pragma unroll
           for (int i = 0; i < 4; ++i) a_i += q[i] * y[i];
@@ -933,6 +937,12 @@ __global__ __launch_bounds__(kThr) void k_decay_step(DecayStepArgs a) {
   int turn = 0;
   for (int n = 0; n < a.N; ++n) {
     const float decay = expf(static_cast<const float*>(a.g.p)[b * a.g.b + h * a.g.h + n * a.g.n]);
+    if (decay == 0.f) {  // gone, NaN and infinities too
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
+    }
     float vc[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) vc[j] = c0 + j < a.Dv ? get(v + n * a.v.n + c0 + j) : 0.f;
