@@ -5,9 +5,10 @@
 //   log p_v = x_v - m - log s,  H = -sum_v p_v log p_v = log s - t / s
 //   dx_v = dlog (1 if v is the token - p_v) - dH p_v (log p_v + H)
 //
-// Bound by memory: a row is read once, 16 bytes per lane, with running maxima and sums per lane that
+// Bound by memory: a row is read once, 16 bytes per lane, with a running maximum per wave and sums per lane that
 // are joined at the end. Rows are cut into parts where there are fewer than fill the GPU, and a
-// second kernel joins those. All of it is in fp32: a difference to the maximum is one rounding, an exponential two more.
+// second kernel joins those. A value's difference z to the maximum is one rounding in fp32, and its exponential is off by
+// that of z log2 e, up to 2^-24 |z|, and one more; sums are in fp64.
 //
 // 2 x 1000 rows of 151936 bf16 logits with the entropy: forward 150 us (608 MB, 4.1 TB/s), gradient 229 us (1216 MB,
 // 5.3 TB/s). 4096 rows with five alternatives: 261 us (1245 MB, 4.8 TB/s). Beside the loads a value costs about ten
@@ -38,20 +39,22 @@ constexpr float kLog2e = 1.44269504088896340736f;
 
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 
-// A row's running sums.
+// A row's running sums, in 64 bits: of a row with nearly all weight in one place s is 1 and what is asked for. In 32 bits
+// the other values of that place's lane were lost, 2e-3 of a log probability of -3e-4 and 1e-4 of the row's entropy.
 struct Sums {
-  float m, s, t;
+  float m;
+  double s, t;
 };
-constexpr Sums kNothing = {-INFINITY, 0.f, 0.f};
+constexpr Sums kNothing = {-INFINITY, 0, 0};
 // What sums over values with maximum m become with the maximum `to`, which is not lower.
 __device__ __forceinline__ void move_to(Sums& x, float to) {
-  if (x.m == to || x.s == 0.f) {
+  if (x.m == to || x.s == 0) {
     x.m = to;
     return;
   }
   const float d = x.m - to, c = exp_of(d);
   // what vanishes leaves nothing, and not zero times infinity
-  x.t = c > 0.f ? (x.t + x.s * d) * c : 0.f;
+  x.t = c > 0.f ? (x.t + x.s * d) * c : 0;
   x.s *= c;
   x.m = to;
 }
@@ -70,21 +73,43 @@ __device__ __forceinline__ float most_of(const float (&x)[N]) {
   for (int e = 1; e < N; ++e) most = fmaxf(most, x[e]);
   return most;
 }
-// Adds N values, the highest of them `most`. What they are taken relative to follows the maximum only where it is passed
-// by more than e^8: so it hardly ever does (276 us for 286 over 4096 rows), and sums of less than e^8 2^30 are as
-// exact as of less than 2^30.
-constexpr float kBeyond = 8.f;
-template <int N, bool ENTROPY>
-__device__ __forceinline__ void add(Sums& a, const float (&x)[N], float most) {
-  if (most > a.m + kBeyond) move_to(a, most);
-  const float m = a.m == -INFINITY ? 0.f : a.m;  // -inf values weigh nothing
-#pragma unroll
-  for (int e = 0; e < N; ++e) {
-    const float z = x[e] - m, y = exp_of(z);
-    a.s += y;
-    // 0 times -inf is no share
-    if (ENTROPY) a.t = fmaf(y, fmaxf(z, -1e30f), a.t);
+// A turn's values, before they go to the sums: 4096 rows take 268 us, with each piece's going there by itself 275, with
+// sums in 32 bits 260.
+struct Few {
+  float s = 0.f, t = 0.f;
+  __device__ __forceinline__ void to(Sums& a) {
+    a.s += s;
+    a.t += t;
+    s = t = 0.f;
   }
+};
+// Adds each lane's N values, the highest of them `most`; all lanes. They are taken relative to the wave's maximum so far,
+// of which the exponential is one. It seldom moves; the values that come with a new one are added one by one in 64 bits.
+template <int N, bool ENTROPY>
+__device__ __forceinline__ void add(Sums& a, Few& few, const float (&x)[N], float most) {
+  const bool moves = __any(most > a.m);
+  if (moves) {
+    few.to(a);
+    float to = fmaxf(most, a.m);
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) to = fmaxf(to, __shfl_xor(to, off, 64));
+    move_to(a, __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(to))));
+  }
+  const float m = a.m == -INFINITY ? 0.f : a.m;  // -inf values weigh nothing
+  auto each = [&](auto& s, auto& t) {
+    typedef std::remove_reference_t<decltype(s)> S;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float z = x[e] - m, y = exp_of(z);
+      s += y;
+      // 0 times -inf is no share
+      if (ENTROPY) t = fma((S)y, (S)fmaxf(z, -1e30f), t);
+    }
+  };
+  if (moves)
+    each(a.s, a.t);
+  else
+    each(few.s, few.t);
 }
 
 // A wave's highest values in order, one per lane. Empty places are below all values, -inf too.
@@ -204,7 +229,8 @@ __device__ __forceinline__ void offer(Best& b, float (&x)[N], float most, uint32
 
 // What a part of a row leaves: its sums, then the values of its best and their places.
 struct Part {
-  float m, s, t, unused;
+  double s, t;
+  float m;
 };
 
 template <typename T>
@@ -290,15 +316,17 @@ template <typename T, bool ENTROPY, bool TOP>
 __device__ __forceinline__ void finish(const ScoreArgs& a, const ScoreOut& out, int64_t row, const Sums& sum,
                                        const Best& b) {
   const int t = threadIdx.x;
-  const float log = logf(sum.s);
+  const double lse = sum.m + log(sum.s);
   if (t == 0) {
     const int64_t token = a.tokens[row];
-    out.logp[row] = token < 0 ? 0.f : token < a.V ? get(row_at<T>(a, row) + token) - sum.m - log : __builtin_nanf("");
-    if (ENTROPY) out.entropy[row] = log - sum.t / sum.s;
-    if (out.saved) out.saved[2 * row] = sum.m, out.saved[2 * row + 1] = sum.s;
+    out.logp[row] = token < 0        ? 0.f
+                    : token < a.V ? (float)(get(row_at<T>(a, row) + token) - lse)
+                                  : __builtin_nanf("");
+    if (ENTROPY) out.entropy[row] = (float)(log(sum.s) - sum.t / sum.s);
+    if (out.saved) out.saved[2 * row] = sum.m, out.saved[2 * row + 1] = (float)sum.s;
   }
   if (TOP && t < a.top) {
-    out.top[row * a.top + t] = b.x - sum.m - log;
+    out.top[row * a.top + t] = (float)(b.x - lse);
     out.place[row * a.top + t] = b.at == 0xffffffffu ? -1 : (int64_t)b.at;
   }
 }
@@ -318,6 +346,7 @@ __global__ __launch_bounds__(kThr) void k_scores(ScoreArgs a, ScoreOut out, int 
   const T* x = row_at<T>(a, row);
   const int pieces = a.V / P, first = (int)((int64_t)pieces * part / parts), end = (int)((int64_t)pieces * (part + 1) / parts);
   Sums mine = kNothing;
+  Few few;
   Best b;
   // The waves tell one another the last value that counts, when they come to it: late news lets more through, no less
   // (286 us for 303 over 4096 rows).
@@ -336,7 +365,7 @@ __global__ __launch_bounds__(kThr) void k_scores(ScoreArgs a, ScoreOut out, int 
   auto take = [&](auto& v, uint32_t i, bool in) {
     constexpr int N = sizeof(v) / sizeof(v[0]);
     const float most = most_of(v);
-    add<N, ENTROPY>(mine, v, most);
+    add<N, ENTROPY>(mine, few, v, most);
     if constexpr (TOP) offer<N>(b, v, most, i, in, limit, a.top, lane);
   };
   // A wave's turns: whole ones, of which the next is on its way, then piece by piece, with lanes past the end that have
@@ -363,6 +392,7 @@ __global__ __launch_bounds__(kThr) void k_scores(ScoreArgs a, ScoreOut out, int 
         values(v, raw[n]);
         take(v, (uint32_t)(i + n * kThr + lane) * P, true);
       }
+      few.to(mine);
       i = after;
     } while (i + kWhole <= end);
   }
@@ -377,12 +407,14 @@ __global__ __launch_bounds__(kThr) void k_scores(ScoreArgs a, ScoreOut out, int 
       for (int e = 0; e < P; ++e) v[e] = -INFINITY;
     if constexpr (TOP) hear();
     take(v, (uint32_t)p * P, p < end);
+    few.to(mine);
   }
   // values behind the last whole piece
   if (part == parts - 1 && w == kWaves - 1 && pieces * P < a.V) {
     const int p = pieces * P + lane;
     float v[1] = {p < a.V ? get(x + p) : -INFINITY};
     take(v, p, p < a.V);
+    few.to(mine);
   }
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) {
@@ -400,7 +432,7 @@ __global__ __launch_bounds__(kThr) void k_scores(ScoreArgs a, ScoreOut out, int 
     finish<T, ENTROPY, TOP>(a, out, row, mine, b);
     return;
   }
-  if (t == 0) sums[blockIdx.x] = {mine.m, mine.s, mine.t, 0.f};
+  if (t == 0) sums[blockIdx.x] = {mine.s, mine.t, mine.m};
   if (TOP && t < a.top) {
     best[(size_t)blockIdx.x * a.top + t] = b.x;
     best_at[(size_t)blockIdx.x * a.top + t] = b.at;

@@ -7,6 +7,7 @@ import pytest
 import torch
 
 from oal_amd.decay_attention import decay_attention
+from oal_amd.token_scores import token_log_probs
 from oracle.decay_oracle import decay_attention as definition
 
 pytestmark = pytest.mark.gpu
@@ -66,3 +67,29 @@ def test_results_with_decays_are_rounded_once(heads, dtype):
         err = _error(got[name], want[name].to(dtype))
         print(f"{heads} {dtype} {name}: {err:.2e} of {bound:.2e}", flush=True)
         assert got[name].dtype == dtype and err <= bound, f"{name}: {err:.3g}"
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,vocab,peaks", [(24, 151936, (14, 24)), (1100, 20000, (12, 22)), (7, 1000, (10, 20))])
+def test_scores_of_rows_with_nearly_all_weight_in_one_place(rows, vocab, peaks, dtype):
+    """A model that is sure: the log probability of what it expects and the entropy are small sums over all the
+    other tokens, whose terms have one sign. Their exponents, up to 42 in base two, are rounded by half of 2^-18 at most,
+    1.4e-6 of a term, and their sums by 24 roundings of 2^-24 at most: each result is off by 4e-6 of itself at
+    most. In sums of 32 bits from one on it was up to 2e-2."""
+    gen = torch.Generator().manual_seed(vocab)
+    logits = torch.randn(rows, vocab, generator=gen)
+    tokens = torch.randint(0, vocab, (rows,), generator=gen)
+    logits[torch.arange(rows), tokens] = torch.linspace(*peaks, rows)
+    logits = logits.to(dtype).to(_dev())
+    tokens = tokens.to(logits.device)
+    log = torch.log_softmax(logits.double(), -1)
+    # 1 - p as a sum, which is what float64 has left of it too
+    rest = log.exp().scatter(-1, tokens[:, None], 0.0)
+    sure = torch.log1p(-rest.sum(-1))
+    want = {"log_probs": sure, "entropy": -(rest * log).sum(-1) - sure.exp() * sure, "top_log_probs": sure}
+    got = token_log_probs(logits, tokens, entropy=True, top=1)
+    assert torch.equal(got.top_tokens[:, 0], tokens)
+    for name, y in want.items():
+        err = float(((getattr(got, name).double().view(rows) - y) / y).abs().max())
+        print(f"{rows} {vocab} {dtype} {name}: {err:.2e}", flush=True)
+        assert err <= 4e-6, f"{name}: {err:.3g}"
