@@ -38,6 +38,8 @@ constexpr int kWaves = kThr / 64;
 constexpr float kLog2e = 1.44269504088896340736f;
 
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
+// A logarithm whose exponential is zero: lower ones, -inf among them, are this where they are multiplied with it.
+constexpr float kGone = -200.f;
 
 // A row's running sums, in 64 bits: of a row with nearly all weight in one place s is 1 and what is asked for. In 32 bits
 // the other values of that place's lane were lost, 2e-3 of a log probability of -3e-4 and 1e-4 of the row's entropy.
@@ -102,8 +104,7 @@ __device__ __forceinline__ void add(Sums& a, Few& few, const float (&x)[N], floa
     for (int e = 0; e < N; ++e) {
       const float z = x[e] - m, y = exp_of(z);
       s += y;
-      // 0 times -inf is no share
-      if (ENTROPY) t = fma((S)y, (S)fmaxf(z, -1e30f), t);
+      if (ENTROPY) t = fma((S)y, (S)fmaxf(z, kGone), t);
     }
   };
   if (moves)
@@ -500,7 +501,7 @@ __global__ __launch_bounds__(kThr) void k_scores_bwd(ScoreArgs a, int parts, con
   auto grad = [&](float v, int64_t i) {
     if (!asked) return 0.f;
     const float z = v - m;
-    const float d = exp_of(z) * fmaf(slope, fmaxf(z, -1e30f), flat);  // where p is zero it is
+    const float d = exp_of(z) * fmaf(slope, fmaxf(z, kGone), flat);  // where p is zero it is
     return i == token ? d + dl : d;
   };
   const int64_t pieces = a.V / P, first = pieces * part / parts, end = pieces * (part + 1) / parts;

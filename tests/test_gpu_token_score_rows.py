@@ -75,3 +75,18 @@ def test_rows_that_nothing_is_asked_about_have_no_gradient(rows, vocab, dtype):
     assert not grad[:4].any() and torch.equal(grad, want)
     grad, = torch.autograd.grad(token_log_probs(leaf, tokens.to(dev)).log_probs, leaf, up)
     assert not grad[:4].any() and torch.isfinite(grad).all() and grad[4:].any()
+
+
+@pytest.mark.parametrize("scale", [1.0, 1e10, 1e30])
+def test_masked_logits_under_large_gradients(scale):
+    """A logit of -inf has no gradient, however large the entropy's is (a scaled loss)."""
+    dev = _dev()
+    logits, tokens, up = _inputs(5, 3001, seed=5)
+    logits[:, ::3] = -math.inf
+    tokens = tokens // 3 * 3 + 1
+    leaf = logits.double().requires_grad_()
+    want, = torch.autograd.grad(token_scores(leaf, tokens)[1], leaf, scale * up.double())
+    mine = logits.to(dev).requires_grad_()
+    grad, = torch.autograd.grad(token_log_probs(mine, tokens.to(dev), entropy=True).entropy, mine, scale * up.to(dev))
+    assert not grad[:, ::3].any()
+    assert float((grad.cpu().double() - want).norm()) <= _SUM * float(want.norm())
