@@ -1,7 +1,9 @@
 """Gradients of token scores' rows that something is wrong with: a token past the vocabulary, no
 token, no distribution. What does not depend on it stays as it is.
 
-Tolerances as for ordinary rows: 200 roundings of 2^-24 of the norm, and of one for numbers of order one."""
+And the alternatives of all rows of a large call.
+
+Tolerances: 200 roundings of 2^-24 of the norm for gradients; two where exponentials' errors go either way."""
 
 import math
 
@@ -9,7 +11,7 @@ import pytest
 import torch
 
 from oal_amd.token_scores import token_log_probs
-from oracle.heads_oracle import token_scores
+from oracle.heads_oracle import token_scores, top_tokens
 
 pytestmark = pytest.mark.gpu
 
@@ -90,3 +92,20 @@ def test_masked_logits_under_large_gradients(scale):
     grad, = torch.autograd.grad(token_log_probs(mine, tokens.to(dev), entropy=True).entropy, mine, scale * up.to(dev))
     assert not grad[:, ::3].any()
     assert float((grad.cpu().double() - want).norm()) <= _SUM * float(want.norm())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,vocab,top", [(1100, 20003, 20), (300, 60000, 5), (1030, 50001, 64)])
+def test_alternatives_of_every_row_over_many_turns(rows, vocab, top, dtype):
+    """Rows of several turns of a block's waves, whole and in parts: the lists that the waves of a row share a limit for, with
+    the many equal values that 16-bit logits have."""
+    gen = torch.Generator().manual_seed(top)
+    logits = (2 * torch.randn(rows, vocab, generator=gen)).to(dtype).to(_dev())
+    tokens = torch.randint(0, vocab, (rows,), generator=gen).to(logits.device)
+    values, places = top_tokens(logits, top)
+    got = token_log_probs(logits, tokens, entropy=True, top=top)
+    assert torch.equal(got.top_tokens, places)
+    lse = torch.logsumexp(logits.double(), -1, keepdim=True)
+    for x, y in ((got.top_log_probs, values - lse), (got.log_probs, logits.double().gather(-1, tokens[:, None])[:, 0] - lse[:, 0]),
+                 (got.entropy, token_scores(logits, tokens)[1])):
+        assert float((x.double() - y).norm()) <= 2 * 2.0 ** -24 * float(y.norm())
