@@ -108,18 +108,20 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(2) < 1 << 23 or t.shape[2] == 1 else t.contiguous()
 
 
+def _ready(q, k, v, g, state):
+    """The operands as the kernels read them."""
+    return (*map(_rows, (q, k, v)), g, None if state is None else _native._aligned(state.contiguous()))
+
+
 class _DecayFunction(torch.autograd.Function):
     """(q, k, v, g, state or None, scale) -> (out, final state); dimensions multiples of 8, on one ROCm device."""
 
     @staticmethod
     def forward(ctx: Any, q, k, v, g, state, scale: float):
-        q, k, v = map(_rows, (q, k, v))
-        start = None if state is None else _native._aligned(state.contiguous())
-        keep = any(ctx.needs_input_grad)
-        out, final, saved = _native.decay_forward(q, k, v, g, start, scale=scale, keep=keep)
-        if keep:
-            ctx.save_for_backward(q, k, v, g, saved)
-            ctx.scale = scale
+        operands = _ready(q, k, v, g, state)
+        out, final, saved = _native.decay_forward(*operands, scale=scale, keep=True)
+        ctx.save_for_backward(*operands[:4], saved)
+        ctx.scale = scale
         return out, final
 
     @staticmethod
@@ -150,13 +152,16 @@ def decay_attention(
     scale = _validate_scale(scale, d)
     _native.require_eager("decay_attention", q, k, v, g, initial_state)
     _native._require_device(q)
-    if d % 8 == 0 and dv % 8 == 0:
-        return _DecayFunction.apply(q, k, v, g, initial_state, scale)
-    state = initial_state
-    if state is not None:
-        state = torch.nn.functional.pad(state, (0, -dv % 8, 0, -d % 8))
-    out, final = _DecayFunction.apply(_pad8(q), _pad8(k), _pad8(v), g, state, scale)
-    return out[..., :dv], final[..., :d, :dv].contiguous()  # as decay_step takes it
+    operands, narrow = (q, k, v, g, initial_state), d % 8 or dv % 8
+    if narrow:
+        state = None if initial_state is None else torch.nn.functional.pad(initial_state, (0, -dv % 8, 0, -d % 8))
+        operands = (_pad8(q), _pad8(k), _pad8(v), g, state)
+    # a prompt keeps no states for a backward, also where a head's decay is a parameter
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in operands):
+        out, final = _DecayFunction.apply(*operands, scale)
+    else:
+        out, final = _native.decay_forward(*_ready(*operands), scale=scale, keep=False)[:2]
+    return (out[..., :dv], final[..., :d, :dv].contiguous()) if narrow else (out, final)  # as decay_step takes it
 
 
 def decay_step(
