@@ -17,11 +17,11 @@
 // Decays enter as differences of sums, held in two floats (48 bits): a token that
 // forgets everything (g of -inf, the first of a new text) leaves large sums whose differences still matter.
 //
-// 4 x 4096 tokens of 14/14/14 heads of 64, bf16, forward and backward: 191 us of kernels, of which the gradients are 98,
+// 4 x 4096 tokens of 14/14/14 heads of 64, bf16, forward and backward: 199 us of kernels, of which the gradients are 106,
 // the outputs 39, both sums 35, both scans 14. What has to be read and written takes 47 us at the rate of a large copy. What
-// bounds it is the vector unit's work on operands (decays, splits into parts, fragments from LDS), 1600 instructions a
+// bounds it is the vector unit's work on operands (decays, splits into parts, fragments from LDS), 1800 instructions a
 // wave and chunk in the backward, and waiting between phases that depend on one another: there the vector units
-// are busy for 45 % of the time, the matrix units for 15 %, and waves wait for 42 % of theirs. A prompt of 32768 tokens, 7/7/14 heads: 85 us, copied in 35.
+// are busy for 45 % of the time, the matrix units for 14 %, and waves wait for 42 % of theirs. A prompt of 32768 tokens, 7/7/14 heads: 91 us, copied in 35.
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -350,14 +350,13 @@ __device__ __forceinline__ int here(int x) {
   return x;
 }
 
-// Parts of the scores inside a chunk. bf16 ones in two, off by 2^-16, as float16 ones: results are then off by their own
-// rounding and the states' (1.0 to 1.07 of it over 1 to 500 tokens; with scores of one part 1.4), in the same time:
-// 4 x 4096 tokens, forward and backward, 197 us either way.
+// Parts of the scores inside a chunk. bf16 ones in two, off by 2^-17, as float16 ones, so that a result is rounded once, to
+// its own type: in one part bf16 results were 2.2e-3 off where a rounding is 1.7e-3 (4 x 4096 tokens, forward and
+// backward, 192 us for 199); three parts take 9 us more.
 template <typename T>
 constexpr int kScoreParts = kPartsOf<T> == 1 ? 2 : kPartsOf<T>;
-// Parts of the states that 16-bit results read: two too, off by 2^-17, so that a result is rounded once, to its own
-// type. In one part bf16 outputs were 1.9e-3 off where a rounding is 1.7e-3 (32768 tokens, k_decay_out 51 us for 56);
-// three parts leave room for three blocks a CU in place of four (69 us).
+// Parts of the states that 16-bit results read: two too. In one part bf16 outputs were 1.9e-3 off (32768 tokens,
+// k_decay_out 51 us for 56); three parts leave room for three blocks a CU in place of four (67 us).
 template <typename T>
 constexpr int kStateParts = kPartsOf<T> == 1 ? 2 : kPartsOf<T>;
 
@@ -546,8 +545,8 @@ __global__ __launch_bounds__(kThr) void k_decay_scan(Scan a) {
 // accumulators and, as bf16 parts (kStateParts), in LDS. Outputs are transposed: a wave's 16 queries
 // are the columns, so the scores are an operand of the product with V as they are.
 // UP: parts of what the state takes on, three where it goes on to the caller or (states: kept before every
-// chunk) to the backward, two where no further than the segment's own outputs (32768 tokens: 51 us for 56).
-// In training 39 us over 4 x 4096 tokens, 117 MB of heads and 59 MB of states (4.5 TB/s).
+// chunk) to the backward, two, off by 2^-17 as what outputs read of it, where no further than the segment's own outputs (32768 tokens: 56 us
+// for 62). In training 39 us over 4 x 4096 tokens, 117 MB of heads and 59 MB of states (4.5 TB/s).
 template <typename T, int UP>
 __global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 4 : 2) void k_decay_out(DecayArgs a, DecaySegments sg, int each,
                                                                               From from, T* __restrict__ out,
@@ -646,7 +645,7 @@ __global__ __launch_bounds__(kThr, kPartsOf<T> == 1 ? 4 : 2) void k_decay_out(De
 // A block walks back with dS' in its accumulators; S the forward has kept. Both take turns in one tile of LDS. All
 // products are transposed: a wave's 16 tokens are the columns. dg
 // sees all 24 bits of the states, in three parts of X, and so do dq and dk; dv takes kStateParts.
-// 105 us over 4 x 4096 tokens, 448 blocks at two a CU with all their registers (bf16: twenty of them in scratch): 64 CUs have
+// 106 us over 4 x 4096 tokens, 448 blocks at two a CU with all their registers (bf16: ten of them in scratch): 64 CUs have
 // but one. dg as a difference of sums over all pairs took 96 us and left noise of 1e-7 of the largest sum.
 // ---------------------------------------------------------------------------
 template <typename T>
@@ -1016,8 +1015,8 @@ int heads_each(const DecayArgs& a, const DecaySegments& sg) {
   return (rep + parts - 1) / parts;
 }
 // Segments so that `blocks` blocks have one each, those that the GPU holds at once: four a CU in the forward, two in the
-// backward. Forward with 512, 1024 and 2048 blocks: 98, 85 and 90 us for 32768 tokens, 189, 191 and 203 for training over
-// 4 x 4096; backward with 256, 512 and 1024: 241, 191 and 190.
+// backward. Forward with 512, 1024 and 2048 blocks: 106, 92 and 94 us for 32768 tokens, 202, 201 and 211 for training over
+// 4 x 4096; backward with 256, 512 and 1024: 257, 201 and 200.
 DecaySegments segments(int U, int NC, int blocks) {
   const int count = std::clamp(blocks / U, 1, NC), len = (NC + count - 1) / count;
   return {(NC + len - 1) / len, len};

@@ -11,8 +11,9 @@
 // that of z log2 e, up to 2^-24 |z|, and one more; sums are in fp64.
 //
 // 2 x 1000 rows of 151936 bf16 logits with the entropy: forward 150 us (608 MB, 4.1 TB/s), gradient 229 us (1216 MB,
-// 5.3 TB/s). 4096 rows with five alternatives: 261 us (1245 MB, 4.8 TB/s). Beside the loads a value costs about ten
-// instructions, an exponential of four times the price among them. One row with 20 alternatives: 12 us in 49 parts and 6 to join them, most of it the lists' beginnings;
+// 5.3 TB/s). 4096 rows with five alternatives: 266 us (1245 MB, 4.7 TB/s). Beside the loads a value costs about ten
+// instructions, an exponential of four times the price among them. One row with 20 alternatives: 13 us in 49 parts, whose loads
+// are waited for one by one (score_parts) while the lists begin, and 7 to join them;
 // 48 rows of 32003 fp32 logits in 10 parts each: 16 and 5.
 //
 // The alternatives: a wave keeps the highest 64 of its values so far in order, one per lane, and
@@ -236,9 +237,9 @@ struct Part {
 
 template <typename T>
 constexpr int kPiece = 16 / sizeof(T);
-// Pieces of a lane in flight at once, in the forward with as many of the next turn: with 2, 3 and 4 the 4096 rows take 254,
-// 261 and 258 us, 2 x 1000 rows forward 152, 150 and 145, back 230, 229 and 256, 48 short rows 20, 20 and 23. Without the
-// next turn on its way the forward takes 276 and 152.
+// Pieces of a lane in flight at once, in the forward with as many of the next turn: with 2, 3 and 4 the 4096 rows take 262,
+// 266 and 260 us, 2 x 1000 rows forward 153, 152 and 152, back 230, 227 and 226, 48 short rows 20, 21 and 24. Without the
+// next turn on its way the forward takes 267 and 156.
 constexpr int kTurn = 3;
 
 // 16 bytes of a row, at any address of its type: rows of an odd vocabulary begin where they may.
@@ -350,7 +351,7 @@ __global__ __launch_bounds__(kThr) void k_scores(ScoreArgs a, ScoreOut out, int 
   Few few;
   Best b;
   // The waves tell one another the last value that counts, when they come to it: late news lets more through, no less
-  // (286 us for 303 over 4096 rows).
+  // (266 us for 273 over 4096 rows).
   __shared__ float lasts[kWaves];
   if constexpr (TOP) {
     if (lane == 0) lasts[w] = -INFINITY;
@@ -527,8 +528,10 @@ __global__ __launch_bounds__(kThr) void k_scores_bwd(ScoreArgs a, int parts, con
 namespace {
 int score_parts(const ScoreArgs& a) {
   const int64_t rows = (int64_t)a.B * a.N;
-  // Parts fill the GPU's 256 CUs four times; a part has a turn of the block's pieces or more, and a wave joins 64 parts at
-  // most. With twice or half as many blocks one row, 48 and 2000 take the same within 1%.
+  // Parts fill the GPU's 256 CUs four times, and a wave joins 64 parts at most. A part has a turn of the block's pieces
+  // of fp32 logits or more; of 16-bit ones, whose pieces hold twice as many values, half a turn, so that few rows of them
+  // (one of 151936: 49 parts of 387 pieces) go piece by piece, in more blocks. With twice or half as many blocks one row,
+  // 48 and 2000 take the same within 1%.
   const int64_t most = std::max(1, a.V / (kThr * kTurn * 4));
   return (int)std::clamp<int64_t>((1024 + rows - 1) / rows, 1, std::min<int64_t>(most, 64));
 }

@@ -7,9 +7,10 @@ The mean of -log p over a text is its next-token loss: :func:`token_log_probs` i
 logits, through log_probs and entropy. It holds no float32 copy of the logits, and its backward keeps two
 numbers for each row beside them.
 
-Logits are float32, bfloat16 or float16; sums and results are float32. A logit of -inf is a token
-that cannot be; a row of such logits alone, and one with NaN or +inf, has NaN scores, as log_softmax has. Results repeat bit
-by bit from call to call; few rows are cut into parts by a rule on their number, so that last bits
+Logits are float32, bfloat16 or float16; exponentials and results are float32, sums over a row float64, so that small
+log probabilities and entropies, of a model that is sure, are as exact as others. A logit of -inf is a token
+that cannot be; a row of such logits alone, and one with NaN or +inf, has NaN scores, as log_softmax has, and a gradient of NaN
+if one is asked of it. Results repeat bit by bit from call to call; few rows are cut into parts by a rule on their number, so that last bits
 depend on how many others are in the call.
 
 Calls are eager: tracers, functorch's transforms and forward-mode derivatives are refused
