@@ -344,8 +344,10 @@ def score_tokens(model: QwenOALModel, tokens: torch.Tensor, *, lengths: torch.Te
     tokens of each sequence of a batch padded at its end; behind them log probabilities are zero."""
     if tokens.ndim != 2:
         raise ValueError("tokens must be [B, N]")
-    if lengths is not None and (lengths.shape != tokens.shape[:1] or lengths.is_floating_point()):
-        raise ValueError("lengths must be integers [B]")
+    if lengths is not None and (
+            not isinstance(lengths, torch.Tensor) or lengths.shape != tokens.shape[:1] or lengths.dtype is torch.bool
+            or lengths.is_floating_point() or lengths.is_complex() or lengths.device != tokens.device):
+        raise ValueError("lengths must be integers [B], on the tokens' device")
     targets = tokens[:, 1:]
     if lengths is not None:
         places = torch.arange(1, tokens.shape[1], device=tokens.device)
