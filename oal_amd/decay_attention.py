@@ -23,8 +23,8 @@ query head o // (H / Hq) from state head o // (H / Hv).
 Sums over tokens do not depend on the type of q, k and v, which may be
 float32, bfloat16 or float16: states, decays and their gradients are exact to float32, those of each decay by itself. 16-bit
 results are rounded once, from sums whose terms are off by 2^-17 at most.
-Values have to be finite: a token that is not spoils the 64 tokens of its chunk (in :func:`decay_step` itself), what
-depends on those behind them and before them, and the state. What was forgotten by g = -inf in another chunk, or in an
+Values have to be finite: a token that is not spoils the 64 tokens of its chunk (in :func:`decay_step` itself), and with them
+the state, the results behind and the gradients before. What was forgotten by g = -inf in another chunk, or in an
 initial state or a step before, does not matter, whatever it is. Results repeat bit by bit from call to call;
 sequences are cut into segments by a rule on batch, heads and length, so that last bits depend on those.
 
